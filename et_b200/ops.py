@@ -16,7 +16,7 @@ __all__ = [
     "gen_sparse_tile_mat", "gen_sparse_row_mat", "build_head_ptr", "Encoder", "encoder_buffer_size",
     "encoder_batch_buffer_size", "KIND_TILE", "KIND_PRUNE", "KIND_LENGTH", "KIND_PRUNE_QKV",
     "Model", "attention_check", "prune_dense_to_tiles", "select_rows_magnitude", "compact_rows", "set_tuning_goal",
-    "set_attention_scores_fp32", "attention_scores_fp32",
+    "set_attention_scores_fp32", "attention_scores_fp32", "rotary_axes", "AdapterBank", "attention_rules", "attention_rules_scratch_size",
 ]
 
 _i = ctypes.c_int
@@ -29,7 +29,8 @@ _SIGNATURES = {
     "et_tile_spmm_bias": "pppppiiipip", "et_attention_otf": "pppppiiip", "et_attention_prune": "ppppppipiiip",
     "et_qk_scores": "pppiiip", "et_attention_sharedqk": "ppppiiip", "et_attention_static_scores": "pppppiiip",
     "et_attention_batch": "ppppiippppippiiiiiip", "et_encoder_run": "pppp", "et_encoder_run_batch": "pppppipsp",
-    "et_model_run_batch": "pppppip",
+    "et_model_run_batch": "pppppip", "et_rotary_axes": "ppiiippiiiiipippiip", "et_adapter_add": "ppppiiippiip",
+    "et_attention_rules": "ppppiiiiiiipppiiiiippsp",
 }
 
 
@@ -265,6 +266,172 @@ def attention_batch(out, Q, K, V, d_model, nhead, cu_seqlens=None, valid_lens=No
         _a(out), _a(Q), _a(K), _a(V), Q.shape[1] if qk_pitch is None else qk_pitch, V.shape[1] if v_pitch is None else v_pitch,
         _a(qk_head_ptr), _a(v_col_id), _a(v_head_ptr), _a(mask), mask_ld, _a(cu_seqlens), _a(valid_lens), batch, uniform_len,
         max_seq_len, total, d_model, nhead, raw_stream(stream))
+    if rc:
+        check(rc)
+    return out
+
+
+# ---------------------------------------------------------------------------------- positions, adapters, rules on scores
+_current_device = None
+
+
+def _device():
+    global _current_device
+    if _current_device is None:
+        import torch
+        torch.cuda.init()
+        try:
+            _current_device = torch._C._cuda_getDevice
+        except AttributeError:
+            _current_device = torch.cuda.current_device
+    return _current_device()
+
+
+def _checked(name, t, dtype, dims, device, last=True):
+    """Refuses a tensor that is not what the library would take it for: type, dimensions, neighbouring elements, device."""
+    if t.dtype != dtype or t.dim() != dims:
+        raise ValueError(f"{name}: {dims}-dimensional {dtype} expected, not {t.dim()}-dimensional {t.dtype}")
+    if t.device.type != "cuda" or t.device.index != device:
+        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device {device}")
+    if dims and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}: the elements of a row must be neighbours")
+    if not last and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t
+
+
+def _pitch(t):
+    """Elements from one row to the next (of a single row: its width)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rotary_axes(q_out, k_out, q, k, positions, inv_freq, axis, head_dim, interleaved=False, stream=None):
+    """Rotary positions over several axes on the heads of q [tokens, heads * head_dim] and k (either may be None); rows may be slices of
+    wider ones, q_out may be q and k_out may be k. positions [tokens, axes] int32; inv_freq float32 and axis int32, one for each
+    pair of features (twice as many features are turned). Returns (q_out, k_out)."""
+    import torch
+    device = _device()
+    f16, i32 = torch.float16, torch.int32
+    heads, pitches = [], []
+    tokens, axes = _checked("positions", positions, i32, 2, device, last=False).shape
+    pairs, = _checked("inv_freq", inv_freq, torch.float32, 1, device, last=False).shape
+    if _checked("axis", axis, i32, 1, device, last=False).shape[0] != pairs:
+        raise ValueError("inv_freq and axis: one element for each pair")
+    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
+        if x is None:
+            heads.append(0)
+            pitches.append((0, 0))
+            continue
+        _checked(name, x, f16, 2, device)
+        _checked(name + "_out", out, f16, 2, device)
+        if x.shape != out.shape or x.shape[0] != tokens or x.shape[1] % head_dim:
+            raise ValueError(f"{name}: {tokens} rows of whole heads of {head_dim}, the result alike")
+        heads.append(x.shape[1] // head_dim)
+        pitches.append((_pitch(out), _pitch(x)))
+    rc = (_entries or _lib()).et_rotary_axes(
+        _a(q_out if q is not None else None), _a(q), *pitches[0], heads[0], _a(k_out if k is not None else None), _a(k), *pitches[1], heads[1], head_dim,
+        2 * pairs, positions.data_ptr(), axes, inv_freq.data_ptr(), axis.data_ptr(), 1 if interleaved else 0, tokens, raw_stream(stream))
+    if rc:
+        check(rc)
+    return q_out, k_out
+
+
+class AdapterBank:
+    """Low-rank adapters of one projection, for sequences that each have one of them (or none): out = base + scale B (A x)."""
+
+    def __init__(self, in_feat, out_feat, max_rank, slots):
+        self.in_feat, self.out_feat, self.max_rank, self.slots = in_feat, out_feat, max_rank, slots
+        self._h = ctypes.c_void_p(0)
+        check(lib().et_adapter_bank_create(ctypes.byref(self._h), _i(in_feat), _i(out_feat), _i(max_rank), _i(slots)))
+
+    def set(self, slot, A, B, scale=1.0):
+        """Fills a slot: A [rank, in_feat], B [out_feat, rank], host arrays. Synchronises the device."""
+        A, B = np.ascontiguousarray(A, dtype=np.float16), np.ascontiguousarray(B, dtype=np.float16)
+        if A.ndim != 2 or B.ndim != 2 or A.shape[1] != self.in_feat or B.shape[0] != self.out_feat or A.shape[0] != B.shape[1]:
+            raise ValueError(f"A [rank, {self.in_feat}] and B [{self.out_feat}, rank] expected, not {A.shape} and {B.shape}")
+        check(lib().et_adapter_bank_set(self._h, _i(slot), _i(A.shape[0]), ptr(A), ptr(B), ctypes.c_float(scale)))
+
+    def clear(self, slot):
+        """Empties a slot: its sequences get base. Synchronises the device."""
+        check(lib().et_adapter_bank_set(self._h, _i(slot), _i(0), None, None, ctypes.c_float(0.0)))
+
+    def add(self, out, base, x, adapter_ids, cu_seqlens=None, stream=None):
+        """out = base + the adapter's product for each sequence's tokens. adapter_ids int32 [batch] (-1: none), cu_seqlens int32 [batch + 1]
+        or None (one token to a sequence). out may be base; rows may be slices of wider ones."""
+        import torch
+        device = _device()
+        for name, t, width in (("out", out, self.out_feat), ("base", base, self.out_feat), ("x", x, self.in_feat)):
+            if _checked(name, t, torch.float16, 2, device).shape[1] != width or t.shape[0] != x.shape[0]:
+                raise ValueError(f"{name}: {x.shape[0]} rows of {width} expected, not {tuple(t.shape)}")
+        batch, = _checked("adapter_ids", adapter_ids, torch.int32, 1, device, last=False).shape
+        if cu_seqlens is not None and _checked("cu_seqlens", cu_seqlens, torch.int32, 1, device, last=False).shape[0] != batch + 1:
+            raise ValueError("cu_seqlens: one element more than adapter_ids")
+        rc = (_entries or _lib()).et_adapter_add(self._h, out.data_ptr(), base.data_ptr(), x.data_ptr(), _pitch(out), _pitch(base), _pitch(x), _a(cu_seqlens),
+                                                 adapter_ids.data_ptr(), batch, x.shape[0], raw_stream(stream))
+        if rc:
+            check(rc)
+        return out
+
+    def close(self):
+        if self._h:
+            lib().et_adapter_bank_destroy(self._h)
+            self._h = ctypes.c_void_p(0)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class _ScoreRules(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("distance_bias", ctypes.c_void_p), ("reach", ctypes.c_int),
+                ("window_left", ctypes.c_int), ("window_right", ctypes.c_int), ("prefix_lens", ctypes.c_void_p), ("q_docs", ctypes.c_void_p),
+                ("k_docs", ctypes.c_void_p)]
+
+
+def attention_rules_scratch_size(batch, max_k_len):
+    """Bytes of scratch that attention_rules needs with documents."""
+    f = lib().et_attention_rules_scratch_size
+    f.restype = ctypes.c_size_t
+    return int(f(_i(batch), _i(max_k_len)))
+
+
+def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_lens=None, batch=1, max_q_len=0, max_k_len=0, scale=0.0, cap=0.0, slopes=None,
+                    distance_bias=None, window=(-1, -1), prefix_lens=None, q_docs=None, k_docs=None, scratch=None, stream=None):
+    """Attention with rules on its scores (capped, biased by distance, seen through windows, prefixes and documents) over packed sequences, or of
+    tokens over keys kept from before (k_start, k_lens). Q and out [tokens, heads * head_dim], K and V [rows, kv_heads * head_dim], rows may be
+    slices of wider ones; see et_attention_rules for each argument. max_q_len, max_k_len: 0 takes the number of rows."""
+    import torch
+    device = _device()
+    f16, i32 = torch.float16, torch.int32
+    for name, t in (("out", out), ("Q", Q), ("K", K), ("V", V)):
+        _checked(name, t, f16, 2, device)
+        if t.shape[1] % head_dim or not t.shape[1]:
+            raise ValueError(f"{name}: whole heads of {head_dim} expected, not {t.shape[1]} features")
+    if out.shape != Q.shape or K.shape != V.shape:
+        raise ValueError("out like Q and V like K expected")
+    nhead, nhead_kv = Q.shape[1] // head_dim, K.shape[1] // head_dim
+    for name, t, n in (("cu_seqlens", cu_seqlens, batch + 1), ("k_start", k_start, batch), ("k_lens", k_lens, batch), ("prefix_lens", prefix_lens, batch),
+                       ("q_docs", q_docs, Q.shape[0]), ("k_docs", k_docs, K.shape[0])):
+        if t is not None and _checked(name, t, i32, 1, device, last=False).shape[0] != n:
+            raise ValueError(f"{name}: {n} elements expected, not {t.shape[0]}")
+    if slopes is not None and _checked("slopes", slopes, torch.float32, 1, device, last=False).shape[0] != nhead:
+        raise ValueError("slopes: one for each head")
+    reach = 0
+    if distance_bias is not None:
+        _checked("distance_bias", distance_bias, f16, 2, device, last=False)
+        if distance_bias.shape[0] != nhead or distance_bias.shape[1] % 2 == 0:
+            raise ValueError("distance_bias: [heads, 2 reach + 1] expected")
+        reach = distance_bias.shape[1] // 2
+    scratch_bytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    if scratch is not None and (scratch.device.type != "cuda" or scratch.device.index != device or not scratch.is_contiguous()):
+        raise ValueError("scratch must be contiguous, on the current CUDA device")
+    rules = _ScoreRules(scale, cap, _a(slopes), _a(distance_bias), reach, window[0], window[1], _a(prefix_lens), _a(q_docs), _a(k_docs))
+    rc = (_entries or _lib()).et_attention_rules(
+        out.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), _pitch(out), _pitch(Q), _pitch(K), _pitch(V), nhead, nhead_kv, head_dim, _a(cu_seqlens),
+        _a(k_start), _a(k_lens), batch, Q.shape[0], K.shape[0], max_q_len or Q.shape[0], max_k_len or K.shape[0], ctypes.addressof(rules), _a(scratch),
+        scratch_bytes, raw_stream(stream))
     if rc:
         check(rc)
     return out

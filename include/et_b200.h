@@ -161,6 +161,65 @@ int et_attention_batch(void* out, const void* Q, const void* K, const void* V, i
                        int mask_ld, const int* cu_seqlens, const int* valid_lens, int batch, int uniform_len,
                        int max_seq_len, int total_tokens, int d_model, int nhead, void* stream);
 
+/* ---- rotary positions over several axes (no counterpart in the reference, whose encoders place tokens by what their input holds) ----
+ * Turns the features of every head of Q and K in pairs: pair i of token t by the angle positions[t * n_axes + axis[i]] * inv_freq[i]
+ * (taken in 64 bits), (x, y) -> (x cos - y sin, x sin + y cos). Pairs are features i and i + rot_dim / 2 of a head, or 2i and 2i + 1
+ * when interleaved != 0; features from rot_dim on are passed on unchanged. positions [tokens x n_axes] int32, inv_freq [rot_dim / 2]
+ * fp32 and axis [rot_dim / 2] int32 are device arrays; a pair whose axis is not 0 .. n_axes - 1 is not turned. Rows may be slices of
+ * wider ones (pitches in elements): Q and K as a fused projection leaves them. q_out may be q and k_out may be k, with equal pitches;
+ * any other overlap is the caller's error. nhead_q or nhead_k may be 0. head_dim 2 to 256, rot_dim even. Rows and heads that start on 16
+ * bytes go fastest. */
+int et_rotary_axes(void* q_out, const void* q, int q_out_pitch, int q_pitch, int nhead_q, void* k_out, const void* k, int k_out_pitch,
+                   int k_pitch, int nhead_k, int head_dim, int rot_dim, const int* positions, int n_axes, const float* inv_freq,
+                   const int* axis, int interleaved, int tokens, void* stream);
+
+/* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference, which holds one set of weights) ----
+ * A bank holds n_slots adapters of one projection, each of rank up to max_rank (1 to 128): A [rank x in_feat], B [out_feat x rank] and a
+ * scale. It allocates its memory on the current device and synchronises it, as et_adapter_bank_set does, which copies an adapter from HOST
+ * arrays into a slot (rank 0: the slot is empty again). in_feat and out_feat are multiples of 16. */
+typedef struct et_adapter_bank et_adapter_bank;
+int et_adapter_bank_create(et_adapter_bank** out, int in_feat, int out_feat, int max_rank, int n_slots);
+int et_adapter_bank_destroy(et_adapter_bank* bank);
+int et_adapter_bank_set(et_adapter_bank* bank, int slot, int rank, const void* a_host, const void* b_host, float scale);
+/* out[t] = base[t] + scale_a B_a (A_a x[t]) for the tokens of each sequence, a = adapter_ids[sequence] (device, batch ints; an id that
+ * is no slot, or an empty one, adds nothing). base is what the shared projection left (et_tile_linear, et_row_linear); out may be base with the same
+ * pitch. cu_seqlens (device, batch + 1 ints) are the sequences' token offsets, or NULL: one token each (single tokens of many requests). Rows of
+ * out in no sequence are left as they are. tokens: the rows that there are; none beyond is touched. Rows start on 16 bytes (pitches multiples
+ * of 8). Sums in fp32; A x is rounded to fp16, each row scaled so that it can not overflow. */
+int et_adapter_add(const et_adapter_bank* bank, void* out, const void* base, const void* x, int out_pitch, int base_pitch, int x_pitch,
+                   const int* cu_seqlens, const int* adapter_ids, int batch, int tokens, void* stream);
+
+/* ---- attention with rules on its scores (no counterpart in the reference, whose masks are additive and shared by all heads) ----
+ *   score(q, k) = cap tanh(scale Q_q . K_k / cap) + bias(k - q);   out_q = sum of softmax(score) V_k over the keys that q sees
+ * A query that sees no key gets zeros; what it does not see takes no part, whatever it holds (infinities, not a number). */
+typedef struct et_score_rules {
+    float scale;               /* 0: 1 / sqrt(head_dim) */
+    float cap;                 /* 0: scores are not capped */
+    const float* slopes;       /* [nhead] or NULL: bias = -slopes[head] |k - q| */
+    const void* distance_bias; /* fp16 [nhead][2 reach + 1] or NULL: bias = distance_bias[head][reach + max(-reach, min(reach, k - q))] */
+    int reach;
+    int window_left;           /* keys before q - window_left are not seen; below 0: no limit */
+    int window_right;          /* keys behind q + window_right are not seen (0: none behind q); below 0: no limit */
+    const int* prefix_lens;    /* [batch] or NULL: the first prefix_lens[sequence] keys are seen whatever the window is */
+    const int* q_docs;         /* [q_tokens] and [k_rows], or both NULL: a query sees only keys of its own document (of those that */
+    const int* k_docs;         /* the window and the prefix leave); documents below 0 see and are seen by nothing */
+} et_score_rules;
+/* Q and out [q_tokens x nhead * head_dim], K and V [k_rows x nhead_kv * head_dim], nhead a multiple of nhead_kv (query head h reads
+ * K/V head h / (nhead / nhead_kv)), head_dim 1 to 256, each with a pitch of its own in elements. Sequence b has the queries of rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] (device, batch + 1 ints; NULL: max_q_len each). Its keys:
+ *   k_start NULL: the rows of its queries; the first k_lens[b] of them where k_lens is given (key padding). Query i is at position i.
+ *   k_start given (device, batch ints): rows k_start[b] .. k_start[b] + k_lens[b], kept from before; the last query is at the last
+ *     key: query i is at position k_lens[b] - (number of queries) + i. Places may overlap (a shared beginning).
+ * All arrays of the rules are device arrays. max_q_len and max_k_len: at least the longest sequence's queries and keys; keys beyond
+ * max_k_len, or beyond k_rows, are not seen. Single tokens (max_q_len 1 with k_start) take a kernel that splits the keys. scratch: device memory of
+ * et_attention_rules_scratch_size bytes when documents are given (contents do not matter; calls that may overlap need one each), else NULL.
+ * out may not overlap the inputs. Rows of out in no sequence are left as they are. */
+int et_attention_rules(void* out, const void* Q, const void* K, const void* V, int out_pitch, int q_pitch, int k_pitch, int v_pitch,
+                       int nhead, int nhead_kv, int head_dim, const int* cu_seqlens, const int* k_start, const int* k_lens, int batch,
+                       int q_tokens, int k_rows, int max_q_len, int max_k_len, const et_score_rules* rules, void* scratch,
+                       size_t scratch_bytes, void* stream);
+size_t et_attention_rules_scratch_size(int batch, int max_k_len);
+
 /* ---- pruned-format generators (host) ----------------------------------------------------------
  * Seeded and reproducible. bernoulli == 0 keeps exactly floor(total*(1-sparsity)) tiles (a block-row's
  * tiles in draw order); otherwise each tile is kept with probability 1-sparsity (ascending offsets).

@@ -1,0 +1,79 @@
+"""What the operators for positions, adapters and rules on scores refuse, before any CUDA call, and what they do with nothing to do."""
+import ctypes
+import math
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import et_b200
+    from et_b200 import build
+    build.build()
+    return et_b200.lib()
+
+
+P = ctypes.c_void_p(16)   # an address that nothing reads
+
+
+def rotary(lib, **change):
+    a = dict(q_out=P, q=P, q_out_pitch=64, q_pitch=64, nhead_q=1, k_out=P, k=P, k_out_pitch=64, k_pitch=64, nhead_k=1, head_dim=64, rot_dim=64, positions=P, n_axes=1,
+             inv_freq=P, axis=P, interleaved=0, tokens=0, stream=None)
+    a.update(change)
+    return lib.et_rotary_axes(*a.values())
+
+
+@pytest.mark.parametrize("change", [dict(tokens=-1), dict(nhead_q=-1), dict(head_dim=0), dict(head_dim=257), dict(rot_dim=63), dict(rot_dim=66), dict(rot_dim=-2), dict(n_axes=0),
+                                    dict(tokens=1, q=None), dict(tokens=1, k_out=None), dict(tokens=1, positions=None), dict(tokens=1, axis=None), dict(tokens=1, q_pitch=63),
+                                    dict(tokens=1, k_out_pitch=8), dict(tokens=1, q_out_pitch=128)])
+def test_rotary_refuses(lib, change):
+    assert rotary(lib, **change) == 1 and b"et_rotary_axes" in lib.et_last_error()
+
+
+def test_rotary_of_nothing(lib):
+    assert rotary(lib) == 0
+    assert rotary(lib, tokens=5, nhead_q=0, nhead_k=0) == 0
+
+
+@pytest.mark.parametrize("sizes", [(0, 64, 8, 1), (24, 64, 8, 1), (64, 40, 8, 1), (64, 64, 0, 1), (64, 64, 129, 1), (64, 64, 8, 0), (-16, 64, 8, 1)])
+def test_adapter_bank_refuses(lib, sizes):
+    bank = ctypes.c_void_p(16)
+    assert lib.et_adapter_bank_create(ctypes.byref(bank), *sizes) == 1 and not bank
+    assert lib.et_adapter_bank_create(None, 64, 64, 8, 1) == 1
+
+
+def test_adapter_without_a_bank(lib):
+    assert lib.et_adapter_bank_set(None, 0, 1, P, P, ctypes.c_float(1)) == 1
+    assert lib.et_adapter_add(None, P, P, P, 64, 64, 64, None, P, 1, 1, None) == 1
+    assert lib.et_adapter_bank_destroy(None) == 0
+
+
+def attention(lib, rules=None, **change):
+    from et_b200 import ops
+    a = dict(out=P, Q=P, K=P, V=P, out_pitch=128, q_pitch=128, k_pitch=64, v_pitch=64, nhead=2, nhead_kv=1, head_dim=64, cu=None, k_start=None, k_lens=None, batch=1, q_tokens=4,
+             k_rows=4, max_q_len=4, max_k_len=4)
+    a.update(change)
+    values = dict(window_left=-1, window_right=-1)
+    values.update(rules or {})
+    r = ops._ScoreRules(**values)
+    return lib.et_attention_rules(*a.values(), ctypes.byref(r), None, ctypes.c_size_t(0), None)
+
+
+@pytest.mark.parametrize("change", [dict(batch=-1), dict(q_tokens=-1), dict(max_k_len=-1), dict(nhead=0), dict(nhead_kv=0), dict(nhead=3, nhead_kv=2), dict(head_dim=0), dict(head_dim=257),
+                                    dict(nhead=1 << 16), dict(max_q_len=1 << 30), dict(k_start=P), dict(out=None), dict(Q=None), dict(V=None), dict(batch=2), dict(q_pitch=127),
+                                    dict(v_pitch=63), dict(rules=dict(cap=-1.0)), dict(rules=dict(cap=math.inf)), dict(rules=dict(scale=math.nan)), dict(rules=dict(scale=-1.0)),
+                                    dict(rules=dict(slopes=16, distance_bias=16)), dict(rules=dict(distance_bias=16, reach=-1)), dict(rules=dict(q_docs=16)),
+                                    dict(rules=dict(q_docs=16, k_docs=16))])
+def test_attention_refuses(lib, change):
+    assert attention(lib, **change) == 1 and b"et_attention_rules" in lib.et_last_error()
+
+
+def test_attention_of_nothing(lib):
+    for change in (dict(batch=0), dict(q_tokens=0), dict(max_q_len=0)):
+        assert attention(lib, **change) == 0
+
+
+def test_attention_scratch_size(lib):
+    import et_b200 as et
+    assert et.attention_rules_scratch_size(0, 100) == 0 and et.attention_rules_scratch_size(3, 0) == 0
+    assert et.attention_rules_scratch_size(3, 129) == 3 * 2 * 8 and et.attention_rules_scratch_size(1 << 20, 1 << 20) == (1 << 20) * (1 << 13) * 8

@@ -23,6 +23,8 @@ int attention_tc_launch(half* Z, const half* Q, const half* K, const half* V, in
                         int d_model, int nhead, cudaStream_t st);
 // Reads and clears the current device's error word of the tcgen05 kernel's bounded waits (synchronises).
 int attention_tc_error(int* code);
+// Address of that word on the current device; looked up once per device.
+int attn_err_address(int** out);
 // One-time per-device set-up of that error word (no allocation); safe to call repeatedly.
 int attention_prepare_device();
 // pitch: row pitch of Q and K in elements (0 = d_model).

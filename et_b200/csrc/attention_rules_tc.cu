@@ -1,0 +1,1032 @@
+// Attention with rules on its scores, on the 5th-generation tensor cores (tcgen05 + TMEM + TMA): whole sequences, heads of a multiple of 16 up to 128.
+//
+// A work item is 128 queries of one head of one sequence; a block is 128 keys of it. Blocks that no query of the item sees are left out: the
+// window and the prefix give two ranges of blocks, documents are looked up in a summary (lowest and highest document of every block) that a small kernel
+// makes first. Blocks that all queries see take no mask; in the others a row has one bit for each of its scores.
+//   S = Q K^T        SS UMMAs 128x128x16, fp32 in 128 TMEM columns
+//   softmax          four warps, a thread to a query row, in two passes over the scores in tensor memory: the first caps them, adds the bias, takes out
+//                    what is not seen (what it changes goes back) and takes the maximum, the second takes the exponentials
+//   O += P V         TS UMMAs 128 x head x 16: A = P (fp16) from tensor memory, B = V as loaded
+//   epilogue         O / row sum -> fp16 -> global
+// Two CTAs share an SM (256 TMEM columns each), so that one's loads, maxima and hand-overs run under the other's exponentials. Heads of 64 keep P in
+// columns of its own, and Q K^T of the next block runs while this one's exponentials become P V; wider heads have no columns left, P takes the place of
+// the scores it came from, and Q K^T of the next block follows P V.
+//
+// Not a number times the weight 0 is not a number: V rows behind the last key are cleared in shared memory before P V, and a row whose result is not
+// finite is computed again from the keys that it sees (rules_row). So is one whose result, a mean of values near fp16's largest, has left the range by the
+// rounding of its weights.
+//
+// Every mbarrier wait is bounded; a wait that gives up sets the error word that et_attention_check reads and the CTA leaves through the common exit.
+#include "attention.h"
+#include "attention_rules.h"
+#include "common.h"
+#include "ptx.cuh"
+#include "tmap.h"
+#include "vec_math.cuh"
+
+namespace et {
+
+namespace {
+
+constexpr int kBQ = 128, kBK = 128;
+constexpr int kPanel = 128 * 128;         // 128 rows of 64 fp16 features
+constexpr int kSoftmaxWarps = 4;
+constexpr int kLoadWarp = 4, kMmaWarp = 5, kHelpWarp = 6, kHelpWarps = 2;
+constexpr int kThreads = 256;
+constexpr int kCtasPerSm = 2;
+constexpr int kTmemCols = 256;
+constexpr float kRescaleStep = 8.f;       // log2 units by which a row's maximum must grow before O is rescaled
+constexpr int kItemRing = 4, kBlockRing = 8;
+constexpr int kMaxSorted = 128;           // sequences of a ragged batch that a CTA keeps in order of length
+constexpr int kLenClasses = 9;
+constexpr int kShiftPitch = 528;          // bytes of one of eight copies of a block's biases, each shifted by one more: 256 values and 16 bytes against conflicts
+constexpr int kShiftBytes = 8 * kShiftPitch;
+
+enum Bias { kNoBias = 0, kSlopes = 1, kTable = 2 };
+enum BlockFlags { kPartial = 1, kFirst = 2, kLast = 4, kEnd = 8 };
+
+struct TcRules {
+    RuleParams r;
+    const int2* summary;      // documents: lowest and highest of each block of keys, [batch][summary_blocks]
+    int summary_blocks;
+    bool take_over;           // CTAs ask for items that have not started
+    bool sorted;              // a ragged batch of at most kMaxSorted sequences, the longest first
+    bool heavy_first;         // equal lengths: late queries, which see more, first
+    int* err;
+};
+
+struct Item {
+    RuleSeq seq;
+    int b, qi0, head;
+    int state;                // -1: no more items, 0: no query sees a key, 1: blocks follow
+};
+struct Block {
+    int j, left, flags, item; // number of the block, keys from its first one on, what it is, slot of its item
+};
+
+template <int kHD>
+struct Cfg {
+    static constexpr int kPanels = kHD / 64;
+    static constexpr int kTile = kPanels * kPanel;          // 128 rows of Q, K or V
+    static constexpr bool kOwnP = kHD == 64;
+    static constexpr int kStages = kHD == 64 ? 2 : 1;       // of Q, K and V each
+    static constexpr uint32_t kSCol = 0, kPCol = kOwnP ? 128 : 0, kOCol = kOwnP ? 192 : 128;
+    static constexpr int kHelpAt = 3 * kStages * kTile;
+};
+
+struct TcShared {
+    uint4 clc;
+    uint64_t clc_full;
+    uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t s_full, s_free, p_full, pv_done;
+    uint64_t m_full[2], m_empty[2];       // what the helping warps bring of a block: documents of its keys, its biases
+    uint64_t item_full[kItemRing], item_empty[kItemRing];
+    uint64_t block_full[kBlockRing];
+    Item item[kItemRing];
+    Block block[kBlockRing];
+    alignas(16) int docs[2][kBK];         // read four at a time
+    uint32_t tmem_base;
+};
+struct SeqTable {
+    RuleSeq seq[kMaxSorted];
+    int b[kMaxSorted];
+    int before[kMaxSorted + 1];
+    int class_at[kLenClasses + 1];
+};
+
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const float (&v)[32]) {
+    const uint32_t(&r)[32] = reinterpret_cast<const uint32_t(&)[32]>(v);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+        "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// 2^x for two values on the FMA and ALU pipes, x <= 127: x = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves n in the low bits of
+// the sum) and |f| <= 1/2; 2^f by the cubic that interpolates it at the Chebyshev nodes of [-1/2, 1/2] (largest relative error 1.0e-4, below half
+// a unit of the fp16 that the result is rounded to); n goes into the exponent. Not a number stays so.
+__device__ __forceinline__ float2 exp2_cubic2(float2 x) {
+    x.x = max_nan(x.x, -126.f);
+    x.y = max_nan(x.y, -126.f);
+    const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
+    const float2 t = add2(x, big);
+    const float2 n = add2(t, nbig);
+    const float2 f = add2(x, make_float2(-n.x, -n.y));
+    float2 r = fma2(f, make_float2(0.0558382832f, 0.0558382832f), make_float2(0.242639482f, 0.242639482f));
+    r = fma2(r, f, make_float2(0.693136752f, 0.693136752f));
+    r = fma2(r, f, make_float2(0.999924541f, 0.999924541f));
+    float2 y;
+    y.x = __int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23));
+    y.y = __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23));
+    return fma2(x, make_float2(0.f, 0.f), y);
+}
+// c - 2 c / (1 + 2^(x cap_in)) of four scores, with one reciprocal for the four: of the product of the denominators, which are at most 2^25 + 1 (from there
+// on the result is c).
+__device__ __forceinline__ void cap4(float& a, float& b, float& c, float& d, float cap_in, float cap_out) {
+    const float2 in2 = make_float2(cap_in, cap_in), one2 = make_float2(1.f, 1.f);
+    float2 x = mul2(make_float2(a, b), in2), y = mul2(make_float2(c, d), in2);
+    x.x = ex2_fast(min_nan(x.x, 25.f));
+    x.y = ex2_fast(min_nan(x.y, 25.f));
+    y.x = ex2_fast(min_nan(y.x, 25.f));
+    y.y = ex2_fast(min_nan(y.y, 25.f));
+    x = add2(x, one2);
+    y = add2(y, one2);
+    const float2 xy = mul2(x, y);
+    const float r = rcp_fast(xy.x * xy.y);
+    const float2 inv = mul2(make_float2(r, r), make_float2(xy.y, xy.x));   // 1 / (x y), each
+    const float2 out2 = make_float2(cap_out, cap_out), n2 = make_float2(-2.f * cap_out, -2.f * cap_out);
+    const float2 ab = fma2(mul2(inv, y), n2, out2), cd = fma2(mul2(inv, x), n2, out2);
+    a = ab.x; b = ab.y; c = cd.x; d = cd.y;
+}
+// Bits i >= from of a word (from: any whole number).
+__device__ __forceinline__ uint32_t bits_from(int from) { return from <= 0 ? ~0u : from >= 32 ? 0u : ~0u << from; }
+
+__device__ __forceinline__ void tma_load_heads(void* dst, const void* tmap, int x, int head, int row, uint64_t* bar) { tma_load_3d(dst, tmap, x, head, row, bar); }
+
+__device__ __forceinline__ void clc_ask(uint4* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool clc_answer(const uint4* answer, int& x) {
+    uint32_t ok, cx;
+    asm volatile(
+        "{\n.reg .b128 h;\n.reg .pred p;\nld.shared.b128 h, [%2];\n"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\nselp.u32 %0, 1, 0, p;\nmov.u32 %1, 0;\n"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n}"
+        : "=r"(ok), "=r"(cx)
+        : "r"(smem_u32(answer))
+        : "memory");
+    x = (int)cx;
+    return ok != 0;
+}
+
+// A ragged batch in order of its sequences' key blocks, the most first (whole warp), so that what is left when CTAs run out of items are short
+// ones, and an item is found without reading memory.
+__device__ __forceinline__ void sort_sequences(const RuleParams& p, SeqTable* t, int lane) {
+    if (lane <= kLenClasses) t->class_at[lane] = 0;
+    __syncwarp();
+    const unsigned below = (1u << lane) - 1u;
+    for (int pass = 0; pass < 2; ++pass) {   // count, place
+        for (int base = 0; base < p.batch; base += 32) {
+            const int i = base + lane;
+            const bool in = i < p.batch;
+            RuleSeq s = {};
+            if (in) s = rule_seq(p, i);
+            const int c = in ? 8 - min((s.klen + kBK - 1) / kBK, 8) : kLenClasses;
+            const unsigned same = __match_any_sync(0xffffffffu, c);
+            const int at = t->class_at[c];
+            __syncwarp();
+            if ((same & below) == 0) t->class_at[c] = at + __popc(same);
+            __syncwarp();
+            if (pass == 1 && in) {
+                const int pos = at + __popc(same & below);
+                t->seq[pos] = s;
+                t->b[pos] = i;
+            }
+        }
+        __syncwarp();
+        if (pass == 0) {   // counts -> where each class starts
+            const int n = lane < kLenClasses ? t->class_at[lane] : 0;
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            __syncwarp();
+            if (lane < kLenClasses) t->class_at[lane] = incl - n;
+            __syncwarp();
+        }
+    }
+    int before = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+        const int i = base + lane;
+        int incl = i < p.batch ? (t->seq[i].qlen + kBQ - 1) / kBQ : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (i < p.batch) t->before[i + 1] = before + incl;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) t->before[0] = 0;
+    __syncwarp();
+}
+
+// Which queries block `blk` is (whole warp); false: it lies beyond the batch (the grid of a ragged batch has slack).
+__device__ __forceinline__ bool find_item(const TcRules& p, const SeqTable* t, int blk, int lane, Item& it) {
+    const RuleParams& r = p.r;
+    if (p.sorted) {
+        for (int base = 0; base < r.batch; base += 32) {
+            const unsigned hit = __ballot_sync(0xffffffffu, base + lane < r.batch && blk < t->before[min(base + lane, kMaxSorted - 1) + 1]);
+            if (!hit) continue;
+            const int pos = base + __ffs(hit) - 1;
+            it.seq = t->seq[pos];
+            it.b = t->b[pos];
+            it.qi0 = (t->before[pos + 1] - 1 - blk) * kBQ;   // late queries first
+            return true;
+        }
+        return false;
+    } else if (r.cu_seqlens) {
+        for (int base = 0; base < r.batch; base += 32) {
+            const int i = base + lane;
+            RuleSeq s = {};
+            if (i < r.batch) s = rule_seq(r, i);
+            const int n = (s.qlen + kBQ - 1) / kBQ;
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, blk < incl);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                it.b = base + src;
+                it.qi0 = (__shfl_sync(0xffffffffu, incl, src) - 1 - blk) * kBQ;
+                it.seq.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+                it.seq.qlen = __shfl_sync(0xffffffffu, s.qlen, src);
+                it.seq.k0 = __shfl_sync(0xffffffffu, s.k0, src);
+                it.seq.klen = __shfl_sync(0xffffffffu, s.klen, src);
+                it.seq.qpos0 = __shfl_sync(0xffffffffu, s.qpos0, src);
+                it.seq.prefix = __shfl_sync(0xffffffffu, s.prefix, src);
+                return true;
+            }
+            blk -= __shfl_sync(0xffffffffu, incl, 31);
+        }
+        return false;
+    } else {
+        const int nb = (r.max_q_len + kBQ - 1) / kBQ;
+        if (blk >= nb * r.batch) return false;
+        it.b = p.heavy_first ? blk % r.batch : blk / nb;
+        it.qi0 = (p.heavy_first ? nb - 1 - blk / r.batch : blk % nb) * kBQ;
+        it.seq = rule_seq(r, it.b);
+        return true;
+    }
+}
+
+// The blocks of keys that an item's queries see, in order (whole warp): the prefix's blocks, then the window's; of documents those whose range meets the queries'.
+struct Blocks {
+    const int2* summary;
+    int n_prefix, first, n;        // blocks of the prefix, the window's first block behind them, all of them
+    int at;                        // the next one to look at; documents: behind the 32 looked at
+    unsigned seen, whole;          // documents: of the 32 looked at, those to come, and those of one document with all queries
+    int d_lo, d_hi;
+
+    __device__ __forceinline__ int number(int i) const { return i < n_prefix ? i : first + i - n_prefix; }
+    __device__ __forceinline__ void start(const TcRules& p, const Item& it, int lane) {
+        const RuleParams& r = p.r;
+        const RuleSeq& s = it.seq;
+        const int qa = s.qpos0 + it.qi0, qb = s.qpos0 + min(it.qi0 + kBQ, s.qlen) - 1;
+        const int pre = max(0, min(s.prefix, s.klen));
+        n_prefix = (pre + kBK - 1) / kBK;
+        const int lo = r.window_left == kNoLimit ? 0 : max(qa - r.window_left, 0);
+        const int hi = r.window_right == kNoLimit ? s.klen - 1 : min(qb + r.window_right, s.klen - 1);
+        first = max(lo / kBK, n_prefix);
+        n = n_prefix + (hi >= lo ? max(hi / kBK - first + 1, 0) : 0);
+        at = 0;
+        if (p.summary) {
+            int mn = 0x7fffffff, mx = -0x7fffffff - 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int q = it.qi0 + i * 32 + lane;
+                if (q < s.qlen) {
+                    const int d = r.q_docs[s.q0 + q];
+                    mn = min(mn, d);
+                    mx = max(mx, d);
+                }
+            }
+            d_lo = __reduce_min_sync(0xffffffffu, mn);
+            d_hi = __reduce_max_sync(0xffffffffu, mx);
+            summary = p.summary + (size_t)it.b * p.summary_blocks;
+            seen = whole = 0;
+        }
+    }
+    // -1: no more
+    __device__ __forceinline__ int next(const TcRules& p, const Item& it, int lane, bool& partial) {
+        int i;
+        bool one_document = true;
+        if (p.summary) {
+            while (!seen) {
+                if (at >= n) return -1;
+                const int mine = at + lane;
+                bool meets = false, same = false;
+                if (mine < n) {
+                    const int2 d = summary[number(mine)];
+                    meets = d_hi >= 0 && d.y >= max(d_lo, 0) && d.x <= d_hi;
+                    same = d.x == d.y && d_lo == d_hi && d.x == d_lo;
+                }
+                seen = __ballot_sync(0xffffffffu, meets);
+                whole = __ballot_sync(0xffffffffu, same);
+                at += 32;
+            }
+            const int bit = __ffs(seen) - 1;
+            i = at - 32 + bit;
+            one_document = (whole >> bit) & 1u;
+            seen &= seen - 1;
+        } else {
+            if (at >= n) return -1;
+            i = at++;
+        }
+        const int j = number(i);
+        const RuleParams& r = p.r;
+        const RuleSeq& s = it.seq;
+        const int qa = s.qpos0 + it.qi0, qb = s.qpos0 + min(it.qi0 + kBQ, s.qlen) - 1;
+        const int ka = j * kBK, kb = ka + kBK - 1;
+        const bool inside = (r.window_left == kNoLimit || ka >= qb - r.window_left) && (r.window_right == kNoLimit || kb <= qa + r.window_right);
+        partial = !(one_document && kb < s.klen && (inside || kb < s.prefix));
+        return j;
+    }
+};
+
+template <int kHD, int kBias, bool kCap>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                                                                                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcRules p) {
+    using C = Cfg<kHD>;
+    const bool docs = p.summary != nullptr, help = kBias == kTable || docs;
+    constexpr bool kChanged = kCap || kBias != kNoBias;   // the first pass leaves scores in the log2 domain
+    constexpr int kPolyPairs = 2;                         // of 16 pairs of exponentials, how many go to the FMA pipe
+    const RuleParams& r = p.r;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* const sQ = smem;
+    uint8_t* const sK = sQ + C::kStages * C::kTile;
+    uint8_t* const sV = sK + C::kStages * C::kTile;
+    uint8_t* const sBias = smem + C::kHelpAt;
+    TcShared* const sh = reinterpret_cast<TcShared*>(smem + C::kHelpAt + (kBias == kTable ? 2 * kShiftBytes : 0));
+    SeqTable* const table = reinterpret_cast<SeqTable*>(sh + 1);   // p.sorted
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int hd = r.head_dim, osteps = hd >> 4;
+    pdl_launch_dependents();
+
+    if (warp == kLoadWarp) {
+        if (lane == 0) {
+            mbar_init(&sh->clc_full, 1);
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh->q_full[i], 1); mbar_init(&sh->q_empty[i], 1);
+                mbar_init(&sh->k_full[i], 1); mbar_init(&sh->k_empty[i], 1);
+                mbar_init(&sh->v_full[i], 1); mbar_init(&sh->v_empty[i], 1);
+                mbar_init(&sh->m_full[i], 32 * kHelpWarps);
+                mbar_init(&sh->m_empty[i], kSoftmaxWarps);
+            }
+            mbar_init(&sh->s_full, 1);
+            mbar_init(&sh->s_free, kSoftmaxWarps);
+            mbar_init(&sh->p_full, kSoftmaxWarps);
+            mbar_init(&sh->pv_done, 1);
+            for (int i = 0; i < kItemRing; ++i) {
+                mbar_init(&sh->item_full[i], 1);
+                mbar_init(&sh->item_empty[i], kSoftmaxWarps);
+            }
+            for (int i = 0; i < kBlockRing; ++i) mbar_init(&sh->block_full[i], 1);
+            fence_mbar_init();
+            prefetch_tmap(&tmQ);
+            prefetch_tmap(&tmK);
+            prefetch_tmap(&tmV);
+        }
+    } else if (warp == kMmaWarp) {
+        tmem_alloc(&sh->tmem_base, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+
+    if (warp == kLoadWarp) {
+        // ---- items, their blocks and the loads (all lanes stay together; lane 0 issues)
+        pdl_wait();
+        if (p.sorted) sort_sequences(r, table, lane);
+        int id = blockIdx.x;
+        int ni = 0, nq = 0, nk = 0, nv = 0, g = 0;   // items handed out, tiles requested, blocks announced
+        uint32_t clc_phase = 0;
+        bool ok = true;
+        auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int row, uint64_t* full, uint64_t* empty, int& count) {
+            const int st = count % C::kStages;
+            if (!mbar_wait(&empty[st], ((uint32_t)(count / C::kStages) & 1u) ^ 1u)) return false;
+            if (lane == 0) {
+                mbar_expect_tx(&full[st], C::kTile);
+#pragma unroll
+                for (int c = 0; c < C::kPanels; ++c) tma_load_heads(dst + st * C::kTile + c * kPanel, tm, c * 64, head, row, &full[st]);
+            }
+            ++count;
+            return true;
+        };
+        // A block's entry may be overwritten kBlockRing blocks later: by then the K tile in between has been used, so the scores two blocks
+        // before that have been read, and with them everything of this block by everyone.
+        auto announce = [&](int j, int left, int flags, int slot) {
+            if (lane == 0) {
+                Block& b = sh->block[g % kBlockRing];
+                b.j = j; b.left = left; b.flags = flags; b.item = slot;
+                mbar_arrive(&sh->block_full[g % kBlockRing]);
+            }
+            __syncwarp();
+            ++g;
+        };
+        for (;;) {
+            if (lane == 0 && p.take_over) {
+                mbar_expect_tx(&sh->clc_full, 16);
+                clc_ask(&sh->clc, &sh->clc_full);
+            }
+            Item it = {};
+            it.head = id % r.nhead;
+            if (find_item(p, table, id / r.nhead, lane, it)) {
+                Blocks blocks;
+                blocks.start(p, it, lane);
+                bool partial = false, partial_next = false;
+                int j = blocks.next(p, it, lane, partial);
+                it.state = j >= 0 ? 1 : 0;
+                const int slot = ni % kItemRing;
+                if ((ok = mbar_wait(&sh->item_empty[slot], ((uint32_t)(ni / kItemRing) & 1u) ^ 1u))) {
+                    if (lane == 0) {
+                        sh->item[slot] = it;
+                        mbar_arrive(&sh->item_full[slot]);
+                    }
+                    __syncwarp();
+                    ++ni;
+                    const int kv_head = it.head / r.group;
+                    if (j >= 0) ok = load(sQ, &tmQ, it.head, it.seq.q0 + it.qi0, sh->q_full, sh->q_empty, nq);
+                    // K of the first block; then K of the next block ahead of V of this one, if there is a place for it before this one's P V
+                    if (ok && j >= 0) ok = load(sK, &tmK, kv_head, it.seq.k0 + j * kBK, sh->k_full, sh->k_empty, nk);
+                    int flags = kFirst;
+                    while (ok && j >= 0) {
+                        const int jn = blocks.next(p, it, lane, partial_next);
+                        announce(j, it.seq.klen - j * kBK, flags | (partial ? kPartial : 0) | (jn < 0 ? kLast : 0), slot);
+                        if (C::kStages == 1) ok = load(sV, &tmV, kv_head, it.seq.k0 + j * kBK, sh->v_full, sh->v_empty, nv);
+                        if (ok && jn >= 0) ok = load(sK, &tmK, kv_head, it.seq.k0 + jn * kBK, sh->k_full, sh->k_empty, nk);
+                        if (ok && C::kStages > 1) ok = load(sV, &tmV, kv_head, it.seq.k0 + j * kBK, sh->v_full, sh->v_empty, nv);
+                        j = jn;
+                        partial = partial_next;
+                        flags = 0;
+                    }
+                }
+            }
+            if (!p.take_over) break;
+            // the answer is awaited even on the way out: nothing may be in flight towards shared memory when the CTA leaves
+            const bool answered = mbar_wait(&sh->clc_full, clc_phase);
+            clc_phase ^= 1u;
+            ok = ok && answered;
+            if (!ok) break;
+            const bool more = clc_answer(&sh->clc, id);
+            fence_proxy_async_smem();   // the answer has been read before the next one may be written
+            __syncwarp();
+            if (!more) break;
+        }
+        if (ok) {
+            const int slot = ni % kItemRing;
+            ok = mbar_wait(&sh->item_empty[slot], ((uint32_t)(ni / kItemRing) & 1u) ^ 1u);
+            if (ok) {
+                if (lane == 0) {
+                    sh->item[slot].state = -1;
+                    mbar_arrive(&sh->item_full[slot]);
+                }
+                announce(0, 0, kEnd, slot);
+            }
+        }
+        if (!ok) {
+            if (lane == 0) atomicExch(p.err, 21);
+            // copies still in flight land before the CTA leaves (bounded)
+            for (int i = max(nq - C::kStages, 0); i < nq; ++i) mbar_wait(&sh->q_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
+            for (int i = max(nk - C::kStages, 0); i < nk; ++i) mbar_wait(&sh->k_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
+            for (int i = max(nv - C::kStages, 0); i < nv; ++i) mbar_wait(&sh->v_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == kMmaWarp) {
+        // ---- UMMAs: the warp stays converged, one elected lane issues. Blocks are numbered through across items.
+        const int steps = hd >> 4;
+        const uint32_t idesc_qk = make_idesc_f16(128, kBK), idesc_qk_half = make_idesc_f16(128, kBK / 2), idesc_pv = make_idesc_f16(128, hd, false, true);
+        int nq = 0;
+        uint32_t g = 0;
+        bool ok = true;
+        struct { int left, flags; } cur = {0, 0}, nxt = {0, 0};   // the block in work, and the one behind it
+        auto entry = [&](uint32_t n) {
+            nxt.left = sh->block[n % kBlockRing].left;
+            nxt.flags = sh->block[n % kBlockRing].flags;
+            __syncwarp();
+        };
+        auto entry_wait = [&](uint32_t n) { return mbar_wait(&sh->block_full[n % kBlockRing], (n / kBlockRing) & 1u); };
+        // S = Q K_n^T of the block whose entry is `nxt`
+        auto issue_qk = [&](uint32_t n) {
+            const int qs = (nq - 1) % C::kStages;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t qa = smem_u32(sQ + qs * C::kTile), ka = smem_u32(sK + (n % C::kStages) * C::kTile);
+                const uint32_t idesc = nxt.left <= kBK / 2 ? idesc_qk_half : idesc_qk;
+                for (int ks = 0; ks < steps; ++ks) {
+                    const uint32_t at = (ks >> 2) * kPanel + (ks & 3) * 32;
+                    umma_f16(tmem + C::kSCol, make_smem_desc(qa + at, 16, 1024, 2), make_smem_desc(ka + at, 16, 1024, 2), idesc, ks > 0);
+                }
+                umma_commit(&sh->s_full);
+                umma_commit(&sh->k_empty[n % C::kStages]);
+                if (nxt.flags & kLast) umma_commit(&sh->q_empty[qs]);
+            }
+            __syncwarp();
+        };
+        auto wait_operands = [&](uint32_t n) {   // of block n, whose entry is `nxt`
+            if (nxt.flags & kFirst) {
+                if (!mbar_wait(&sh->q_full[nq % C::kStages], (uint32_t)(nq / C::kStages) & 1u)) return false;
+                ++nq;
+            }
+            return mbar_wait(&sh->k_full[n % C::kStages], (n / C::kStages) & 1u);
+        };
+        ok = entry_wait(0);
+        if (ok) {
+            entry(0);
+            if (!(nxt.flags & kEnd)) {
+                ok = wait_operands(0);
+                if (ok) issue_qk(0);
+            }
+        }
+        while (ok && !(nxt.flags & kEnd)) {
+            cur = nxt;
+            bool issued = false;
+            if constexpr (C::kOwnP) {
+                // the next block's Q K^T ahead of this one's P V: always within an item; of the next item if its operands are there already
+                bool ahead = !(cur.flags & kLast);
+                if (!ahead && mbar_poll_warp(&sh->block_full[(g + 1) % kBlockRing], ((g + 1) / kBlockRing) & 1u) &&
+                    !(sh->block[(g + 1) % kBlockRing].flags & kEnd))
+                    ahead = mbar_poll_warp(&sh->q_full[nq % C::kStages], (uint32_t)(nq / C::kStages) & 1u) &&
+                            mbar_poll_warp(&sh->k_full[(g + 1) % C::kStages], ((g + 1) / C::kStages) & 1u);
+                if (ahead) {
+                    ok = entry_wait(g + 1);
+                    if (!ok) break;
+                    entry(g + 1);
+                    ok = wait_operands(g + 1) && mbar_wait(&sh->s_free, g & 1);
+                    if (!ok) break;
+                    issue_qk(g + 1);
+                    issued = true;
+                }
+            }
+            // O += P V of block g
+            const int vs = g % C::kStages;
+            ok = mbar_wait(&sh->v_full[vs], (g / C::kStages) & 1u);
+            if (!ok) break;
+            const int keys = min(cur.left, kBK);
+            if (keys & 15) {   // V rows behind the last key, up to the end of a step: cleared
+                const int end = (keys + 15) & ~15;
+                uint8_t* const v = sV + vs * C::kTile;
+                for (int i = lane; i < (end - keys) * 8 * C::kPanels; i += 32) {
+                    const int row = keys + i / (8 * C::kPanels), c = i % (8 * C::kPanels);
+                    *reinterpret_cast<uint4*>(v + (c >> 3) * kPanel + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+            }
+            ok = mbar_wait(&sh->p_full, g & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t va = smem_u32(sV + vs * C::kTile);
+                const int n = (keys + 15) >> 4;
+                for (int ks = 0; ks < n; ++ks)   // P of keys 16ks .. 16ks + 15: 8 packed columns; V: panels of 64 features
+                    umma_f16_ts(tmem + C::kOCol, tmem + C::kPCol + (uint32_t)(ks * 8), make_smem_desc(va + ks * 2048, kPanel, 1024, 2), idesc_pv,
+                                (!(cur.flags & kFirst) || ks > 0) ? 1u : 0u);
+                umma_commit(&sh->pv_done);
+                umma_commit(&sh->v_empty[vs]);
+            }
+            __syncwarp();
+            if (!issued) {
+                ok = entry_wait(g + 1);
+                if (!ok) break;
+                entry(g + 1);
+                if (!(nxt.flags & kEnd)) {
+                    // the scores have been read: P comes after them. Where P lies in their place its P V must be over.
+                    ok = wait_operands(g + 1) && (C::kOwnP ? mbar_wait(&sh->s_free, g & 1) : mbar_wait(&sh->pv_done, g & 1));
+                    if (!ok) break;
+                    issue_qk(g + 1);
+                }
+            }
+            ++g;
+        }
+        if (!ok && lane == 0) atomicExch(p.err, 21);
+        __syncwarp();
+    } else if (warp >= kHelpWarp) {
+        // ---- what a block needs beside K and V: the documents of its keys, its biases by distance
+        if (help) {
+            pdl_wait();
+            const int t = tid - 32 * kHelpWarp;
+            bool ok = true;
+            for (uint32_t g = 0;; ++g) {
+                ok = mbar_wait(&sh->block_full[g % kBlockRing], (g / kBlockRing) & 1u);
+                if (!ok) break;
+                const Block b = sh->block[g % kBlockRing];
+                if (b.flags & kEnd) break;
+                const int m = g & 1;
+                ok = mbar_wait(&sh->m_empty[m], ((g >> 1) & 1u) ^ 1u);
+                if (!ok) break;
+                const Item& it = sh->item[b.item];
+                if (docs) {
+                    if (b.flags & kPartial) {
+#pragma unroll
+                        for (int i = 0; i < kBK; i += 32 * kHelpWarps)
+                            sh->docs[m][i + t] = i + t < b.left ? r.k_docs[it.seq.k0 + b.j * kBK + i + t] : -1;
+                    }
+                }
+                if constexpr (kBias == kTable) {
+                    // value n of copy s: the bias of the distance of key - query n + s - 127 within the block's corner distance
+                    const half* const row = r.table + (size_t)it.head * (2 * r.reach + 1) + r.reach;
+                    const int corner = b.j * kBK - (it.seq.qpos0 + it.qi0) - 127;
+#pragma unroll 2
+                    for (int e = t; e < 8 * 32; e += 32 * kHelpWarps) {
+                        const int s = e >> 5, n = (e & 31) * 8;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int d = corner + n + s + 2 * i;
+                            const half2 two = __halves2half2(row[max(-r.reach, min(r.reach, d))], row[max(-r.reach, min(r.reach, d + 1))]);
+                            w[i] = *reinterpret_cast<const uint32_t*>(&two);
+                        }
+                        *reinterpret_cast<uint4*>(sBias + m * kShiftBytes + s * kShiftPitch + n * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                mbar_arrive(&sh->m_full[m]);
+            }
+            if (!ok && lane == 0) atomicExch(p.err, 23);
+            __syncwarp();
+        }
+    } else {
+        // ---- softmax: one thread per query row (TMEM lane)
+        pdl_wait();
+        const int row = warp * 32 + lane;
+        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        const uint32_t s_addr = tmem + lane_base + C::kSCol, p_addr = tmem + lane_base + C::kPCol, o_addr = tmem + lane_base + C::kOCol;
+        const bool wide = (r.out_pitch & 15) == 0 && (reinterpret_cast<uintptr_t>(r.out) & 31) == 0;
+        uint32_t g = 0;
+        bool ok = true;
+        int done_slot = -1;     // item whose P V is on its way and whose rows are still to be written
+        float done_sum = 0.f;   // its row sum
+        auto release = [&](int slot) {
+            __syncwarp();
+            if (elect_one()) mbar_arrive(&sh->item_empty[slot]);
+            __syncwarp();
+        };
+        // O / row sum -> fp16 -> global, when the item's last P V has completed: inside the next item's first block, whose scores cover the wait.
+        auto finish = [&]() {
+            const Item& it = sh->item[done_slot];
+            const float inv = done_sum > 0.f ? 1.f / done_sum : done_sum == 0.f ? 0.f : done_sum;   // (not a number stays so)
+            const int qi = it.qi0 + row;
+            const bool in = qi < it.seq.qlen;
+            half* const orow = r.out + (it.seq.q0 + qi) * r.out_pitch + it.head * hd;
+            half2 top = __float2half2_rn(0.f);   // largest result; infinity or not a number if one of them is
+#pragma unroll 1
+            for (int c = 0; c < osteps; ++c) {
+                uint32_t o[16];
+                tmem_ld16(o_addr + c * 16, o);
+                tmem_ld_wait(o);
+                uint32_t ow[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    ow[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                    top = __hmax2_nan(top, __habs2(*reinterpret_cast<const half2*>(&ow[i])));
+                }
+                if (in) {
+                    half* const z = orow + c * 16;
+                    if (wide) {
+                        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(z), "r"(ow[0]), "r"(ow[1]), "r"(ow[2]), "r"(ow[3]), "r"(ow[4]),
+                                     "r"(ow[5]), "r"(ow[6]), "r"(ow[7])
+                                     : "memory");
+                    } else {
+                        *reinterpret_cast<uint4*>(z) = make_uint4(ow[0], ow[1], ow[2], ow[3]);
+                        *reinterpret_cast<uint4*>(z + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
+                    }
+                }
+            }
+            const float largest = fmaxf(__low2float(top), __high2float(top)), sum = __low2float(top) + __high2float(top);
+            unsigned again = __ballot_sync(0xffffffffu, in && !(largest <= 65504.f && sum == sum));
+            for (; again; again &= again - 1) rules_row(r, it.seq, it.qi0 + warp * 32 + __ffs(again) - 1, it.head);
+            release(done_slot);
+            done_slot = -1;
+        };
+        for (int ni = 0; ok; ++ni) {
+            const int slot = ni % kItemRing;
+            ok = mbar_wait(&sh->item_full[slot], (uint32_t)(ni / kItemRing) & 1u);
+            if (!ok) break;
+            const Item& it = sh->item[slot];
+            const int state = it.state;
+            if (state <= 0) {
+                if (done_slot >= 0) {   // (the ring could run out of slots if an item waited behind empty ones)
+                    ok = mbar_wait(&sh->pv_done, (g - 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    finish();
+                }
+                if (state < 0) break;
+                const int qi = it.qi0 + row;   // no query sees a key: zeros
+                if (qi < it.seq.qlen) {
+                    uint4* const z = reinterpret_cast<uint4*>(r.out + (it.seq.q0 + qi) * r.out_pitch + it.head * hd);
+                    for (int i = 0; i < hd / 8; ++i) z[i] = make_uint4(0u, 0u, 0u, 0u);
+                }
+                release(slot);
+                continue;
+            }
+            const int qpos = it.seq.qpos0 + it.qi0 + row;
+            const int prefix = it.seq.prefix;
+            int my_doc = 0;
+            if (docs) my_doc = it.qi0 + row < it.seq.qlen ? r.q_docs[it.seq.q0 + it.qi0 + row] : -1;
+            float slope = 0.f;
+            if constexpr (kBias == kSlopes) slope = r.slopes[it.head] * -kRulesLog2e;
+            float m_run = -INFINITY;
+            float2 l2 = make_float2(0.f, 0.f);
+            bool last = false;
+            for (; !last; ++g) {
+                ok = mbar_wait(&sh->s_full, g & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const Block& b = sh->block[g % kBlockRing];
+                const int k0 = b.j * kBK, left = b.left, flags = b.flags;
+                const bool partial = flags & kPartial, first = flags & kFirst;
+                last = flags & kLast;
+                const int chunks = left > kBK / 2 ? 4 : 2;
+                const int m = g & 1;
+                if (help) {
+                    ok = mbar_wait(&sh->m_full[m], (g >> 1) & 1u);
+                    if (!ok) break;
+                }
+                // the maximum, half a block at a time; scores that change go back to where they came from
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int c = 0; c < chunks; c += 2) {
+                    uint32_t seen[2] = {~0u, ~0u};
+                    if (partial) {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            const int at = k0 + (c + x) * 32;
+                            uint32_t w = r.window_left == kNoLimit ? ~0u : bits_from(qpos - r.window_left - at);
+                            if (r.window_right != kNoLimit) w &= ~bits_from(qpos + r.window_right + 1 - at);
+                            w |= ~bits_from(prefix - at);
+                            w &= ~bits_from(left - (c + x) * 32);
+                            if (docs) {
+                                uint32_t same = 0;
+                                const int4* const d = reinterpret_cast<const int4*>(sh->docs[m] + (c + x) * 32);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const int4 four = d[i];
+                                    same |= (four.x == my_doc ? 1u : 0u) << (4 * i) | (four.y == my_doc ? 2u : 0u) << (4 * i) | (four.z == my_doc ? 4u : 0u) << (4 * i) |
+                                            (four.w == my_doc ? 8u : 0u) << (4 * i);
+                                }
+                                w &= my_doc >= 0 ? same : 0u;
+                            }
+                            seen[x] = w;
+                        }
+                    }
+                    float v[2][32];
+                    tmem_ld32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                    tmem_ld32(s_addr + c * 32 + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
+                    tmem_ld_wait(v[0], v[1]);
+                    if constexpr (kCap) {
+                        if (partial) {   // four scores share a reciprocal: what is not seen must not be not a number
+#pragma unroll
+                            for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = (seen[i >> 5] >> (i & 31)) & 1u ? v[i >> 5][i & 31] : 0.f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) cap4(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1], v[i >> 5][(i & 31) + 2], v[i >> 5][(i & 31) + 3], r.cap_in, r.cap_out);
+                    }
+                    const float sc = kCap ? 1.f : r.scale_log2;
+                    const float2 sc2 = make_float2(sc, sc);
+                    if constexpr (kBias == kSlopes) {
+                        const float base = (float)(k0 + c * 32 - qpos);
+                        const float2 slope2 = make_float2(slope, slope);
+#pragma unroll
+                        for (int i = 0; i < 64; i += 2) {
+                            float2 d = add2(make_float2(base, base), make_float2((float)i, (float)(i + 1)));
+                            d.x = fabsf(d.x);
+                            d.y = fabsf(d.y);
+                            float2 x = make_float2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1]);
+                            if constexpr (!kCap) x = mul2(x, sc2);
+                            x = fma2(d, slope2, x);
+                            v[i >> 5][i & 31] = x.x;
+                            v[i >> 5][(i & 31) + 1] = x.y;
+                        }
+                    }
+                    if constexpr (kBias == kTable) {
+                        // row's first value is number 127 - row: eight values at a time from the copy in which they start on 16 bytes
+                        const int start = 127 - row;
+                        const uint8_t* const biases = sBias + m * kShiftBytes + (start & 7) * kShiftPitch + ((start & ~7) + c * 32) * 2;
+                        const float2 log2 = make_float2(kRulesLog2e, kRulesLog2e);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const uint4 eight = *reinterpret_cast<const uint4*>(biases + e * 16);
+                            const half2* const h = reinterpret_cast<const half2*>(&eight);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float& a = v[e >> 2][(e & 3) * 8 + 2 * i];
+                                float& bb = v[e >> 2][(e & 3) * 8 + 2 * i + 1];
+                                float2 x = make_float2(a, bb);
+                                if constexpr (!kCap) x = mul2(x, sc2);
+                                x = fma2(__half22float2(h[i]), log2, x);
+                                a = x.x;
+                                bb = x.y;
+                            }
+                        }
+                    }
+                    if (partial) {
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = (seen[i >> 5] >> (i & 31)) & 1u ? v[i >> 5][i & 31] : -INFINITY;
+                    }
+                    if (kChanged || partial) {
+                        tmem_store32(s_addr + c * 32, v[0]);
+                        tmem_store32(s_addr + c * 32 + 32, v[1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) mx[i & 3] = max3(mx[i & 3], v[i >> 4][2 * (i & 15)], v[i >> 4][2 * (i & 15) + 1]);
+                }
+                if (kChanged || partial) tmem_st_wait();
+                if (help) {
+                    __syncwarp();
+                    if (elect_one()) mbar_arrive(&sh->m_empty[m]);
+                    __syncwarp();
+                }
+                const float sc = kChanged ? 1.f : r.scale_log2;
+                const float bmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sc;   // the scale is positive
+                // The reference point moves only when the row maximum has grown by more than 2^8; the final division by the row sum makes the
+                // result independent of it.
+                const bool grow = bmax > m_run + kRescaleStep;   // also true for the first finite score of a row
+                const bool any = __any_sync(0xffffffffu, grow);
+                float alpha = 1.f;
+                if (grow) {
+                    alpha = m_run == -INFINITY ? 0.f : ex2_fast(m_run - bmax);
+                    m_run = bmax;
+                    l2.x *= alpha;
+                    l2.y *= alpha;
+                }
+                const float nshift = (m_run == -INFINITY) ? 0.f : -m_run;
+                const float2 sc2 = make_float2(sc, sc), sh2 = make_float2(nshift, nshift);
+                // P and O may be written once P V of the previous block has completed
+                if (g > 0) {
+                    ok = mbar_wait(&sh->pv_done, (g - 1) & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                if (first) {
+                    if (done_slot >= 0) finish();
+                } else if (any) {
+#pragma unroll 1
+                    for (int c = 0; c < osteps; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(o_addr + c * 16, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_store16(o_addr + c * 16, o);
+                    }
+                }
+                // exponentials of 32 scores, while the next 32 are fetched
+                auto chunk = [&](const float (&v)[32], int c) {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float2 e = kChanged ? add2(make_float2(v[2 * i], v[2 * i + 1]), sh2) : fma2(make_float2(v[2 * i], v[2 * i + 1]), sc2, sh2);
+                        if ((i * kPolyPairs) / 16 != ((i + 1) * kPolyPairs) / 16) {   // spread over the chunk so that both pipes stay busy
+                            e = exp2_cubic2(e);
+                        } else {
+                            e.x = ex2_fast(e.x);
+                            e.y = ex2_fast(e.y);
+                        }
+                        l2 = add2(l2, e);
+                        pk[i] = pack2(e.x, e.y);
+                    }
+                    tmem_store16(p_addr + c * 16, pk);
+                };
+                {
+                    float v[32], w[32];
+                    tmem_ld32(s_addr, reinterpret_cast<uint32_t(&)[32]>(v));
+                    tmem_ld_wait(v);
+                    int c = 0;
+#pragma unroll 1
+                    for (;; c += 2) {
+                        tmem_ld32(s_addr + c * 32 + 32, reinterpret_cast<uint32_t(&)[32]>(w));
+                        chunk(v, c);
+                        tmem_ld_wait(w);
+                        if (c + 2 == chunks) break;
+                        tmem_ld32(s_addr + c * 32 + 64, reinterpret_cast<uint32_t(&)[32]>(v));
+                        chunk(w, c + 1);
+                        tmem_ld_wait(v);
+                    }
+                    if constexpr (C::kOwnP) {
+                        tc_fence_before();   // the next block's scores may be written
+                        __syncwarp();
+                        if (elect_one()) mbar_arrive(&sh->s_free);
+                        __syncwarp();
+                    }
+                    chunk(w, c + 1);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(&sh->p_full);
+                __syncwarp();
+            }
+            if (!ok) break;
+            done_slot = slot;
+            done_sum = l2.x + l2.y;
+        }
+        if (!ok && lane == 0) atomicExch(p.err, 22);
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
+}
+
+// Lowest and highest document of every block of 128 keys of every sequence: a warp to a block.
+__global__ void __launch_bounds__(128) document_summary_kernel(const __grid_constant__ RuleParams p, int2* __restrict__ summary, int blocks) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 31, j = blockIdx.x * 4 + (threadIdx.x >> 5);
+    for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
+        const RuleSeq s = rule_seq(p, b);
+        if (j * kBK >= s.klen) continue;
+        int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = j * kBK + i * 32 + lane;
+            if (k < s.klen) {
+                const int d = p.k_docs[s.k0 + k];
+                lo = min(lo, d);
+                hi = max(hi, d);
+            }
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        if (lane == 0) summary[(size_t)b * blocks + j] = make_int2(lo, hi);
+    }
+}
+
+template <int kHD, int kBias, bool kCap>
+cudaError_t launch(int grid, cudaStream_t st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcRules& p) {
+    const auto kernel = attention_rules_tc_kernel<kHD, kBias, kCap>;
+    static_assert(Cfg<kHD>::kHelpAt + 2 * kShiftBytes + sizeof(TcShared) + sizeof(SeqTable) + 2048 <= 233472 / kCtasPerSm, "two CTAs to an SM");
+    static PerDeviceOnce once;
+    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448); });
+    if (e != cudaSuccess) return e;
+    const size_t smem = Cfg<kHD>::kHelpAt + (kBias == kTable ? 2 * kShiftBytes : 0) + sizeof(TcShared) + (p.sorted ? sizeof(SeqTable) : 0) + 1024;
+    return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, tq, tk, tv, p);
+}
+template <int kHD>
+cudaError_t launch_for(int grid, cudaStream_t st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcRules& p) {
+    const bool cap = p.r.cap_out > 0.f;
+    const auto run = p.r.slopes  ? (cap ? launch<kHD, kSlopes, true> : launch<kHD, kSlopes, false>)
+                     : p.r.table ? (cap ? launch<kHD, kTable, true> : launch<kHD, kTable, false>)
+                                 : (cap ? launch<kHD, kNoBias, true> : launch<kHD, kNoBias, false>);
+    return run(grid, st, tq, tk, tv, p);
+}
+
+}  // namespace
+
+bool attention_rules_tc_takes(const RuleParams& p) {
+    return p.head_dim % 16 == 0 && p.head_dim <= 128 && ((p.q_pitch | p.k_pitch | p.v_pitch | p.out_pitch) & 7) == 0 && aligned16(p.q) && aligned16(p.k) &&
+           aligned16(p.v) && aligned16(p.out) && p.k_rows > 0 && p.max_k_len > 0 &&
+           ((long long)p.q_tokens / kBQ + p.batch) * p.nhead <= 0x7fffffff;
+}
+
+int attention_rules_tc_launch(const RuleParams& r, void* scratch, cudaStream_t st) {
+    TcRules p;
+    p.r = r;
+    int rc = attn_err_address(&p.err);
+    if (rc) return rc;
+    CUtensorMap tq, tk, tv;
+    if (!make_tmap_heads_f16(&tq, r.q, r.q_tokens, r.nhead, r.head_dim, r.q_pitch, kBQ) ||
+        !make_tmap_heads_f16(&tk, r.k, r.k_rows, r.nhead / r.group, r.head_dim, r.k_pitch, kBK) ||
+        !make_tmap_heads_f16(&tv, r.v, r.k_rows, r.nhead / r.group, r.head_dim, r.v_pitch, kBK))
+        return fail(ET_ERR_CUDA, "et_attention_rules: cuTensorMapEncodeTiled failed");
+    p.summary = static_cast<const int2*>(scratch);
+    p.summary_blocks = (r.max_k_len + kBK - 1) / kBK;
+    if (scratch) {
+        const cudaError_t e = launch_pdl(document_summary_kernel, dim3((p.summary_blocks + 3) / 4, min(r.batch, 0xffff)), dim3(128), 0, st, r, static_cast<int2*>(scratch), p.summary_blocks);
+        if (e != cudaSuccess) return cuda_status(e, "et_attention_rules: summary of the documents");
+    }
+    const int blocks = r.cu_seqlens ? r.q_tokens / kBQ + r.batch : r.batch * ((r.max_q_len + kBQ - 1) / kBQ);
+    // CTAs that all fit are left to the hardware: one that starts early would take an item for which a place is still free. (Of a ragged batch only the
+    // tokens are known here: at least this many blocks.)
+    const long long items = r.cu_seqlens ? (r.q_tokens + kBQ - 1) / kBQ : blocks;
+    p.take_over = items * r.nhead > (long long)kCtasPerSm * sm_count();
+    p.sorted = p.take_over && r.cu_seqlens && r.batch <= kMaxSorted;
+    p.heavy_first = r.window_right != kNoLimit;
+    const cudaError_t e = r.head_dim <= 64 ? launch_for<64>(blocks * r.nhead, st, tq, tk, tv, p) : launch_for<128>(blocks * r.nhead, st, tq, tk, tv, p);
+    return cuda_status(e, "et_attention_rules launch");
+}
+
+}  // namespace et

@@ -981,6 +981,8 @@ constexpr int kMaxDevices = 64;
 std::mutex g_err_mu;
 int* g_err_ptr[kMaxDevices] = {nullptr};
 
+}  // namespace
+
 int attn_err_address(int** out) {
     int dev = -1;
     cudaError_t e = cudaGetDevice(&dev);
@@ -996,6 +998,8 @@ int attn_err_address(int** out) {
     *out = g_err_ptr[dev];
     return ET_OK;
 }
+
+namespace {
 
 template <bool kMask, int kForm, bool kSorted>
 cudaError_t opt_in() {

@@ -62,7 +62,7 @@ __device__ __forceinline__ RuleSeq rule_seq(const RuleParams& p, int b) {
 
 // One query of one head by one warp, for any head width up to 256 and any alignment: a key to a lane for the scores, features to the lanes for
 // the sum of V. Scores and sums in fp32. What is not seen is not read into any sum.
-__device__ __noinline__ void rules_row(const RuleParams& p, const RuleSeq& s, int i, int h) {
+static __device__ __noinline__ void rules_row(const RuleParams& p, const RuleSeq& s, int i, int h) {
     const int lane = threadIdx.x & 31, hd = p.head_dim;
     const half* const q = p.q + (s.q0 + i) * p.q_pitch + (size_t)h * hd;
     const half* const k = p.k + s.k0 * p.k_pitch + (size_t)(h / p.group) * hd;

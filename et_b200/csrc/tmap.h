@@ -61,4 +61,18 @@ inline bool make_tmap_panels_f16(CUtensorMap* out, const void* base, uint64_t ro
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Rows of heads side by side, seen as [rows][heads][head_dim]: one box = 64 features (from a multiple of 64 on) of one head of `box_rows` rows, as a
+// 128-byte-swizzled [box_rows x 64] block. Features beyond the head and rows beyond the last read as zero. head_dim a multiple of 8.
+inline bool make_tmap_heads_f16(CUtensorMap* out, const void* base, uint64_t rows, uint64_t heads, uint64_t head_dim, uint64_t pitch_elems, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {head_dim, heads, rows};
+    cuuint64_t strides[2] = {head_dim * 2, pitch_elems * 2};
+    cuuint32_t box[3] = {64, 1, box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace et

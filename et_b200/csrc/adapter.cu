@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kMaxRank = 128;
+constexpr int kMaxCluster = 8;
 
 struct Slot {
     int rank;      // 0: nothing to add
@@ -40,7 +41,7 @@ struct AdapterParams {
     const Slot* slots;
     const half *a, *b;                  // packed, all slots
     long long out_pitch, base_pitch, x_pitch, a_stride, b_stride;   // of a slot, in elements
-    int batch, tokens, n_slots, in_feat, out_feat, rank_tiles;
+    int batch, tokens, n_slots, in_feat, out_feat;
     bool copy;                          // out is not base: what has no adapter is copied
 };
 
@@ -92,7 +93,7 @@ template <int kRt, int kMt, int kWk, bool kCluster>
 __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant__ AdapterParams p) {
     constexpr int kWm = kWarps / kWk, kTile = kWm * kMt * 16;
     constexpr int kFrags = kMt * kRt * 2;                  // accumulator fragments of a warp
-    extern __shared__ float4 parts[];                      // [kWarps][kFrags][32]: shares of A x, as accumulator fragments
+    extern __shared__ float4 parts[];                      // [kWarps][kFrags][32]: shares of A x, as accumulator fragments; then their sums
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp / kWk, wk = warp % kWk;
     const int g = lane >> 2, t = lane & 3;
     unsigned crank = 0, csize = 1;
@@ -108,7 +109,6 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
     const int id = p.ids[seq];
     Slot slot = {0, 0.f};
     if (id >= 0 && id < p.n_slots) slot = p.slots[id];
-    const int tiles = (slot.rank + 15) / 16;
     const int part = crank * kWk + wk, n_parts = csize * kWk;   // this warp's share of K and of the columns
     const int col_groups = (p.out_feat + 31) / 32;
     int row[kMt][2];        // the lane's rows, -1 beyond the tile
@@ -163,8 +163,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
             if (c >= chunks) break;
 #pragma unroll
             for (int j = 0; j < kRt * 2; ++j) {
-                if (j >= tiles * 2) break;
-                const uint4 w = __ldg(a + ((size_t)c * (p.rank_tiles * 2) + j) * 32 + lane);
+                const uint4 w = __ldg(a + ((size_t)c * (kRt * 2) + j) * 32 + lane);
 #pragma unroll
                 for (int m = 0; m < kMt; ++m) {
                     mma_16816(acc[m][j], xv[u][m][0].x, xv[u][m][1].x, xv[u][m][0].y, xv[u][m][1].y, w.x, w.y);
@@ -173,37 +172,51 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
             }
         }
     }
-    // ---- the shares are added, in the order of the warps and CTAs
-    if constexpr (kWk > 1 || kCluster) {
+    // ---- the shares are added, in the order of the warps, then of the CTAs: each thread adds a few places of all of them, so that what another CTA
+    // holds crosses to this one once
+    float4* const sums = parts + kWarps * kFrags * 32;     // [kWm][kFrags][32]: of this CTA's warps
+    float4* const all = sums + kWm * kFrags * 32;          // of all CTAs
 #pragma unroll
-        for (int m = 0; m < kMt; ++m)
+    for (int m = 0; m < kMt; ++m)
 #pragma unroll
-            for (int j = 0; j < kRt * 2; ++j)
-                parts[(warp * kFrags + m * kRt * 2 + j) * 32 + lane] = make_float4(acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]);
-        auto add_shares = [&](const float4* from, int first_warp, int n, bool fresh) {
+        for (int j = 0; j < kRt * 2; ++j)
+            parts[(warp * kFrags + m * kRt * 2 + j) * 32 + lane] = make_float4(acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]);
+    __syncthreads();
+    for (int e = threadIdx.x; e < kWm * kFrags * 32; e += kThreads) {
+        const int group = e / (kFrags * 32), at = e % (kFrags * 32);
+        float4 s = parts[group * kWk * kFrags * 32 + at];
 #pragma unroll
-            for (int m = 0; m < kMt; ++m)
-#pragma unroll
-                for (int j = 0; j < kRt * 2; ++j) {
-                    if (j >= tiles * 2) break;
-                    float4 s = fresh ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]);
-                    for (int w = 0; w < n; ++w) {
-                        const float4 v = from[((first_warp + w) * kFrags + m * kRt * 2 + j) * 32 + lane];
-                        s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
-                    }
-                    acc[m][j][0] = s.x; acc[m][j][1] = s.y; acc[m][j][2] = s.z; acc[m][j][3] = s.w;
-                }
-        };
-        if constexpr (kCluster) {
-            cg::cluster_group cluster = cg::this_cluster();
-            cluster.sync();
-            for (unsigned r = 0; r < csize; ++r) add_shares(cluster.map_shared_rank(parts, r), wm * kWk, kWk, r == 0);
-            cluster.sync();   // nobody leaves while its shares are read
-        } else {
-            __syncthreads();
-            add_shares(parts, wm * kWk, kWk, true);
+        for (int w = 1; w < kWk; ++w) {
+            const float4 v = parts[(group * kWk + w) * kFrags * 32 + at];
+            s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
+        sums[e] = s;
     }
+    if constexpr (kCluster) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        for (int e = threadIdx.x; e < kWm * kFrags * 32; e += kThreads) {
+            float4 v[kMaxCluster];
+#pragma unroll
+            for (int c = 0; c < kMaxCluster; ++c)
+                if (c < (int)csize) v[c] = cluster.map_shared_rank(sums, c)[e];
+            float4 s = v[0];
+#pragma unroll
+            for (int c = 1; c < kMaxCluster; ++c)
+                if (c < (int)csize) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
+            all[e] = s;
+        }
+        cluster.sync();   // nobody leaves while its shares are read
+    } else {
+        __syncthreads();
+    }
+#pragma unroll
+    for (int m = 0; m < kMt; ++m)
+#pragma unroll
+        for (int j = 0; j < kRt * 2; ++j) {
+            const float4 v = (kCluster ? all : sums)[(wm * kFrags + m * kRt * 2 + j) * 32 + lane];
+            acc[m][j][0] = v.x; acc[m][j][1] = v.y; acc[m][j][2] = v.z; acc[m][j][3] = v.w;
+        }
     // ---- to fp16, each row by a power of two of its own; ranks that only pad a step are zeros even where x is not finite
 #pragma unroll
     for (int j = 0; j < kRt * 2; ++j)
@@ -262,8 +275,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
                 for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
 #pragma unroll
         for (int q = 0; q < kRt; ++q) {
-            if (q >= tiles) break;
-            const uint4* const w = b + (((size_t)c * p.rank_tiles + q) * 32 + lane) * 2;
+            const uint4* const w = b + (((size_t)c * kRt + q) * 32 + lane) * 2;
             const uint4 w0 = __ldg(w), w1 = __ldg(w + 1);
 #pragma unroll
             for (int m = 0; m < kMt; ++m) {
@@ -291,7 +303,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
 
 template <int kRt, int kMt, int kWk, bool kCluster>
 cudaError_t launch(const AdapterParams& p, int tiles, int csize, cudaStream_t st) {
-    const size_t smem = (size_t)kWarps * kMt * kRt * 2 * 32 * sizeof(float4);
+    const size_t smem = (size_t)(kWarps + kWarps / kWk * (kCluster ? 2 : 1)) * kMt * kRt * 2 * 32 * sizeof(float4);
     const auto kernel = adapter_kernel<kRt, kMt, kWk, kCluster>;
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
@@ -315,12 +327,12 @@ cudaError_t launch(const AdapterParams& p, int tiles, int csize, cudaStream_t st
 template <int kRt>
 cudaError_t launch_for(const AdapterParams& p, cudaStream_t st) {
     constexpr int kBigMt = kRt <= 4 ? 2 : 1;     // a rank of 128 has no registers for two tiles' sums
-    constexpr int kBigTile = 2 * kBigMt * 16;
-    const bool big = p.cu_seqlens && p.tokens > 16 * p.batch;
-    if (big) return launch<kRt, kBigMt, 4, false>(p, p.tokens / kBigTile + p.batch, 1, st);
+    constexpr int kBigTile = kBigMt * 16;
+    const bool big = kBigMt > 1 && p.cu_seqlens && p.tokens > 16 * p.batch;
+    if (big) return launch<kRt, kBigMt, 8, false>(p, p.tokens / kBigTile + p.batch, 1, st);
     const int tiles = p.cu_seqlens ? p.tokens / 16 + p.batch : p.batch;
     int csize = 1;
-    while (csize < 8 && tiles * csize * 2 <= sm_count() * 2) csize *= 2;
+    while (csize < kMaxCluster && tiles * csize * 2 <= sm_count() * 2) csize *= 2;
     return csize == 1 ? launch<kRt, 1, 8, false>(p, tiles, 1, st) : launch<kRt, 1, 8, true>(p, tiles, csize, st);
 }
 
@@ -344,7 +356,7 @@ extern "C" int et_adapter_bank_create(et_adapter_bank** out, int in_feat, int ou
     auto* bank = new (std::nothrow) et_adapter_bank;
     if (!bank) return fail(ET_ERR_CUDA, "et_adapter_bank_create: out of host memory");
     bank->in_feat = in_feat; bank->out_feat = out_feat; bank->max_rank = max_rank; bank->n_slots = n_slots;
-    bank->rank_tiles = (max_rank + 15) / 16;
+    bank->rank_tiles = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : max_rank <= 64 ? 4 : 8;   // 16-wide steps: what the kernels are made for
     bank->a_stride = (long long)((in_feat + 31) / 32) * bank->rank_tiles * 2 * 256;
     bank->b_stride = (long long)((out_feat + 31) / 32) * bank->rank_tiles * 512;
     cudaError_t e = cudaGetDevice(&bank->device);
@@ -434,7 +446,6 @@ extern "C" int et_adapter_add(const et_adapter_bank* bank, void* out, const void
     p.cu_seqlens = cu_seqlens; p.ids = adapter_ids; p.slots = bank->slots; p.a = bank->a; p.b = bank->b;
     p.out_pitch = out_pitch; p.base_pitch = base_pitch; p.x_pitch = x_pitch; p.a_stride = bank->a_stride; p.b_stride = bank->b_stride;
     p.batch = batch; p.tokens = tokens; p.n_slots = bank->n_slots; p.in_feat = bank->in_feat; p.out_feat = bank->out_feat;
-    p.rank_tiles = bank->rank_tiles;
     p.copy = out != base;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int rt = bank->rank_tiles;

@@ -5,6 +5,7 @@ function forwards to `libet_b200.so`.
 """
 import array
 import ctypes
+import struct
 
 import numpy as np
 
@@ -272,65 +273,73 @@ def attention_batch(out, Q, K, V, d_model, nhead, cu_seqlens=None, valid_lens=No
 
 
 # ---------------------------------------------------------------------------------- positions, adapters, rules on scores
-_current_device = None
+_kept = None
 
 
-def _device():
-    global _current_device
-    if _current_device is None:
+def _torch_kept():
+    """(lookup of the current device, float16, int32, float32): fetched once, these calls are short."""
+    global _kept
+    if _kept is None:
         import torch
         torch.cuda.init()
-        try:
-            _current_device = torch._C._cuda_getDevice
-        except AttributeError:
-            _current_device = torch.cuda.current_device
-    return _current_device()
+        _kept = (getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device), torch.float16, torch.int32, torch.float32)
+    return _kept
 
 
-def _checked(name, t, dtype, dims, device, last=True):
-    """Refuses a tensor that is not what the library would take it for: type, dimensions, neighbouring elements, device."""
-    if t.dtype != dtype or t.dim() != dims:
-        raise ValueError(f"{name}: {dims}-dimensional {dtype} expected, not {t.dim()}-dimensional {t.dtype}")
-    if t.device.type != "cuda" or t.device.index != device:
-        raise ValueError(f"{name} is on {t.device}, not on the current CUDA device {device}")
-    if dims and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}: the elements of a row must be neighbours")
-    if not last and not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t
+def _refuse(name, t, dtype, dims, device):
+    raise ValueError(f"{name}: a {dims}-dimensional {dtype} tensor on the current CUDA device ({device}) expected, the elements of a row neighbours, rows "
+                     f"one behind the other; not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
-def _pitch(t):
-    """Elements from one row to the next (of a single row: its width)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _rows(name, t, dtype, device):
+    """(rows, features, pitch) of a matrix that may be a slice of a wider one."""
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2:
+        _refuse(name, t, dtype, 2, device)
+    rows, features = t.shape
+    pitch, step = t.stride()
+    if step != 1 and features > 1:
+        _refuse(name, t, dtype, 2, device)
+    return rows, features, pitch if rows > 1 else features
+
+
+def _array(name, t, dtype, device, n):
+    """Address of a contiguous array of n elements, or None."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 1 or not t.is_contiguous():
+        _refuse(name, t, dtype, 1, device)
+    if t.shape[0] != n:
+        raise ValueError(f"{name}: {n} elements expected, not {t.shape[0]}")
+    return t.data_ptr()
+
+
+def _matrix(name, t, dtype, device):
+    """(rows, columns) of a contiguous matrix."""
+    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2 or not t.is_contiguous():
+        _refuse(name, t, dtype, 2, device)
+    return t.shape
 
 
 def rotary_axes(q_out, k_out, q, k, positions, inv_freq, axis, head_dim, interleaved=False, stream=None):
     """Rotary positions over several axes on the heads of q [tokens, heads * head_dim] and k (either may be None); rows may be slices of
     wider ones, q_out may be q and k_out may be k. positions [tokens, axes] int32; inv_freq float32 and axis int32, one for each
     pair of features (twice as many features are turned). Returns (q_out, k_out)."""
-    import torch
-    device = _device()
-    f16, i32 = torch.float16, torch.int32
-    heads, pitches = [], []
-    tokens, axes = _checked("positions", positions, i32, 2, device, last=False).shape
-    pairs, = _checked("inv_freq", inv_freq, torch.float32, 1, device, last=False).shape
-    if _checked("axis", axis, i32, 1, device, last=False).shape[0] != pairs:
-        raise ValueError("inv_freq and axis: one element for each pair")
+    current, f16, i32, f32 = _kept or _torch_kept()
+    device = current()
+    tokens, axes = _matrix("positions", positions, i32, device)
+    pairs = inv_freq.shape[0]
+    args = []
     for name, x, out in (("q", q, q_out), ("k", k, k_out)):
         if x is None:
-            heads.append(0)
-            pitches.append((0, 0))
+            args += (None, None, 0, 0, 0)
             continue
-        _checked(name, x, f16, 2, device)
-        _checked(name + "_out", out, f16, 2, device)
-        if x.shape != out.shape or x.shape[0] != tokens or x.shape[1] % head_dim:
-            raise ValueError(f"{name}: {tokens} rows of whole heads of {head_dim}, the result alike")
-        heads.append(x.shape[1] // head_dim)
-        pitches.append((_pitch(out), _pitch(x)))
-    rc = (_entries or _lib()).et_rotary_axes(
-        _a(q_out if q is not None else None), _a(q), *pitches[0], heads[0], _a(k_out if k is not None else None), _a(k), *pitches[1], heads[1], head_dim,
-        2 * pairs, positions.data_ptr(), axes, inv_freq.data_ptr(), axis.data_ptr(), 1 if interleaved else 0, tokens, raw_stream(stream))
+        rows, width, pitch = _rows(name, x, f16, device)
+        rows_out, width_out, pitch_out = _rows(name + "_out", out, f16, device)
+        if rows != tokens or rows_out != rows or width_out != width or width % head_dim:
+            raise ValueError(f"{name}: {tokens} rows of whole heads of {head_dim}, the result alike, not {tuple(x.shape)} and {tuple(out.shape)}")
+        args += (out.data_ptr(), x.data_ptr(), pitch_out, pitch, width // head_dim)
+    rc = (_entries or _lib()).et_rotary_axes(*args, head_dim, 2 * pairs, positions.data_ptr(), axes, _array("inv_freq", inv_freq, f32, device, pairs),
+                                             _array("axis", axis, i32, device, pairs), 1 if interleaved else 0, tokens, raw_stream(stream))
     if rc:
         check(rc)
     return q_out, k_out
@@ -358,16 +367,17 @@ class AdapterBank:
     def add(self, out, base, x, adapter_ids, cu_seqlens=None, stream=None):
         """out = base + the adapter's product for each sequence's tokens. adapter_ids int32 [batch] (-1: none), cu_seqlens int32 [batch + 1]
         or None (one token to a sequence). out may be base; rows may be slices of wider ones."""
-        import torch
-        device = _device()
-        for name, t, width in (("out", out, self.out_feat), ("base", base, self.out_feat), ("x", x, self.in_feat)):
-            if _checked(name, t, torch.float16, 2, device).shape[1] != width or t.shape[0] != x.shape[0]:
-                raise ValueError(f"{name}: {x.shape[0]} rows of {width} expected, not {tuple(t.shape)}")
-        batch, = _checked("adapter_ids", adapter_ids, torch.int32, 1, device, last=False).shape
-        if cu_seqlens is not None and _checked("cu_seqlens", cu_seqlens, torch.int32, 1, device, last=False).shape[0] != batch + 1:
-            raise ValueError("cu_seqlens: one element more than adapter_ids")
-        rc = (_entries or _lib()).et_adapter_add(self._h, out.data_ptr(), base.data_ptr(), x.data_ptr(), _pitch(out), _pitch(base), _pitch(x), _a(cu_seqlens),
-                                                 adapter_ids.data_ptr(), batch, x.shape[0], raw_stream(stream))
+        current, f16, i32, _ = _kept or _torch_kept()
+        device = current()
+        rows, width, x_pitch = _rows("x", x, f16, device)
+        base_rows, base_width, base_pitch = _rows("base", base, f16, device)
+        out_rows, out_width, out_pitch = _rows("out", out, f16, device)
+        if width != self.in_feat or base_width != self.out_feat or out_width != self.out_feat or base_rows != rows or out_rows != rows:
+            raise ValueError(f"x [{rows}, {self.in_feat}], base and out [{rows}, {self.out_feat}] expected, not {tuple(x.shape)}, {tuple(base.shape)}, {tuple(out.shape)}")
+        batch = adapter_ids.shape[0]
+        rc = (_entries or _lib()).et_adapter_add(self._h, out.data_ptr(), base.data_ptr(), x.data_ptr(), out_pitch, base_pitch, x_pitch,
+                                                 _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), _array("adapter_ids", adapter_ids, i32, device, batch),
+                                                 batch, rows, raw_stream(stream))
         if rc:
             check(rc)
         return out
@@ -384,10 +394,8 @@ class AdapterBank:
             pass
 
 
-class _ScoreRules(ctypes.Structure):
-    _fields_ = [("scale", ctypes.c_float), ("cap", ctypes.c_float), ("slopes", ctypes.c_void_p), ("distance_bias", ctypes.c_void_p), ("reach", ctypes.c_int),
-                ("window_left", ctypes.c_int), ("window_right", ctypes.c_int), ("prefix_lens", ctypes.c_void_p), ("q_docs", ctypes.c_void_p),
-                ("k_docs", ctypes.c_void_p)]
+# et_score_rules as it lies in memory: scale, cap, slopes, distance_bias, reach, window_left, window_right, prefix_lens, q_docs, k_docs
+_score_rules = struct.Struct("@ffPPiiiPPP").pack
 
 
 def attention_rules_scratch_size(batch, max_k_len):
@@ -402,36 +410,32 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
     """Attention with rules on its scores (capped, biased by distance, seen through windows, prefixes and documents) over packed sequences, or of
     tokens over keys kept from before (k_start, k_lens). Q and out [tokens, heads * head_dim], K and V [rows, kv_heads * head_dim], rows may be
     slices of wider ones; see et_attention_rules for each argument. max_q_len, max_k_len: 0 takes the number of rows."""
-    import torch
-    device = _device()
-    f16, i32 = torch.float16, torch.int32
-    for name, t in (("out", out), ("Q", Q), ("K", K), ("V", V)):
-        _checked(name, t, f16, 2, device)
-        if t.shape[1] % head_dim or not t.shape[1]:
-            raise ValueError(f"{name}: whole heads of {head_dim} expected, not {t.shape[1]} features")
-    if out.shape != Q.shape or K.shape != V.shape:
-        raise ValueError("out like Q and V like K expected")
-    nhead, nhead_kv = Q.shape[1] // head_dim, K.shape[1] // head_dim
-    for name, t, n in (("cu_seqlens", cu_seqlens, batch + 1), ("k_start", k_start, batch), ("k_lens", k_lens, batch), ("prefix_lens", prefix_lens, batch),
-                       ("q_docs", q_docs, Q.shape[0]), ("k_docs", k_docs, K.shape[0])):
-        if t is not None and _checked(name, t, i32, 1, device, last=False).shape[0] != n:
-            raise ValueError(f"{name}: {n} elements expected, not {t.shape[0]}")
-    if slopes is not None and _checked("slopes", slopes, torch.float32, 1, device, last=False).shape[0] != nhead:
-        raise ValueError("slopes: one for each head")
-    reach = 0
+    current, f16, i32, f32 = _kept or _torch_kept()
+    device = current()
+    tokens, width, q_pitch = _rows("Q", Q, f16, device)
+    out_rows, out_width, out_pitch = _rows("out", out, f16, device)
+    k_rows, kv_width, k_pitch = _rows("K", K, f16, device)
+    v_rows, v_width, v_pitch = _rows("V", V, f16, device)
+    if out_rows != tokens or out_width != width or v_rows != k_rows or v_width != kv_width or width % head_dim or kv_width % head_dim or not kv_width or not width:
+        raise ValueError(f"whole heads of {head_dim}, out like Q and V like K expected, not {tuple(Q.shape)}, {tuple(out.shape)}, {tuple(K.shape)}, {tuple(V.shape)}")
+    nhead, nhead_kv = width // head_dim, kv_width // head_dim
+    reach, table = 0, None
     if distance_bias is not None:
-        _checked("distance_bias", distance_bias, f16, 2, device, last=False)
-        if distance_bias.shape[0] != nhead or distance_bias.shape[1] % 2 == 0:
+        heads, places = _matrix("distance_bias", distance_bias, f16, device)
+        if heads != nhead or places % 2 == 0:
             raise ValueError("distance_bias: [heads, 2 reach + 1] expected")
-        reach = distance_bias.shape[1] // 2
-    scratch_bytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    if scratch is not None and (scratch.device.type != "cuda" or scratch.device.index != device or not scratch.is_contiguous()):
-        raise ValueError("scratch must be contiguous, on the current CUDA device")
-    rules = _ScoreRules(scale, cap, _a(slopes), _a(distance_bias), reach, window[0], window[1], _a(prefix_lens), _a(q_docs), _a(k_docs))
+        reach, table = places // 2, distance_bias.data_ptr()
+    scratch_bytes = 0
+    if scratch is not None:
+        scratch_bytes = scratch.numel() * scratch.element_size()
+        if scratch.get_device() != device or not scratch.is_contiguous():
+            raise ValueError("scratch must be contiguous, on the current CUDA device")
+    rules = _score_rules(scale, cap, _array("slopes", slopes, f32, device, nhead) or 0, table or 0, reach, *window, _array("prefix_lens", prefix_lens, i32, device, batch) or 0,
+                         _array("q_docs", q_docs, i32, device, tokens) or 0, _array("k_docs", k_docs, i32, device, k_rows) or 0)
     rc = (_entries or _lib()).et_attention_rules(
-        out.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), _pitch(out), _pitch(Q), _pitch(K), _pitch(V), nhead, nhead_kv, head_dim, _a(cu_seqlens),
-        _a(k_start), _a(k_lens), batch, Q.shape[0], K.shape[0], max_q_len or Q.shape[0], max_k_len or K.shape[0], ctypes.addressof(rules), _a(scratch),
-        scratch_bytes, raw_stream(stream))
+        out.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), out_pitch, q_pitch, k_pitch, v_pitch, nhead, nhead_kv, head_dim,
+        _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), _array("k_start", k_start, i32, device, batch), _array("k_lens", k_lens, i32, device, batch), batch, tokens,
+        k_rows, max_q_len or tokens, max_k_len or k_rows, rules, _a(scratch), scratch_bytes, raw_stream(stream))
     if rc:
         check(rc)
     return out

@@ -53,10 +53,9 @@ def attention(lib, rules=None, **change):
     a = dict(out=P, Q=P, K=P, V=P, out_pitch=128, q_pitch=128, k_pitch=64, v_pitch=64, nhead=2, nhead_kv=1, head_dim=64, cu=None, k_start=None, k_lens=None, batch=1, q_tokens=4,
              k_rows=4, max_q_len=4, max_k_len=4)
     a.update(change)
-    values = dict(window_left=-1, window_right=-1)
+    values = dict(scale=0.0, cap=0.0, slopes=0, distance_bias=0, reach=0, window_left=-1, window_right=-1, prefix_lens=0, q_docs=0, k_docs=0)
     values.update(rules or {})
-    r = ops._ScoreRules(**values)
-    return lib.et_attention_rules(*a.values(), ctypes.byref(r), None, ctypes.c_size_t(0), None)
+    return lib.et_attention_rules(*a.values(), ops._score_rules(*values.values()), None, ctypes.c_size_t(0), None)
 
 
 @pytest.mark.parametrize("change", [dict(batch=-1), dict(q_tokens=-1), dict(max_k_len=-1), dict(nhead=0), dict(nhead_kv=0), dict(nhead=3, nhead_kv=2), dict(head_dim=0), dict(head_dim=257),

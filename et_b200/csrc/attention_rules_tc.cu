@@ -1,16 +1,14 @@
 // Attention with rules on its scores, on the 5th-generation tensor cores (tcgen05 + TMEM + TMA): whole sequences, heads of a multiple of 16 up to 128.
 //
-// A work item is 128 queries of one head of one sequence; a block is 128 keys of it. Blocks that no query of the item sees are left out: the
+// A work item is 128 queries of one head of one sequence; a block is 64 keys of it. Blocks that no query of the item sees are left out: the
 // window and the prefix give two ranges of blocks, documents are looked up in a summary (lowest and highest document of every block) that a small kernel
-// makes first. Blocks that all queries see take no mask; in the others a row has one bit for each of its scores.
-//   S = Q K^T        SS UMMAs 128x128x16, fp32 in 128 TMEM columns
-//   softmax          four warps, a thread to a query row, in two passes over the scores in tensor memory: the first caps them, adds the bias, takes out
-//                    what is not seen (what it changes goes back) and takes the maximum, the second takes the exponentials
-//   O += P V         TS UMMAs 128 x head x 16: A = P (fp16) from tensor memory, B = V as loaded
+// makes first. Blocks that all queries see take no mask.
+//   S = Q K^T        SS UMMAs 128x64x16, fp32 in 64 TMEM columns; two places, so that the next block's scores are made during this one's softmax
+//   softmax          four warps, a thread to a query row with its 64 scores in registers: capped, biased, masked, their maximum, exponentials
+//   O += P V         TS UMMAs 128 x head x 16: A = P (fp16) in the place of the scores it came from, B = V as loaded
 //   epilogue         O / row sum -> fp16 -> global
-// Two CTAs share an SM (256 TMEM columns each), so that one's loads, maxima and hand-overs run under the other's exponentials. Heads of 64 keep P in
-// columns of its own, and Q K^T of the next block runs while this one's exponentials become P V; wider heads have no columns left, P takes the place of
-// the scores it came from, and Q K^T of the next block follows P V.
+// Two CTAs share an SM (256 TMEM columns each), so that one's waits and maxima run under the other's exponentials. Heads of 64 have two places for
+// O: an item's rows are written during the next one.
 //
 // Not a number times the weight 0 is not a number: V rows behind the last key are cleared in shared memory before P V, and a row whose result is not
 // finite is computed again from the keys that it sees (rules_row). So is one whose result, a mean of values near fp16's largest, has left the range by the
@@ -28,8 +26,7 @@ namespace et {
 
 namespace {
 
-constexpr int kBQ = 128, kBK = 128;
-constexpr int kPanel = 128 * 128;         // 128 rows of 64 fp16 features
+constexpr int kBQ = 128, kBK = 64;
 constexpr int kSoftmaxWarps = 4;
 constexpr int kLoadWarp = 4, kMmaWarp = 5, kHelpWarp = 6, kHelpWarps = 2;
 constexpr int kThreads = 256;
@@ -39,15 +36,15 @@ constexpr float kRescaleStep = 8.f;       // log2 units by which a row's maximum
 constexpr int kItemRing = 4, kBlockRing = 8;
 constexpr int kMaxSorted = 128;           // sequences of a ragged batch that a CTA keeps in order of length
 constexpr int kLenClasses = 9;
-constexpr int kShiftPitch = 528;          // bytes of one of eight copies of a block's biases, each shifted by one more: 256 values and 16 bytes against conflicts
-constexpr int kShiftBytes = 8 * kShiftPitch;
+constexpr int kShiftPitch = 800;          // bytes of one of four copies of a block's biases (fp32, log2 domain), each shifted by one more: 196 values and some against conflicts
+constexpr int kShiftBytes = 4 * kShiftPitch;
 
 enum Bias { kNoBias = 0, kSlopes = 1, kTable = 2 };
-enum BlockFlags { kPartial = 1, kFirst = 2, kLast = 4, kEnd = 8 };
+enum BlockFlags { kPartial = 1, kFirst = 2, kLast = 4, kEnd = 8, kMixed = 16 };   // kPartial: by place, kMixed: by document
 
 struct TcRules {
     RuleParams r;
-    const int2* summary;      // documents: lowest and highest of each block of keys, [batch][summary_blocks]
+    const int2* summary;      // documents: document_summary_kernel's, [batch][summary_blocks]; null without documents
     int summary_blocks;
     bool take_over;           // CTAs ask for items that have not started
     bool sorted;              // a ragged batch of at most kMaxSorted sequences, the longest first
@@ -66,19 +63,21 @@ struct Block {
 
 template <int kHD>
 struct Cfg {
-    static constexpr int kPanels = kHD / 64;
-    static constexpr int kTile = kPanels * kPanel;          // 128 rows of Q, K or V
-    static constexpr bool kOwnP = kHD == 64;
-    static constexpr int kStages = kHD == 64 ? 2 : 1;       // of Q, K and V each
-    static constexpr uint32_t kSCol = 0, kPCol = kOwnP ? 128 : 0, kOCol = kOwnP ? 192 : 128;
-    static constexpr int kHelpAt = 3 * kStages * kTile;
+    static constexpr int kPanels = kHD / 64;                // of 64 features: rows of 128 bytes
+    static constexpr int kQPanel = kBQ * 128, kKPanel = kBK * 128;
+    static constexpr int kQTile = kPanels * kQPanel, kKTile = kPanels * kKPanel;
+    static constexpr int kQStages = kHD == 64 ? 2 : 1;
+    static constexpr int kStages = kHD == 64 ? 4 : 2;       // of K and V each
+    static constexpr int kOPlaces = kHD == 64 ? 2 : 1;
+    static constexpr uint32_t kSCol = 0, kOCol = 2 * kBK;   // S, 64 columns twice; O
+    static constexpr int kKAt = kQStages * kQTile, kVAt = kKAt + kStages * kKTile, kHelpAt = kVAt + kStages * kKTile;
 };
 
 struct TcShared {
     uint4 clc;
     uint64_t clc_full;
-    uint64_t q_full[2], q_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full, s_free, p_full, pv_done;
+    uint64_t q_full[2], q_empty[2], k_full[4], k_empty[4], v_full[4], v_empty[4];
+    uint64_t s_full[2], p_full[2], pv_done[2];   // by place of the scores
     uint64_t m_full[2], m_empty[2];       // what the helping warps bring of a block: documents of its keys, its biases
     uint64_t item_full[kItemRing], item_empty[kItemRing];
     uint64_t block_full[kBlockRing];
@@ -99,16 +98,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_store32(uint32_t taddr, const float (&v)[32]) {
-    const uint32_t(&r)[32] = reinterpret_cast<const uint32_t(&)[32]>(v);
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
-        "%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -163,8 +152,6 @@ __device__ __forceinline__ void cap4(float& a, float& b, float& c, float& d, flo
 }
 // Bits i >= from of a word (from: any whole number).
 __device__ __forceinline__ uint32_t bits_from(int from) { return from <= 0 ? ~0u : from >= 32 ? 0u : ~0u << from; }
-
-__device__ __forceinline__ void tma_load_heads(void* dst, const void* tmap, int x, int head, int row, uint64_t* bar) { tma_load_3d(dst, tmap, x, head, row, bar); }
 
 __device__ __forceinline__ void clc_ask(uint4* answer, uint64_t* bar) {
     asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
@@ -294,7 +281,8 @@ struct Blocks {
     int n_prefix, first, n;        // blocks of the prefix, the window's first block behind them, all of them
     int at;                        // the next one to look at; documents: behind the 32 looked at
     unsigned seen, whole;          // documents: of the 32 looked at, those to come, and those of one document with all queries
-    int d_lo, d_hi;
+    int d_lo, d_hi;                // lowest and highest of the queries
+    bool d_odd;                    // some query is of none
 
     __device__ __forceinline__ int number(int i) const { return i < n_prefix ? i : first + i - n_prefix; }
     __device__ __forceinline__ void start(const TcRules& p, const Item& it, int lane) {
@@ -309,26 +297,29 @@ struct Blocks {
         n = n_prefix + (hi >= lo ? max(hi / kBK - first + 1, 0) : 0);
         at = 0;
         if (p.summary) {
-            int mn = 0x7fffffff, mx = -0x7fffffff - 1;
+            int lowest = 0x7fffffff, highest = -1;
+            bool none = false;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kBQ / 32; ++i) {
                 const int q = it.qi0 + i * 32 + lane;
                 if (q < s.qlen) {
                     const int d = r.q_docs[s.q0 + q];
-                    mn = min(mn, d);
-                    mx = max(mx, d);
+                    if (d >= 0) lowest = min(lowest, d);
+                    highest = max(highest, d);
+                    none = none || d < 0;
                 }
             }
-            d_lo = __reduce_min_sync(0xffffffffu, mn);
-            d_hi = __reduce_max_sync(0xffffffffu, mx);
+            d_lo = __reduce_min_sync(0xffffffffu, lowest);
+            d_hi = __reduce_max_sync(0xffffffffu, highest);
+            d_odd = __any_sync(0xffffffffu, none);
             summary = p.summary + (size_t)it.b * p.summary_blocks;
             seen = whole = 0;
         }
     }
-    // -1: no more
-    __device__ __forceinline__ int next(const TcRules& p, const Item& it, int lane, bool& partial) {
+    // Number of the next block, -1: no more; what: kPartial, kMixed
+    __device__ __forceinline__ int next(const TcRules& p, const Item& it, int lane, int& what) {
         int i;
-        bool one_document = true;
+        what = 0;
         if (p.summary) {
             while (!seen) {
                 if (at >= n) return -1;
@@ -336,8 +327,8 @@ struct Blocks {
                 bool meets = false, same = false;
                 if (mine < n) {
                     const int2 d = summary[number(mine)];
-                    meets = d_hi >= 0 && d.y >= max(d_lo, 0) && d.x <= d_hi;
-                    same = d.x == d.y && d_lo == d_hi && d.x == d_lo;
+                    meets = d.y >= d_lo && (d.x & 0x7fffffff) <= d_hi;   // (without a document on one side never)
+                    same = d.x == d.y && d_lo == d_hi && d.x == d_lo && !d_odd;
                 }
                 seen = __ballot_sync(0xffffffffu, meets);
                 whole = __ballot_sync(0xffffffffu, same);
@@ -345,7 +336,7 @@ struct Blocks {
             }
             const int bit = __ffs(seen) - 1;
             i = at - 32 + bit;
-            one_document = (whole >> bit) & 1u;
+            if (!((whole >> bit) & 1u)) what = kMixed;
             seen &= seen - 1;
         } else {
             if (at >= n) return -1;
@@ -357,7 +348,7 @@ struct Blocks {
         const int qa = s.qpos0 + it.qi0, qb = s.qpos0 + min(it.qi0 + kBQ, s.qlen) - 1;
         const int ka = j * kBK, kb = ka + kBK - 1;
         const bool inside = (r.window_left == kNoLimit || ka >= qb - r.window_left) && (r.window_right == kNoLimit || kb <= qa + r.window_right);
-        partial = !(one_document && kb < s.klen && (inside || kb < s.prefix));
+        if (!(kb < s.klen && (inside || kb < s.prefix))) what |= kPartial;
         return j;
     }
 };
@@ -367,17 +358,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                                                                                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcRules p) {
     using C = Cfg<kHD>;
     const bool docs = p.summary != nullptr, help = kBias == kTable || docs;
-    constexpr bool kChanged = kCap || kBias != kNoBias;   // the first pass leaves scores in the log2 domain
+    constexpr bool kChanged = kCap || kBias != kNoBias;   // scores are in the log2 domain before the maximum is taken
     constexpr int kPolyPairs = 2;                         // of 16 pairs of exponentials, how many go to the FMA pipe
     const RuleParams& r = p.r;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint8_t* const sQ = smem;
-    uint8_t* const sK = sQ + C::kStages * C::kTile;
-    uint8_t* const sV = sK + C::kStages * C::kTile;
     uint8_t* const sBias = smem + C::kHelpAt;
     TcShared* const sh = reinterpret_cast<TcShared*>(smem + C::kHelpAt + (kBias == kTable ? 2 * kShiftBytes : 0));
     SeqTable* const table = reinterpret_cast<SeqTable*>(sh + 1);   // p.sorted
+    const uint32_t smem_at = smem_u32(smem), sh_at = smem_u32(sh);
+    // Barriers by their 32-bit addresses: through a pointer that was rounded up a wait costs several times as much.
+    auto bar = [&](size_t member, uint32_t i = 0) { return sh_at + (uint32_t)member + i * 8; };
+#define ET_BAR(name, ...) bar(offsetof(TcShared, name), ##__VA_ARGS__)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hd = r.head_dim, osteps = hd >> 4;
     pdl_launch_dependents();
@@ -387,15 +379,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             mbar_init(&sh->clc_full, 1);
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh->q_full[i], 1); mbar_init(&sh->q_empty[i], 1);
-                mbar_init(&sh->k_full[i], 1); mbar_init(&sh->k_empty[i], 1);
-                mbar_init(&sh->v_full[i], 1); mbar_init(&sh->v_empty[i], 1);
+                mbar_init(&sh->s_full[i], 1);
+                mbar_init(&sh->p_full[i], kSoftmaxWarps);
+                mbar_init(&sh->pv_done[i], 1);
                 mbar_init(&sh->m_full[i], 32 * kHelpWarps);
                 mbar_init(&sh->m_empty[i], kSoftmaxWarps);
             }
-            mbar_init(&sh->s_full, 1);
-            mbar_init(&sh->s_free, kSoftmaxWarps);
-            mbar_init(&sh->p_full, kSoftmaxWarps);
-            mbar_init(&sh->pv_done, 1);
+            for (int i = 0; i < C::kStages; ++i) {
+                mbar_init(&sh->k_full[i], 1); mbar_init(&sh->k_empty[i], 1);
+                mbar_init(&sh->v_full[i], 1); mbar_init(&sh->v_empty[i], 1);
+            }
             for (int i = 0; i < kItemRing; ++i) {
                 mbar_init(&sh->item_full[i], 1);
                 mbar_init(&sh->item_empty[i], kSoftmaxWarps);
@@ -423,24 +416,28 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         int ni = 0, nq = 0, nk = 0, nv = 0, g = 0;   // items handed out, tiles requested, blocks announced
         uint32_t clc_phase = 0;
         bool ok = true;
-        auto load = [&](uint8_t* dst, const CUtensorMap* tm, int head, int row, uint64_t* full, uint64_t* empty, int& count) {
-            const int st = count % C::kStages;
-            if (!mbar_wait(&empty[st], ((uint32_t)(count / C::kStages) & 1u) ^ 1u)) return false;
+        auto load = [&](int at, int panel, int stages, const CUtensorMap* tm, int head, int row, size_t full, size_t empty, int& count) {
+            const int st = count % stages;
+            if (!mbar_wait_at(bar(empty, st), ((uint32_t)(count / stages) & 1u) ^ 1u)) return false;
             if (lane == 0) {
-                mbar_expect_tx(&full[st], C::kTile);
+                mbar_expect_tx_at(bar(full, st), C::kPanels * panel);
 #pragma unroll
-                for (int c = 0; c < C::kPanels; ++c) tma_load_heads(dst + st * C::kTile + c * kPanel, tm, c * 64, head, row, &full[st]);
+                for (int c = 0; c < C::kPanels; ++c) tma_load_3d_at(smem_at + at + (st * C::kPanels + c) * panel, tm, c * 64, head, row, bar(full, st));
             }
             ++count;
             return true;
         };
-        // A block's entry may be overwritten kBlockRing blocks later: by then the K tile in between has been used, so the scores two blocks
-        // before that have been read, and with them everything of this block by everyone.
+        auto load_q = [&](int head, int row) { return load(0, C::kQPanel, C::kQStages, &tmQ, head, row, offsetof(TcShared, q_full), offsetof(TcShared, q_empty), nq); };
+        auto load_k = [&](int head, int row) { return load(C::kKAt, C::kKPanel, C::kStages, &tmK, head, row, offsetof(TcShared, k_full), offsetof(TcShared, k_empty), nk); };
+        auto load_v = [&](int head, int row) { return load(C::kVAt, C::kKPanel, C::kStages, &tmV, head, row, offsetof(TcShared, v_full), offsetof(TcShared, v_empty), nv); };
+        // A block's entry may be overwritten kBlockRing blocks later: K of the block before that one has then been requested, so scores have been made
+        // kStages blocks before, for which the weights two blocks before those were in place: everyone has passed this block.
+        static_assert(C::kStages + 3 <= kBlockRing, "entries stay until everyone has read them");
         auto announce = [&](int j, int left, int flags, int slot) {
             if (lane == 0) {
                 Block& b = sh->block[g % kBlockRing];
                 b.j = j; b.left = left; b.flags = flags; b.item = slot;
-                mbar_arrive(&sh->block_full[g % kBlockRing]);
+                mbar_arrive_at(ET_BAR(block_full, g % kBlockRing));
             }
             __syncwarp();
             ++g;
@@ -455,30 +452,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             if (find_item(p, table, id / r.nhead, lane, it)) {
                 Blocks blocks;
                 blocks.start(p, it, lane);
-                bool partial = false, partial_next = false;
-                int j = blocks.next(p, it, lane, partial);
+                int what = 0, what_next = 0;
+                int j = blocks.next(p, it, lane, what);
                 it.state = j >= 0 ? 1 : 0;
                 const int slot = ni % kItemRing;
-                if ((ok = mbar_wait(&sh->item_empty[slot], ((uint32_t)(ni / kItemRing) & 1u) ^ 1u))) {
+                if ((ok = mbar_wait_at(ET_BAR(item_empty, slot), ((uint32_t)(ni / kItemRing) & 1u) ^ 1u))) {
                     if (lane == 0) {
                         sh->item[slot] = it;
-                        mbar_arrive(&sh->item_full[slot]);
+                        mbar_arrive_at(ET_BAR(item_full, slot));
                     }
                     __syncwarp();
                     ++ni;
                     const int kv_head = it.head / r.group;
-                    if (j >= 0) ok = load(sQ, &tmQ, it.head, it.seq.q0 + it.qi0, sh->q_full, sh->q_empty, nq);
-                    // K of the first block; then K of the next block ahead of V of this one, if there is a place for it before this one's P V
-                    if (ok && j >= 0) ok = load(sK, &tmK, kv_head, it.seq.k0 + j * kBK, sh->k_full, sh->k_empty, nk);
+                    if (j >= 0) ok = load_q(it.head, it.seq.q0 + it.qi0) && load_k(kv_head, it.seq.k0 + j * kBK);
                     int flags = kFirst;
-                    while (ok && j >= 0) {
-                        const int jn = blocks.next(p, it, lane, partial_next);
-                        announce(j, it.seq.klen - j * kBK, flags | (partial ? kPartial : 0) | (jn < 0 ? kLast : 0), slot);
-                        if (C::kStages == 1) ok = load(sV, &tmV, kv_head, it.seq.k0 + j * kBK, sh->v_full, sh->v_empty, nv);
-                        if (ok && jn >= 0) ok = load(sK, &tmK, kv_head, it.seq.k0 + jn * kBK, sh->k_full, sh->k_empty, nk);
-                        if (ok && C::kStages > 1) ok = load(sV, &tmV, kv_head, it.seq.k0 + j * kBK, sh->v_full, sh->v_empty, nv);
+                    while (ok && j >= 0) {   // K of the next block ahead of V of this one
+                        const int jn = blocks.next(p, it, lane, what_next);
+                        announce(j, it.seq.klen - j * kBK, flags | what | (jn < 0 ? kLast : 0), slot);
+                        if (jn >= 0) ok = load_k(kv_head, it.seq.k0 + jn * kBK);
+                        if (ok) ok = load_v(kv_head, it.seq.k0 + j * kBK);
                         j = jn;
-                        partial = partial_next;
+                        what = what_next;
                         flags = 0;
                     }
                 }
@@ -496,11 +490,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         }
         if (ok) {
             const int slot = ni % kItemRing;
-            ok = mbar_wait(&sh->item_empty[slot], ((uint32_t)(ni / kItemRing) & 1u) ^ 1u);
+            ok = mbar_wait_at(ET_BAR(item_empty, slot), ((uint32_t)(ni / kItemRing) & 1u) ^ 1u);
             if (ok) {
                 if (lane == 0) {
                     sh->item[slot].state = -1;
-                    mbar_arrive(&sh->item_full[slot]);
+                    mbar_arrive_at(ET_BAR(item_full, slot));
                 }
                 announce(0, 0, kEnd, slot);
             }
@@ -508,115 +502,92 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         if (!ok) {
             if (lane == 0) atomicExch(p.err, 21);
             // copies still in flight land before the CTA leaves (bounded)
-            for (int i = max(nq - C::kStages, 0); i < nq; ++i) mbar_wait(&sh->q_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
-            for (int i = max(nk - C::kStages, 0); i < nk; ++i) mbar_wait(&sh->k_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
-            for (int i = max(nv - C::kStages, 0); i < nv; ++i) mbar_wait(&sh->v_full[i % C::kStages], (uint32_t)(i / C::kStages) & 1u);
+            for (int i = max(nq - C::kQStages, 0); i < nq; ++i) mbar_wait_at(ET_BAR(q_full, i % C::kQStages), (uint32_t)(i / C::kQStages) & 1u);
+            for (int i = max(nk - C::kStages, 0); i < nk; ++i) mbar_wait_at(ET_BAR(k_full, i % C::kStages), (uint32_t)(i / C::kStages) & 1u);
+            for (int i = max(nv - C::kStages, 0); i < nv; ++i) mbar_wait_at(ET_BAR(v_full, i % C::kStages), (uint32_t)(i / C::kStages) & 1u);
         }
         __syncwarp();
     } else if (warp == kMmaWarp) {
         // ---- UMMAs: the warp stays converged, one elected lane issues. Blocks are numbered through across items.
         const int steps = hd >> 4;
-        const uint32_t idesc_qk = make_idesc_f16(128, kBK), idesc_qk_half = make_idesc_f16(128, kBK / 2), idesc_pv = make_idesc_f16(128, hd, false, true);
-        int nq = 0;
+        const uint32_t idesc_qk = make_idesc_f16(128, kBK), idesc_pv = make_idesc_f16(128, hd, false, true);
+        int nq = 0, place = 0;        // Q tiles taken, place of the current item's O
         uint32_t g = 0;
         bool ok = true;
         struct { int left, flags; } cur = {0, 0}, nxt = {0, 0};   // the block in work, and the one behind it
-        auto entry = [&](uint32_t n) {
+        auto entry_wait = [&](uint32_t n) {
+            if (!mbar_wait_at(ET_BAR(block_full, n % kBlockRing), (n / kBlockRing) & 1u)) return false;
             nxt.left = sh->block[n % kBlockRing].left;
             nxt.flags = sh->block[n % kBlockRing].flags;
             __syncwarp();
+            return true;
         };
-        auto entry_wait = [&](uint32_t n) { return mbar_wait(&sh->block_full[n % kBlockRing], (n / kBlockRing) & 1u); };
-        // S = Q K_n^T of the block whose entry is `nxt`
-        auto issue_qk = [&](uint32_t n) {
-            const int qs = (nq - 1) % C::kStages;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t qa = smem_u32(sQ + qs * C::kTile), ka = smem_u32(sK + (n % C::kStages) * C::kTile);
-                const uint32_t idesc = nxt.left <= kBK / 2 ? idesc_qk_half : idesc_qk;
-                for (int ks = 0; ks < steps; ++ks) {
-                    const uint32_t at = (ks >> 2) * kPanel + (ks & 3) * 32;
-                    umma_f16(tmem + C::kSCol, make_smem_desc(qa + at, 16, 1024, 2), make_smem_desc(ka + at, 16, 1024, 2), idesc, ks > 0);
-                }
-                umma_commit(&sh->s_full);
-                umma_commit(&sh->k_empty[n % C::kStages]);
-                if (nxt.flags & kLast) umma_commit(&sh->q_empty[qs]);
-            }
-            __syncwarp();
-        };
-        auto wait_operands = [&](uint32_t n) {   // of block n, whose entry is `nxt`
+        // S = Q K_n^T of the block whose entry is `nxt`; its place holds P of block n - 2 until P V of that is over
+        auto qk = [&](uint32_t n) {
             if (nxt.flags & kFirst) {
-                if (!mbar_wait(&sh->q_full[nq % C::kStages], (uint32_t)(nq / C::kStages) & 1u)) return false;
+                if (!mbar_wait_at(ET_BAR(q_full, nq % C::kQStages), (uint32_t)(nq / C::kQStages) & 1u)) return false;
                 ++nq;
             }
-            return mbar_wait(&sh->k_full[n % C::kStages], (n / C::kStages) & 1u);
+            if (!mbar_wait_at(ET_BAR(k_full, n % C::kStages), (n / C::kStages) & 1u)) return false;
+            if (n >= 2 && !mbar_wait_at(ET_BAR(pv_done, n & 1), ((n - 2) >> 1) & 1u)) return false;
+            const int qs = (nq - 1) % C::kQStages;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t qa = smem_at + qs * C::kQTile, ka = smem_at + C::kKAt + (n % C::kStages) * C::kKTile;
+                for (int ks = 0; ks < steps; ++ks)
+                    umma_f16(tmem + C::kSCol + (n & 1) * kBK, make_smem_desc(qa + (ks >> 2) * C::kQPanel + (ks & 3) * 32, 16, 1024, 2),
+                             make_smem_desc(ka + (ks >> 2) * C::kKPanel + (ks & 3) * 32, 16, 1024, 2), idesc_qk, ks > 0);
+                umma_commit_at(ET_BAR(s_full, n & 1));
+                umma_commit_at(ET_BAR(k_empty, n % C::kStages));
+                if (nxt.flags & kLast) umma_commit_at(ET_BAR(q_empty, qs));
+            }
+            __syncwarp();
+            return true;
         };
         ok = entry_wait(0);
-        if (ok) {
-            entry(0);
-            if (!(nxt.flags & kEnd)) {
-                ok = wait_operands(0);
-                if (ok) issue_qk(0);
-            }
-        }
+        if (ok && !(nxt.flags & kEnd)) ok = qk(0);
         while (ok && !(nxt.flags & kEnd)) {
             cur = nxt;
-            bool issued = false;
-            if constexpr (C::kOwnP) {
-                // the next block's Q K^T ahead of this one's P V: always within an item; of the next item if its operands are there already
-                bool ahead = !(cur.flags & kLast);
-                if (!ahead && mbar_poll_warp(&sh->block_full[(g + 1) % kBlockRing], ((g + 1) / kBlockRing) & 1u) &&
-                    !(sh->block[(g + 1) % kBlockRing].flags & kEnd))
-                    ahead = mbar_poll_warp(&sh->q_full[nq % C::kStages], (uint32_t)(nq / C::kStages) & 1u) &&
-                            mbar_poll_warp(&sh->k_full[(g + 1) % C::kStages], ((g + 1) / C::kStages) & 1u);
-                if (ahead) {
-                    ok = entry_wait(g + 1);
-                    if (!ok) break;
-                    entry(g + 1);
-                    ok = wait_operands(g + 1) && mbar_wait(&sh->s_free, g & 1);
-                    if (!ok) break;
-                    issue_qk(g + 1);
-                    issued = true;
-                }
+            if (C::kOPlaces > 1 && (cur.flags & kFirst)) place ^= 1;
+            // the next block's scores ahead of this one's P V: always within an item; of the next item if its operands are there already
+            bool ahead = !(cur.flags & kLast);
+            if (!ahead && mbar_poll_warp(&sh->block_full[(g + 1) % kBlockRing], ((g + 1) / kBlockRing) & 1u) && !(sh->block[(g + 1) % kBlockRing].flags & kEnd))
+                ahead = mbar_poll_warp(&sh->q_full[nq % C::kQStages], (uint32_t)(nq / C::kQStages) & 1u) &&
+                        mbar_poll_warp(&sh->k_full[(g + 1) % C::kStages], ((g + 1) / C::kStages) & 1u);
+            if (ahead) {
+                ok = entry_wait(g + 1) && qk(g + 1);
+                if (!ok) break;
             }
             // O += P V of block g
             const int vs = g % C::kStages;
-            ok = mbar_wait(&sh->v_full[vs], (g / C::kStages) & 1u);
+            ok = mbar_wait_at(ET_BAR(v_full, vs), (g / C::kStages) & 1u);
             if (!ok) break;
             const int keys = min(cur.left, kBK);
             if (keys & 15) {   // V rows behind the last key, up to the end of a step: cleared
                 const int end = (keys + 15) & ~15;
-                uint8_t* const v = sV + vs * C::kTile;
                 for (int i = lane; i < (end - keys) * 8 * C::kPanels; i += 32) {
                     const int row = keys + i / (8 * C::kPanels), c = i % (8 * C::kPanels);
-                    *reinterpret_cast<uint4*>(v + (c >> 3) * kPanel + row * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    sts128(smem_at + C::kVAt + (vs * C::kPanels + (c >> 3)) * C::kKPanel + row * 128 + (c & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
             }
-            ok = mbar_wait(&sh->p_full, g & 1);
+            ok = mbar_wait_at(ET_BAR(p_full, g & 1), (g >> 1) & 1u);
             if (!ok) break;
             tc_fence_after();
             if (elect_one()) {
-                const uint32_t va = smem_u32(sV + vs * C::kTile);
+                const uint32_t va = smem_at + C::kVAt + vs * C::kKTile;
                 const int n = (keys + 15) >> 4;
                 for (int ks = 0; ks < n; ++ks)   // P of keys 16ks .. 16ks + 15: 8 packed columns; V: panels of 64 features
-                    umma_f16_ts(tmem + C::kOCol, tmem + C::kPCol + (uint32_t)(ks * 8), make_smem_desc(va + ks * 2048, kPanel, 1024, 2), idesc_pv,
-                                (!(cur.flags & kFirst) || ks > 0) ? 1u : 0u);
-                umma_commit(&sh->pv_done);
-                umma_commit(&sh->v_empty[vs]);
+                    umma_f16_ts(tmem + C::kOCol + place * 64, tmem + C::kSCol + (g & 1) * kBK + (uint32_t)(ks * 8), make_smem_desc(va + ks * 2048, C::kKPanel, 1024, 2),
+                                idesc_pv, (!(cur.flags & kFirst) || ks > 0) ? 1u : 0u);
+                umma_commit_at(ET_BAR(pv_done, g & 1));
+                umma_commit_at(ET_BAR(v_empty, vs));
             }
             __syncwarp();
-            if (!issued) {
+            if (!ahead) {
                 ok = entry_wait(g + 1);
-                if (!ok) break;
-                entry(g + 1);
-                if (!(nxt.flags & kEnd)) {
-                    // the scores have been read: P comes after them. Where P lies in their place its P V must be over.
-                    ok = wait_operands(g + 1) && (C::kOwnP ? mbar_wait(&sh->s_free, g & 1) : mbar_wait(&sh->pv_done, g & 1));
-                    if (!ok) break;
-                    issue_qk(g + 1);
-                }
+                if (ok && !(nxt.flags & kEnd)) ok = qk(g + 1);
             }
             ++g;
         }
@@ -629,39 +600,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             const int t = tid - 32 * kHelpWarp;
             bool ok = true;
             for (uint32_t g = 0;; ++g) {
-                ok = mbar_wait(&sh->block_full[g % kBlockRing], (g / kBlockRing) & 1u);
+                ok = mbar_wait_at(ET_BAR(block_full, g % kBlockRing), (g / kBlockRing) & 1u);
                 if (!ok) break;
                 const Block b = sh->block[g % kBlockRing];
                 if (b.flags & kEnd) break;
                 const int m = g & 1;
-                ok = mbar_wait(&sh->m_empty[m], ((g >> 1) & 1u) ^ 1u);
+                ok = mbar_wait_at(ET_BAR(m_empty, m), ((g >> 1) & 1u) ^ 1u);
                 if (!ok) break;
                 const Item& it = sh->item[b.item];
-                if (docs) {
-                    if (b.flags & kPartial) {
-#pragma unroll
-                        for (int i = 0; i < kBK; i += 32 * kHelpWarps)
-                            sh->docs[m][i + t] = i + t < b.left ? r.k_docs[it.seq.k0 + b.j * kBK + i + t] : -1;
-                    }
-                }
+                if (b.flags & kMixed) sh->docs[m][t] = t < b.left ? r.k_docs[it.seq.k0 + b.j * kBK + t] : -1;
                 if constexpr (kBias == kTable) {
-                    // value n of copy s: the bias of the distance of key - query n + s - 127 within the block's corner distance
+                    // value n of copy s: the bias of a key n + s - 127 behind the first key's distance to the first query
                     const half* const row = r.table + (size_t)it.head * (2 * r.reach + 1) + r.reach;
                     const int corner = b.j * kBK - (it.seq.qpos0 + it.qi0) - 127;
-#pragma unroll 2
-                    for (int e = t; e < 8 * 32; e += 32 * kHelpWarps) {
-                        const int s = e >> 5, n = (e & 31) * 8;
-                        uint32_t w[4];
+                    float* const to = reinterpret_cast<float*>(sBias + m * kShiftBytes);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int d = corner + n + s + 2 * i;
-                            const half2 two = __halves2half2(row[max(-r.reach, min(r.reach, d))], row[max(-r.reach, min(r.reach, d + 1))]);
-                            w[i] = *reinterpret_cast<const uint32_t*>(&two);
-                        }
-                        *reinterpret_cast<uint4*>(sBias + m * kShiftBytes + s * kShiftPitch + n * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int i = 0; i < 4; ++i) {
+                        const int n = t + 64 * i;
+                        if (n >= kShiftPitch / 4) break;
+                        const float v = __half2float(row[max(-r.reach, min(r.reach, corner + n))]) * kRulesLog2e;
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            if (n >= s) to[s * (kShiftPitch / 4) + n - s] = v;
                     }
                 }
-                mbar_arrive(&sh->m_full[m]);
+                mbar_arrive_at(ET_BAR(m_full, m));
             }
             if (!ok && lane == 0) atomicExch(p.err, 23);
             __syncwarp();
@@ -671,19 +634,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         pdl_wait();
         const int row = warp * 32 + lane;
         const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-        const uint32_t s_addr = tmem + lane_base + C::kSCol, p_addr = tmem + lane_base + C::kPCol, o_addr = tmem + lane_base + C::kOCol;
         const bool wide = (r.out_pitch & 15) == 0 && (reinterpret_cast<uintptr_t>(r.out) & 31) == 0;
         uint32_t g = 0;
+        int place = 0;          // of the current item's O
         bool ok = true;
         int done_slot = -1;     // item whose P V is on its way and whose rows are still to be written
         float done_sum = 0.f;   // its row sum
-        auto release = [&](int slot) {
+        auto arrive = [&](uint32_t at) {
             __syncwarp();
-            if (elect_one()) mbar_arrive(&sh->item_empty[slot]);
+            if (elect_one()) mbar_arrive_at(at);
             __syncwarp();
         };
-        // O / row sum -> fp16 -> global, when the item's last P V has completed: inside the next item's first block, whose scores cover the wait.
-        auto finish = [&]() {
+        // O / row sum -> fp16 -> global, of the item whose last block is n - 1.
+        auto finish = [&](uint32_t n, int from) {
+            if (!mbar_wait_at(ET_BAR(pv_done, (n - 1) & 1), ((n - 1) >> 1) & 1u)) return false;
+            tc_fence_after();
             const Item& it = sh->item[done_slot];
             const float inv = done_sum > 0.f ? 1.f / done_sum : done_sum == 0.f ? 0.f : done_sum;   // (not a number stays so)
             const int qi = it.qi0 + row;
@@ -693,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
 #pragma unroll 1
             for (int c = 0; c < osteps; ++c) {
                 uint32_t o[16];
-                tmem_ld16(o_addr + c * 16, o);
+                tmem_ld16(tmem + lane_base + C::kOCol + from * 64 + c * 16, o);
                 tmem_ld_wait(o);
                 uint32_t ow[8];
 #pragma unroll
@@ -716,97 +681,85 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             const float largest = fmaxf(__low2float(top), __high2float(top)), sum = __low2float(top) + __high2float(top);
             unsigned again = __ballot_sync(0xffffffffu, in && !(largest <= 65504.f && sum == sum));
             for (; again; again &= again - 1) rules_row(r, it.seq, it.qi0 + warp * 32 + __ffs(again) - 1, it.head);
-            release(done_slot);
+            arrive(ET_BAR(item_empty, done_slot));
             done_slot = -1;
+            return true;
         };
         for (int ni = 0; ok; ++ni) {
             const int slot = ni % kItemRing;
-            ok = mbar_wait(&sh->item_full[slot], (uint32_t)(ni / kItemRing) & 1u);
+            ok = mbar_wait_at(ET_BAR(item_full, slot), (uint32_t)(ni / kItemRing) & 1u);
             if (!ok) break;
             const Item& it = sh->item[slot];
             const int state = it.state;
-            if (state <= 0) {
-                if (done_slot >= 0) {   // (the ring could run out of slots if an item waited behind empty ones)
-                    ok = mbar_wait(&sh->pv_done, (g - 1) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    finish();
-                }
-                if (state < 0) break;
-                const int qi = it.qi0 + row;   // no query sees a key: zeros
+            // The rows of the item before are written within this one's first block where O has a second place. (The ring could run out of slots if an item
+            // waited behind empty ones.)
+            if (done_slot >= 0 && (C::kOPlaces == 1 || state <= 0)) {
+                ok = finish(g, place);
+                if (!ok) break;
+            }
+            if (state < 0) break;
+            if (state == 0) {   // no query sees a key: zeros
+                const int qi = it.qi0 + row;
                 if (qi < it.seq.qlen) {
                     uint4* const z = reinterpret_cast<uint4*>(r.out + (it.seq.q0 + qi) * r.out_pitch + it.head * hd);
                     for (int i = 0; i < hd / 8; ++i) z[i] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                release(slot);
+                arrive(ET_BAR(item_empty, slot));
                 continue;
             }
+            if (C::kOPlaces > 1) place ^= 1;
+            const uint32_t o_addr = tmem + lane_base + C::kOCol + place * 64;
             const int qpos = it.seq.qpos0 + it.qi0 + row;
             const int prefix = it.seq.prefix;
             int my_doc = 0;
             if (docs) my_doc = it.qi0 + row < it.seq.qlen ? r.q_docs[it.seq.q0 + it.qi0 + row] : -1;
+            if (my_doc < 0) my_doc = -2;   // (keys behind the last one count as -1)
             float slope = 0.f;
             if constexpr (kBias == kSlopes) slope = r.slopes[it.head] * -kRulesLog2e;
             float m_run = -INFINITY;
             float2 l2 = make_float2(0.f, 0.f);
             bool last = false;
             for (; !last; ++g) {
-                ok = mbar_wait(&sh->s_full, g & 1);
+                const uint32_t s_addr = tmem + lane_base + C::kSCol + (g & 1) * kBK;
+                ok = mbar_wait_at(ET_BAR(s_full, g & 1), (g >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 const Block& b = sh->block[g % kBlockRing];
                 const int k0 = b.j * kBK, left = b.left, flags = b.flags;
-                const bool partial = flags & kPartial, first = flags & kFirst;
+                const bool first = flags & kFirst;
                 last = flags & kLast;
-                const int chunks = left > kBK / 2 ? 4 : 2;
                 const int m = g & 1;
-                if (help) {
-                    ok = mbar_wait(&sh->m_full[m], (g >> 1) & 1u);
-                    if (!ok) break;
+                float v[2][32];
+                tmem_ld32(s_addr, reinterpret_cast<uint32_t(&)[32]>(v[0]));
+                tmem_ld32(s_addr + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
+                tmem_ld_wait(v[0], v[1]);
+                if constexpr (kCap) {
+                    if (left < kBK) {   // four scores share a reciprocal: what lies behind the last key must not be not a number
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = i < left ? v[i >> 5][i & 31] : 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4) cap4(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1], v[i >> 5][(i & 31) + 2], v[i >> 5][(i & 31) + 3], r.cap_in, r.cap_out);
                 }
-                // the maximum, half a block at a time; scores that change go back to where they came from
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int c = 0; c < chunks; c += 2) {
-                    uint32_t seen[2] = {~0u, ~0u};
-                    if (partial) {
+                const float sc = kCap ? 1.f : r.scale_log2;
+                const float2 scale2 = make_float2(sc, sc);
+                if constexpr (kBias == kSlopes) {
+                    // On one side of the queries the bias is linear in the key; in the blocks around them it is not.
+                    const int near = k0 - qpos;
+                    const bool behind = k0 >= qpos, before = k0 + kBK - 1 <= qpos;
+                    if (__all_sync(0xffffffffu, behind) || __all_sync(0xffffffffu, before)) {
+                        const float signed_slope = behind ? slope : -slope, base = (float)near * signed_slope;
+                        const float2 slope2 = make_float2(signed_slope, signed_slope), base2 = make_float2(base, base);
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            const int at = k0 + (c + x) * 32;
-                            uint32_t w = r.window_left == kNoLimit ? ~0u : bits_from(qpos - r.window_left - at);
-                            if (r.window_right != kNoLimit) w &= ~bits_from(qpos + r.window_right + 1 - at);
-                            w |= ~bits_from(prefix - at);
-                            w &= ~bits_from(left - (c + x) * 32);
-                            if (docs) {
-                                uint32_t same = 0;
-                                const int4* const d = reinterpret_cast<const int4*>(sh->docs[m] + (c + x) * 32);
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) {
-                                    const int4 four = d[i];
-                                    same |= (four.x == my_doc ? 1u : 0u) << (4 * i) | (four.y == my_doc ? 2u : 0u) << (4 * i) | (four.z == my_doc ? 4u : 0u) << (4 * i) |
-                                            (four.w == my_doc ? 8u : 0u) << (4 * i);
-                                }
-                                w &= my_doc >= 0 ? same : 0u;
-                            }
-                            seen[x] = w;
+                        for (int i = 0; i < 64; i += 2) {
+                            const float2 bias = fma2(make_float2((float)i, (float)(i + 1)), slope2, base2);
+                            float2 x = make_float2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1]);
+                            x = kCap ? add2(x, bias) : fma2(x, scale2, bias);
+                            v[i >> 5][i & 31] = x.x;
+                            v[i >> 5][(i & 31) + 1] = x.y;
                         }
-                    }
-                    float v[2][32];
-                    tmem_ld32(s_addr + c * 32, reinterpret_cast<uint32_t(&)[32]>(v[0]));
-                    tmem_ld32(s_addr + c * 32 + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
-                    tmem_ld_wait(v[0], v[1]);
-                    if constexpr (kCap) {
-                        if (partial) {   // four scores share a reciprocal: what is not seen must not be not a number
-#pragma unroll
-                            for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = (seen[i >> 5] >> (i & 31)) & 1u ? v[i >> 5][i & 31] : 0.f;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 64; i += 4) cap4(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1], v[i >> 5][(i & 31) + 2], v[i >> 5][(i & 31) + 3], r.cap_in, r.cap_out);
-                    }
-                    const float sc = kCap ? 1.f : r.scale_log2;
-                    const float2 sc2 = make_float2(sc, sc);
-                    if constexpr (kBias == kSlopes) {
-                        const float base = (float)(k0 + c * 32 - qpos);
+                    } else {
+                        const float base = (float)near;
                         const float2 slope2 = make_float2(slope, slope);
 #pragma unroll
                         for (int i = 0; i < 64; i += 2) {
@@ -814,91 +767,98 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                             d.x = fabsf(d.x);
                             d.y = fabsf(d.y);
                             float2 x = make_float2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1]);
-                            if constexpr (!kCap) x = mul2(x, sc2);
+                            if constexpr (!kCap) x = mul2(x, scale2);
                             x = fma2(d, slope2, x);
                             v[i >> 5][i & 31] = x.x;
                             v[i >> 5][(i & 31) + 1] = x.y;
                         }
                     }
-                    if constexpr (kBias == kTable) {
-                        // row's first value is number 127 - row: eight values at a time from the copy in which they start on 16 bytes
-                        const int start = 127 - row;
-                        const uint8_t* const biases = sBias + m * kShiftBytes + (start & 7) * kShiftPitch + ((start & ~7) + c * 32) * 2;
-                        const float2 log2 = make_float2(kRulesLog2e, kRulesLog2e);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint4 eight = *reinterpret_cast<const uint4*>(biases + e * 16);
-                            const half2* const h = reinterpret_cast<const half2*>(&eight);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float& a = v[e >> 2][(e & 3) * 8 + 2 * i];
-                                float& bb = v[e >> 2][(e & 3) * 8 + 2 * i + 1];
-                                float2 x = make_float2(a, bb);
-                                if constexpr (!kCap) x = mul2(x, sc2);
-                                x = fma2(__half22float2(h[i]), log2, x);
-                                a = x.x;
-                                bb = x.y;
-                            }
-                        }
-                    }
-                    if (partial) {
-#pragma unroll
-                        for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = (seen[i >> 5] >> (i & 31)) & 1u ? v[i >> 5][i & 31] : -INFINITY;
-                    }
-                    if (kChanged || partial) {
-                        tmem_store32(s_addr + c * 32, v[0]);
-                        tmem_store32(s_addr + c * 32 + 32, v[1]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) mx[i & 3] = max3(mx[i & 3], v[i >> 4][2 * (i & 15)], v[i >> 4][2 * (i & 15) + 1]);
                 }
-                if (kChanged || partial) tmem_st_wait();
                 if (help) {
-                    __syncwarp();
-                    if (elect_one()) mbar_arrive(&sh->m_empty[m]);
-                    __syncwarp();
+                    ok = mbar_wait_at(ET_BAR(m_full, m), (g >> 1) & 1u);
+                    if (!ok) break;
                 }
-                const float sc = kChanged ? 1.f : r.scale_log2;
-                const float bmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sc;   // the scale is positive
+                if constexpr (kBias == kTable) {
+                    // the row's first value is number 127 - row: four at a time from the copy in which they start on 16 bytes
+                    const int start = 127 - row;
+                    const uint32_t biases = smem_u32(sBias) + m * kShiftBytes + (start & 3) * kShiftPitch + (start & ~3) * 4;
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4) {
+                        const uint4 four = lds128(biases + i * 4);
+                        float* const x = &v[i >> 5][i & 31];
+                        const float2 lo = make_float2(__uint_as_float(four.x), __uint_as_float(four.y)), hi = make_float2(__uint_as_float(four.z), __uint_as_float(four.w));
+                        float2 a = make_float2(x[0], x[1]), bb = make_float2(x[2], x[3]);
+                        a = kCap ? add2(a, lo) : fma2(a, scale2, lo);
+                        bb = kCap ? add2(bb, hi) : fma2(bb, scale2, hi);
+                        x[0] = a.x; x[1] = a.y; x[2] = bb.x; x[3] = bb.y;
+                    }
+                }
+                if (flags & kMixed) {
+                    const uint32_t ids = sh_at + (uint32_t)offsetof(TcShared, docs) + m * (kBK * 4);
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4) {
+                        const uint4 four = lds128(ids + i * 4);
+                        float* const x = &v[i >> 5][i & 31];
+                        x[0] = (int)four.x == my_doc ? x[0] : -INFINITY;
+                        x[1] = (int)four.y == my_doc ? x[1] : -INFINITY;
+                        x[2] = (int)four.z == my_doc ? x[2] : -INFINITY;
+                        x[3] = (int)four.w == my_doc ? x[3] : -INFINITY;
+                    }
+                }
+                if (help) arrive(ET_BAR(m_empty, m));
+                if (flags & kPartial) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int at = k0 + h * 32;
+                        uint32_t w = r.window_left == kNoLimit ? ~0u : bits_from(qpos - r.window_left - at);
+                        if (r.window_right != kNoLimit) w &= ~bits_from(qpos + r.window_right + 1 - at);
+                        w |= ~bits_from(prefix - at);
+                        w &= ~bits_from(left - h * 32);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[h][i] = (w >> i) & 1u ? v[h][i] : -INFINITY;
+                    }
+                }
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx[i & 3] = max3(mx[i & 3], v[i >> 4][2 * (i & 15)], v[i >> 4][2 * (i & 15) + 1]);
+                const float to_log2 = kChanged ? 1.f : r.scale_log2;
+                const float bmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * to_log2;   // the scale is positive
                 // The reference point moves only when the row maximum has grown by more than 2^8; the final division by the row sum makes the
                 // result independent of it.
                 const bool grow = bmax > m_run + kRescaleStep;   // also true for the first finite score of a row
-                const bool any = __any_sync(0xffffffffu, grow);
-                float alpha = 1.f;
-                if (grow) {
-                    alpha = m_run == -INFINITY ? 0.f : ex2_fast(m_run - bmax);
-                    m_run = bmax;
-                    l2.x *= alpha;
-                    l2.y *= alpha;
-                }
-                const float nshift = (m_run == -INFINITY) ? 0.f : -m_run;
-                const float2 sc2 = make_float2(sc, sc), sh2 = make_float2(nshift, nshift);
-                // P and O may be written once P V of the previous block has completed
-                if (g > 0) {
-                    ok = mbar_wait(&sh->pv_done, (g - 1) & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                }
-                if (first) {
-                    if (done_slot >= 0) finish();
-                } else if (any) {
+                if (__any_sync(0xffffffffu, grow)) {
+                    float alpha = 1.f;
+                    if (grow) {
+                        alpha = m_run == -INFINITY ? 0.f : ex2_fast(m_run - bmax);
+                        m_run = bmax;
+                        l2.x *= alpha;
+                        l2.y *= alpha;
+                    }
+                    if (!first) {   // O holds what the blocks before this one gave
+                        ok = mbar_wait_at(ET_BAR(pv_done, (g - 1) & 1), ((g - 1) >> 1) & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < osteps; ++c) {
-                        uint32_t o[16];
-                        tmem_ld16(o_addr + c * 16, o);
-                        tmem_ld_wait(o);
+                        for (int c = 0; c < osteps; ++c) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + c * 16, o);
+                            tmem_ld_wait(o);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_store16(o_addr + c * 16, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_store16(o_addr + c * 16, o);
+                        }
                     }
                 }
-                // exponentials of 32 scores, while the next 32 are fetched
-                auto chunk = [&](const float (&v)[32], int c) {
+                const float nshift = (m_run == -INFINITY) ? 0.f : -m_run;
+                const float2 to_log22 = make_float2(to_log2, to_log2), shift2 = make_float2(nshift, nshift);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
                     uint32_t pk[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float2 e = kChanged ? add2(make_float2(v[2 * i], v[2 * i + 1]), sh2) : fma2(make_float2(v[2 * i], v[2 * i + 1]), sc2, sh2);
-                        if ((i * kPolyPairs) / 16 != ((i + 1) * kPolyPairs) / 16) {   // spread over the chunk so that both pipes stay busy
+                        float2 e = make_float2(v[h][2 * i], v[h][2 * i + 1]);
+                        e = kChanged ? add2(e, shift2) : fma2(e, to_log22, shift2);
+                        if ((i * kPolyPairs) / 16 != ((i + 1) * kPolyPairs) / 16) {   // spread so that both pipes stay busy
                             e = exp2_cubic2(e);
                         } else {
                             e.x = ex2_fast(e.x);
@@ -907,36 +867,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                         l2 = add2(l2, e);
                         pk[i] = pack2(e.x, e.y);
                     }
-                    tmem_store16(p_addr + c * 16, pk);
-                };
-                {
-                    float v[32], w[32];
-                    tmem_ld32(s_addr, reinterpret_cast<uint32_t(&)[32]>(v));
-                    tmem_ld_wait(v);
-                    int c = 0;
-#pragma unroll 1
-                    for (;; c += 2) {
-                        tmem_ld32(s_addr + c * 32 + 32, reinterpret_cast<uint32_t(&)[32]>(w));
-                        chunk(v, c);
-                        tmem_ld_wait(w);
-                        if (c + 2 == chunks) break;
-                        tmem_ld32(s_addr + c * 32 + 64, reinterpret_cast<uint32_t(&)[32]>(v));
-                        chunk(w, c + 1);
-                        tmem_ld_wait(v);
-                    }
-                    if constexpr (C::kOwnP) {
-                        tc_fence_before();   // the next block's scores may be written
-                        __syncwarp();
-                        if (elect_one()) mbar_arrive(&sh->s_free);
-                        __syncwarp();
-                    }
-                    chunk(w, c + 1);
+                    tmem_store16(s_addr + h * 16, pk);   // where this block's first scores were: they have all been read
                 }
                 tmem_st_wait();
                 tc_fence_before();
-                __syncwarp();
-                if (elect_one()) mbar_arrive(&sh->p_full);
-                __syncwarp();
+                arrive(ET_BAR(p_full, g & 1));
+                if (C::kOPlaces > 1 && first && done_slot >= 0) {
+                    ok = finish(g, place ^ 1);
+                    if (!ok) break;
+                }
             }
             if (!ok) break;
             done_slot = slot;
@@ -945,13 +884,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         if (!ok && lane == 0) atomicExch(p.err, 22);
         __syncwarp();
     }
+#undef ET_BAR
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == kMmaWarp) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Lowest and highest document of every block of 128 keys of every sequence: a warp to a block.
+// Lowest and highest document of every block of keys of every sequence (the lowest with its sign set where some key is of none): a warp to a block.
 __global__ void __launch_bounds__(128) document_summary_kernel(const __grid_constant__ RuleParams p, int2* __restrict__ summary, int blocks) {
     pdl_launch_dependents();
     pdl_wait();
@@ -959,18 +899,21 @@ __global__ void __launch_bounds__(128) document_summary_kernel(const __grid_cons
     for (int b = blockIdx.y; b < p.batch; b += gridDim.y) {
         const RuleSeq s = rule_seq(p, b);
         if (j * kBK >= s.klen) continue;
-        int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+        int lo = 0x7fffffff, hi = -1;
+        bool none = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kBK / 32; ++i) {
             const int k = j * kBK + i * 32 + lane;
             if (k < s.klen) {
                 const int d = p.k_docs[s.k0 + k];
-                lo = min(lo, d);
+                if (d >= 0) lo = min(lo, d);
                 hi = max(hi, d);
+                none = none || d < 0;
             }
         }
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
+        if (__any_sync(0xffffffffu, none)) lo |= 0x80000000;   // never equal to the highest
         if (lane == 0) summary[(size_t)b * blocks + j] = make_int2(lo, hi);
     }
 }

@@ -75,4 +75,4 @@ def test_attention_of_nothing(lib):
 def test_attention_scratch_size(lib):
     import et_b200 as et
     assert et.attention_rules_scratch_size(0, 100) == 0 and et.attention_rules_scratch_size(3, 0) == 0
-    assert et.attention_rules_scratch_size(3, 129) == 3 * 2 * 8 and et.attention_rules_scratch_size(1 << 20, 1 << 20) == (1 << 20) * (1 << 13) * 8
+    assert et.attention_rules_scratch_size(3, 129) == 3 * 3 * 8 and et.attention_rules_scratch_size(1 << 20, 1 << 20) == (1 << 20) * (1 << 14) * 8

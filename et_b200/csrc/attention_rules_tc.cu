@@ -78,6 +78,7 @@ struct TcShared {
     uint64_t clc_full;
     uint64_t q_full[2], q_empty[2], k_full[4], k_empty[4], v_full[4], v_empty[4];
     uint64_t s_full[2], p_full[2], pv_done[2];   // by place of the scores
+    uint64_t v_ready[4];                  // V has landed and is cleared behind the last key
     uint64_t m_full[2], m_empty[2];       // what the helping warps bring of a block: documents of its keys, its biases
     uint64_t item_full[kItemRing], item_empty[kItemRing];
     uint64_t block_full[kBlockRing];
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             }
             for (int i = 0; i < C::kStages; ++i) {
                 mbar_init(&sh->k_full[i], 1); mbar_init(&sh->k_empty[i], 1);
-                mbar_init(&sh->v_full[i], 1); mbar_init(&sh->v_empty[i], 1);
+                mbar_init(&sh->v_full[i], 1); mbar_init(&sh->v_empty[i], 1); mbar_init(&sh->v_ready[i], kHelpWarps);
             }
             for (int i = 0; i < kItemRing; ++i) {
                 mbar_init(&sh->item_full[i], 1);
@@ -430,9 +431,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         auto load_q = [&](int head, int row) { return load(0, C::kQPanel, C::kQStages, &tmQ, head, row, offsetof(TcShared, q_full), offsetof(TcShared, q_empty), nq); };
         auto load_k = [&](int head, int row) { return load(C::kKAt, C::kKPanel, C::kStages, &tmK, head, row, offsetof(TcShared, k_full), offsetof(TcShared, k_empty), nk); };
         auto load_v = [&](int head, int row) { return load(C::kVAt, C::kKPanel, C::kStages, &tmV, head, row, offsetof(TcShared, v_full), offsetof(TcShared, v_empty), nv); };
-        // A block's entry may be overwritten kBlockRing blocks later: K of the block before that one has then been requested, so scores have been made
-        // kStages blocks before, for which the weights two blocks before those were in place: everyone has passed this block.
-        static_assert(C::kStages + 3 <= kBlockRing, "entries stay until everyone has read them");
+        // A block's entry may be overwritten kBlockRing blocks later: V of the block before that has then been requested, in a place that P V has
+        // left kStages blocks before, and before P V of a block everyone has passed it.
+        static_assert(C::kStages + 1 <= kBlockRing, "entries stay until everyone has read them");
         auto announce = [&](int j, int left, int flags, int slot) {
             if (lane == 0) {
                 Block& b = sh->block[g % kBlockRing];
@@ -508,102 +509,84 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         }
         __syncwarp();
     } else if (warp == kMmaWarp) {
-        // ---- UMMAs: the warp stays converged, one elected lane issues. Blocks are numbered through across items.
-        const int steps = hd >> 4;
-        const uint32_t idesc_qk = make_idesc_f16(128, kBK), idesc_pv = make_idesc_f16(128, hd, false, true);
-        int nq = 0, place = 0;        // Q tiles taken, place of the current item's O
-        uint32_t g = 0;
-        bool ok = true;
-        struct { int left, flags; } cur = {0, 0}, nxt = {0, 0};   // the block in work, and the one behind it
-        auto entry_wait = [&](uint32_t n) {
-            if (!mbar_wait_at(ET_BAR(block_full, n % kBlockRing), (n / kBlockRing) & 1u)) return false;
-            nxt.left = sh->block[n % kBlockRing].left;
-            nxt.flags = sh->block[n % kBlockRing].flags;
-            __syncwarp();
-            return true;
-        };
-        // S = Q K_n^T of the block whose entry is `nxt`; its place holds P of block n - 2 until P V of that is over
-        auto qk = [&](uint32_t n) {
-            if (nxt.flags & kFirst) {
-                if (!mbar_wait_at(ET_BAR(q_full, nq % C::kQStages), (uint32_t)(nq / C::kQStages) & 1u)) return false;
-                ++nq;
-            }
-            if (!mbar_wait_at(ET_BAR(k_full, n % C::kStages), (n / C::kStages) & 1u)) return false;
-            if (n >= 2 && !mbar_wait_at(ET_BAR(pv_done, n & 1), ((n - 2) >> 1) & 1u)) return false;
-            const int qs = (nq - 1) % C::kQStages;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t qa = smem_at + qs * C::kQTile, ka = smem_at + C::kKAt + (n % C::kStages) * C::kKTile;
-                for (int ks = 0; ks < steps; ++ks)
-                    umma_f16(tmem + C::kSCol + (n & 1) * kBK, make_smem_desc(qa + (ks >> 2) * C::kQPanel + (ks & 3) * 32, 16, 1024, 2),
-                             make_smem_desc(ka + (ks >> 2) * C::kKPanel + (ks & 3) * 32, 16, 1024, 2), idesc_qk, ks > 0);
-                umma_commit_at(ET_BAR(s_full, n & 1));
-                umma_commit_at(ET_BAR(k_empty, n % C::kStages));
-                if (nxt.flags & kLast) umma_commit_at(ET_BAR(q_empty, qs));
-            }
-            __syncwarp();
-            return true;
-        };
-        ok = entry_wait(0);
-        if (ok && !(nxt.flags & kEnd)) ok = qk(0);
-        while (ok && !(nxt.flags & kEnd)) {
-            cur = nxt;
-            if (C::kOPlaces > 1 && (cur.flags & kFirst)) place ^= 1;
-            // the next block's scores ahead of this one's P V: always within an item; of the next item if its operands are there already
-            bool ahead = !(cur.flags & kLast);
-            if (!ahead && mbar_poll_warp(&sh->block_full[(g + 1) % kBlockRing], ((g + 1) / kBlockRing) & 1u) && !(sh->block[(g + 1) % kBlockRing].flags & kEnd))
-                ahead = mbar_poll_warp(&sh->q_full[nq % C::kQStages], (uint32_t)(nq / C::kQStages) & 1u) &&
-                        mbar_poll_warp(&sh->k_full[(g + 1) % C::kStages], ((g + 1) / C::kStages) & 1u);
-            if (ahead) {
-                ok = entry_wait(g + 1) && qk(g + 1);
-                if (!ok) break;
-            }
-            // O += P V of block g
-            const int vs = g % C::kStages;
-            ok = mbar_wait_at(ET_BAR(v_full, vs), (g / C::kStages) & 1u);
-            if (!ok) break;
-            const int keys = min(cur.left, kBK);
-            if (keys & 15) {   // V rows behind the last key, up to the end of a step: cleared
-                const int end = (keys + 15) & ~15;
-                for (int i = lane; i < (end - keys) * 8 * C::kPanels; i += 32) {
-                    const int row = keys + i / (8 * C::kPanels), c = i % (8 * C::kPanels);
-                    sts128(smem_at + C::kVAt + (vs * C::kPanels + (c >> 3)) * C::kKPanel + row * 128 + (c & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+        // ---- UMMAs: one elected lane does everything, by 32-bit addresses. Blocks are numbered through across items. (As a converged warp that elects a lane for
+        // each batch, with descriptors made in the loop, this role took 1900 clocks a block and bounded the kernel: heads of 64, 4 x 4096 tokens 451 us.)
+        if (elect_one()) {
+            const int steps = hd >> 4;
+            const uint32_t idesc_qk = make_idesc_f16(128, kBK), idesc_pv = make_idesc_f16(128, hd, false, true);
+            const uint64_t q_desc = make_smem_desc(smem_at, 16, 1024, 2), k_desc = make_smem_desc(smem_at + C::kKAt, 16, 1024, 2);
+            const uint64_t v_desc = make_smem_desc(smem_at + C::kVAt, C::kKPanel, 1024, 2);
+            int qs = C::kQStages - 1, q_phase = 1;    // of the current item's Q
+            int place = 0;                            // of the current item's O
+            uint32_t g = 0;
+            int left = 0, flags = 0, next_left = 0, next_flags = 0;   // of the block in work, and of the one behind it
+            auto entry = [&](uint32_t n) {
+                if (!mbar_wait_at(ET_BAR(block_full, n % kBlockRing), (n / kBlockRing) & 1u)) return false;
+                next_left = sh->block[n % kBlockRing].left;
+                next_flags = sh->block[n % kBlockRing].flags;
+                return true;
+            };
+            // S = Q K_n^T of the block whose entry has been read last; its place holds P of block n - 2 until P V of that is over
+            auto qk = [&](uint32_t n) {
+                if (next_flags & kFirst) {
+                    qs = qs + 1 == C::kQStages ? 0 : qs + 1;
+                    if (qs == 0) q_phase ^= 1;
+                    if (!mbar_wait_at(ET_BAR(q_full, qs), q_phase)) return false;
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-            }
-            ok = mbar_wait_at(ET_BAR(p_full, g & 1), (g >> 1) & 1u);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-                const uint32_t va = smem_at + C::kVAt + vs * C::kKTile;
-                const int n = (keys + 15) >> 4;
-                for (int ks = 0; ks < n; ++ks)   // P of keys 16ks .. 16ks + 15: 8 packed columns; V: panels of 64 features
-                    umma_f16_ts(tmem + C::kOCol + place * 64, tmem + C::kSCol + (g & 1) * kBK + (uint32_t)(ks * 8), make_smem_desc(va + ks * 2048, C::kKPanel, 1024, 2),
-                                idesc_pv, (!(cur.flags & kFirst) || ks > 0) ? 1u : 0u);
+                const uint32_t ks0 = n % C::kStages;
+                if (!mbar_wait_at(ET_BAR(k_full, ks0), (n / C::kStages) & 1u)) return false;
+                if (n >= 2 && !mbar_wait_at(ET_BAR(pv_done, n & 1), ((n - 2) >> 1) & 1u)) return false;
+                tc_fence_after();
+                const uint64_t a = q_desc + qs * (C::kQTile >> 4), b = k_desc + ks0 * (C::kKTile >> 4);
+                const uint32_t to = tmem + C::kSCol + (n & 1) * kBK;
+#pragma unroll
+                for (int ks = 0; ks < kHD / 16; ++ks)
+                    if (ks < steps)
+                        umma_f16(to, a + ((ks >> 2) * C::kQPanel + (ks & 3) * 32) / 16, b + ((ks >> 2) * C::kKPanel + (ks & 3) * 32) / 16, idesc_qk, ks > 0);
+                umma_commit_at(ET_BAR(s_full, n & 1));
+                umma_commit_at(ET_BAR(k_empty, ks0));
+                if (next_flags & kLast) umma_commit_at(ET_BAR(q_empty, qs));
+                return true;
+            };
+            bool ok = entry(0) && ((next_flags & kEnd) || qk(0));
+            while (ok && !(next_flags & kEnd)) {
+                left = next_left;
+                flags = next_flags;
+                if (C::kOPlaces > 1 && (flags & kFirst)) place ^= 1;
+                // The next block's scores ahead of this one's P V; of the next item only where its Q has a place of its own (else it has just been requested).
+                const bool ahead = C::kQStages > 1 || !(flags & kLast);
+                if (ahead && !(ok = entry(g + 1) && ((next_flags & kEnd) || qk(g + 1)))) break;
+                // O += P V of block g
+                const uint32_t vs = g % C::kStages;
+                const int keys = min(left, kBK);
+                ok = mbar_wait_at(ET_BAR(v_ready, vs), (g / C::kStages) & 1u) && mbar_wait_at(ET_BAR(p_full, g & 1), (g >> 1) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t b = v_desc + vs * (C::kKTile >> 4);
+                const uint32_t a = tmem + C::kSCol + (g & 1) * kBK, to = tmem + C::kOCol + place * 64;
+#pragma unroll
+                for (int ks = 0; ks < kBK / 16; ++ks)   // P of keys 16ks .. 16ks + 15: 8 packed columns; V: panels of 64 features
+                    if (ks * 16 < keys) umma_f16_ts(to, a + ks * 8, b + ks * (2048 / 16), idesc_pv, (!(flags & kFirst) || ks > 0) ? 1u : 0u);
                 umma_commit_at(ET_BAR(pv_done, g & 1));
                 umma_commit_at(ET_BAR(v_empty, vs));
+                if (!ahead) ok = entry(g + 1) && ((next_flags & kEnd) || qk(g + 1));
+                ++g;
             }
-            __syncwarp();
-            if (!ahead) {
-                ok = entry_wait(g + 1);
-                if (ok && !(nxt.flags & kEnd)) ok = qk(g + 1);
-            }
-            ++g;
+            if (!ok) atomicExch(p.err, 21);
         }
-        if (!ok && lane == 0) atomicExch(p.err, 21);
         __syncwarp();
     } else if (warp >= kHelpWarp) {
-        // ---- what a block needs beside K and V: the documents of its keys, its biases by distance
-        if (help) {
-            pdl_wait();
-            const int t = tid - 32 * kHelpWarp;
-            bool ok = true;
-            for (uint32_t g = 0;; ++g) {
-                ok = mbar_wait_at(ET_BAR(block_full, g % kBlockRing), (g / kBlockRing) & 1u);
-                if (!ok) break;
-                const Block b = sh->block[g % kBlockRing];
-                if (b.flags & kEnd) break;
+        // ---- what a block needs beside K and V: the documents of its keys, its biases by distance; and V's rows behind the last key, up to the end of a
+        // 16-key step, are cleared (they may hold anything)
+        pdl_wait();
+        const int t = tid - 32 * kHelpWarp;
+        bool ok = true;
+        for (uint32_t g = 0;; ++g) {
+            ok = mbar_wait_at(ET_BAR(block_full, g % kBlockRing), (g / kBlockRing) & 1u);
+            if (!ok) break;
+            const Block b = sh->block[g % kBlockRing];
+            if (b.flags & kEnd) break;
+            if (help) {
                 const int m = g & 1;
                 ok = mbar_wait_at(ET_BAR(m_empty, m), ((g >> 1) & 1u) ^ 1u);
                 if (!ok) break;
@@ -626,9 +609,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 }
                 mbar_arrive_at(ET_BAR(m_full, m));
             }
-            if (!ok && lane == 0) atomicExch(p.err, 23);
+            const int vs = g % C::kStages;
+            ok = mbar_wait_at(ET_BAR(v_full, vs), (g / C::kStages) & 1u);
+            if (!ok) break;
+            const int keys = min(b.left, kBK);
+            if (keys & 15) {
+                const int end = (keys + 15) & ~15;
+                for (int i = t; i < (end - keys) * 8 * C::kPanels; i += 32 * kHelpWarps) {
+                    const int row = keys + i / (8 * C::kPanels), c = i % (8 * C::kPanels);
+                    sts128(smem_at + C::kVAt + (vs * C::kPanels + (c >> 3)) * C::kKPanel + row * 128 + (c & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+                }
+                fence_proxy_async_smem();
+            }
             __syncwarp();
+            if (elect_one()) mbar_arrive_at(ET_BAR(v_ready, vs));
         }
+        if (!ok && lane == 0) atomicExch(p.err, 23);
+        __syncwarp();
     } else {
         // ---- softmax: one thread per query row (TMEM lane)
         pdl_wait();

@@ -203,6 +203,7 @@ def run_attention(et, Q, K, V, hd, seqs, cu=None, k_start=None, k_lens=None, pre
     et.attention_rules(out, Q, K, V, hd, cu_seqlens=None if cu is None else dev(cu), k_start=None if k_start is None else dev(k_start), k_lens=None if k_lens is None else dev(k_lens),
                        batch=batch, max_q_len=max_q, max_k_len=max_k, scale=scale, cap=cap, slopes=slopes, distance_bias=table, window=window,
                        prefix_lens=None if prefixes is None else dev(prefixes), q_docs=docs[0] if docs else None, k_docs=docs[1] if docs else None, scratch=scratch)
+    et.attention_check()   # no wait has given up
     want, bound = ol.attention(Q, K, V, hd, seqs, scale=scale or None, cap=cap, slopes=slopes, table=table, window=window, prefixes=prefixes,
                                q_docs=docs[0] if docs else None, k_docs=docs[1] if docs else None)
     ol.assert_within(out, want, bound, "attention")
@@ -258,6 +259,17 @@ def test_attention_of_whole_sequences(et, hq, hk, hd, lengths, rule):
     args = rules_of(rule, lengths, hq)
     Q, K, V, cu, seqs = packed(1, lengths, hq, hk, hd, std=3.0 if args["cap"] else 1.0)
     run_attention(et, Q, K, V, hd, seqs, cu=cu, **args)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch,longest", [(48, 701), (128, 150), (300, 90)])
+@pytest.mark.parametrize("rule", ["plain", "window", "documents", "cap table documents", "all"])
+def test_attention_of_ragged_batches_of_several_waves(et, batch, longest, rule, hd):
+    """CTAs take over many short items, each with a last block of its own size, in order of length (up to 128 sequences) or as they come."""
+    r = np.random.default_rng(batch)
+    lengths = [int(n) for n in r.integers(0, longest + 1, batch)]
+    Q, K, V, cu, seqs = packed(5, lengths, 12, 4, hd)
+    run_attention(et, Q, K, V, hd, seqs, cu=cu, **rules_of(rule, lengths, 12))
 
 
 @pytest.mark.parametrize("hq,hk,hd", [(3, 1, 16), (2, 2, 32), (6, 3, 48), (4, 1, 80), (2, 1, 96), (5, 5, 112), (2, 2, 20), (3, 1, 7), (2, 1, 192), (4, 2, 256)])

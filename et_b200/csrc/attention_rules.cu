@@ -85,7 +85,7 @@ extern "C" int et_attention_rules(void* out, const void* Q, const void* K, const
     p.window_right = r.window_right < 0 || r.window_right >= kNoLimit ? kNoLimit : r.window_right;
     p.prefix_lens = r.prefix_lens; p.q_docs = r.q_docs; p.k_docs = r.k_docs;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (attention_rules_token_takes(p)) return cuda_status(attention_rules_token_launch(p, st), "et_attention_rules launch");
+    if (attention_rules_token_takes(p)) return attention_rules_token_launch(p, st);
     if (attention_rules_tc_takes(p)) return attention_rules_tc_launch(p, p.k_docs ? scratch : nullptr, st);
     return cuda_status(attention_rules_rows_launch(p, st), "et_attention_rules launch");
 }

@@ -293,24 +293,21 @@ def _refuse(name, t, dtype, dims, device):
 
 def _rows(name, t, dtype, device):
     """(rows, features, pitch) of a matrix that may be a slice of a wider one."""
-    if t.dtype is not dtype or t.get_device() != device or t.dim() != 2:
-        _refuse(name, t, dtype, 2, device)
-    rows, features = t.shape
-    pitch, step = t.stride()
-    if step != 1 and features > 1:
-        _refuse(name, t, dtype, 2, device)
-    return rows, features, pitch if rows > 1 else features
+    if t.dtype is dtype and t.get_device() == device and t.dim() == 2:
+        rows, features = t.shape
+        pitch, step = t.stride()
+        if step == 1 or features == 1:
+            return rows, features, pitch if rows > 1 else features
+    _refuse(name, t, dtype, 2, device)
 
 
 def _array(name, t, dtype, device, n):
-    """Address of a contiguous array of n elements, or None."""
-    if t is None:
-        return None
-    if t.dtype is not dtype or t.get_device() != device or t.dim() != 1 or not t.is_contiguous():
-        _refuse(name, t, dtype, 1, device)
-    if t.shape[0] != n:
-        raise ValueError(f"{name}: {n} elements expected, not {t.shape[0]}")
-    return t.data_ptr()
+    """Address of a contiguous array of n elements."""
+    if t.dtype is dtype and t.get_device() == device and t.dim() == 1 and t.is_contiguous():
+        if t.numel() == n:
+            return t.data_ptr()
+        raise ValueError(f"{name}: {n} elements expected, not {t.numel()}")
+    _refuse(name, t, dtype, 1, device)
 
 
 def _matrix(name, t, dtype, device):
@@ -376,7 +373,7 @@ class AdapterBank:
             raise ValueError(f"x [{rows}, {self.in_feat}], base and out [{rows}, {self.out_feat}] expected, not {tuple(x.shape)}, {tuple(base.shape)}, {tuple(out.shape)}")
         batch = adapter_ids.shape[0]
         rc = (_entries or _lib()).et_adapter_add(self._h, out.data_ptr(), base.data_ptr(), x.data_ptr(), out_pitch, base_pitch, x_pitch,
-                                                 _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), _array("adapter_ids", adapter_ids, i32, device, batch),
+                                                 None if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), _array("adapter_ids", adapter_ids, i32, device, batch),
                                                  batch, rows, raw_stream(stream))
         if rc:
             check(rc)
@@ -419,7 +416,7 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
     if out_rows != tokens or out_width != width or v_rows != k_rows or v_width != kv_width or width % head_dim or kv_width % head_dim or not kv_width or not width:
         raise ValueError(f"whole heads of {head_dim}, out like Q and V like K expected, not {tuple(Q.shape)}, {tuple(out.shape)}, {tuple(K.shape)}, {tuple(V.shape)}")
     nhead, nhead_kv = width // head_dim, kv_width // head_dim
-    reach, table = 0, None
+    reach = table = 0
     if distance_bias is not None:
         heads, places = _matrix("distance_bias", distance_bias, f16, device)
         if heads != nhead or places % 2 == 0:
@@ -430,12 +427,14 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
         scratch_bytes = scratch.numel() * scratch.element_size()
         if scratch.get_device() != device or not scratch.is_contiguous():
             raise ValueError("scratch must be contiguous, on the current CUDA device")
-    rules = _score_rules(scale, cap, _array("slopes", slopes, f32, device, nhead) or 0, table or 0, reach, *window, _array("prefix_lens", prefix_lens, i32, device, batch) or 0,
-                         _array("q_docs", q_docs, i32, device, tokens) or 0, _array("k_docs", k_docs, i32, device, k_rows) or 0)
+    rules = _score_rules(scale, cap, 0 if slopes is None else _array("slopes", slopes, f32, device, nhead), table, reach, window[0], window[1],
+                         0 if prefix_lens is None else _array("prefix_lens", prefix_lens, i32, device, batch),
+                         0 if q_docs is None else _array("q_docs", q_docs, i32, device, tokens), 0 if k_docs is None else _array("k_docs", k_docs, i32, device, k_rows))
     rc = (_entries or _lib()).et_attention_rules(
         out.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), out_pitch, q_pitch, k_pitch, v_pitch, nhead, nhead_kv, head_dim,
-        _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), _array("k_start", k_start, i32, device, batch), _array("k_lens", k_lens, i32, device, batch), batch, tokens,
-        k_rows, max_q_len or tokens, max_k_len or k_rows, rules, _a(scratch), scratch_bytes, raw_stream(stream))
+        None if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), None if k_start is None else _array("k_start", k_start, i32, device, batch),
+        None if k_lens is None else _array("k_lens", k_lens, i32, device, batch), batch, tokens, k_rows, max_q_len or tokens, max_k_len or k_rows, rules,
+        None if scratch is None else scratch.data_ptr(), scratch_bytes, raw_stream(stream))
     if rc:
         check(rc)
     return out

@@ -2,30 +2,32 @@
 //
 // A bank holds the adapters of one projection in the order in which the tensor cores take them, so that a warp loads its fragments of
 // A and B with 16 bytes a lane, side by side, and needs no shared memory for them: they come from L1 and L2, where a bank stays.
-// One launch does both products. 16 or 32 tokens of one sequence are kWk warps' work: each takes a share of the K range for A x, the
-// shares are added in shared memory, and each takes a share of the output columns for B (A x), which go straight into base's granules.
-// Where there are few tokens a cluster of CTAs takes the place of one: its CTAs split K and the columns once more and add the
-// shares through distributed shared memory.
+// One launch does both products. 16 or 32 tokens of one sequence are a CTA's work: its eight warps each take a share of the K range for A x, the
+// shares are added in shared memory, and each takes a share of the output columns for B (A x). Where there are many tokens base and out move by TMA, 64
+// columns at a time through a ring of each warp; where there are few, CTAs share a tile's columns, each with all of A x.
 //
 // Sums are fp32. A x is rounded to fp16 between the products, as the second one needs it, each row scaled by a power of two so that its
 // largest value lies in [1, 2): it can not overflow, and the rounding (2^-11 of a term of the delta) is that of the result's own type.
 // Both products' fragments are permuted so that a lane has eight neighbouring elements of X, of base and of the result: the sum over k
 // does not depend on the order of k, and which column a lane of the second product computes is free.
 //
-// What bounds it: HBM. X is read once, base read and out written once; two operations a byte and rank, far below what mma.sync delivers.
-#include <cooperative_groups.h>
+// What bounds it: X is read once, base read and out written once; two operations a byte and rank, far below what mma.sync delivers. 32 prompts of 18 thousand
+// tokens, 1024 -> 4096, rank 32: 88 us, 61 at copy bandwidth (a plain copy of base in tiles of 32 rows takes 55); the rest is the weights, which every
+// tile of 32 tokens reads again (195 MB beside 340, from L2: rings of two stages, which leave them more of L1, gain 6 us over three), and the start of a
+// tile. 64 single tokens 4.0 us. Tried: clusters of 2, 4, 8 CTAs that share a tile's K range and columns through distributed shared memory (103, 131, 235 us;
+// single tokens 5.0, 5.3, 7.3), tiles of 64 tokens (103), CTAs that share the columns where there are many tokens (91).
 #include <new>
 #include <vector>
+#include "attention.h"
 #include "common.h"
-
-namespace cg = cooperative_groups;
+#include "ptx.cuh"
+#include "tmap.h"
 
 namespace et {
 namespace {
 
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kMaxRank = 128;
-constexpr int kMaxCluster = 8;
 
 struct Slot {
     int rank;      // 0: nothing to add
@@ -42,6 +44,8 @@ struct AdapterParams {
     const half *a, *b;                  // packed, all slots
     long long out_pitch, base_pitch, x_pitch, a_stride, b_stride;   // of a slot, in elements
     int batch, tokens, n_slots, in_feat, out_feat;
+    int n_split;                        // CTAs that share a tile's columns, each with all of A x
+    int* err;                           // of bounded waits
     bool copy;                          // out is not base: what has no adapter is copied
 };
 
@@ -55,7 +59,41 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The tile of kTile tokens that CTA or cluster `tile` has: sequence, first token, tokens (whole warp). Without cu_seqlens a sequence is one token.
+// 16 rows and 32 columns of B (A x): the lane's columns 8t .. 8t + 7 of rows g (elements 0 and 1 of each fragment) and g + 8 (2 and 3).
+template <int kRt>
+__device__ __forceinline__ void product(float (&d)[4][4], const uint32_t (&h)[kRt][4], const uint4 (&w)[kRt][2]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[j][i] = 0.f;
+#pragma unroll
+    for (int q = 0; q < kRt; ++q) {
+        mma_16816(d[0], h[q][0], h[q][1], h[q][2], h[q][3], w[q][0].x, w[q][0].y);
+        mma_16816(d[1], h[q][0], h[q][1], h[q][2], h[q][3], w[q][0].z, w[q][0].w);
+        mma_16816(d[2], h[q][0], h[q][1], h[q][2], h[q][3], w[q][1].x, w[q][1].y);
+        mma_16816(d[3], h[q][0], h[q][1], h[q][2], h[q][3], w[q][1].z, w[q][1].w);
+    }
+}
+// Adds it to eight elements of base; i: which of the two rows.
+__device__ __forceinline__ void add_to(uint4& old, const float (&d)[4][4], int i, float factor) {
+    half2* const o = reinterpret_cast<half2*>(&old);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 v = __half22float2(o[j]);
+        o[j] = __floats2half2_rn(fmaf(factor, d[j][2 * i], v.x), fmaf(factor, d[j][2 * i + 1], v.y));
+    }
+}
+
+// Where base passes through, by warps.
+template <int kMt>
+struct Ring {
+    static constexpr int kStage = kMt * 16 * 128;          // 64 columns of a tile's rows, 128-byte swizzle
+    static constexpr int kStages = 2;
+    static constexpr int kBarAt = kWarps * kStages * kStage;
+    static constexpr int kBytes = kBarAt + kWarps * kStages * 8 + 1024;
+};
+
+// The tile of kTile tokens with number `tile`: sequence, first token, tokens (whole warp). Without cu_seqlens a sequence is one token.
 template <int kTile>
 __device__ __forceinline__ int find_tile(const AdapterParams& p, int tile, int& seq, int& t0) {
     const int lane = threadIdx.x & 31;
@@ -88,40 +126,39 @@ __device__ __forceinline__ int find_tile(const AdapterParams& p, int tile, int& 
     return 0;
 }
 
-// kRt: 16-wide steps of the bank's largest rank; kMt: 16-token tiles of a warp; kWk: warps that share them.
-template <int kRt, int kMt, int kWk, bool kCluster>
-__global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant__ AdapterParams p) {
-    constexpr int kWm = kWarps / kWk, kTile = kWm * kMt * 16;
+// kRt: 16-wide steps of the bank's largest rank; kMt: 16-token tiles of a CTA. kTma: base and out move by TMA, 64 columns of a
+// tile at a time, through a ring of each warp; only a tile that ends inside a sequence's last rows is written row by row.
+template <int kRt, int kMt, bool kTma>
+__global__ void __launch_bounds__(kThreads, kTma && kRt <= 4 ? 2 : 1) adapter_kernel(const __grid_constant__ AdapterParams p, const __grid_constant__ CUtensorMap tm_base,
+                                                           const __grid_constant__ CUtensorMap tm_out) {
+    constexpr int kTile = kMt * 16;
     constexpr int kFrags = kMt * kRt * 2;                  // accumulator fragments of a warp
-    extern __shared__ float4 parts[];                      // [kWarps][kFrags][32]: shares of A x, as accumulator fragments; then their sums
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp / kWk, wk = warp % kWk;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = kTma ? (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) : smem_raw;
+    float4* const parts = reinterpret_cast<float4*>(smem);   // [kWarps][kFrags][32]: shares of A x, as accumulator fragments; then their sums
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
-    unsigned crank = 0, csize = 1;
-    if constexpr (kCluster) {
-        crank = cg::this_cluster().block_rank();
-        csize = cg::this_cluster().num_blocks();
-    }
     pdl_launch_dependents();
     pdl_wait();
     int seq = 0, t0 = 0;
-    const int rows_in_tile = find_tile<kTile>(p, blockIdx.x / csize, seq, t0);
-    if (rows_in_tile <= 0) return;   // the same for the whole cluster
+    const int rows_in_tile = find_tile<kTile>(p, blockIdx.x / p.n_split, seq, t0);
+    if (rows_in_tile <= 0) return;
     const int id = p.ids[seq];
     Slot slot = {0, 0.f};
     if (id >= 0 && id < p.n_slots) slot = p.slots[id];
-    const int part = crank * kWk + wk, n_parts = csize * kWk;   // this warp's share of K and of the columns
-    const int col_groups = (p.out_feat + 31) / 32;
+    const int all_groups = (p.out_feat + 31) / 32, split = blockIdx.x % p.n_split;
+    const int first_group = split * all_groups / p.n_split, col_groups = (split + 1) * all_groups / p.n_split;
     int row[kMt][2];        // the lane's rows, -1 beyond the tile
 #pragma unroll
     for (int m = 0; m < kMt; ++m)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const int r = (wm * kMt + m) * 16 + h * 8 + g;
+            const int r = m * 16 + h * 8 + g;
             row[m][h] = r < rows_in_tile ? t0 + r : -1;
         }
     if (slot.rank == 0) {
         if (!p.copy) return;
-        for (int c = part; c < col_groups; c += n_parts) {
+        for (int c = first_group + warp; c < col_groups; c += kWarps) {
             const int col = c * 32 + t * 8;
             if (col >= p.out_feat) continue;
 #pragma unroll
@@ -143,12 +180,12 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
             for (int i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
     const int chunks = (p.in_feat + 31) / 32;
     const uint4* const a = reinterpret_cast<const uint4*>(p.a + id * p.a_stride);
-    constexpr int kUnroll = kMt == 1 ? 4 : 2;
-    for (int c0 = part; c0 < chunks; c0 += n_parts * kUnroll) {
+    constexpr int kUnroll = kMt == 1 ? 4 : kMt == 2 ? 2 : 1;
+    for (int c0 = warp; c0 < chunks; c0 += kWarps * kUnroll) {
         uint4 xv[kUnroll][kMt][2];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int k = (c0 + u * n_parts) * 32 + t * 8;
+            const int k = (c0 + u * kWarps) * 32 + t * 8;
 #pragma unroll
             for (int m = 0; m < kMt; ++m)
 #pragma unroll
@@ -159,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int c = c0 + u * n_parts;
+            const int c = c0 + u * kWarps;
             if (c >= chunks) break;
 #pragma unroll
             for (int j = 0; j < kRt * 2; ++j) {
@@ -172,49 +209,47 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
             }
         }
     }
-    // ---- the shares are added, in the order of the warps, then of the CTAs: each thread adds a few places of all of them, so that what another CTA
-    // holds crosses to this one once
-    float4* const sums = parts + kWarps * kFrags * 32;     // [kWm][kFrags][32]: of this CTA's warps
-    float4* const all = sums + kWm * kFrags * 32;          // of all CTAs
+    const uint4* const b = reinterpret_cast<const uint4*>(p.b + id * p.b_stride);
+    uint4 old_next[kMt][2], w_next[kRt][2];
+    auto request = [&](int c) {
+        if (c >= col_groups) return;
+        const int col = c * 32 + t * 8;
+#pragma unroll
+        for (int m = 0; m < kMt; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (col < p.out_feat && row[m][i] >= 0) old_next[m][i] = *reinterpret_cast<const uint4*>(p.base + row[m][i] * p.base_pitch + col);
+#pragma unroll
+        for (int q = 0; q < kRt; ++q) {
+            const uint4* const w = b + (((size_t)c * kRt + q) * 32 + lane) * 2;
+            w_next[q][0] = __ldg(w);
+            w_next[q][1] = __ldg(w + 1);
+        }
+    };
+    if constexpr (!kTma) request(first_group + warp);   // before the shares are exchanged
+    // ---- the shares are added, in the order of the warps: each thread adds a few places of all of them
+    float4* const sums = parts + kWarps * kFrags * 32;     // [kFrags][32]
 #pragma unroll
     for (int m = 0; m < kMt; ++m)
 #pragma unroll
         for (int j = 0; j < kRt * 2; ++j)
             parts[(warp * kFrags + m * kRt * 2 + j) * 32 + lane] = make_float4(acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]);
     __syncthreads();
-    for (int e = threadIdx.x; e < kWm * kFrags * 32; e += kThreads) {
-        const int group = e / (kFrags * 32), at = e % (kFrags * 32);
-        float4 s = parts[group * kWk * kFrags * 32 + at];
+    for (int e = threadIdx.x; e < kFrags * 32; e += kThreads) {
+        float4 s = parts[e];
 #pragma unroll
-        for (int w = 1; w < kWk; ++w) {
-            const float4 v = parts[(group * kWk + w) * kFrags * 32 + at];
+        for (int w = 1; w < kWarps; ++w) {
+            const float4 v = parts[w * kFrags * 32 + e];
             s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
         }
         sums[e] = s;
     }
-    if constexpr (kCluster) {
-        cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
-        for (int e = threadIdx.x; e < kWm * kFrags * 32; e += kThreads) {
-            float4 v[kMaxCluster];
-#pragma unroll
-            for (int c = 0; c < kMaxCluster; ++c)
-                if (c < (int)csize) v[c] = cluster.map_shared_rank(sums, c)[e];
-            float4 s = v[0];
-#pragma unroll
-            for (int c = 1; c < kMaxCluster; ++c)
-                if (c < (int)csize) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
-            all[e] = s;
-        }
-        cluster.sync();   // nobody leaves while its shares are read
-    } else {
-        __syncthreads();
-    }
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < kMt; ++m)
 #pragma unroll
         for (int j = 0; j < kRt * 2; ++j) {
-            const float4 v = (kCluster ? all : sums)[(wm * kFrags + m * kRt * 2 + j) * 32 + lane];
+            const float4 v = sums[(m * kRt * 2 + j) * 32 + lane];
             acc[m][j][0] = v.x; acc[m][j][1] = v.y; acc[m][j][2] = v.z; acc[m][j][3] = v.w;
         }
     // ---- to fp16, each row by a power of two of its own; ranks that only pad a step are zeros even where x is not finite
@@ -254,86 +289,142 @@ __global__ void __launch_bounds__(kThreads) adapter_kernel(const __grid_constant
             h[m][q][3] = pack_h2(acc[m][2 * q + 1][2] * down[1], acc[m][2 * q + 1][3] * down[1]);
         }
     }
-    // ---- base + B (A x): groups of 32 columns, of which a lane has eight neighbouring ones in each of its rows
-    const uint4* const b = reinterpret_cast<const uint4*>(p.b + id * p.b_stride);
-#pragma unroll 2
-    for (int c = part; c < col_groups; c += n_parts) {
-        const int col = c * 32 + t * 8;
-        const bool in = col < p.out_feat;
-        uint4 old[kMt][2];
+    if constexpr (kTma) {
+        // ---- base + B (A x): units of 64 columns. A unit's base lands in a stage, is added to there and leaves from there.
+        using R = Ring<kMt>;
+        const uint32_t ring = smem_u32(smem) + warp * R::kStages * R::kStage, bars = smem_u32(smem) + R::kBarAt + warp * R::kStages * 8;
+        if (lane == 0) {
+            for (int i = 0; i < R::kStages; ++i) mbar_init(reinterpret_cast<uint64_t*>(smem + R::kBarAt) + warp * R::kStages + i, 1);
+            fence_mbar_init();
+            fence_proxy_async_smem();
+        }
+        __syncthreads();   // everyone has read the sums, which lie where the rings are
+        const int first_unit = split * ((p.out_feat + 63) / 64) / p.n_split, units = (split + 1) * ((p.out_feat + 63) / 64) / p.n_split;
+        const bool whole = rows_in_tile == kTile;
+        auto fetch = [&](int u, int stage) {
+            if (lane == 0 && u < units) {
+                mbar_expect_tx_at(bars + stage * 8, R::kStage);
+                tma_load_2d_at(ring + stage * R::kStage, &tm_base, u * 64, t0, bars + stage * 8);
+            }
+        };
 #pragma unroll
-        for (int m = 0; m < kMt; ++m)
+        for (int i = 0; i < R::kStages - 1; ++i) fetch(first_unit + warp + i * kWarps, i);
+        auto weights = [&](uint4 (&w)[kRt][2], int c) {
+            if (c >= all_groups) return;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (in && row[m][i] >= 0) old[m][i] = *reinterpret_cast<const uint4*>(p.base + row[m][i] * p.base_pitch + col);
-        float d[kMt][4][4];
+            for (int q = 0; q < kRt; ++q) {
+                const uint4* const from = b + (((size_t)c * kRt + q) * 32 + lane) * 2;
+                w[q][0] = __ldg(from);
+                w[q][1] = __ldg(from + 1);
+            }
+        };
+        uint4 w[2][kRt][2];
+        weights(w[0], (first_unit + warp) * 2);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int u = first_unit + warp; u < units; u += kWarps) {
+            weights(w[1], u * 2 + 1);
+            ok = mbar_wait_at(bars + stage * 8, phase);
+            if (!ok) break;
+            const uint32_t at = ring + stage * R::kStage;
 #pragma unroll
-        for (int m = 0; m < kMt; ++m)
+            for (int x = 0; x < 2; ++x) {
+                if (u * 2 + x >= all_groups) break;
+                const int col = u * 64 + x * 32 + t * 8;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+                for (int m = 0; m < kMt; ++m) {
+                    float d[4][4];
+                    product(d, h[m], w[x]);
+                    if (x == 0 && m == kMt - 1) weights(w[0], (u + kWarps) * 2);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[m][j][i] = 0.f;
-#pragma unroll
-        for (int q = 0; q < kRt; ++q) {
-            const uint4* const w = b + (((size_t)c * kRt + q) * 32 + lane) * 2;
-            const uint4 w0 = __ldg(w), w1 = __ldg(w + 1);
-#pragma unroll
-            for (int m = 0; m < kMt; ++m) {
-                mma_16816(d[m][0], h[m][q][0], h[m][q][1], h[m][q][2], h[m][q][3], w0.x, w0.y);
-                mma_16816(d[m][1], h[m][q][0], h[m][q][1], h[m][q][2], h[m][q][3], w0.z, w0.w);
-                mma_16816(d[m][2], h[m][q][0], h[m][q][1], h[m][q][2], h[m][q][3], w1.x, w1.y);
-                mma_16816(d[m][3], h[m][q][0], h[m][q][1], h[m][q][2], h[m][q][3], w1.z, w1.w);
+                    for (int i = 0; i < 2; ++i) {
+                        const int r = m * 16 + i * 8 + g;
+                        const uint32_t place = at + r * 128 + (((x * 4 + t) ^ (r & 7)) << 4);
+                        uint4 old = lds128(place);
+                        add_to(old, d, i, factor[m][i]);
+                        if (whole) sts128(place, old);
+                        else if (col < p.out_feat && row[m][i] >= 0) *reinterpret_cast<uint4*>(p.out + row[m][i] * p.out_pitch + col) = old;
+                    }
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (whole) tma_store_2d_at(&tm_out, at, u * 64, t0);
+                tma_store_commit();
+                tma_store_wait_read_but_one();   // the unit before this one has left its stage
+            }
+            fetch(u + (R::kStages - 1) * kWarps, stage == 0 ? R::kStages - 1 : stage - 1);
+            if (++stage == R::kStages) {
+                stage = 0;
+                phase ^= 1u;
             }
         }
+        if (lane == 0) tma_store_wait();
+        if (!ok) {   // (copies on their way land before the CTA leaves; bounded)
+            if (lane == 0) atomicExch(p.err, 51);
+            for (int i = 0; i < R::kStages; ++i) mbar_wait_at(bars + i * 8, i < stage ? phase ^ 1u : phase);
+        }
+    } else
+    // ---- base + B (A x): groups of 32 columns, of which a lane has eight neighbouring ones in each of its rows
+    for (int c = first_group + warp; c < col_groups; c += kWarps) {
+        const int col = c * 32 + t * 8;
+        uint4 old[kMt][2], w[kRt][2];
 #pragma unroll
-        for (int m = 0; m < kMt; ++m)
+        for (int q = 0; q < kRt; ++q) {
+            w[q][0] = w_next[q][0];
+            w[q][1] = w_next[q][1];
+        }
+#pragma unroll
+        for (int m = 0; m < kMt; ++m) {
+            old[m][0] = old_next[m][0];
+            old[m][1] = old_next[m][1];
+        }
+        request(c + kWarps);
+#pragma unroll
+        for (int m = 0; m < kMt; ++m) {
+            float d[4][4];
+            product(d, h[m], w);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (!in || row[m][i] < 0) continue;
-                half2* const o = reinterpret_cast<half2*>(&old[m][i]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 v = __half22float2(o[j]);
-                    o[j] = __floats2half2_rn(fmaf(factor[m][i], d[m][j][2 * i], v.x), fmaf(factor[m][i], d[m][j][2 * i + 1], v.y));
-                }
+                if (col >= p.out_feat || row[m][i] < 0) continue;
+                add_to(old[m][i], d, i, factor[m][i]);
                 *reinterpret_cast<uint4*>(p.out + row[m][i] * p.out_pitch + col) = old[m][i];
             }
+        }
     }
 }
 
-template <int kRt, int kMt, int kWk, bool kCluster>
-cudaError_t launch(const AdapterParams& p, int tiles, int csize, cudaStream_t st) {
-    const size_t smem = (size_t)(kWarps + kWarps / kWk * (kCluster ? 2 : 1)) * kMt * kRt * 2 * 32 * sizeof(float4);
-    const auto kernel = adapter_kernel<kRt, kMt, kWk, kCluster>;
+template <int kRt, int kMt, bool kTma>
+cudaError_t launch(const AdapterParams& p, const CUtensorMap& tm_base, const CUtensorMap& tm_out, long long tiles, cudaStream_t st) {
+    constexpr size_t sums = (size_t)(kWarps + 1) * kMt * kRt * 2 * 32 * sizeof(float4);
+    constexpr size_t smem = kTma && Ring<kMt>::kBytes > sums + 1024 ? Ring<kMt>::kBytes : sums + (kTma ? 1024 : 0);
+    const auto kernel = adapter_kernel<kRt, kMt, kTma>;
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles * csize));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)csize;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = kCluster ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    return launch_pdl(kernel, dim3((unsigned)(tiles * p.n_split)), dim3(kThreads), smem, st, p, tm_base, tm_out);
 }
 
 template <int kRt>
-cudaError_t launch_for(const AdapterParams& p, cudaStream_t st) {
+int launch_for(AdapterParams p, cudaStream_t st) {
     constexpr int kBigMt = kRt <= 4 ? 2 : 1;     // a rank of 128 has no registers for two tiles' sums
-    constexpr int kBigTile = kBigMt * 16;
-    const bool big = kBigMt > 1 && p.cu_seqlens && p.tokens > 16 * p.batch;
-    if (big) return launch<kRt, kBigMt, 8, false>(p, p.tokens / kBigTile + p.batch, 1, st);
-    const int tiles = p.cu_seqlens ? p.tokens / 16 + p.batch : p.batch;
-    int csize = 1;
-    while (csize < kMaxCluster && tiles * csize * 2 <= sm_count() * 2) csize *= 2;
-    return csize == 1 ? launch<kRt, 1, 8, false>(p, tiles, 1, st) : launch<kRt, 1, 8, true>(p, tiles, csize, st);
+    CUtensorMap tm_base = {}, tm_out = {};
+    // Tiles of 32 tokens where they give every SM two CTAs; with fewer tokens, or sequences that would not fill a tile, tiles of 16, whose columns are
+    // shared by CTAs as long as each warp has three groups of them. (1100 tokens of nine sequences, 768 -> 2304, rank 8: 11.0 us in the former form, 7.5 in the latter;
+    // single tokens of 64 sequences, 1024 -> 1024: 4.0 us, with two CTAs to a tile 4.2.)
+    const long long big_tiles = p.tokens / (kBigMt * 16) + p.batch;
+    if (p.cu_seqlens && p.tokens > 16 * p.batch && big_tiles > 2 * sm_count()) {
+        p.n_split = 1;
+        if (!make_tmap_2d_f16(&tm_base, p.base, p.tokens, p.out_feat, p.base_pitch, kBigMt * 16, 64, 128) ||
+            !make_tmap_2d_f16(&tm_out, p.out, p.tokens, p.out_feat, p.out_pitch, kBigMt * 16, 64, 128))
+            return fail(ET_ERR_CUDA, "et_adapter_add: cuTensorMapEncodeTiled failed");
+        return cuda_status(launch<kRt, kBigMt, true>(p, tm_base, tm_out, big_tiles, st), "et_adapter_add launch");
+    }
+    const long long tiles = p.cu_seqlens ? p.tokens / 16 + p.batch : p.batch;
+    p.n_split = (int)max(1LL, min(2LL * sm_count() / tiles, (long long)((p.out_feat + 31) / 32 / (3 * kWarps))));
+    return cuda_status(launch<kRt, 1, false>(p, tm_base, tm_out, tiles, st), "et_adapter_add launch");
 }
 
 }  // namespace
@@ -447,8 +538,9 @@ extern "C" int et_adapter_add(const et_adapter_bank* bank, void* out, const void
     p.out_pitch = out_pitch; p.base_pitch = base_pitch; p.x_pitch = x_pitch; p.a_stride = bank->a_stride; p.b_stride = bank->b_stride;
     p.batch = batch; p.tokens = tokens; p.n_slots = bank->n_slots; p.in_feat = bank->in_feat; p.out_feat = bank->out_feat;
     p.copy = out != base;
+    const int rc = attn_err_address(&p.err);
+    if (rc) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int rt = bank->rank_tiles;
-    const cudaError_t r = rt <= 1 ? launch_for<1>(p, st) : rt <= 2 ? launch_for<2>(p, st) : rt <= 4 ? launch_for<4>(p, st) : launch_for<8>(p, st);
-    return cuda_status(r, "et_adapter_add launch");
+    return rt <= 1 ? launch_for<1>(p, st) : rt <= 2 ? launch_for<2>(p, st) : rt <= 4 ? launch_for<4>(p, st) : launch_for<8>(p, st);
 }

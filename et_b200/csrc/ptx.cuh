@@ -96,13 +96,16 @@ __device__ __forceinline__ bool mbar_poll_warp(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity));
 }
 // ------------------------------------------------------------------ TMA
-__device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int x, int y,
-                                            uint64_t* bar) {
+__device__ __forceinline__ void tma_load_2d_at(uint32_t dst, const void* tmap, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-        "{%2, %3}], [%4];" ::"r"(smem_u32(dst)),
-        "l"(tmap), "r"(x), "r"(y), "r"(smem_u32(bar))
+        "{%2, %3}], [%4];" ::"r"(dst),
+        "l"(tmap), "r"(x), "r"(y), "r"(bar)
         : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int x, int y,
+                                            uint64_t* bar) {
+    tma_load_2d_at(smem_u32(dst), tmap, x, y, smem_u32(bar));
 }
 __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
     asm volatile(
@@ -114,18 +117,21 @@ __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const void* tmap, i
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
     tma_load_3d_at(smem_u32(dst), tmap, x, y, z, smem_u32(bar));
 }
-__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int x, int y) {
+__device__ __forceinline__ void tma_store_2d_at(const void* tmap, uint32_t src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                      tmap),
-                 "r"(smem_u32(src)), "r"(x), "r"(y)
+                 "r"(src), "r"(x), "r"(y)
                  : "memory");
 }
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int x, int y) { tma_store_2d_at(tmap, smem_u32(src), x, y); }
 __device__ __forceinline__ void tma_store_commit() {
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 __device__ __forceinline__ void tma_store_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
+// All but the latest committed group of this thread's stores have left shared memory.
+__device__ __forceinline__ void tma_store_wait_read_but_one() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 // The stores of this thread are complete: their results may be read back (by other threads after a barrier and the fence below).
 __device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_proxy_async_global() { asm volatile("fence.proxy.async.global;" ::: "memory"); }

@@ -57,7 +57,7 @@ struct Item {
     int b, qi0, head;
     int state;                // -1: no more items, 0: no query sees a key, 1: blocks follow
 };
-struct Block {
+struct alignas(16) Block {
     int j, left, flags, item; // number of the block, keys from its first one on, what it is, slot of its item
 };
 
@@ -78,7 +78,6 @@ struct TcShared {
     uint64_t clc_full;
     uint64_t q_full[2], q_empty[2], k_full[4], k_empty[4], v_full[4], v_empty[4];
     uint64_t s_full[2], p_full[2], pv_done[2];   // by place of the scores
-    uint64_t v_ready[4];                  // V has landed and is cleared behind the last key
     uint64_t m_full[2], m_empty[2];       // what the helping warps bring of a block: documents of its keys, its biases
     uint64_t item_full[kItemRing], item_empty[kItemRing];
     uint64_t block_full[kBlockRing];
@@ -115,24 +114,6 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
-// 2^x for two values on the FMA and ALU pipes, x <= 127: x = n + f with n the nearest whole number (adding 1.5 * 2^23 leaves n in the low bits of
-// the sum) and |f| <= 1/2; 2^f by the cubic that interpolates it at the Chebyshev nodes of [-1/2, 1/2] (largest relative error 1.0e-4, below half
-// a unit of the fp16 that the result is rounded to); n goes into the exponent. Not a number stays so.
-__device__ __forceinline__ float2 exp2_cubic2(float2 x) {
-    x.x = max_nan(x.x, -126.f);
-    x.y = max_nan(x.y, -126.f);
-    const float2 big = make_float2(12582912.f, 12582912.f), nbig = make_float2(-12582912.f, -12582912.f);
-    const float2 t = add2(x, big);
-    const float2 n = add2(t, nbig);
-    const float2 f = add2(x, make_float2(-n.x, -n.y));
-    float2 r = fma2(f, make_float2(0.0558382832f, 0.0558382832f), make_float2(0.242639482f, 0.242639482f));
-    r = fma2(r, f, make_float2(0.693136752f, 0.693136752f));
-    r = fma2(r, f, make_float2(0.999924541f, 0.999924541f));
-    float2 y;
-    y.x = __int_as_float(__float_as_int(r.x) + (__float_as_int(t.x) << 23));
-    y.y = __int_as_float(__float_as_int(r.y) + (__float_as_int(t.y) << 23));
-    return fma2(x, make_float2(0.f, 0.f), y);
-}
 // c - 2 c / (1 + 2^(x cap_in)) of four scores, with one reciprocal for the four: of the product of the denominators, which are at most 2^25 + 1 (from there
 // on the result is c).
 __device__ __forceinline__ void cap4(float& a, float& b, float& c, float& d, float cap_in, float cap_out) {
@@ -146,7 +127,7 @@ __device__ __forceinline__ void cap4(float& a, float& b, float& c, float& d, flo
     y = add2(y, one2);
     const float2 xy = mul2(x, y);
     const float r = rcp_fast(xy.x * xy.y);
-    const float2 inv = mul2(make_float2(r, r), make_float2(xy.y, xy.x));   // 1 / (x y), each
+    const float2 inv = make_float2(r * xy.y, r * xy.x);   // 1 / (x y), each
     const float2 out2 = make_float2(cap_out, cap_out), n2 = make_float2(-2.f * cap_out, -2.f * cap_out);
     const float2 ab = fma2(mul2(inv, y), n2, out2), cd = fma2(mul2(inv, x), n2, out2);
     a = ab.x; b = ab.y; c = cd.x; d = cd.y;
@@ -174,15 +155,21 @@ __device__ __forceinline__ bool clc_answer(const uint4* answer, int& x) {
 // ones, and an item is found without reading memory.
 __device__ __forceinline__ void sort_sequences(const RuleParams& p, SeqTable* t, int lane) {
     if (lane <= kLenClasses) t->class_at[lane] = 0;
+    RuleSeq mine[kMaxSorted / 32];   // read at once, kept for both passes
+#pragma unroll
+    for (int n = 0; n < kMaxSorted / 32; ++n) {
+        mine[n] = RuleSeq{};
+        if (n * 32 + lane < p.batch) mine[n] = rule_seq(p, n * 32 + lane);
+    }
     __syncwarp();
     const unsigned below = (1u << lane) - 1u;
     for (int pass = 0; pass < 2; ++pass) {   // count, place
-        for (int base = 0; base < p.batch; base += 32) {
-            const int i = base + lane;
+#pragma unroll
+        for (int n = 0; n < kMaxSorted / 32; ++n) {
+            if (n * 32 >= p.batch) break;
+            const int i = n * 32 + lane;
             const bool in = i < p.batch;
-            RuleSeq s = {};
-            if (in) s = rule_seq(p, i);
-            const int c = in ? 8 - min((s.klen + kBK - 1) / kBK, 8) : kLenClasses;
+            const int c = in ? 8 - min((mine[n].klen + 127) / 128, 8) : kLenClasses;   // by 128 keys
             const unsigned same = __match_any_sync(0xffffffffu, c);
             const int at = t->class_at[c];
             __syncwarp();
@@ -190,7 +177,7 @@ __device__ __forceinline__ void sort_sequences(const RuleParams& p, SeqTable* t,
             __syncwarp();
             if (pass == 1 && in) {
                 const int pos = at + __popc(same & below);
-                t->seq[pos] = s;
+                t->seq[pos] = mine[n];
                 t->b[pos] = i;
             }
         }
@@ -360,7 +347,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
     using C = Cfg<kHD>;
     const bool docs = p.summary != nullptr, help = kBias == kTable || docs;
     constexpr bool kChanged = kCap || kBias != kNoBias;   // scores are in the log2 domain before the maximum is taken
-    constexpr int kPolyPairs = 2;                         // of 16 pairs of exponentials, how many go to the FMA pipe
     const RuleParams& r = p.r;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -388,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             }
             for (int i = 0; i < C::kStages; ++i) {
                 mbar_init(&sh->k_full[i], 1); mbar_init(&sh->k_empty[i], 1);
-                mbar_init(&sh->v_full[i], 1); mbar_init(&sh->v_empty[i], 1); mbar_init(&sh->v_ready[i], kHelpWarps);
+                mbar_init(&sh->v_full[i], 1); mbar_init(&sh->v_empty[i], 1);
             }
             for (int i = 0; i < kItemRing; ++i) {
                 mbar_init(&sh->item_full[i], 1);
@@ -559,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 // O += P V of block g
                 const uint32_t vs = g % C::kStages;
                 const int keys = min(left, kBK);
-                ok = mbar_wait_at(ET_BAR(v_ready, vs), (g / C::kStages) & 1u) && mbar_wait_at(ET_BAR(p_full, g & 1), (g >> 1) & 1u);
+                ok = mbar_wait_at(ET_BAR(v_full, vs), (g / C::kStages) & 1u) && mbar_wait_at(ET_BAR(p_full, g & 1), (g >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 const uint64_t b = v_desc + vs * (C::kKTile >> 4);
@@ -576,17 +562,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         }
         __syncwarp();
     } else if (warp >= kHelpWarp) {
-        // ---- what a block needs beside K and V: the documents of its keys, its biases by distance; and V's rows behind the last key, up to the end of a
-        // 16-key step, are cleared (they may hold anything)
-        pdl_wait();
-        const int t = tid - 32 * kHelpWarp;
-        bool ok = true;
-        for (uint32_t g = 0;; ++g) {
-            ok = mbar_wait_at(ET_BAR(block_full, g % kBlockRing), (g / kBlockRing) & 1u);
-            if (!ok) break;
-            const Block b = sh->block[g % kBlockRing];
-            if (b.flags & kEnd) break;
-            if (help) {
+        // ---- what a block needs beside K and V: the documents of its keys, its biases by distance
+        if (help) {
+            pdl_wait();
+            const int t = tid - 32 * kHelpWarp;
+            bool ok = true;
+            for (uint32_t g = 0;; ++g) {
+                ok = mbar_wait_at(ET_BAR(block_full, g % kBlockRing), (g / kBlockRing) & 1u);
+                if (!ok) break;
+                const Block b = sh->block[g % kBlockRing];
+                if (b.flags & kEnd) break;
                 const int m = g & 1;
                 ok = mbar_wait_at(ET_BAR(m_empty, m), ((g >> 1) & 1u) ^ 1u);
                 if (!ok) break;
@@ -609,22 +594,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 }
                 mbar_arrive_at(ET_BAR(m_full, m));
             }
-            const int vs = g % C::kStages;
-            ok = mbar_wait_at(ET_BAR(v_full, vs), (g / C::kStages) & 1u);
-            if (!ok) break;
-            const int keys = min(b.left, kBK);
-            if (keys & 15) {
-                const int end = (keys + 15) & ~15;
-                for (int i = t; i < (end - keys) * 8 * C::kPanels; i += 32 * kHelpWarps) {
-                    const int row = keys + i / (8 * C::kPanels), c = i % (8 * C::kPanels);
-                    sts128(smem_at + C::kVAt + (vs * C::kPanels + (c >> 3)) * C::kKPanel + row * 128 + (c & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
-                }
-                fence_proxy_async_smem();
-            }
-            __syncwarp();
-            if (elect_one()) mbar_arrive_at(ET_BAR(v_ready, vs));
+            if (!ok && lane == 0) atomicExch(p.err, 23);
         }
-        if (!ok && lane == 0) atomicExch(p.err, 23);
         __syncwarp();
     } else {
         // ---- softmax: one thread per query row (TMEM lane)
@@ -639,8 +610,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         float done_sum = 0.f;   // its row sum
         auto arrive = [&](uint32_t at) {
             __syncwarp();
-            if (elect_one()) mbar_arrive_at(at);
-            __syncwarp();
+            if (lane == 0) mbar_arrive_at(at);
         };
         // O / row sum -> fp16 -> global, of the item whose last block is n - 1.
         auto finish = [&](uint32_t n, int from) {
@@ -652,15 +622,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             const bool in = qi < it.seq.qlen;
             half* const orow = r.out + (it.seq.q0 + qi) * r.out_pitch + it.head * hd;
             half2 top = __float2half2_rn(0.f);   // largest result; infinity or not a number if one of them is
-#pragma unroll 1
-            for (int c = 0; c < osteps; ++c) {
-                uint32_t o[16];
-                tmem_ld16(tmem + lane_base + C::kOCol + from * 64 + c * 16, o);
-                tmem_ld_wait(o);
+            auto sixteen = [&](const uint32_t (&o)[32], int at, int c) {   // columns 16c .. 16c + 15 of the head, o[at] on
+                if (c >= osteps) return;
                 uint32_t ow[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    ow[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+                    ow[i] = pack2(__uint_as_float(o[at + 2 * i]) * inv, __uint_as_float(o[at + 2 * i + 1]) * inv);
                     top = __hmax2_nan(top, __habs2(*reinterpret_cast<const half2*>(&ow[i])));
                 }
                 if (in) {
@@ -674,6 +641,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                         *reinterpret_cast<uint4*>(z + 8) = make_uint4(ow[4], ow[5], ow[6], ow[7]);
                     }
                 }
+            };
+#pragma unroll 1
+            for (int c = 0; c < osteps; c += 4) {   // (columns beyond the head are there, whatever they hold)
+                uint32_t o[2][32];
+                tmem_ld32(tmem + lane_base + C::kOCol + from * 64 + c * 16, o[0]);
+                tmem_ld32(tmem + lane_base + C::kOCol + from * 64 + c * 16 + 32, o[1]);
+                tmem_ld_wait(o[0], o[1]);
+                sixteen(o[0], 0, c);
+                sixteen(o[0], 16, c + 1);
+                sixteen(o[1], 0, c + 2);
+                sixteen(o[1], 16, c + 3);
             }
             const float largest = fmaxf(__low2float(top), __high2float(top)), sum = __low2float(top) + __high2float(top);
             unsigned again = __ballot_sync(0xffffffffu, in && !(largest <= 65504.f && sum == sum));
@@ -721,8 +699,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 ok = mbar_wait_at(ET_BAR(s_full, g & 1), (g >> 1) & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                const Block& b = sh->block[g % kBlockRing];
-                const int k0 = b.j * kBK, left = b.left, flags = b.flags;
+                const uint4 b = lds128(sh_at + (uint32_t)offsetof(TcShared, block) + (g % kBlockRing) * (uint32_t)sizeof(Block));
+                const int k0 = (int)b.x * kBK, left = (int)b.y, flags = (int)b.z;
                 const bool first = flags & kFirst;
                 last = flags & kLast;
                 const int m = g & 1;
@@ -742,33 +720,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 const float2 scale2 = make_float2(sc, sc);
                 if constexpr (kBias == kSlopes) {
                     // On one side of the queries the bias is linear in the key; in the blocks around them it is not.
-                    const int near = k0 - qpos;
+                    const float near = (float)(k0 - qpos);
                     const bool behind = k0 >= qpos, before = k0 + kBK - 1 <= qpos;
                     if (__all_sync(0xffffffffu, behind) || __all_sync(0xffffffffu, before)) {
-                        const float signed_slope = behind ? slope : -slope, base = (float)near * signed_slope;
-                        const float2 slope2 = make_float2(signed_slope, signed_slope), base2 = make_float2(base, base);
+                        const float s1 = behind ? slope : -slope;
+                        const float2 step2 = make_float2(16.f * s1, 16.f * s1);
+                        float2 bias[8];   // (chains of sums: as constants in registers the distances cost two moves each)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) bias[i] = make_float2((near + 2 * i) * s1, (near + 2 * i + 1) * s1);
 #pragma unroll
                         for (int i = 0; i < 64; i += 2) {
-                            const float2 bias = fma2(make_float2((float)i, (float)(i + 1)), slope2, base2);
-                            float2 x = make_float2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1]);
-                            x = kCap ? add2(x, bias) : fma2(x, scale2, bias);
-                            v[i >> 5][i & 31] = x.x;
-                            v[i >> 5][(i & 31) + 1] = x.y;
+                            float2& y = bias[(i >> 1) & 7];
+                            float* const w = &v[i >> 5][i & 31];
+                            const float2 x = kCap ? add2(make_float2(w[0], w[1]), y) : fma2(make_float2(w[0], w[1]), scale2, y);
+                            w[0] = x.x;
+                            w[1] = x.y;
+                            if (i < 48) y = add2(y, step2);
                         }
                     } else {
-                        const float base = (float)near;
-                        const float2 slope2 = make_float2(slope, slope);
 #pragma unroll
-                        for (int i = 0; i < 64; i += 2) {
-                            float2 d = add2(make_float2(base, base), make_float2((float)i, (float)(i + 1)));
-                            d.x = fabsf(d.x);
-                            d.y = fabsf(d.y);
-                            float2 x = make_float2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1]);
-                            if constexpr (!kCap) x = mul2(x, scale2);
-                            x = fma2(d, slope2, x);
-                            v[i >> 5][i & 31] = x.x;
-                            v[i >> 5][(i & 31) + 1] = x.y;
-                        }
+                        for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = fmaf(fabsf(near + (float)i), slope, kCap ? v[i >> 5][i & 31] : v[i >> 5][i & 31] * sc);
                     }
                 }
                 if (help) {
@@ -855,16 +826,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                     for (int i = 0; i < 16; ++i) {
                         float2 e = make_float2(v[h][2 * i], v[h][2 * i + 1]);
                         e = kChanged ? add2(e, shift2) : fma2(e, to_log22, shift2);
-                        if ((i * kPolyPairs) / 16 != ((i + 1) * kPolyPairs) / 16) {   // spread so that both pipes stay busy
-                            e = exp2_cubic2(e);
-                        } else {
-                            e.x = ex2_fast(e.x);
-                            e.y = ex2_fast(e.y);
-                        }
+                        e.x = ex2_fast(e.x);
+                        e.y = ex2_fast(e.y);
                         l2 = add2(l2, e);
                         pk[i] = pack2(e.x, e.y);
                     }
                     tmem_store16(s_addr + h * 16, pk);   // where this block's first scores were: they have all been read
+                }
+                // V's rows behind the last key, up to the end of a 16-key step, may hold anything: they are cleared
+                if (left < kBK && (left & 15)) {
+                    const int vs = g % C::kStages, end = (left + 15) & ~15;
+                    ok = mbar_wait_at(ET_BAR(v_full, vs), (g / C::kStages) & 1u);
+                    if (!ok) break;
+                    for (int i = row; i < (end - left) * 8 * C::kPanels; i += kBQ) {
+                        const int key = left + i / (8 * C::kPanels), c = i % (8 * C::kPanels);
+                        sts128(smem_at + C::kVAt + (vs * C::kPanels + (c >> 3)) * C::kKPanel + key * 128 + (c & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
+                    }
+                    fence_proxy_async_smem();
                 }
                 tmem_st_wait();
                 tc_fence_before();

@@ -4,14 +4,15 @@
 //
 // What bounds it: HBM, each head is read and written once. The angle is taken in 64 bits: of a position of a million an fp32 product keeps
 // four digits behind the point. In turns (multiplied by 1 / 2 pi) it loses its whole part there, and sine and cosine of the rest are fp32
-// (sincospif). A block takes the angles of its tokens once, for all heads, through shared memory; then a thread keeps the eight it needs in
-// registers and goes through the heads, 16 bytes at a time and four heads in flight.
+// (sincospif). A block requests its heads, 16 bytes and four heads to a thread, takes the angles of its tokens meanwhile, once for all heads, and leaves
+// them in shared memory; a thread keeps the eight that it needs in registers. 32768 tokens of 32 heads of 64 take 43 us, 6.2 TB/s; with the heads requested
+// behind the angles and a warp's rows in different tokens 56.
 #include "common.h"
 
 namespace et {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kMaxThreads = 512;
 constexpr int kHeadsInFlight = 4;
 
 enum Pairing {
@@ -30,7 +31,7 @@ struct RotaryParams {
     const int* axis;
     int nhead_q, nhead_k, head_dim, rot, n_axes, tokens;
     int lanes;            // threads to a head (a power of two, so that a head lies inside a warp)
-    int block_tokens;     // tokens to a block
+    int block_tokens, head_step;   // tokens of a block, heads of each that it takes at a time
     bool interleaved;
     bool in_place_q, in_place_k;
 };
@@ -54,28 +55,15 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
 }
 
 template <int kPairing>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
     extern __shared__ float2 turns[];   // [block_tokens][rot / 2]: cosine, sine
     const int pairs = p.rot >> 1, heads = p.nhead_q + p.nhead_k;
     const int t0 = blockIdx.x * p.block_tokens, nt = min(p.block_tokens, p.tokens - t0);
     pdl_launch_dependents();
     pdl_wait();
-    for (int i = threadIdx.x; i < nt * pairs; i += kThreads) {
-        const int t = i / pairs, pair = i - t * pairs;
-        const int ax = p.axis[pair];
-        float2 cs = make_float2(1.f, 0.f);
-        if (ax >= 0 && ax < p.n_axes) {   // (a pair of no axis is not turned)
-            double turn = (double)p.positions[(size_t)(t0 + t) * p.n_axes + ax] * (double)p.inv_freq[pair] * 0.15915494309189535;
-            turn -= rint(turn);
-            sincospif(2.f * (float)turn, &cs.y, &cs.x);
-        }
-        turns[i] = cs;
-    }
-    __syncthreads();
-    const int rows = kThreads / p.lanes;   // heads that the block takes at a time
-    const int row = threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;
-    const int t = row % p.block_tokens, head_step = rows / p.block_tokens;
-    const bool token_in = t < nt && row / p.block_tokens < head_step;
+    const int row = threadIdx.x / p.lanes, lane = threadIdx.x % p.lanes;   // (neighbouring heads of a token lie side by side)
+    const int head_step = p.head_step, t = row / head_step, first_head = row % head_step;
+    const bool token_in = t < nt;
     const float2* const cs = turns + min(t, nt - 1) * pairs;
     auto src = [&](int h) {
         return h < p.nhead_q ? p.q + (size_t)(t0 + t) * p.q_pitch + h * p.head_dim : p.k + (size_t)(t0 + t) * p.k_pitch + (h - p.nhead_q) * p.head_dim;
@@ -85,10 +73,26 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
                              : p.k_out + (size_t)(t0 + t) * p.k_out_pitch + (h - p.nhead_q) * p.head_dim;
     };
     auto in_place = [&](int h) { return h < p.nhead_q ? p.in_place_q : p.in_place_k; };
+    // The block's angles, into shared memory. Called when the first heads are already on their way.
+    auto take_angles = [&]() {
+        for (int i = threadIdx.x; i < nt * pairs; i += blockDim.x) {
+            const int pair = i % pairs;
+            const int ax = p.axis[pair];
+            float2 v = make_float2(1.f, 0.f);
+            if (ax >= 0 && ax < p.n_axes) {   // (a pair of no axis is not turned)
+                double turn = (double)p.positions[(size_t)(t0 + i / pairs) * p.n_axes + ax] * (double)p.inv_freq[pair] * 0.15915494309189535;
+                turn -= rint(turn);
+                sincospif(2.f * (float)turn, &v.y, &v.x);
+            }
+            turns[i] = v;
+        }
+        __syncthreads();
+    };
 
     if constexpr (kPairing == kScalar) {
+        take_angles();
         if (!token_in) return;
-        for (int h = row / p.block_tokens; h < heads; h += head_step) {
+        for (int h = first_head; h < heads; h += head_step) {
             const half* const x = src(h);
             half* const y = dst(h);
             for (int i = lane; i < pairs; i += p.lanes) {
@@ -104,7 +108,20 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         const int turned = pairs / 8;   // lanes below have eight pairs, the others a granule that is passed on
         const bool turns_it = lane < turned;
         const int at = turns_it ? lane * 8 : p.rot + (lane - turned) * 8;
-        if (!token_in || at >= p.head_dim) return;
+        const bool in = token_in && at < p.head_dim;
+        uint4 a[kHeadsInFlight], b[kHeadsInFlight];
+        auto fetch = [&](int h0) {
+#pragma unroll
+            for (int k = 0; k < kHeadsInFlight; ++k) {
+                const int h = h0 + k * head_step;
+                if (!in || h >= heads || (!turns_it && in_place(h))) continue;
+                a[k] = *reinterpret_cast<const uint4*>(src(h) + at);
+                if (turns_it) b[k] = *reinterpret_cast<const uint4*>(src(h) + at + pairs);
+            }
+        };
+        fetch(first_head);
+        take_angles();
+        if (!in) return;
         float c[8], s[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -112,15 +129,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
             c[i] = v.x;
             s[i] = v.y;
         }
-        for (int h0 = row / p.block_tokens; h0 < heads; h0 += head_step * kHeadsInFlight) {
-            uint4 a[kHeadsInFlight], b[kHeadsInFlight];
-#pragma unroll
-            for (int k = 0; k < kHeadsInFlight; ++k) {
-                const int h = h0 + k * head_step;
-                if (h >= heads || (!turns_it && in_place(h))) continue;
-                a[k] = *reinterpret_cast<const uint4*>(src(h) + at);
-                if (turns_it) b[k] = *reinterpret_cast<const uint4*>(src(h) + at + pairs);
-            }
+        for (int h0 = first_head; h0 < heads; h0 += head_step * kHeadsInFlight) {
+            if (h0 != first_head) fetch(h0);
 #pragma unroll
             for (int k = 0; k < kHeadsInFlight; ++k) {
                 const int h = h0 + k * head_step;
@@ -147,16 +157,6 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         const int at = lane * 8;
         const bool in = token_in && at < p.head_dim;
         const int n_turned = max(0, min(8, p.rot - at));   // the others are passed on
-        float c[8], s[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int d = at + i;
-            const bool second = kPairing == kNeighbours ? (i & 1) : d >= pairs;
-            const int pair = kPairing == kNeighbours ? d >> 1 : (second ? d - pairs : d);
-            const float2 v = cs[i < n_turned ? pair : 0];
-            c[i] = v.x;
-            s[i] = second ? v.y : -v.y;
-        }
         // kHalves: the partners of features at .. at + 7 are at + pairs .. (first half) or at - pairs .. (second half); a granule that
         // holds features of both halves has partners of both kinds, eight of each
         const int up = at + pairs, down = at - pairs;
@@ -182,10 +182,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
             r.w = (shift & 1) ? __funnelshift_r(w[3], w[4], 16) : w[3];
             return r;
         };
-        const int iterations = (heads + head_step * kHeadsInFlight - 1) / (head_step * kHeadsInFlight);
-        for (int n = 0; n < iterations; ++n) {
-            const int h0 = row / p.block_tokens + n * head_step * kHeadsInFlight;
-            uint4 a[kHeadsInFlight], bu[kHeadsInFlight], bd[kHeadsInFlight];
+        uint4 a[kHeadsInFlight], bu[kHeadsInFlight], bd[kHeadsInFlight];
+        auto fetch = [&](int h0) {
 #pragma unroll
             for (int k = 0; k < kHeadsInFlight; ++k) {
                 const int h = h0 + k * head_step;
@@ -197,6 +195,23 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
                     if (need_down) bd[k] = eight_from(src(h), down);
                 }
             }
+        };
+        fetch(first_head);
+        take_angles();
+        float c[8], s[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = at + i;
+            const bool second = kPairing == kNeighbours ? (i & 1) : d >= pairs;
+            const int pair = kPairing == kNeighbours ? d >> 1 : (second ? d - pairs : d);
+            const float2 v = cs[i < n_turned ? pair : 0];
+            c[i] = v.x;
+            s[i] = second ? v.y : -v.y;
+        }
+        const int iterations = (heads + head_step * kHeadsInFlight - 1) / (head_step * kHeadsInFlight);
+        for (int n = 0; n < iterations; ++n) {
+            const int h0 = first_head + n * head_step * kHeadsInFlight;
+            if (n) fetch(h0);
             if constexpr (kPairing == kHalves) __syncwarp();
 #pragma unroll
             for (int k = 0; k < kHeadsInFlight; ++k) {
@@ -258,11 +273,15 @@ extern "C" int et_rotary_axes(void* q_out, const void* q, int q_out_pitch, int q
     const int want = pairing == kScalar ? min(32, max(1, pairs)) : pairing == kHalves8 ? pairs / 8 + (head_dim - rot_dim) / 8 : head_dim / 8;
     p.lanes = 1;
     while (p.lanes < want) p.lanes *= 2;
-    // Tokens to a block: as many as keep all SMs busy with several blocks each, but no more angles than threads.
-    const int rows = kThreads / p.lanes;
-    p.block_tokens = max(1, min(min(rows, kThreads / max(pairs, 1)), tokens / (sm_count() * 6)));
+    // A thread has kHeadsInFlight heads, all requested at once, one where there are few tokens; a block has as many tokens as make 128 threads, but no more
+    // than leave every SM four blocks. (32768 tokens of 32 heads of 64 in blocks of 128, 256, 512 threads: 43.4, 45.7, 61.1 us, with two heads to a thread 48.8,
+    // eight 53.9; 64 tokens of 24 heads with one, two, four, eight: 2.2, 2.2, 2.9, 4.2.)
+    const int heads = nhead_q + nhead_k, in_flight = tokens > sm_count() * 4 ? kHeadsInFlight : 1;
+    p.head_step = max(1, min((heads + in_flight - 1) / in_flight, kMaxThreads / p.lanes));
+    p.block_tokens = max(1, min(128 / (p.head_step * p.lanes), tokens / (sm_count() * 4)));
+    const int threads = (p.block_tokens * p.head_step * p.lanes + 31) / 32 * 32;
     const int blocks = (tokens + p.block_tokens - 1) / p.block_tokens;
     const size_t smem = (size_t)p.block_tokens * max(pairs, 1) * sizeof(float2);
     const auto kernel = pairing == kScalar ? rotary_kernel<kScalar> : pairing == kHalves8 ? rotary_kernel<kHalves8> : pairing == kHalves ? rotary_kernel<kHalves> : rotary_kernel<kNeighbours>;
-    return cuda_status(launch_pdl(kernel, dim3(blocks), dim3(kThreads), smem, static_cast<cudaStream_t>(stream), p), "et_rotary_axes launch");
+    return cuda_status(launch_pdl(kernel, dim3(blocks), dim3(threads), smem, static_cast<cudaStream_t>(stream), p), "et_rotary_axes launch");
 }

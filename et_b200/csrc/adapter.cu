@@ -16,6 +16,7 @@
 // tile of 32 tokens reads again (195 MB beside 340, from L2: rings of two stages, which leave them more of L1, gain 6 us over three), and the start of a
 // tile. 64 single tokens 4.0 us. Tried: clusters of 2, 4, 8 CTAs that share a tile's K range and columns through distributed shared memory (103, 131, 235 us;
 // single tokens 5.0, 5.3, 7.3), tiles of 64 tokens (103), CTAs that share the columns where there are many tokens (91).
+#include <cstring>
 #include <new>
 #include <vector>
 #include "attention.h"
@@ -494,19 +495,17 @@ extern "C" int et_adapter_bank_set(et_adapter_bank* bank, int slot, int rank, co
     const half* const B = static_cast<const half*>(b_host);   // [out_feat x rank]
     // A: [chunk of 32 features][8 ranks][lane = rank * 4 + t][features 8t .. 8t + 7 of the chunk]
     for (int r = 0; r < rank; ++r)
-        for (int k = 0; k < bank->in_feat; ++k) {
+        for (int k = 0; k < bank->in_feat; k += 8) {
             const size_t tile = (size_t)(k / 32) * (bank->rank_tiles * 2) + r / 8;
-            pa[(tile * 32 + (r % 8) * 4 + (k % 32) / 8) * 8 + k % 8] = A[(size_t)r * bank->in_feat + k];
+            std::memcpy(&pa[(tile * 32 + (r % 8) * 4 + (k % 32) / 8) * 8], A + (size_t)r * bank->in_feat + k, 16);
         }
     // B: [group of 32 columns][16 ranks][lane][tile 0 .. 3][ranks 2t, 2t + 1, 2t + 8, 2t + 9]; column c of the group is column
     // 2 (c / 8) + c % 2 of tile (c / 2) % 4, which is the lane's number / 4
-    for (int n = 0; n < bank->out_feat; ++n)
-        for (int r = 0; r < rank; ++r) {
-            const int c = n % 32, q = r % 16;
-            const int lane = (2 * (c / 8) + c % 2) * 4 + (q % 8) / 2;
-            const size_t tile = (size_t)(n / 32) * bank->rank_tiles + r / 16;
-            pb[(tile * 32 + lane) * 16 + (c / 2) % 4 * 4 + q / 8 * 2 + q % 2] = B[(size_t)n * rank + r];
-        }
+    for (int n = 0; n < bank->out_feat; ++n) {
+        const int c = n % 32;
+        half* const column = &pb[((size_t)(n / 32) * bank->rank_tiles * 32 + (2 * (c / 8) + c % 2) * 4) * 16 + (c / 2) % 4 * 4];
+        for (int r = 0; r < rank; ++r) column[(size_t)(r / 16) * 512 + (r % 8) / 2 * 16 + r % 16 / 8 * 2 + r % 2] = B[(size_t)n * rank + r];
+    }
     const Slot entry = {rank, scale};
     e = cudaDeviceSynchronize();   // launches that read the slot as it was have finished
     if (e == cudaSuccess) e = cudaMemcpy(bank->a + slot * bank->a_stride, pa.data(), pa.size() * sizeof(half), cudaMemcpyHostToDevice);

@@ -80,6 +80,7 @@ extern "C" int et_attention_rules(void* out, const void* Q, const void* K, const
     p.scale_log2 = (float)(scale * 1.4426950408889634);
     p.cap_in = r.cap > 0.f ? (float)(2.0 * scale * 1.4426950408889634 / r.cap) : 0.f;
     p.cap_out = (float)(r.cap * 1.4426950408889634);
+    ET_REQUIRE(std::isfinite(p.scale_log2) && std::isfinite(p.cap_in) && std::isfinite(p.cap_out), "et_attention_rules: scale and cap are too far apart");
     p.slopes = r.slopes; p.table = static_cast<const half*>(r.distance_bias); p.reach = r.distance_bias ? r.reach : 0;
     p.window_left = r.window_left < 0 || r.window_left >= kNoLimit ? kNoLimit : r.window_left;
     p.window_right = r.window_right < 0 || r.window_right >= kNoLimit ? kNoLimit : r.window_right;

@@ -114,6 +114,12 @@ static __device__ __noinline__ void rules_row(const RuleParams& p, const RuleSeq
         const float w = seen ? exp2f(score - shift) : 0.f, keep = top == -INFINITY ? 0.f : exp2f(top - shift);
         top = m;
         sum = sum * keep + w;   // each lane its own keys'
+        if (__any_sync(0xffffffffu, w != w)) {   // so is the whole row, whatever follows
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[c] = NAN;
+            sum = 1.f;
+            break;
+        }
 #pragma unroll
         for (int c = 0; c < 8; ++c) o[c] *= keep;
         for (unsigned left = any; left; left &= left - 1) {

@@ -324,22 +324,28 @@ def rotary_axes(q_out, k_out, q, k, positions, inv_freq, axis, head_dim, interle
     current, f16, i32, f32 = _kept or _torch_kept()
     device = current()
     tokens, axes = _matrix("positions", positions, i32, device)
-    pairs = inv_freq.shape[0]
-    args = []
-    for name, x, out in (("q", q, q_out), ("k", k, k_out)):
-        if x is None:
-            args += (None, None, 0, 0, 0)
-            continue
-        rows, width, pitch = _rows(name, x, f16, device)
-        rows_out, width_out, pitch_out = _rows(name + "_out", out, f16, device)
-        if rows != tokens or rows_out != rows or width_out != width or width % head_dim:
-            raise ValueError(f"{name}: {tokens} rows of whole heads of {head_dim}, the result alike, not {tuple(x.shape)} and {tuple(out.shape)}")
-        args += (out.data_ptr(), x.data_ptr(), pitch_out, pitch, width // head_dim)
-    rc = (_entries or _lib()).et_rotary_axes(*args, head_dim, 2 * pairs, positions.data_ptr(), axes, _array("inv_freq", inv_freq, f32, device, pairs),
-                                             _array("axis", axis, i32, device, pairs), 1 if interleaved else 0, tokens, raw_stream(stream))
+    pairs = inv_freq.numel()
+    rc = (_entries or _lib()).et_rotary_axes(*_turned("q", q, q_out, tokens, head_dim, f16, device), *_turned("k", k, k_out, tokens, head_dim, f16, device), head_dim, 2 * pairs,
+                                             positions.data_ptr(), axes, _array("inv_freq", inv_freq, f32, device, pairs), _array("axis", axis, i32, device, pairs),
+                                             1 if interleaved else 0, tokens, raw_stream(stream))
     if rc:
         check(rc)
     return q_out, k_out
+
+
+def _turned(name, x, out, tokens, head_dim, f16, device):
+    """(addresses and pitches of the result and of x, heads)."""
+    if x is None:
+        return None, None, 0, 0, 0
+    if x.dtype is f16 and out.dtype is f16 and x.get_device() == device and out.get_device() == device and x.dim() == 2:
+        shape = rows, width = x.shape
+        pitch, step = x.stride()
+        if rows == tokens and width % head_dim == 0 and step == 1 and out.shape == shape:
+            pitch_out, step = out.stride()
+            if step == 1:
+                return out.data_ptr(), x.data_ptr(), pitch_out if rows > 1 else width, pitch if rows > 1 else width, width // head_dim
+    raise ValueError(f"{name}: {tokens} rows of whole float16 heads of {head_dim} on the current CUDA device ({device}), neighbouring elements, and the result alike expected, "
+                     f"not {x.dtype} {tuple(x.shape)} on {x.device} and {out.dtype} {tuple(out.shape)} on {out.device}")
 
 
 class AdapterBank:
@@ -410,10 +416,10 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
     current, f16, i32, f32 = _kept or _torch_kept()
     device = current()
     tokens, width, q_pitch = _rows("Q", Q, f16, device)
-    out_rows, out_width, out_pitch = _rows("out", out, f16, device)
     k_rows, kv_width, k_pitch = _rows("K", K, f16, device)
-    v_rows, v_width, v_pitch = _rows("V", V, f16, device)
-    if out_rows != tokens or out_width != width or v_rows != k_rows or v_width != kv_width or width % head_dim or kv_width % head_dim or not kv_width or not width:
+    _, _, out_pitch = _rows("out", out, f16, device)
+    _, _, v_pitch = _rows("V", V, f16, device)
+    if out.shape != Q.shape or V.shape != K.shape or width % head_dim or kv_width % head_dim or not kv_width or not width:
         raise ValueError(f"whole heads of {head_dim}, out like Q and V like K expected, not {tuple(Q.shape)}, {tuple(out.shape)}, {tuple(K.shape)}, {tuple(V.shape)}")
     nhead, nhead_kv = width // head_dim, kv_width // head_dim
     reach = table = 0

@@ -146,7 +146,7 @@ int et_attention_static_scores(void* out, const void* Q, const void* K, const vo
  * ET_ERR_DEVICE_TIMEOUT and the code in *code (21: the issuing thread's wait, 22: the final accumulator wait, 23: a warp
  * that copies masks)
  * when a bounded wait inside the kernel gave up since the last check; the rows of that CTA are then not
- * written. The word is one per device, shared by every launch on it. No counterpart in the reference, whose
+ * written. The word is one per device, shared by every launch on it, those of et_attention_rules (24: single tokens) and et_adapter_add (51) among them. No counterpart in the reference, whose
  * only error handling is cudaChk's exit(1) (encoder/utils.h:4-12). */
 int et_attention_check(int* code);
 /* Batched, variable-length form (no counterpart in the reference, which handles one sequence per call):
@@ -176,7 +176,7 @@ int et_rotary_axes(void* q_out, const void* q, int q_out_pitch, int q_pitch, int
 /* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference, which holds one set of weights) ----
  * A bank holds n_slots adapters of one projection, each of rank up to max_rank (1 to 128): A [rank x in_feat], B [out_feat x rank] and a
  * scale. It allocates its memory on the current device and synchronises it, as et_adapter_bank_set does, which copies an adapter from HOST
- * arrays into a slot (rank 0: the slot is empty again). in_feat and out_feat are multiples of 16. */
+ * arrays into a slot (rank 0: the slot is empty again): not while another thread launches with the bank. in_feat and out_feat are multiples of 16. */
 typedef struct et_adapter_bank et_adapter_bank;
 int et_adapter_bank_create(et_adapter_bank** out, int in_feat, int out_feat, int max_rank, int n_slots);
 int et_adapter_bank_destroy(et_adapter_bank* bank);
@@ -213,7 +213,8 @@ typedef struct et_score_rules {
  * All arrays of the rules are device arrays. max_q_len and max_k_len: at least the longest sequence's queries and keys; keys beyond
  * max_k_len, or beyond k_rows, are not seen. Single tokens (max_q_len 1 with k_start) take a kernel that splits the keys. scratch: device memory of
  * et_attention_rules_scratch_size bytes when documents are given (contents do not matter; calls that may overlap need one each), else NULL.
- * out may not overlap the inputs. Rows of out in no sequence are left as they are. */
+ * out may not overlap the inputs. Rows of out in no sequence are left as they are. The first call on a device looks up the device's error
+ * word (et_attention_check): make it before a stream capture, as et_adapter_add's. */
 int et_attention_rules(void* out, const void* Q, const void* K, const void* V, int out_pitch, int q_pitch, int k_pitch, int v_pitch,
                        int nhead, int nhead_kv, int head_dim, const int* cu_seqlens, const int* k_start, const int* k_lens, int batch,
                        int q_tokens, int k_rows, int max_q_len, int max_k_len, const et_score_rules* rules, void* scratch,

@@ -60,7 +60,7 @@ def attention(lib, rules=None, **change):
 
 @pytest.mark.parametrize("change", [dict(batch=-1), dict(q_tokens=-1), dict(max_k_len=-1), dict(nhead=0), dict(nhead_kv=0), dict(nhead=3, nhead_kv=2), dict(head_dim=0), dict(head_dim=257),
                                     dict(nhead=1 << 16), dict(max_q_len=1 << 30), dict(k_start=P), dict(out=None), dict(Q=None), dict(V=None), dict(batch=2), dict(q_pitch=127),
-                                    dict(v_pitch=63), dict(rules=dict(cap=-1.0)), dict(rules=dict(cap=math.inf)), dict(rules=dict(scale=math.nan)), dict(rules=dict(scale=-1.0)),
+                                    dict(v_pitch=63), dict(rules=dict(cap=-1.0)), dict(rules=dict(cap=math.inf)), dict(rules=dict(cap=1e-39)), dict(rules=dict(scale=3e38)), dict(rules=dict(scale=math.nan)), dict(rules=dict(scale=-1.0)),
                                     dict(rules=dict(slopes=16, distance_bias=16)), dict(rules=dict(distance_bias=16, reach=-1)), dict(rules=dict(q_docs=16)),
                                     dict(rules=dict(q_docs=16, k_docs=16))])
 def test_attention_refuses(lib, change):

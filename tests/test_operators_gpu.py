@@ -130,6 +130,14 @@ def test_adapters_of_sequences(et, k, n, max_rank, ranks, lengths):
     check_adapter(et, bank, held, lengths, ids, k, n)
 
 
+@pytest.mark.parametrize("k,n,max_rank,ranks", [(768, 768, 16, [16, 8, 0]), (1024, 368, 32, [32, 17]), (256, 2304, 64, [64, 40]), (208, 48, 128, [128, 100]), (96, 16, 4, [4])])
+def test_adapters_of_many_tokens(et, k, n, max_rank, ranks):
+    """Enough tokens for the form in which base and out move by TMA: whole tiles, ends of sequences inside one, sequences of one token, without an adapter, empty."""
+    bank, held = make_bank(et, k, n, max_rank, ranks)
+    lengths = [3001, 2500, 31, 0, 4096, 1, 33, 640]
+    check_adapter(et, bank, held, lengths, [0, 1, -1, 0, 0, 1, 0, -1], k, n, pad=8)
+
+
 @pytest.mark.parametrize("batch", [1, 3, 64, 300])
 @pytest.mark.parametrize("k,n,max_rank,ranks", [(1024, 1024, 16, [16] * 5), (768, 2304, 64, [64, 1, 0, 40]), (4096, 1024, 128, [128, 16]), (32, 48, 8, [8, 8])])
 def test_adapters_of_single_tokens(et, k, n, max_rank, ranks, batch):
@@ -316,6 +324,52 @@ def test_attention_of_single_tokens(et, hq, hk, hd, lens, rule):
     if "docs" in args:
         args["docs"] = (dev(np.arange(len(lens)) % 3 - (len(lens) > 2)), dev(np.arange(room * len(lens)) // 40 % 3))
     run_attention(et, Q, K, V, hd, [(b, 1, starts[b], n, n - 1) for b, n in enumerate(lens)], k_start=starts, k_lens=lens, max_q=1, **args)
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(4, 4, 64), (16, 2, 128), (40, 1, 64), (6, 3, 32)])
+@pytest.mark.parametrize("rule", ["causal", "all", "cap table documents"])
+def test_attention_of_a_few_tokens(et, hq, hk, hd, rule):
+    """Up to four new tokens of a sequence over its kept keys, which see one another as the rules say: several tiles of rows, sequences with fewer."""
+    nq, nk = [4, 1, 0, 3, 2], [700, 64, 9, 3, 1]
+    starts = [0, 700, 800, 900, 1000]
+    cu = np.concatenate([[0], np.cumsum(nq)]).astype(int)
+    Q, K, V = normal(4, int(cu[-1]), hq * hd), normal(5, 1010, hk * hd), normal(6, 1010, hk * hd)
+    args = rules_of(rule, nk, hq)
+    if "docs" in args:
+        args["docs"] = (dev(np.arange(int(cu[-1])) % 4 - 1), dev(np.arange(1010) // 100 % 4))
+    run_attention(et, Q, K, V, hd, [(int(cu[b]), nq[b], starts[b], nk[b], nk[b] - nq[b]) for b in range(5)], cu=cu, k_start=starts, k_lens=nk, max_q=4, **args)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 24])
+def test_attention_of_values_that_are_not_numbers(et, hd):
+    """What a row sees and is not a number makes it not a number, in all its features or in those of V, and no other row."""
+    import torch
+    Q, K, V, cu, seqs = packed(3, [600, 300], 4, 2, hd)
+    K[610, 3] = math.nan                 # of the second sequence, first K/V head: its first two query heads
+    V[20, hd + 5] = math.inf             # of the first sequence, second K/V head: its last two query heads, one feature each
+    out = run_attention(et, Q, K, V, hd, seqs, cu=cu, window=(-1, 0))
+    bad = torch.zeros(900, 4, hd, dtype=torch.bool, device="cuda")
+    bad[610:, :2] = True
+    bad[20:600, 2:, 5] = True
+    assert torch.equal(~torch.isfinite(out.view(900, 4, hd)), bad)
+    Q[:] = math.nan
+    out = et.attention_rules(torch.zeros_like(out), Q, K, V, hd, cu_seqlens=dev(cu), batch=2, max_q_len=600, max_k_len=600, window=(-1, 0))
+    assert torch.isnan(out).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_scores_that_keep_growing(et, hd):
+    """Every block's scores are far above those of the block before: the reference moves each time; and far below: it stays."""
+    import torch
+    n = 1000
+    Q, K, V = normal(1, 200, 2 * hd, std=0.1), normal(2, n, 2 * hd, std=0.1), normal(3, n, 2 * hd)
+    Q[:, 0] = Q[:, hd] = 8.0
+    ramp = (torch.arange(n, device="cuda") // 50).half() * 4
+    for sign in (1, -1):
+        K[:, 0] = K[:, hd] = sign * ramp
+        for rows in (200, 1):
+            run_attention(et, Q[:rows], K, V, hd, [(0, rows, 0, n, n - rows)], k_start=[0], k_lens=[n], max_q=rows)
+            run_attention(et, Q[:rows], K, V, hd, [(0, rows, 0, n, n - rows)], k_start=[0], k_lens=[n], max_q=rows, slopes=torch.tensor([0.5, 0.01], device="cuda"), window=(-1, 0))
 
 
 @pytest.mark.parametrize("single", [False, True])

@@ -277,28 +277,21 @@ _kept = None
 
 
 def _torch_kept():
-    """(lookup of the current device, float16, int32, float32): fetched once, these calls are short."""
+    """(lookup of the current device, of a device's current stream, float16, int32, float32): fetched once, these calls are short."""
     global _kept
     if _kept is None:
         import torch
-        torch.cuda.init()
-        _kept = (getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device), torch.float16, torch.int32, torch.float32)
+        raw_stream()   # initialises CUDA
+        try:
+            _kept = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.float16, torch.int32, torch.float32)
+        except AttributeError:
+            _kept = (torch.cuda.current_device, lambda device: raw_stream(), torch.float16, torch.int32, torch.float32)
     return _kept
 
 
 def _refuse(name, t, dtype, dims, device):
     raise ValueError(f"{name}: a {dims}-dimensional {dtype} tensor on the current CUDA device ({device}) expected, the elements of a row neighbours, rows "
                      f"one behind the other; not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-
-
-def _rows(name, t, dtype, device):
-    """(rows, features, pitch) of a matrix that may be a slice of a wider one."""
-    if t.dtype is dtype and t.get_device() == device and t.dim() == 2:
-        rows, features = t.shape
-        pitch, step = t.stride()
-        if step == 1 or features == 1:
-            return rows, features, pitch if rows > 1 else features
-    _refuse(name, t, dtype, 2, device)
 
 
 def _array(name, t, dtype, device, n):
@@ -321,29 +314,35 @@ def rotary_axes(q_out, k_out, q, k, positions, inv_freq, axis, head_dim, interle
     """Rotary positions over several axes on the heads of q [tokens, heads * head_dim] and k (either may be None); rows may be slices of
     wider ones, q_out may be q and k_out may be k. positions [tokens, axes] int32; inv_freq float32 and axis int32, one for each
     pair of features (twice as many features are turned). Returns (q_out, k_out)."""
-    current, f16, i32, f32 = _kept or _torch_kept()
+    current, stream_of, f16, i32, f32 = _kept or _torch_kept()
     device = current()
-    tokens, axes = _matrix("positions", positions, i32, device)
+    tokens, axes = positions.shape
     pairs = inv_freq.numel()
-    rc = (_entries or _lib()).et_rotary_axes(*_turned("q", q, q_out, tokens, head_dim, f16, device), *_turned("k", k, k_out, tokens, head_dim, f16, device), head_dim, 2 * pairs,
-                                             positions.data_ptr(), axes, _array("inv_freq", inv_freq, f32, device, pairs), _array("axis", axis, i32, device, pairs),
-                                             1 if interleaved else 0, tokens, raw_stream(stream))
+    if (positions.dtype is not i32 or axis.dtype is not i32 or inv_freq.dtype is not f32 or positions.get_device() != device or axis.get_device() != device
+            or inv_freq.get_device() != device or axis.numel() != pairs or not positions.is_contiguous() or not axis.is_contiguous() or not inv_freq.is_contiguous()):
+        raise ValueError(f"positions int32 [tokens, axes], inv_freq float32 and axis int32 [pairs], contiguous, on the current CUDA device ({device}) expected, not "
+                         + ", ".join(f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for t in (positions, inv_freq, axis)))
+    nq = nk = q_pitch = k_pitch = q_out_pitch = k_out_pitch = 0
+    q_at = k_at = q_out_at = k_out_at = None
+    if q is not None:
+        q_at, q_out_at, q_pitch, q_out_pitch, nq = _turned("q", q, q_out, tokens, head_dim, f16, device)
+    if k is not None:
+        k_at, k_out_at, k_pitch, k_out_pitch, nk = _turned("k", k, k_out, tokens, head_dim, f16, device)
+    rc = (_entries or _lib()).et_rotary_axes(q_out_at, q_at, q_out_pitch, q_pitch, nq, k_out_at, k_at, k_out_pitch, k_pitch, nk, head_dim, 2 * pairs, positions.data_ptr(), axes,
+                                             inv_freq.data_ptr(), axis.data_ptr(), 1 if interleaved else 0, tokens, stream_of(device) if stream is None else stream.cuda_stream)
     if rc:
         check(rc)
     return q_out, k_out
 
 
 def _turned(name, x, out, tokens, head_dim, f16, device):
-    """(addresses and pitches of the result and of x, heads)."""
-    if x is None:
-        return None, None, 0, 0, 0
-    if x.dtype is f16 and out.dtype is f16 and x.get_device() == device and out.get_device() == device and x.dim() == 2:
-        shape = rows, width = x.shape
-        pitch, step = x.stride()
-        if rows == tokens and width % head_dim == 0 and step == 1 and out.shape == shape:
-            pitch_out, step = out.stride()
-            if step == 1:
-                return out.data_ptr(), x.data_ptr(), pitch_out if rows > 1 else width, pitch if rows > 1 else width, width // head_dim
+    """(addresses and pitches of x and of its result, heads)."""
+    rows, width = shape = x.shape
+    pitch, step = x.stride()
+    out_pitch, out_step = out.stride()
+    if (x.dtype is f16 and out.dtype is f16 and x.get_device() == device and out.get_device() == device and rows == tokens and width % head_dim == 0 and out.shape == shape
+            and step == 1 and out_step == 1):
+        return (x.data_ptr(), out.data_ptr(), pitch, out_pitch, width // head_dim) if rows > 1 else (x.data_ptr(), out.data_ptr(), width, width, width // head_dim)
     raise ValueError(f"{name}: {tokens} rows of whole float16 heads of {head_dim} on the current CUDA device ({device}), neighbouring elements, and the result alike expected, "
                      f"not {x.dtype} {tuple(x.shape)} on {x.device} and {out.dtype} {tuple(out.shape)} on {out.device}")
 
@@ -370,17 +369,23 @@ class AdapterBank:
     def add(self, out, base, x, adapter_ids, cu_seqlens=None, stream=None):
         """out = base + the adapter's product for each sequence's tokens. adapter_ids int32 [batch] (-1: none), cu_seqlens int32 [batch + 1]
         or None (one token to a sequence). out may be base; rows may be slices of wider ones."""
-        current, f16, i32, _ = _kept or _torch_kept()
+        current, stream_of, f16, i32, _ = _kept or _torch_kept()
         device = current()
-        rows, width, x_pitch = _rows("x", x, f16, device)
-        base_rows, base_width, base_pitch = _rows("base", base, f16, device)
-        out_rows, out_width, out_pitch = _rows("out", out, f16, device)
-        if width != self.in_feat or base_width != self.out_feat or out_width != self.out_feat or base_rows != rows or out_rows != rows:
-            raise ValueError(f"x [{rows}, {self.in_feat}], base and out [{rows}, {self.out_feat}] expected, not {tuple(x.shape)}, {tuple(base.shape)}, {tuple(out.shape)}")
-        batch = adapter_ids.shape[0]
+        rows, width = x.shape
+        shape = base.shape
+        x_pitch, x_step = x.stride()
+        base_pitch, base_step = base.stride()
+        out_pitch, out_step = out.stride()
+        if (x.dtype is not f16 or base.dtype is not f16 or out.dtype is not f16 or x.get_device() != device or base.get_device() != device or out.get_device() != device
+                or width != self.in_feat or shape != out.shape or shape != (rows, self.out_feat) or x_step != 1 or base_step != 1 or out_step != 1):
+            raise ValueError(f"float16 x [{rows}, {self.in_feat}], base and out [{rows}, {self.out_feat}] on the current CUDA device ({device}) with neighbouring elements expected, not "
+                             f"{x.dtype} {tuple(x.shape)} on {x.device}, {base.dtype} {tuple(base.shape)} on {base.device}, {out.dtype} {tuple(out.shape)} on {out.device}")
+        if rows <= 1:
+            x_pitch, base_pitch, out_pitch = width, self.out_feat, self.out_feat
+        batch = adapter_ids.numel()
         rc = (_entries or _lib()).et_adapter_add(self._h, out.data_ptr(), base.data_ptr(), x.data_ptr(), out_pitch, base_pitch, x_pitch,
-                                                 None if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), _array("adapter_ids", adapter_ids, i32, device, batch),
-                                                 batch, rows, raw_stream(stream))
+                                                 None if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1),
+                                                 _array("adapter_ids", adapter_ids, i32, device, batch), batch, rows, stream_of(device) if stream is None else stream.cuda_stream)
         if rc:
             check(rc)
         return out
@@ -413,14 +418,24 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
     """Attention with rules on its scores (capped, biased by distance, seen through windows, prefixes and documents) over packed sequences, or of
     tokens over keys kept from before (k_start, k_lens). Q and out [tokens, heads * head_dim], K and V [rows, kv_heads * head_dim], rows may be
     slices of wider ones; see et_attention_rules for each argument. max_q_len, max_k_len: 0 takes the number of rows."""
-    current, f16, i32, f32 = _kept or _torch_kept()
+    current, stream_of, f16, i32, f32 = _kept or _torch_kept()
     device = current()
-    tokens, width, q_pitch = _rows("Q", Q, f16, device)
-    k_rows, kv_width, k_pitch = _rows("K", K, f16, device)
-    _, _, out_pitch = _rows("out", out, f16, device)
-    _, _, v_pitch = _rows("V", V, f16, device)
-    if out.shape != Q.shape or V.shape != K.shape or width % head_dim or kv_width % head_dim or not kv_width or not width:
-        raise ValueError(f"whole heads of {head_dim}, out like Q and V like K expected, not {tuple(Q.shape)}, {tuple(out.shape)}, {tuple(K.shape)}, {tuple(V.shape)}")
+    q_shape, k_shape = Q.shape, K.shape
+    tokens, width = q_shape
+    k_rows, kv_width = k_shape
+    q_pitch, q_step = Q.stride()
+    k_pitch, k_step = K.stride()
+    v_pitch, v_step = V.stride()
+    out_pitch, out_step = out.stride()
+    if (Q.dtype is not f16 or K.dtype is not f16 or V.dtype is not f16 or out.dtype is not f16 or Q.get_device() != device or K.get_device() != device
+            or V.get_device() != device or out.get_device() != device or out.shape != q_shape or V.shape != k_shape or width % head_dim or kv_width % head_dim
+            or not kv_width or not width or (q_step, k_step, v_step, out_step) != (1, 1, 1, 1) and min(width, kv_width) > 1):
+        raise ValueError(f"float16 rows of whole heads of {head_dim} on the current CUDA device ({device}) with neighbouring elements, out like Q and V like K expected, not "
+                         + ", ".join(f"{n} {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for n, t in (("Q", Q), ("out", out), ("K", K), ("V", V))))
+    if tokens <= 1:
+        q_pitch = out_pitch = width
+    if k_rows <= 1:
+        k_pitch = v_pitch = kv_width
     nhead, nhead_kv = width // head_dim, kv_width // head_dim
     reach = table = 0
     if distance_bias is not None:
@@ -440,7 +455,7 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
         out.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), out_pitch, q_pitch, k_pitch, v_pitch, nhead, nhead_kv, head_dim,
         None if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), None if k_start is None else _array("k_start", k_start, i32, device, batch),
         None if k_lens is None else _array("k_lens", k_lens, i32, device, batch), batch, tokens, k_rows, max_q_len or tokens, max_k_len or k_rows, rules,
-        None if scratch is None else scratch.data_ptr(), scratch_bytes, raw_stream(stream))
+        None if scratch is None else scratch.data_ptr(), scratch_bytes, stream_of(device) if stream is None else stream.cuda_stream)
     if rc:
         check(rc)
     return out

@@ -1,0 +1,76 @@
+// Low-rank adapters: what the two kernels share.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace et {
+
+struct AdapterSlot {
+    int rank;      // 0: nothing to add
+    float scale;
+};
+
+struct AdapterParams {
+    half* out;
+    const half* base;
+    const half* x;
+    const int* cu_seqlens;
+    const int* ids;
+    const AdapterSlot* slots;
+    const half *a, *b;                  // packed, all slots: for the kernel that is launched
+    long long out_pitch, base_pitch, x_pitch, a_stride, b_stride;   // of a slot, in elements
+    int batch, tokens, n_slots, in_feat, out_feat;
+    int n_split;                        // CTAs that share a tile's columns, each with all of A x
+    int* err;                           // of bounded waits
+    bool copy;                          // out is not base: what has no adapter is copied
+};
+
+// The tile of `size` tokens with number `tile`: sequence, first token, tokens (whole warp). Without cu_seqlens a sequence is one token.
+__device__ __forceinline__ int find_tile(const AdapterParams& p, int tile, int size, int& seq, int& t0) {
+    const int lane = threadIdx.x & 31;
+    if (!p.cu_seqlens) {
+        seq = t0 = tile;
+        return tile < p.batch ? 1 : 0;
+    }
+    for (int base = 0; base < p.batch; base += 32) {
+        const int i = base + lane;
+        const int first = i < p.batch ? p.cu_seqlens[i] : 0;
+        const int len = i < p.batch ? max(p.cu_seqlens[i + 1] - first, 0) : 0;
+        const int n = (len + size - 1) / size;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, tile < incl);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            const int at = (tile - __shfl_sync(0xffffffffu, incl - n, src)) * size;
+            seq = base + src;
+            t0 = __shfl_sync(0xffffffffu, first, src) + at;
+            const int end = min(__shfl_sync(0xffffffffu, first + len, src), p.tokens);   // (never beyond the rows that there are)
+            return t0 < 0 ? 0 : max(min(end - t0, size), 0);
+        }
+        tile -= __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return 0;
+}
+
+// The power of two (its exponent's bits) that brings a row of A x with that largest value into [1, 2): infinity stays one; below 2^-100 it makes no difference
+// to the result.
+__device__ __forceinline__ int row_exponent(float top) {
+    const int e = __float_as_int(top) >> 23;
+    return e == 255 ? 127 : max(27, min(e, 227));
+}
+
+// tcgen05 kernel for many tokens (adapter_tc.cu): rank_step 16, 32, 64 or 128, the rank that the bank's slots are laid out for.
+int adapter_tc_launch(AdapterParams p, int rank_step, cudaStream_t st);
+// Elements of a slot in the layouts that it takes, and the layouts: A [chunk of 64 features][rank_step][64] with 128-byte swizzle, B [unit of 64 columns]
+// [8 columns][8 ranks] as core matrices of 8 columns x 16 bytes.
+long long adapter_tc_a_stride(int in_feat, int rank_step);
+long long adapter_tc_b_stride(int out_feat, int rank_step);
+void adapter_tc_pack(half* pa, half* pb, const half* A, const half* B, int rank, int in_feat, int out_feat, int rank_step);
+
+}  // namespace et

@@ -176,7 +176,8 @@ int et_rotary_axes(void* q_out, const void* q, int q_out_pitch, int q_pitch, int
 /* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference, which holds one set of weights) ----
  * A bank holds n_slots adapters of one projection, each of rank up to max_rank (1 to 128): A [rank x in_feat], B [out_feat x rank] and a
  * scale. It allocates its memory on the current device and synchronises it, as et_adapter_bank_set does, which copies an adapter from HOST
- * arrays into a slot (rank 0: the slot is empty again): not while another thread launches with the bank. in_feat and out_feat are multiples of 16. */
+ * arrays into a slot (rank 0: the slot is empty again): not while another thread launches with the bank. in_feat and out_feat are multiples of 16.
+ * The weights are held in two layouts (for few tokens and for many), ranks rounded up to 16, 32, 64 or 128. */
 typedef struct et_adapter_bank et_adapter_bank;
 int et_adapter_bank_create(et_adapter_bank** out, int in_feat, int out_feat, int max_rank, int n_slots);
 int et_adapter_bank_destroy(et_adapter_bank* bank);

@@ -138,6 +138,46 @@ def test_adapters_of_many_tokens(et, k, n, max_rank, ranks):
     check_adapter(et, bank, held, lengths, [0, 1, -1, 0, 0, 1, 0, -1], k, n, pad=8)
 
 
+@pytest.mark.parametrize("k,n,max_rank,ranks,lengths", [
+    (64, 80, 16, [16, 3], [20000, 5, 17000, 3003, 1, 0, 8192]),                              # more than one wave of tiles
+    (144, 64, 32, [20, 32], [9 + i * 7 % 32 for i in range(600)]),                           # many short sequences
+    (1024, 4096, 64, [64, 50], [1800, 1, 1799]), (4096, 1024, 128, [128, 65], [5003]),       # few tokens, wide: the columns of a tile are shared
+    (768, 2304, 8, [8, 5], [128] * 64 + [7] * 3), (80, 1008, 48, [48, 33], [8192]), (32, 16, 100, [100, 1], [72, 8130])])
+def test_adapters_of_many_tokens_in_other_shapes(et, k, n, max_rank, ranks, lengths):
+    bank, held = make_bank(et, k, n, max_rank, ranks)
+    check_adapter(et, bank, held, lengths, [(i + i // 3) % (len(ranks) + 1) - 1 if i else 0 for i in range(len(lengths))], k, n, pad=8)
+    et.attention_check()
+
+
+@pytest.mark.parametrize("rank", [5, 48, 128])
+def test_adapter_rows_of_many_tokens_do_not_mix(et, rank):
+    """Infinities, what is no number and values whose A x is beyond fp16 stay in their rows; so does a sequence's adapter of infinities."""
+    import torch
+    k, n = 256, 320
+    bank, held = make_bank(et, k, n, rank, [rank, rank])
+    lengths, ids = [4500, 3, 4000, 900], [0, 1, -1, 0]
+    cu = np.concatenate([[0], np.cumsum(lengths)])
+    x, base = normal(1, 9403, k), normal(2, 9403, n)
+    x[77], x[4400, 9], x[4502, 0], base[8600, 5] = 60000.0, math.inf, math.nan, math.inf
+    x[9000] = 1.0e-7
+    want, bound = ol.adapter(base, x, cu, ids, held)
+    out = bank.add(torch.zeros_like(base), base, x, dev(ids), cu_seqlens=dev(cu))
+    odd = torch.zeros_like(out, dtype=torch.bool)
+    odd[4400] = odd[4502] = True
+    odd[8600, 5] = True
+    assert not torch.isfinite(out[4400]).any() and torch.isnan(out[4502]).all() and torch.isinf(out[8600, 5])
+    over = want.abs() > 65504 * (1 - 2.0 ** -10)   # the result itself is beyond the type
+    look = ~odd & ~over
+    ol.assert_within(torch.where(look, out, 0.0), torch.where(look, want, 0.0), torch.where(look, bound, 0.0), "rows")
+    huge = A, B = torch.full((rank, k), 60000.0).half(), torch.ones(n, rank).half()
+    bank.set(1, A.numpy(), B.numpy(), 1.0)
+    again = bank.add(torch.zeros_like(base), base, x, dev(ids), cu_seqlens=dev(cu))
+    same = torch.ones(9403, dtype=torch.bool, device="cuda")
+    same[4500:4503] = False
+    same[4400] = False
+    assert torch.equal(again[same], out[same]) and huge
+
+
 @pytest.mark.parametrize("batch", [1, 3, 64, 300])
 @pytest.mark.parametrize("k,n,max_rank,ranks", [(1024, 1024, 16, [16] * 5), (768, 2304, 64, [64, 1, 0, 40]), (4096, 1024, 128, [128, 16]), (32, 48, 8, [8, 8])])
 def test_adapters_of_single_tokens(et, k, n, max_rank, ranks, batch):

@@ -5,8 +5,8 @@
 // What bounds it: HBM, each head is read and written once. The angle is taken in 64 bits: of a position of a million an fp32 product keeps
 // four digits behind the point. In turns (multiplied by 1 / 2 pi) it loses its whole part there, and sine and cosine of the rest are fp32
 // (sincospif). A block requests its heads, 16 bytes and four heads to a thread, takes the angles of its tokens meanwhile, once for all heads, and leaves
-// them in shared memory; a thread keeps the eight that it needs in registers. 32768 tokens of 32 heads of 64 take 43 us, 6.2 TB/s; with the heads requested
-// behind the angles and a warp's rows in different tokens 56.
+// them in shared memory; a thread keeps the eight that it needs in registers. 32768 tokens of 32 heads of 64 take 41 us, 6.5 TB/s; with the heads requested
+// behind the angles and a warp's rows in different tokens 56. 5003 tokens of 40 heads of 128, neighbours, 96 features turned: 18 us, 5.6 TB/s.
 #include "common.h"
 
 namespace et {
@@ -18,7 +18,7 @@ constexpr int kHeadsInFlight = 4;
 enum Pairing {
     kHalves8 = 0,      // pairs half a rotated width apart, that half a multiple of 8: a thread has eight pairs, two granules of 16 bytes
     kHalves = 1,       // the same for any half: a thread has a granule and fetches the partners of its features, which straddle two others
-    kNeighbours = 2,   // pairs of neighbouring features: a granule has its own partners
+    kNeighbours = 2,   // pairs of neighbouring features: a granule has its own partners, a thread four pairs
     kScalar = 3,       // anything else (heads or rows that do not start on 16 bytes): a thread has one pair
 };
 
@@ -30,7 +30,7 @@ struct RotaryParams {
     const float* inv_freq;
     const int* axis;
     int nhead_q, nhead_k, head_dim, rot, n_axes, tokens;
-    int lanes;            // threads to a head (a power of two, so that a head lies inside a warp)
+    int lanes;            // threads to a head (kHalves: a power of two, so that a head lies inside a warp)
     int block_tokens, head_step;   // tokens of a block, heads of each that it takes at a time
     bool interleaved;
     bool in_place_q, in_place_k;
@@ -65,13 +65,10 @@ __global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_consta
     const int head_step = p.head_step, t = row / head_step, first_head = row % head_step;
     const bool token_in = t < nt;
     const float2* const cs = turns + min(t, nt - 1) * pairs;
-    auto src = [&](int h) {
-        return h < p.nhead_q ? p.q + (size_t)(t0 + t) * p.q_pitch + h * p.head_dim : p.k + (size_t)(t0 + t) * p.k_pitch + (h - p.nhead_q) * p.head_dim;
-    };
-    auto dst = [&](int h) {
-        return h < p.nhead_q ? p.q_out + (size_t)(t0 + t) * p.q_out_pitch + h * p.head_dim
-                             : p.k_out + (size_t)(t0 + t) * p.k_out_pitch + (h - p.nhead_q) * p.head_dim;
-    };
+    const long long q_row = (t0 + t) * p.q_pitch, k_row = (t0 + t) * p.k_pitch - p.nhead_q * p.head_dim;
+    const long long q_out_row = (t0 + t) * p.q_out_pitch, k_out_row = (t0 + t) * p.k_out_pitch - p.nhead_q * p.head_dim;
+    auto src = [&](int h) { return (h < p.nhead_q ? p.q + q_row : p.k + k_row) + h * p.head_dim; };
+    auto dst = [&](int h) { return (h < p.nhead_q ? p.q_out + q_out_row : p.k_out + k_out_row) + h * p.head_dim; };
     auto in_place = [&](int h) { return h < p.nhead_q ? p.in_place_q : p.in_place_k; };
     // The block's angles, into shared memory. Called when the first heads are already on their way.
     auto take_angles = [&]() {
@@ -137,31 +134,62 @@ __global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_consta
                 if (h >= heads || (!turns_it && in_place(h))) continue;
                 half* const y = dst(h) + at;
                 if (turns_it) {
-                    float u[8], v[8], x[8], z[8];
-                    unpack8(a[k], u);
-                    unpack8(b[k], v);
+                    half2 *const u = reinterpret_cast<half2*>(&a[k]), *const v = reinterpret_cast<half2*>(&b[k]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        x[i] = u[i] * c[i] - v[i] * s[i];
-                        z[i] = u[i] * s[i] + v[i] * c[i];
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 x = __half22float2(u[i]), z = __half22float2(v[i]);
+                        u[i] = __floats2half2_rn(x.x * c[2 * i] - z.x * s[2 * i], x.y * c[2 * i + 1] - z.y * s[2 * i + 1]);
+                        v[i] = __floats2half2_rn(x.x * s[2 * i] + z.x * c[2 * i], x.y * s[2 * i + 1] + z.y * c[2 * i + 1]);
                     }
-                    a[k] = pack8(x);
-                    *reinterpret_cast<uint4*>(y + pairs) = pack8(z);
+                    *reinterpret_cast<uint4*>(y + pairs) = b[k];
                 }
                 *reinterpret_cast<uint4*>(y) = a[k];
             }
         }
+    } else if constexpr (kPairing == kNeighbours) {
+        const int at = lane * 8, n_turned = max(0, min(4, (p.rot - at) / 2));   // pairs of the granule that are turned; the others are passed on
+        const bool in = token_in && at < p.head_dim && (n_turned > 0 || !(p.in_place_q && p.in_place_k));
+        uint4 a[kHeadsInFlight];
+        auto fetch = [&](int h0) {
+#pragma unroll
+            for (int k = 0; k < kHeadsInFlight; ++k) {
+                const int h = h0 + k * head_step;
+                if (in && h < heads) a[k] = *reinterpret_cast<const uint4*>(src(h) + at);
+            }
+        };
+        fetch(first_head);
+        take_angles();
+        if (!in) return;
+        float2 turn[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) turn[i] = i < n_turned ? cs[at / 2 + i] : make_float2(1.f, 0.f);
+        for (int h0 = first_head; h0 < heads; h0 += head_step * kHeadsInFlight) {
+            if (h0 != first_head) fetch(h0);
+#pragma unroll
+            for (int k = 0; k < kHeadsInFlight; ++k) {
+                const int h = h0 + k * head_step;
+                if (h >= heads) continue;
+                half2* const x = reinterpret_cast<half2*>(&a[k]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 v = __half22float2(x[i]);
+                    const half2 z = __floats2half2_rn(v.x * turn[i].x - v.y * turn[i].y, v.x * turn[i].y + v.y * turn[i].x);
+                    x[i] = i < n_turned ? z : x[i];
+                }
+                *reinterpret_cast<uint4*>(dst(h) + at) = a[k];
+            }
+        }
     } else {
-        // A granule of eight features to a thread. Other threads of the warp may read what this one writes (kHalves in place), so
-        // a warp writes once all its lanes have read; every lane stays for that.
+        // A granule of eight features to a thread. Other threads of the warp may read what this one writes (in place), so a warp writes once all
+        // its lanes have read; every lane stays for that.
         const int at = lane * 8;
         const bool in = token_in && at < p.head_dim;
         const int n_turned = max(0, min(8, p.rot - at));   // the others are passed on
-        // kHalves: the partners of features at .. at + 7 are at + pairs .. (first half) or at - pairs .. (second half); a granule that
+        // The partners of features at .. at + 7 are at + pairs .. (first half) or at - pairs .. (second half); a granule that
         // holds features of both halves has partners of both kinds, eight of each
         const int up = at + pairs, down = at - pairs;
-        const bool need_up = kPairing == kHalves && in && at < pairs && n_turned > 0;
-        const bool need_down = kPairing == kHalves && in && at + n_turned > pairs && n_turned > 0;
+        const bool need_up = in && at < pairs && n_turned > 0;
+        const bool need_down = in && at + n_turned > pairs && n_turned > 0;
         auto eight_from = [&](const half* x, int d) {   // features d .. d + 7 of a head, those outside of it as zeros
             const int g = d >> 3, shift = d & 7;        // (arithmetic: down to -1)
             const int last = (p.head_dim >> 3) - 1;
@@ -189,11 +217,9 @@ __global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_consta
                 const int h = h0 + k * head_step;
                 if (!in || h >= heads) continue;
                 a[k] = *reinterpret_cast<const uint4*>(src(h) + at);
-                if constexpr (kPairing == kHalves) {
-                    bu[k] = bd[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (need_up) bu[k] = eight_from(src(h), up);
-                    if (need_down) bd[k] = eight_from(src(h), down);
-                }
+                bu[k] = bd[k] = make_uint4(0u, 0u, 0u, 0u);
+                if (need_up) bu[k] = eight_from(src(h), up);
+                if (need_down) bd[k] = eight_from(src(h), down);
             }
         };
         fetch(first_head);
@@ -202,8 +228,8 @@ __global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const int d = at + i;
-            const bool second = kPairing == kNeighbours ? (i & 1) : d >= pairs;
-            const int pair = kPairing == kNeighbours ? d >> 1 : (second ? d - pairs : d);
+            const bool second = d >= pairs;
+            const int pair = second ? d - pairs : d;
             const float2 v = cs[i < n_turned ? pair : 0];
             c[i] = v.x;
             s[i] = second ? v.y : -v.y;
@@ -212,23 +238,18 @@ __global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const __grid_consta
         for (int n = 0; n < iterations; ++n) {
             const int h0 = first_head + n * head_step * kHeadsInFlight;
             if (n) fetch(h0);
-            if constexpr (kPairing == kHalves) __syncwarp();
+            __syncwarp();
 #pragma unroll
             for (int k = 0; k < kHeadsInFlight; ++k) {
                 const int h = h0 + k * head_step;
                 if (!in || h >= heads) continue;
                 float x[8], partner[8], z[8];
                 unpack8(a[k], x);
-                if constexpr (kPairing == kNeighbours) {
+                float u[8], d[8];
+                unpack8(bu[k], u);
+                unpack8(bd[k], d);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) partner[i] = x[i ^ 1];
-                } else {
-                    float u[8], d[8];
-                    unpack8(bu[k], u);
-                    unpack8(bd[k], d);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) partner[i] = at + i < pairs ? u[i] : d[i];
-                }
+                for (int i = 0; i < 8; ++i) partner[i] = at + i < pairs ? u[i] : d[i];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) z[i] = i < n_turned ? x[i] * c[i] + partner[i] * s[i] : x[i];
                 *reinterpret_cast<uint4*>(dst(h) + at) = pack8(z);
@@ -273,12 +294,14 @@ extern "C" int et_rotary_axes(void* q_out, const void* q, int q_out_pitch, int q
     const int want = pairing == kScalar ? min(32, max(1, pairs)) : pairing == kHalves8 ? pairs / 8 + (head_dim - rot_dim) / 8 : head_dim / 8;
     p.lanes = 1;
     while (p.lanes < want) p.lanes *= 2;
+    if (pairing == kHalves8 || pairing == kNeighbours) p.lanes = want;   // (5003 tokens of 40 heads of 128, 96 features turned: ten lanes 21.4 us, sixteen 32)
     // A thread has kHeadsInFlight heads, all requested at once, one where there are few tokens; a block has as many tokens as make 128 threads, but no more
-    // than leave every SM four blocks. (32768 tokens of 32 heads of 64 in blocks of 128, 256, 512 threads: 43.4, 45.7, 61.1 us, with two heads to a thread 48.8,
-    // eight 53.9; 64 tokens of 24 heads with one, two, four, eight: 2.2, 2.2, 2.9, 4.2.)
+    // than leave every SM eight blocks. (32768 tokens of 32 heads of 64 in blocks of 128, 256, 512 threads: 42.7, 45.0, 61.1 us, with two heads to a thread 44.4,
+    // three 45.4, four 41.9, neighbours with four, six, eight 41.0, 43.0, 42.3; 4000 tokens of 24 heads with four blocks to an SM 7.2, eight 6.8; 64 tokens
+    // of 24 heads with one, two, four, eight heads: 2.2, 2.2, 2.9, 4.2.)
     const int heads = nhead_q + nhead_k, in_flight = tokens > sm_count() * 4 ? kHeadsInFlight : 1;
     p.head_step = max(1, min((heads + in_flight - 1) / in_flight, kMaxThreads / p.lanes));
-    p.block_tokens = max(1, min(128 / (p.head_step * p.lanes), tokens / (sm_count() * 4)));
+    p.block_tokens = max(1, min(128 / (p.head_step * p.lanes), tokens / (sm_count() * 8)));
     const int threads = (p.block_tokens * p.head_step * p.lanes + 31) / 32 * 32;
     const int blocks = (tokens + p.block_tokens - 1) / p.block_tokens;
     const size_t smem = (size_t)p.block_tokens * max(pairs, 1) * sizeof(float2);

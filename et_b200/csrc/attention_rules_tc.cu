@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 ok = mbar_wait_at(ET_BAR(m_empty, m), ((g >> 1) & 1u) ^ 1u);
                 if (!ok) break;
                 const Item& it = sh->item[b.item];
-                if (b.flags & kMixed) sh->docs[m][t] = t < b.left ? r.k_docs[it.seq.k0 + b.j * kBK + t] : -1;
+                if (b.flags & kMixed) sh->docs[m][t] = t < b.left ? max(r.k_docs[it.seq.k0 + b.j * kBK + t], -1) : -1;
                 if constexpr (kBias == kTable) {
                     // value n of copy s: the bias of a key n + s - 127 behind the first key's distance to the first query
                     const half* const row = r.table + (size_t)it.head * (2 * r.reach + 1) + r.reach;
@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             const int prefix = it.seq.prefix;
             int my_doc = 0;
             if (docs) my_doc = it.qi0 + row < it.seq.qlen ? r.q_docs[it.seq.q0 + it.qi0 + row] : -1;
-            if (my_doc < 0) my_doc = -2;   // (keys behind the last one count as -1)
+            if (my_doc < 0) my_doc = -2;   // (keys behind the last one, and those of no document, count as -1)
             float slope = 0.f;
             if constexpr (kBias == kSlopes) slope = r.slopes[it.head] * -kRulesLog2e;
             float m_run = -INFINITY;

@@ -469,6 +469,24 @@ def test_attention_of_rows_that_see_nothing(et, hd):
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 40])
+@pytest.mark.parametrize("rule", [{}, {"window": (70, 5)}, {"window": (-1, 0), "slopes": True}, {"cap": 20.0, "prefixes": [100, 3]}])
+def test_attention_of_documents_in_any_order(et, hd, rule):
+    """Numbers in any order, as many as keys, up to the largest; several numbers below 0 on both sides, which see and are seen by nothing."""
+    import torch
+    lengths = [500, 203]
+    Q, K, V, cu, seqs = packed(1, lengths, 4, 2, hd)
+    rule = {**rule, **({"slopes": torch.rand(4, device="cuda")} if rule.get("slopes") else {})}
+    r = np.random.default_rng(3)
+    n = len(Q)
+    for docs in (r.integers(-4, 5, n), r.permutation(n) // 2, r.choice([-(1 << 31), -2, -1, 0, (1 << 31) - 1], n), np.arange(n) // 40 - 3, -1 - np.arange(n) % 3):
+        other = np.where(r.random(n) < 0.5, docs, r.permutation(docs))
+        for pair in ((docs, docs), (docs, other)):
+            out = run_attention(et, Q, K, V, hd, seqs, cu=cu, docs=(dev(pair[0]), dev(pair[1])), **rule)
+            assert (out[torch.as_tensor(pair[0] < 0, device="cuda")] == 0).all()
+    et.attention_check()
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("single", [False, True])
 def test_attention_of_large_scores(et, hd, single):

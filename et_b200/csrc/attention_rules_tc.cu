@@ -256,16 +256,22 @@ __device__ __forceinline__ bool find_item(const TcRules& p, const SeqTable* t, i
     }
 }
 
-// The blocks of keys that an item's queries see, in order (whole warp): the prefix's blocks, then the window's; of documents those whose range meets the queries'.
+// The blocks of keys that an item's queries see (whole warp): the prefix's blocks, then the window's; of documents those whose range meets the queries'. With slopes
+// from the queries on to the end, then from the queries back to the beginning: so the largest scores tend to come first, while in order every block before the
+// queries raises the maximum and O is rescaled. (4 x 4096 tokens, 16 heads of 64: 599 us in order, 507 so.)
 struct Blocks {
     const int2* summary;
     int n_prefix, first, n;        // blocks of the prefix, the window's first block behind them, all of them
+    int turn;                      // how many lie before the queries and come last, in reverse
     int at;                        // the next one to look at; documents: behind the 32 looked at
     unsigned seen, whole;          // documents: of the 32 looked at, those to come, and those of one document with all queries
     int d_lo, d_hi;                // lowest and highest of the queries
     bool d_odd;                    // some query is of none
 
-    __device__ __forceinline__ int number(int i) const { return i < n_prefix ? i : first + i - n_prefix; }
+    __device__ __forceinline__ int number(int i) const {
+        i = i < n - turn ? i + turn : n - 1 - i;
+        return i < n_prefix ? i : first + i - n_prefix;
+    }
     __device__ __forceinline__ void start(const TcRules& p, const Item& it, int lane) {
         const RuleParams& r = p.r;
         const RuleSeq& s = it.seq;
@@ -276,6 +282,11 @@ struct Blocks {
         const int hi = r.window_right == kNoLimit ? s.klen - 1 : min(qb + r.window_right, s.klen - 1);
         first = max(lo / kBK, n_prefix);
         n = n_prefix + (hi >= lo ? max(hi / kBK - first + 1, 0) : 0);
+        turn = 0;
+        if (r.slopes) {
+            const int j = max(qa, 0) / kBK;   // the first query's block
+            turn = min(j < n_prefix ? j : n_prefix + max(j - first, 0), n);
+        }
         at = 0;
         if (p.summary) {
             int lowest = 0x7fffffff, highest = -1;

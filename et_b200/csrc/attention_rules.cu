@@ -41,7 +41,7 @@ cudaError_t attention_rules_rows_launch(const RuleParams& p, cudaStream_t st) {
 
 extern "C" size_t et_attention_rules_scratch_size(int batch, int max_k_len) {
     if (batch <= 0 || max_k_len <= 0) return 0;
-    return (size_t)batch * (size_t)((max_k_len + 63) / 64) * 8;
+    return (size_t)batch * (((size_t)max_k_len + 63) / 64) * 8;
 }
 
 extern "C" int et_attention_rules(void* out, const void* Q, const void* K, const void* V, int out_pitch, int q_pitch, int k_pitch, int v_pitch,

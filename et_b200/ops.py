@@ -340,7 +340,7 @@ def _turned(name, x, out, tokens, head_dim, f16, device):
     rows, width = shape = x.shape
     pitch, step = x.stride()
     out_pitch, out_step = out.stride()
-    if (x.dtype is f16 and out.dtype is f16 and x.get_device() == device and out.get_device() == device and rows == tokens and width % head_dim == 0 and out.shape == shape
+    if (x.dtype is f16 and out.dtype is f16 and x.get_device() == device and out.get_device() == device and rows == tokens and head_dim > 0 and width % head_dim == 0 and out.shape == shape
             and step == 1 and out_step == 1):
         return (x.data_ptr(), out.data_ptr(), pitch, out_pitch, width // head_dim) if rows > 1 else (x.data_ptr(), out.data_ptr(), width, width, width // head_dim)
     raise ValueError(f"{name}: {tokens} rows of whole float16 heads of {head_dim} on the current CUDA device ({device}), neighbouring elements, and the result alike expected, "
@@ -428,7 +428,7 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
     v_pitch, v_step = V.stride()
     out_pitch, out_step = out.stride()
     if (Q.dtype is not f16 or K.dtype is not f16 or V.dtype is not f16 or out.dtype is not f16 or Q.get_device() != device or K.get_device() != device
-            or V.get_device() != device or out.get_device() != device or out.shape != q_shape or V.shape != k_shape or width % head_dim or kv_width % head_dim
+            or V.get_device() != device or out.get_device() != device or out.shape != q_shape or V.shape != k_shape or head_dim < 1 or width % head_dim or kv_width % head_dim
             or not kv_width or not width or (q_step, k_step, v_step, out_step) != (1, 1, 1, 1) and min(width, kv_width) > 1):
         raise ValueError(f"float16 rows of whole heads of {head_dim} on the current CUDA device ({device}) with neighbouring elements, out like Q and V like K expected, not "
                          + ", ".join(f"{n} {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for n, t in (("Q", Q), ("out", out), ("K", K), ("V", V))))

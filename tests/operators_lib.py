@@ -47,7 +47,7 @@ def attention(Q, K, V, head_dim, seqs, scale=None, cap=0.0, slopes=None, table=N
     sequence are not a number. What a query does not see takes no part, whatever it holds; a query that sees something that is not finite has bound infinity.
 
     The bound, of a result sum p v: the weights are rounded to fp16 (half a step, or 2^-25 of the reference weight 1 when far below it) after exponentials
-    with a relative error of 1.0e-4 at most, of scores with fp32 errors (head_dim products, then the cap's exponential and quotient, an
+    with a relative error of 2^-20 at most, of scores with fp32 errors (head_dim products, then the cap's exponential and quotient, an
     absolute error of some 2^-21 of the cap, then the bias); the result is rounded to fp16."""
     hd = head_dim
     H, Hk = Q.shape[1] // hd, K.shape[1] // hd
@@ -93,7 +93,7 @@ def attention(Q, K, V, head_dim, seqs, scale=None, cap=0.0, slopes=None, table=N
         total = p.sum(-1, keepdim=True)
         p = p / torch.where(total > 0, total, 1.0)
         err = err + 2.0 ** -22 * torch.where(seen, (top - s).clamp(min=0), 0.0)   # the difference to the maximum is rounded too
-        e = torch.where(seen, HALF + 1.0e-4 + 2.0 ** -20 + err, 0.0)
+        e = torch.where(seen, HALF + 2.0 ** -20 + err, 0.0)
         o = p @ v
         # weights and their sum are both off: the sum's error moves the whole result
         bd = (p * e) @ v.abs() + (p * (e - HALF).clamp(min=0)).sum(-1, keepdim=True) * o.abs()

@@ -185,6 +185,47 @@ def test_adapters_of_single_tokens(et, k, n, max_rank, ranks, batch):
     check_adapter(et, bank, held, [1] * batch, [(i * 5) % (len(ranks) + 1) - 1 for i in range(batch)], k, n, single=True)
 
 
+@pytest.mark.parametrize("lengths", [[1] * 64, [40, 300, 1], [5000, 4100, 77]])
+def test_adapters_in_a_graph_and_on_two_streams(et, lengths):
+    """Captured twice, replayed side by side with direct calls; a slot that is filled anew, ids and lengths that change are those of the replay."""
+    import torch
+    k, n, total = 256, 320, sum(lengths)
+    bank, held = make_bank(et, k, n, 16, [16, 9])
+    single = max(lengths) == 1
+    x, base = normal(5, total, k), normal(6, total, n)
+    cu = np.concatenate([[0], np.cumsum(lengths)])
+    ids = dev([i % 2 for i in range(len(lengths))])
+    cu_dev = None if single else dev(cu)
+    first = bank.add(torch.zeros_like(base), base, x, ids, cu_seqlens=cu_dev)
+    torch.cuda.synchronize()
+    outs, graphs, streams = [torch.zeros_like(base) for _ in range(2)], [], [torch.cuda.Stream() for _ in range(2)]
+    for out in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            bank.add(out, base, x, ids, cu_seqlens=cu_dev)
+        graphs.append(g)
+    direct = torch.zeros_like(base)
+    for _ in range(4):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        bank.add(direct, base, x, ids, cu_seqlens=cu_dev)
+    torch.cuda.synchronize()
+    assert all(torch.equal(t, first) for t in (*outs, direct))
+    A, B = normal(90, 4, k, std=k ** -0.5), normal(91, n, 4)
+    bank.set(1, A.cpu().numpy(), B.cpu().numpy(), 2.0)
+    held[1] = (A, B, 2.0)
+    ids.copy_(dev([1 - i % 2 for i in range(len(lengths))]))
+    if not single:
+        cu = np.array([0, 3, 3, total])
+        cu_dev.copy_(dev(cu))
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    want, bound = ol.adapter(base, x, cu, ids.tolist(), held)
+    ol.assert_within(outs[0], want, bound, "replayed")
+    et.attention_check()
+
+
 def test_adapter_rows_in_slices_and_strange_ids(et):
     bank, held = make_bank(et, 256, 512, 16, [16, 8])
     check_adapter(et, bank, held, [40, 2, 9], [0, 1, 0], 256, 512, pad=24)
@@ -647,4 +688,9 @@ def test_attention_refusals_on_the_device(et):
     for bad in (Q.float(), Q.cpu(), Q.t(), Q[:, :100]):
         with pytest.raises(ValueError):
             et.attention_rules(out, bad, Q, Q, 64, **ok)
+    for hd in (0, -64):
+        with pytest.raises((ValueError, et.EtError)):
+            et.attention_rules(out, Q, Q, Q, hd, **ok)
+        with pytest.raises((ValueError, et.EtError)):
+            et.rotary_axes(out, None, Q, None, dev(np.zeros((8, 1), dtype=int)), torch.ones(32, device="cuda"), dev(np.zeros(32, dtype=int)), hd)
     assert (out == 0).all()

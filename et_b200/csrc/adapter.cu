@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, 1) adapter_kernel(const __grid_const
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
     const int chunks = (p.in_feat + 31) / 32;
-    const uint4* const a = reinterpret_cast<const uint4*>(p.a + id * p.a_stride);
+    const uint4* const a = reinterpret_cast<const uint4*>(p.a + id * p.stride);
     constexpr int kUnroll = 4;
     for (int c0 = warp; c0 < chunks; c0 += kWarps * kUnroll) {
         uint4 xv[kUnroll][2];
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, 1) adapter_kernel(const __grid_const
             }
         }
     }
-    const uint4* const b = reinterpret_cast<const uint4*>(p.b + id * p.b_stride);
+    const uint4* const b = reinterpret_cast<const uint4*>(p.b + id * p.stride);
     uint4 old_next[2], w_next[kRt][2];
     auto request = [&](int c) {
         if (c >= col_groups) return;
@@ -230,8 +230,8 @@ int launch(AdapterParams p, cudaStream_t st) {
 
 struct et_adapter_bank {
     int in_feat, out_feat, max_rank, n_slots, rank_tiles, device;
-    long long a_stride, b_stride, a_tc_stride, b_tc_stride;
-    half *a = nullptr, *b = nullptr, *a_tc = nullptr, *b_tc = nullptr;
+    long long b_at, a_tc_at, b_tc_at, stride;   // of a slot, in elements: where its parts begin (A at 0; for many tokens A and B), all of it
+    half* weights = nullptr;
     et::AdapterSlot* slots = nullptr;
 };
 
@@ -246,15 +246,12 @@ extern "C" int et_adapter_bank_create(et_adapter_bank** out, int in_feat, int ou
     if (!bank) return fail(ET_ERR_CUDA, "et_adapter_bank_create: out of host memory");
     bank->in_feat = in_feat; bank->out_feat = out_feat; bank->max_rank = max_rank; bank->n_slots = n_slots;
     bank->rank_tiles = max_rank <= 16 ? 1 : max_rank <= 32 ? 2 : max_rank <= 64 ? 4 : 8;   // 16-wide steps: what the kernels are made for
-    bank->a_stride = (long long)((in_feat + 31) / 32) * bank->rank_tiles * 2 * 256;
-    bank->b_stride = (long long)((out_feat + 31) / 32) * bank->rank_tiles * 512;
-    bank->a_tc_stride = adapter_tc_a_stride(in_feat, bank->rank_tiles * 16);
-    bank->b_tc_stride = adapter_tc_b_stride(out_feat, bank->rank_tiles * 16);
+    bank->b_at = (long long)((in_feat + 31) / 32) * bank->rank_tiles * 2 * 256;
+    bank->a_tc_at = bank->b_at + (long long)((out_feat + 31) / 32) * bank->rank_tiles * 512;
+    bank->b_tc_at = bank->a_tc_at + adapter_tc_a_stride(in_feat, bank->rank_tiles * 16);
+    bank->stride = bank->b_tc_at + adapter_tc_b_stride(out_feat, bank->rank_tiles * 16);
     cudaError_t e = cudaGetDevice(&bank->device);
-    if (e == cudaSuccess) e = cudaMalloc(&bank->a, (size_t)bank->a_stride * n_slots * sizeof(half));
-    if (e == cudaSuccess) e = cudaMalloc(&bank->b, (size_t)bank->b_stride * n_slots * sizeof(half));
-    if (e == cudaSuccess) e = cudaMalloc(&bank->a_tc, (size_t)bank->a_tc_stride * n_slots * sizeof(half));
-    if (e == cudaSuccess) e = cudaMalloc(&bank->b_tc, (size_t)bank->b_tc_stride * n_slots * sizeof(half));
+    if (e == cudaSuccess) e = cudaMalloc(&bank->weights, (size_t)bank->stride * n_slots * sizeof(half));
     if (e == cudaSuccess) e = cudaMalloc(&bank->slots, (size_t)n_slots * sizeof(AdapterSlot));
     if (e == cudaSuccess) e = cudaMemset(bank->slots, 0, (size_t)n_slots * sizeof(AdapterSlot));
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
@@ -268,10 +265,7 @@ extern "C" int et_adapter_bank_create(et_adapter_bank** out, int in_feat, int ou
 
 extern "C" int et_adapter_bank_destroy(et_adapter_bank* bank) {
     if (!bank) return ET_OK;
-    cudaFree(bank->a);
-    cudaFree(bank->b);
-    cudaFree(bank->a_tc);
-    cudaFree(bank->b_tc);
+    cudaFree(bank->weights);
     cudaFree(bank->slots);
     delete bank;
     return ET_OK;
@@ -287,15 +281,13 @@ extern "C" int et_adapter_bank_set(et_adapter_bank* bank, int slot, int rank, co
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_status(e, "et_adapter_bank_set");
     ET_REQUIRE(dev == bank->device, "et_adapter_bank_set: the bank belongs to another device");
-    std::vector<half> pa, pb, ta, tb;
+    std::vector<half> packed;
     try {
-        pa.assign((size_t)bank->a_stride, __float2half(0.f));
-        pb.assign((size_t)bank->b_stride, __float2half(0.f));
-        ta.assign((size_t)bank->a_tc_stride, __float2half(0.f));
-        tb.assign((size_t)bank->b_tc_stride, __float2half(0.f));
+        packed.assign((size_t)bank->stride, __float2half(0.f));
     } catch (...) {
         return fail(ET_ERR_CUDA, "et_adapter_bank_set: out of host memory");
     }
+    half *const pa = packed.data(), *const pb = pa + bank->b_at;
     const half* const A = static_cast<const half*>(a_host);   // [rank x in_feat]
     const half* const B = static_cast<const half*>(b_host);   // [out_feat x rank]
     // A: [chunk of 32 features][8 ranks][lane = rank * 4 + t][features 8t .. 8t + 7 of the chunk]
@@ -311,13 +303,10 @@ extern "C" int et_adapter_bank_set(et_adapter_bank* bank, int slot, int rank, co
         half* const column = &pb[((size_t)(n / 32) * bank->rank_tiles * 32 + (2 * (c / 8) + c % 2) * 4) * 16 + (c / 2) % 4 * 4];
         for (int r = 0; r < rank; ++r) column[(size_t)(r / 16) * 512 + (r % 8) / 2 * 16 + r % 16 / 8 * 2 + r % 2] = B[(size_t)n * rank + r];
     }
-    adapter_tc_pack(ta.data(), tb.data(), A, B, rank, bank->in_feat, bank->out_feat, bank->rank_tiles * 16);
+    adapter_tc_pack(pa + bank->a_tc_at, pa + bank->b_tc_at, A, B, rank, bank->in_feat, bank->out_feat, bank->rank_tiles * 16);
     const AdapterSlot entry = {rank, scale};
     e = cudaDeviceSynchronize();   // launches that read the slot as it was have finished
-    if (e == cudaSuccess) e = cudaMemcpy(bank->a + slot * bank->a_stride, pa.data(), pa.size() * sizeof(half), cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaMemcpy(bank->b + slot * bank->b_stride, pb.data(), pb.size() * sizeof(half), cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaMemcpy(bank->a_tc + slot * bank->a_tc_stride, ta.data(), ta.size() * sizeof(half), cudaMemcpyHostToDevice);
-    if (e == cudaSuccess) e = cudaMemcpy(bank->b_tc + slot * bank->b_tc_stride, tb.data(), tb.size() * sizeof(half), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess && rank > 0) e = cudaMemcpy(bank->weights + slot * bank->stride, pa, packed.size() * sizeof(half), cudaMemcpyHostToDevice);
     if (e == cudaSuccess) e = cudaMemcpy(bank->slots + slot, &entry, sizeof(entry), cudaMemcpyHostToDevice);
     if (e == cudaSuccess) e = cudaDeviceSynchronize();
     return cuda_status(e, "et_adapter_bank_set");
@@ -341,8 +330,8 @@ extern "C" int et_adapter_add(const et_adapter_bank* bank, void* out, const void
     ET_REQUIRE(dev == bank->device, "et_adapter_add: the bank belongs to another device");
     AdapterParams p;
     p.out = static_cast<half*>(out); p.base = static_cast<const half*>(base); p.x = static_cast<const half*>(x);
-    p.cu_seqlens = cu_seqlens; p.ids = adapter_ids; p.slots = bank->slots; p.a = bank->a; p.b = bank->b;
-    p.out_pitch = out_pitch; p.base_pitch = base_pitch; p.x_pitch = x_pitch; p.a_stride = bank->a_stride; p.b_stride = bank->b_stride;
+    p.cu_seqlens = cu_seqlens; p.ids = adapter_ids; p.slots = bank->slots; p.a = bank->weights; p.b = bank->weights + bank->b_at;
+    p.out_pitch = out_pitch; p.base_pitch = base_pitch; p.x_pitch = x_pitch; p.stride = bank->stride;
     p.batch = batch; p.tokens = tokens; p.n_slots = bank->n_slots; p.in_feat = bank->in_feat; p.out_feat = bank->out_feat;
     p.copy = out != base;
     const int rc = attn_err_address(&p.err);
@@ -352,7 +341,8 @@ extern "C" int et_adapter_add(const et_adapter_bank* bank, void* out, const void
     // The tensor cores' kernel where there is enough to do: it takes some 10 us however little that is, but reads the weights for 64 to 128 tokens where the other
     // reads them for 16. (8 sequences of 6205 tokens, 1024 -> 4096, rank 32: 25 us, 41 in the other; 16 of 2055: 20 and 14; 768 -> 768, rank 16, 32 of 8509: 12.4 and 12.2.)
     if (cu_seqlens && tokens > 16LL * batch && (tokens >= 8192 || (long long)tokens * (bank->in_feat + 2LL * bank->out_feat) >= 30'000'000)) {
-        p.a = bank->a_tc; p.b = bank->b_tc; p.a_stride = bank->a_tc_stride; p.b_stride = bank->b_tc_stride;
+        p.a = bank->weights + bank->a_tc_at;
+        p.b = bank->weights + bank->b_tc_at;
         return adapter_tc_launch(p, rt * 16, st);
     }
     return rt <= 1 ? launch<1>(p, st) : rt <= 2 ? launch<2>(p, st) : rt <= 4 ? launch<4>(p, st) : launch<8>(p, st);

@@ -18,8 +18,8 @@ struct AdapterParams {
     const int* cu_seqlens;
     const int* ids;
     const AdapterSlot* slots;
-    const half *a, *b;                  // packed, all slots: for the kernel that is launched
-    long long out_pitch, base_pitch, x_pitch, a_stride, b_stride;   // of a slot, in elements
+    const half *a, *b;                  // packed, of the first slot: for the kernel that is launched
+    long long out_pitch, base_pitch, x_pitch, stride;   // stride: from slot to slot, in elements
     int batch, tokens, n_slots, in_feat, out_feat;
     int n_split;                        // CTAs that share a tile's columns, each with all of A x
     int* err;                           // of bounded waits
@@ -67,7 +67,7 @@ __device__ __forceinline__ int row_exponent(float top) {
 
 // tcgen05 kernel for many tokens (adapter_tc.cu): rank_step 16, 32, 64 or 128, the rank that the bank's slots are laid out for.
 int adapter_tc_launch(AdapterParams p, int rank_step, cudaStream_t st);
-// Elements of a slot in the layouts that it takes, and the layouts: A [chunk of 64 features][rank_step][64] with 128-byte swizzle, B [unit of 64 columns]
+// Elements of A and B in the layouts that it takes, and the layouts: A [chunk of 64 features][rank_step][64] with 128-byte swizzle, B [unit of 64 columns]
 // [8 columns][8 ranks] as core matrices of 8 columns x 16 bytes.
 long long adapter_tc_a_stride(int in_feat, int rank_step);
 long long adapter_tc_b_stride(int out_feat, int rank_step);

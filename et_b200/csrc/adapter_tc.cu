@@ -111,8 +111,8 @@ __global__ void __launch_bounds__(kThreads, 2) adapter_tc_kernel(const __grid_co
         }
     } else if (rows > 0 && warp == kLoadWarp) {
         if (lane == 0) {
-            const half* const a = p.a + id * p.a_stride;
-            const half* const b = p.b + id * p.b_stride + (long long)first_unit * (kWeights / 2);
+            const half* const a = p.a + id * p.stride;
+            const half* const b = p.b + id * p.stride + (long long)first_unit * (kWeights / 2);
             const int n = chunks + units;
             bool ok = true;
             RingAt at;

@@ -184,7 +184,7 @@ int et_adapter_bank_destroy(et_adapter_bank* bank);
 int et_adapter_bank_set(et_adapter_bank* bank, int slot, int rank, const void* a_host, const void* b_host, float scale);
 /* out[t] = base[t] + scale_a B_a (A_a x[t]) for the tokens of each sequence, a = adapter_ids[sequence] (device, batch ints; an id that
  * is no slot, or an empty one, adds nothing). base is what the shared projection left (et_tile_linear, et_row_linear); out may be base with the same
- * pitch. cu_seqlens (device, batch + 1 ints) are the sequences' token offsets, or NULL: one token each (single tokens of many requests). Rows of
+ * pitch, and overlaps x in nothing. cu_seqlens (device, batch + 1 ints) are the sequences' token offsets, or NULL: one token each (single tokens of many requests). Rows of
  * out in no sequence are left as they are. tokens: the rows that there are; none beyond is touched. Rows start on 16 bytes (pitches multiples
  * of 8). Sums in fp32; A x is rounded to fp16, each row scaled so that it can not overflow. */
 int et_adapter_add(const et_adapter_bank* bank, void* out, const void* base, const void* x, int out_pitch, int base_pitch, int x_pitch,

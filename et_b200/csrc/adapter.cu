@@ -347,3 +347,8 @@ extern "C" int et_adapter_add(const et_adapter_bank* bank, void* out, const void
     }
     return rt <= 1 ? launch<1>(p, st) : rt <= 2 ? launch<2>(p, st) : rt <= 4 ? launch<4>(p, st) : launch<8>(p, st);
 }
+
+extern "C" int et_adapter_add_by(const et_adapter_add_args* a) {
+    ET_REQUIRE(a, "et_adapter_add_by: null pointer");
+    return et_adapter_add(a->bank, a->out, a->base, a->x, a->out_pitch, a->base_pitch, a->x_pitch, a->cu_seqlens, a->adapter_ids, a->batch, a->tokens, a->stream);
+}

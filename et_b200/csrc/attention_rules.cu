@@ -90,3 +90,9 @@ extern "C" int et_attention_rules(void* out, const void* Q, const void* K, const
     if (attention_rules_tc_takes(p)) return attention_rules_tc_launch(p, p.k_docs ? scratch : nullptr, st);
     return cuda_status(attention_rules_rows_launch(p, st), "et_attention_rules launch");
 }
+
+extern "C" int et_attention_rules_by(const et_attention_rules_args* a) {
+    ET_REQUIRE(a, "et_attention_rules_by: null pointer");
+    return et_attention_rules(a->out, a->Q, a->K, a->V, a->out_pitch, a->q_pitch, a->k_pitch, a->v_pitch, a->nhead, a->nhead_kv, a->head_dim, a->cu_seqlens, a->k_start, a->k_lens,
+                              a->batch, a->q_tokens, a->k_rows, a->max_q_len, a->max_k_len, &a->rules, a->scratch, a->scratch_bytes, a->stream);
+}

@@ -308,3 +308,9 @@ extern "C" int et_rotary_axes(void* q_out, const void* q, int q_out_pitch, int q
     const auto kernel = pairing == kScalar ? rotary_kernel<kScalar> : pairing == kHalves8 ? rotary_kernel<kHalves8> : pairing == kHalves ? rotary_kernel<kHalves> : rotary_kernel<kNeighbours>;
     return cuda_status(launch_pdl(kernel, dim3(blocks), dim3(threads), smem, static_cast<cudaStream_t>(stream), p), "et_rotary_axes launch");
 }
+
+extern "C" int et_rotary_axes_by(const et_rotary_axes_args* a) {
+    ET_REQUIRE(a, "et_rotary_axes_by: null pointer");
+    return et_rotary_axes(a->q_out, a->q, a->q_out_pitch, a->q_pitch, a->nhead_q, a->k_out, a->k, a->k_out_pitch, a->k_pitch, a->nhead_k, a->head_dim, a->rot_dim, a->positions,
+                          a->n_axes, a->inv_freq, a->axis, a->interleaved, a->tokens, a->stream);
+}

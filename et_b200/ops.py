@@ -30,8 +30,7 @@ _SIGNATURES = {
     "et_tile_spmm_bias": "pppppiiipip", "et_attention_otf": "pppppiiip", "et_attention_prune": "ppppppipiiip",
     "et_qk_scores": "pppiiip", "et_attention_sharedqk": "ppppiiip", "et_attention_static_scores": "pppppiiip",
     "et_attention_batch": "ppppiippppippiiiiiip", "et_encoder_run": "pppp", "et_encoder_run_batch": "pppppipsp",
-    "et_model_run_batch": "pppppip", "et_rotary_axes": "ppiiippiiiiipippiip", "et_adapter_add": "ppppiiippiip",
-    "et_attention_rules": "ppppiiiiiiipppiiiiippsp",
+    "et_model_run_batch": "pppppip", "et_rotary_axes_by": "p", "et_adapter_add_by": "p", "et_attention_rules_by": "p",
 }
 
 
@@ -273,6 +272,8 @@ def attention_batch(out, Q, K, V, d_model, nhead, cu_seqlens=None, valid_lens=No
 
 
 # ---------------------------------------------------------------------------------- positions, adapters, rules on scores
+# et_rotary_axes_args, et_adapter_add_args and et_attention_rules_args as they lie in memory
+_rotary_args, _adapter_args, _rules_args = struct.Struct("@8P11i0P").pack, struct.Struct("@7P5i0P").pack, struct.Struct("@8PNPffPPiiiPPP12i").pack
 _kept = None
 
 
@@ -323,13 +324,14 @@ def rotary_axes(q_out, k_out, q, k, positions, inv_freq, axis, head_dim, interle
         raise ValueError(f"positions int32 [tokens, axes], inv_freq float32 and axis int32 [pairs], contiguous, on the current CUDA device ({device}) expected, not "
                          + ", ".join(f"{t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for t in (positions, inv_freq, axis)))
     nq = nk = q_pitch = k_pitch = q_out_pitch = k_out_pitch = 0
-    q_at = k_at = q_out_at = k_out_at = None
+    q_at = k_at = q_out_at = k_out_at = 0
     if q is not None:
         q_at, q_out_at, q_pitch, q_out_pitch, nq = _turned("q", q, q_out, tokens, head_dim, f16, device)
     if k is not None:
         k_at, k_out_at, k_pitch, k_out_pitch, nk = _turned("k", k, k_out, tokens, head_dim, f16, device)
-    rc = (_entries or _lib()).et_rotary_axes(q_out_at, q_at, q_out_pitch, q_pitch, nq, k_out_at, k_at, k_out_pitch, k_pitch, nk, head_dim, 2 * pairs, positions.data_ptr(), axes,
-                                             inv_freq.data_ptr(), axis.data_ptr(), 1 if interleaved else 0, tokens, stream_of(device) if stream is None else stream.cuda_stream)
+    rc = (_entries or _lib()).et_rotary_axes_by(_rotary_args(
+        q_out_at, q_at, k_out_at, k_at, positions.data_ptr(), inv_freq.data_ptr(), axis.data_ptr(), stream_of(device) if stream is None else stream.cuda_stream,
+        q_out_pitch, q_pitch, nq, k_out_pitch, k_pitch, nk, head_dim, 2 * pairs, axes, 1 if interleaved else 0, tokens))
     if rc:
         check(rc)
     return q_out, k_out
@@ -383,9 +385,9 @@ class AdapterBank:
         if rows <= 1:
             x_pitch, base_pitch, out_pitch = width, self.out_feat, self.out_feat
         batch = adapter_ids.numel()
-        rc = (_entries or _lib()).et_adapter_add(self._h, out.data_ptr(), base.data_ptr(), x.data_ptr(), out_pitch, base_pitch, x_pitch,
-                                                 None if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1),
-                                                 _array("adapter_ids", adapter_ids, i32, device, batch), batch, rows, stream_of(device) if stream is None else stream.cuda_stream)
+        rc = (_entries or _lib()).et_adapter_add_by(_adapter_args(
+            self._h.value or 0, out.data_ptr(), base.data_ptr(), x.data_ptr(), 0 if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1),
+            _array("adapter_ids", adapter_ids, i32, device, batch), stream_of(device) if stream is None else stream.cuda_stream, out_pitch, base_pitch, x_pitch, batch, rows))
         if rc:
             check(rc)
         return out
@@ -400,10 +402,6 @@ class AdapterBank:
             self.close()
         except Exception:
             pass
-
-
-# et_score_rules as it lies in memory: scale, cap, slopes, distance_bias, reach, window_left, window_right, prefix_lens, q_docs, k_docs
-_score_rules = struct.Struct("@ffPPiiiPPP").pack
 
 
 def attention_rules_scratch_size(batch, max_k_len):
@@ -448,14 +446,14 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
         scratch_bytes = scratch.numel() * scratch.element_size()
         if scratch.get_device() != device or not scratch.is_contiguous():
             raise ValueError("scratch must be contiguous, on the current CUDA device")
-    rules = _score_rules(scale, cap, 0 if slopes is None else _array("slopes", slopes, f32, device, nhead), table, reach, window[0], window[1],
-                         0 if prefix_lens is None else _array("prefix_lens", prefix_lens, i32, device, batch),
-                         0 if q_docs is None else _array("q_docs", q_docs, i32, device, tokens), 0 if k_docs is None else _array("k_docs", k_docs, i32, device, k_rows))
-    rc = (_entries or _lib()).et_attention_rules(
-        out.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), out_pitch, q_pitch, k_pitch, v_pitch, nhead, nhead_kv, head_dim,
-        None if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), None if k_start is None else _array("k_start", k_start, i32, device, batch),
-        None if k_lens is None else _array("k_lens", k_lens, i32, device, batch), batch, tokens, k_rows, max_q_len or tokens, max_k_len or k_rows, rules,
-        None if scratch is None else scratch.data_ptr(), scratch_bytes, stream_of(device) if stream is None else stream.cuda_stream)
+    rc = (_entries or _lib()).et_attention_rules_by(_rules_args(
+        out.data_ptr(), Q.data_ptr(), K.data_ptr(), V.data_ptr(), 0 if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1),
+        0 if k_start is None else _array("k_start", k_start, i32, device, batch), 0 if k_lens is None else _array("k_lens", k_lens, i32, device, batch),
+        0 if scratch is None else scratch.data_ptr(), scratch_bytes, stream_of(device) if stream is None else stream.cuda_stream,
+        scale, cap, 0 if slopes is None else _array("slopes", slopes, f32, device, nhead), table, reach, window[0], window[1],
+        0 if prefix_lens is None else _array("prefix_lens", prefix_lens, i32, device, batch),
+        0 if q_docs is None else _array("q_docs", q_docs, i32, device, tokens), 0 if k_docs is None else _array("k_docs", k_docs, i32, device, k_rows),
+        out_pitch, q_pitch, k_pitch, v_pitch, nhead, nhead_kv, head_dim, batch, tokens, k_rows, max_q_len or tokens, max_k_len or k_rows))
     if rc:
         check(rc)
     return out

@@ -172,6 +172,13 @@ int et_attention_batch(void* out, const void* Q, const void* K, const void* V, i
 int et_rotary_axes(void* q_out, const void* q, int q_out_pitch, int q_pitch, int nhead_q, void* k_out, const void* k, int k_out_pitch,
                    int k_pitch, int nhead_k, int head_dim, int rot_dim, const int* positions, int n_axes, const float* inv_freq,
                    const int* axis, int interleaved, int tokens, void* stream);
+/* The same call, its arguments in one structure: for callers to whom each argument of a foreign call costs time. So for the other calls below. */
+typedef struct et_rotary_axes_args {
+    void* q_out; const void* q; void* k_out; const void* k;
+    const int* positions; const float* inv_freq; const int* axis; void* stream;
+    int q_out_pitch, q_pitch, nhead_q, k_out_pitch, k_pitch, nhead_k, head_dim, rot_dim, n_axes, interleaved, tokens;
+} et_rotary_axes_args;
+int et_rotary_axes_by(const et_rotary_axes_args* args);
 
 /* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference, which holds one set of weights) ----
  * A bank holds n_slots adapters of one projection, each of rank up to max_rank (1 to 128): A [rank x in_feat], B [out_feat x rank] and a
@@ -189,6 +196,12 @@ int et_adapter_bank_set(et_adapter_bank* bank, int slot, int rank, const void* a
  * of 8). Sums in fp32; A x is rounded to fp16, each row scaled so that it can not overflow. */
 int et_adapter_add(const et_adapter_bank* bank, void* out, const void* base, const void* x, int out_pitch, int base_pitch, int x_pitch,
                    const int* cu_seqlens, const int* adapter_ids, int batch, int tokens, void* stream);
+typedef struct et_adapter_add_args {
+    const et_adapter_bank* bank; void* out; const void* base; const void* x;
+    const int* cu_seqlens; const int* adapter_ids; void* stream;
+    int out_pitch, base_pitch, x_pitch, batch, tokens;
+} et_adapter_add_args;
+int et_adapter_add_by(const et_adapter_add_args* args);
 
 /* ---- attention with rules on its scores (no counterpart in the reference, whose masks are additive and shared by all heads) ----
  *   score(q, k) = cap tanh(scale Q_q . K_k / cap) + bias(k - q);   out_q = sum of softmax(score) V_k over the keys that q sees
@@ -221,6 +234,13 @@ int et_attention_rules(void* out, const void* Q, const void* K, const void* V, i
                        int q_tokens, int k_rows, int max_q_len, int max_k_len, const et_score_rules* rules, void* scratch,
                        size_t scratch_bytes, void* stream);
 size_t et_attention_rules_scratch_size(int batch, int max_k_len);
+typedef struct et_attention_rules_args {
+    void* out; const void* Q; const void* K; const void* V;
+    const int* cu_seqlens; const int* k_start; const int* k_lens; void* scratch; size_t scratch_bytes; void* stream;
+    et_score_rules rules;
+    int out_pitch, q_pitch, k_pitch, v_pitch, nhead, nhead_kv, head_dim, batch, q_tokens, k_rows, max_q_len, max_k_len;
+} et_attention_rules_args;
+int et_attention_rules_by(const et_attention_rules_args* args);
 
 /* ---- pruned-format generators (host) ----------------------------------------------------------
  * Seeded and reproducible. bernoulli == 0 keeps exactly floor(total*(1-sparsity)) tiles (a block-row's

@@ -427,7 +427,7 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
     out_pitch, out_step = out.stride()
     if (Q.dtype is not f16 or K.dtype is not f16 or V.dtype is not f16 or out.dtype is not f16 or Q.get_device() != device or K.get_device() != device
             or V.get_device() != device or out.get_device() != device or out.shape != q_shape or V.shape != k_shape or head_dim < 1 or width % head_dim or kv_width % head_dim
-            or not kv_width or not width or (q_step, k_step, v_step, out_step) != (1, 1, 1, 1) and min(width, kv_width) > 1):
+            or not kv_width or not width or (q_step != 1 or out_step != 1) and width > 1 or (k_step != 1 or v_step != 1) and kv_width > 1):
         raise ValueError(f"float16 rows of whole heads of {head_dim} on the current CUDA device ({device}) with neighbouring elements, out like Q and V like K expected, not "
                          + ", ".join(f"{n} {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}" for n, t in (("Q", Q), ("out", out), ("K", K), ("V", V))))
     if tokens <= 1:

@@ -688,6 +688,10 @@ def test_attention_refusals_on_the_device(et):
     for bad in (Q.float(), Q.cpu(), Q.t(), Q[:, :100]):
         with pytest.raises(ValueError):
             et.attention_rules(out, bad, Q, Q, 64, **ok)
+    heads = normal(3, 4, 8).t()   # four heads of one feature, a row's elements apart; one of keys
+    for bad in ((out[:, :4], heads, Q[:, :1], Q[:, :1]), (heads, out[:, :4], Q[:, :1], Q[:, :1]), (out[:, :1], out[:, :1], heads, heads)):
+        with pytest.raises((ValueError, et.EtError)):
+            et.attention_rules(*bad, 1, **ok)
     for hd in (0, -64):
         with pytest.raises((ValueError, et.EtError)):
             et.attention_rules(out, Q, Q, Q, hd, **ok)

@@ -339,8 +339,9 @@ extern "C" int et_adapter_add(const et_adapter_bank* bank, void* out, const void
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int rt = bank->rank_tiles;
     // The tensor cores' kernel where there is enough to do: it takes some 10 us however little that is, but reads the weights for 64 to 128 tokens where the other
-    // reads them for 16. (8 sequences of 6205 tokens, 1024 -> 4096, rank 32: 25 us, 41 in the other; 16 of 2055: 20 and 14; 768 -> 768, rank 16, 32 of 8509: 12.4 and 12.2.)
-    if (cu_seqlens && tokens > 16LL * batch && (tokens >= 8192 || (long long)tokens * (bank->in_feat + 2LL * bank->out_feat) >= 30'000'000)) {
+    // reads them for 16. (8 sequences of 6205 tokens, 1024 -> 4096, rank 32: 25 us, 41 in the other; 16 of 2055: 20 and 14; 768 -> 768, rank 16, 32 of 8509: 12.4 and 12.2. Of short sequences
+    // its tiles are mostly empty: 1000 sequences of 24 tokens, 1024 -> 1024, rank 16: 84 and 49, 200 of 50, 768 -> 2304: 34 and 30, 128 of 64, 1024 -> 1024: 16 and 17.)
+    if (cu_seqlens && tokens >= 56LL * batch && (tokens >= 8192 || (long long)tokens * (bank->in_feat + 2LL * bank->out_feat) >= 30'000'000)) {
         p.a = bank->weights + bank->a_tc_at;
         p.b = bank->weights + bank->b_tc_at;
         return adapter_tc_launch(p, rt * 16, st);

@@ -33,12 +33,14 @@ __device__ __forceinline__ int find_tile(const AdapterParams& p, int tile, int s
         seq = t0 = tile;
         return tile < p.batch ? 1 : 0;
     }
-    for (int base = 0; base < p.batch; base += 32) {
-        const int i = base + lane;
-        const int first = i < p.batch ? p.cu_seqlens[i] : 0;
-        const int len = i < p.batch ? max(p.cu_seqlens[i + 1] - first, 0) : 0;
-        const int n = (len + size - 1) / size;
-        int incl = n;
+    for (int base = 0; base < p.batch; base += 128) {   // four sequences to a lane
+        int first[5], n[4];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) first[j] = p.cu_seqlens[min(base + lane * 4 + j, p.batch)];   // (behind the last one all are empty)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n[j] = (max(first[j + 1] - first[j], 0) + size - 1) / size;
+        const int sum = n[0] + n[1] + n[2] + n[3];
+        int incl = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -47,10 +49,17 @@ __device__ __forceinline__ int find_tile(const AdapterParams& p, int tile, int s
         const unsigned hit = __ballot_sync(0xffffffffu, tile < incl);
         if (hit) {
             const int src = __ffs(hit) - 1;
-            const int at = (tile - __shfl_sync(0xffffffffu, incl - n, src)) * size;
-            seq = base + src;
-            t0 = __shfl_sync(0xffffffffu, first, src) + at;
-            const int end = min(__shfl_sync(0xffffffffu, first + len, src), p.tokens);   // (never beyond the rows that there are)
+            int left = tile - (incl - sum), at = 0;   // (of the lane that has it)
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+                if (at == j && left >= n[j]) {
+                    left -= n[j];
+                    ++at;
+                }
+            const int from = at == 0 ? first[0] : at == 1 ? first[1] : at == 2 ? first[2] : first[3], to = at == 0 ? first[1] : at == 1 ? first[2] : at == 2 ? first[3] : first[4];
+            seq = base + src * 4 + __shfl_sync(0xffffffffu, at, src);
+            t0 = __shfl_sync(0xffffffffu, from + left * size, src);
+            const int end = min(__shfl_sync(0xffffffffu, to, src), p.tokens);   // (never beyond the rows that there are)
             return t0 < 0 ? 0 : max(min(end - t0, size), 0);
         }
         tile -= __shfl_sync(0xffffffffu, incl, 31);

@@ -529,6 +529,30 @@ def test_attention_of_documents_in_any_order(et, hd, rule):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rule", [{}, {"window": (-1, 0)}, {"slopes": True}, {"reach": 30}])
+def test_attention_of_scores_around_half_a_cap(et, hd, rule):
+    """Rows whose scores end just below, at and above half a cap, far above it and near 0, side by side; one that is not a number."""
+    import torch
+    n, cap = 300, 8.0
+    Q, K, V = torch.zeros(n, 2 * hd, device="cuda").half(), torch.zeros(n, 2 * hd, device="cuda").half(), normal(3, n, 2 * hd)
+    K[:, 0] = K[:, hd] = torch.linspace(-1, 1, n, device="cuda").half()
+    K[:, 1] = K[:, hd + 1] = 1.0 / 64
+    rows = torch.arange(n, device="cuda")
+    size = torch.tensor([0.001, 1.0, 3.99, 4.0, 4.01, 9.0, 100.0], device="cuda")[(rows // 32) % 7] * torch.where(rows % 5 == 0, 0.5, 1.0)
+    Q[:, 0] = Q[:, hd] = (size * math.sqrt(hd)).half()
+    Q[:, 1] = 1.0
+    r = {**rule, **({"slopes": torch.tensor([0.02, 0.5], device="cuda")} if "slopes" in rule else {}), **({"table": normal(4, 2, 61)} if "reach" in rule else {})}
+    r.pop("reach", None)
+    out = run_attention(et, Q, K, V, hd, [(0, n, 0, n, 0)], cu=[0, n], cap=cap, **r)
+    K[290, hd + 1] = math.nan   # of the second head, at the end
+    Q[40, hd + 1] = 0.0
+    again = et.attention_rules(torch.zeros_like(out), Q, K, V, hd, cu_seqlens=dev([0, n]), batch=1, max_q_len=n, max_k_len=n, cap=cap, window=r.get("window", (-1, -1)),
+                               slopes=r.get("slopes"), distance_bias=r.get("table"))
+    assert torch.equal(again[:, :hd], out[:, :hd]) and torch.isnan(again[290:, hd:]).all()
+    assert torch.isnan(again[:290, hd:]).all() if "window" not in r else torch.equal(again[41:290, hd:], out[41:290, hd:])
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("single", [False, True])
 def test_attention_of_large_scores(et, hd, single):
     """Scores of hundreds: one key takes all; capped ones are flat again; a scale of its own."""

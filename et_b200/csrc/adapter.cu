@@ -13,7 +13,7 @@
 // does not depend on the order of k, and which column a lane of the second product computes is free.
 //
 // What bounds it: latency, the chain id -> A x -> exchange -> B. 64 single tokens, 1024 -> 1024, rank 16: 4.0 us; nine sequences of 1.1 thousand tokens, 768 -> 2304, rank 8:
-// 7.3 us. Tried: clusters of 2, 4, 8 CTAs that share a tile's K range and columns through distributed shared memory (single tokens 5.0, 5.3, 7.3 us).
+// 8.3 us. Tried: clusters of 2, 4, 8 CTAs that share a tile's K range and columns through distributed shared memory (single tokens 5.0, 5.3, 7.3 us).
 #include <cstring>
 #include <new>
 #include <vector>

@@ -13,7 +13,7 @@
 // does not depend on the order of k, and which column a lane of the second product computes is free.
 //
 // What bounds it: latency, the chain id -> A x -> exchange -> B. 64 single tokens, 1024 -> 1024, rank 16: 4.0 us; nine sequences of 1.1 thousand tokens, 768 -> 2304, rank 8:
-// 8.3 us. Tried: clusters of 2, 4, 8 CTAs that share a tile's K range and columns through distributed shared memory (single tokens 5.0, 5.3, 7.3 us).
+// 6.8 us. Tried: clusters of 2, 4, 8 CTAs that share a tile's K range and columns through distributed shared memory (single tokens 5.0, 5.3, 7.3 us).
 #include <cstring>
 #include <new>
 #include <vector>
@@ -218,10 +218,12 @@ int launch(AdapterParams p, cudaStream_t st) {
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem); });
     if (e != cudaSuccess) return cuda_status(e, "et_adapter_add");
-    // A tile's columns are shared by CTAs as long as each warp has three groups of them and the SMs have two CTAs at most. (Single tokens of 64 sequences, 1024 -> 1024:
-    // 4.0 us, with two CTAs to a tile 4.2.)
+    // A tile's columns are shared by as many CTAs as all find a place at once (by their registers three, two or one to an SM), each with 18 groups of columns at least.
+    // (Nine sequences of 1.1 thousand tokens, 768 -> 2304, rank 8, in two, three, four CTAs to a tile 8.4, 7.3, 6.8 us, in more than there are places for 9.5; 64 single tokens, 1024 -> 4096,
+    // rank 128, in one round 11.2, in two 16.2; 64 single tokens, 1024 -> 1024, rank 16, in one CTA to a tile 4.0, in two 4.2.)
+    constexpr int kPlaces = kRt == 1 ? 3 : kRt == 8 ? 1 : 2;
     const long long tiles = p.cu_seqlens ? (long long)p.tokens / kTile + p.batch : p.batch;
-    p.n_split = (int)max(1LL, min(2LL * sm_count() / tiles, (long long)((p.out_feat + 31) / 32 / (3 * kWarps))));
+    p.n_split = (int)max(1LL, min((long long)kPlaces * sm_count() / tiles, (long long)((p.out_feat + 31) / 32 / 18)));
     return cuda_status(launch_pdl(kernel, dim3((unsigned)(tiles * p.n_split)), dim3(kThreads), smem, st, p), "et_adapter_add launch");
 }
 

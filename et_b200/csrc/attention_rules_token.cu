@@ -313,12 +313,15 @@ __global__ void __launch_bounds__(kThreads) attention_rules_token_kernel(const _
     if (t == 0) {
 #pragma unroll
         for (int x = 0; x < kX; ++x) {
-            warp_ms[warp * 2 * kRows + g + 8 * x] = top[x];
+            // (scores that are not numbers leave no maximum: any finite one makes the part count below)
+            warp_ms[warp * 2 * kRows + g + 8 * x] = sum[x] == sum[x] ? top[x] : 0.f;
             warp_ms[warp * 2 * kRows + kRows + g + 8 * x] = sum[x];
         }
     }
     __syncthreads();
-    auto factor = [](float m, float all) { return m == -INFINITY ? 0.f : ex2_fast(m - all); };   // of sums relative to m, to make them relative to `all`
+    // A part that has a maximum has seen something, and its share counts even times 0: what is not finite in it makes the row not finite, and the row is
+    // computed again. (The sums of a part without one are 0 times what is masked.)
+    auto saw = [](float m) { return m != -INFINITY; };
     for (int e = threadIdx.x; e < rows * hd; e += kThreads) {
         const int r = e / hd, c = e % hd;
         float m = -INFINITY, l = 0.f, v = 0.f;
@@ -326,8 +329,9 @@ __global__ void __launch_bounds__(kThreads) attention_rules_token_kernel(const _
         for (int w = 0; w < kWarps; ++w) m = fmaxf(m, warp_ms[w * 2 * kRows + r]);
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-            const float f = factor(warp_ms[w * 2 * kRows + r], m);
-            if (f != 0.f) {
+            const float part = warp_ms[w * 2 * kRows + r];
+            if (saw(part)) {
+                const float f = ex2_fast(part - m);
                 v = fmaf(f, warp_o[(w * kRows + r) * kHD + c], v);
                 l = fmaf(f, warp_ms[w * 2 * kRows + kRows + r], l);
             }
@@ -350,8 +354,8 @@ __global__ void __launch_bounds__(kThreads) attention_rules_token_kernel(const _
         for (int k = 0; k < kMaxCluster; ++k) m = fmaxf(m, part_m[k]);
 #pragma unroll
         for (int k = 0; k < kMaxCluster; ++k) {
-            const float f = factor(part_m[k], m);
-            if (f != 0.f && c < hd) {
+            if (saw(part_m[k]) && c < hd) {
+                const float f = ex2_fast(part_m[k] - m);
                 v = fmaf(f, cluster.map_shared_rank(cta_o, k)[r * kHD + c], v);
                 l = fmaf(f, cluster.map_shared_rank(cta_ms, k)[kRows + r], l);
             }

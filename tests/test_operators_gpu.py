@@ -722,3 +722,78 @@ def test_attention_refusals_on_the_device(et):
         with pytest.raises((ValueError, et.EtError)):
             et.rotary_axes(out, None, Q, None, dev(np.zeros((8, 1), dtype=int)), torch.ones(32, device="cuda"), dev(np.zeros(32, dtype=int)), hd)
     assert (out == 0).all()
+
+
+# Keys of one CTA with a block to each warp, of two CTAs whose second has the last key alone, of a cluster of sixteen.
+@pytest.mark.parametrize("n", [49, 65, 993])
+@pytest.mark.parametrize("nq", [1, 4, 6])   # single tokens and a few; six are whole sequences to the library
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("hq,hk,hd", [(4, 2, 64), (16, 2, 128), (16, 2, 64), (4, 2, 24)])
+def test_tokens_over_kept_keys_of_values_that_are_not_numbers(et, hq, hk, hd, cap, nq, n):
+    """A query, a block of keys or the last key that is not a number makes exactly the heads of the queries that see it not a number."""
+    import torch
+    Q, K, V = normal(1, nq, hq * hd), normal(2, n, hk * hd), normal(3, n, hk * hd)
+
+    def odd(q, k, v, window=(-1, -1)):
+        """Which elements are not finite."""
+        out = et.attention_rules(torch.zeros_like(q), q, k, v, hd, k_start=dev([0]), k_lens=dev([n]), batch=1, max_q_len=nq, max_k_len=n, cap=cap, window=window)
+        et.attention_check()
+        return ~torch.isfinite(out).view(nq, hq, hd)
+
+    expect = torch.zeros(nq, hq, hd, dtype=torch.bool, device="cuda")
+    assert not odd(Q, K, V).any()
+    assert odd(torch.full_like(Q, math.nan), K, V).all()
+    one = Q.clone()
+    one[nq - 1, hd + 1] = math.nan                       # the last query's second head
+    expect[nq - 1, 1] = True
+    assert torch.equal(odd(one, K, V), expect)
+    for first, last in ((0, 16), (32, 48), (n - 1, n)):  # whole blocks, and the last key
+        bad = K.clone()
+        bad[first:last, hd:2 * hd] = math.nan            # of the second K/V head
+        expect = torch.zeros_like(expect)
+        expect[:, hq // 2:] = True
+        assert torch.equal(odd(Q, bad, V), expect)
+        expect[:] = False
+        expect[max(0, first - (n - nq)):, hq // 2:] = True
+        assert torch.equal(odd(Q, bad, V, window=(-1, 0)), expect)
+        assert odd(Q, torch.full_like(K, math.nan), V).all()
+
+
+@pytest.mark.parametrize("n", [49, 65, 993])
+@pytest.mark.parametrize("nq", [1, 4])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("hq,hk,hd", [(4, 2, 64), (16, 2, 128)])
+def test_tokens_over_kept_keys_keep_their_bits_beside_masked_keys_that_are_not_numbers(et, hq, hk, hd, cap, nq, n):
+    import torch
+    Q, K, V = normal(1, nq, hq * hd), normal(2, n, hk * hd), normal(3, n, hk * hd)
+    seqs, call = [(0, nq, 0, n, n - nq)], dict(k_start=[0], k_lens=[n], cap=cap, max_q=nq)
+    for first, last in ((0, 16), (32, 48), (n - 1, n)):
+        bad, k_docs = K.clone(), np.zeros(n, dtype=int)
+        bad[first:last], k_docs[first:last] = math.nan, 3
+        docs = (dev(np.zeros(nq, dtype=int)), dev(k_docs))
+        assert torch.equal(run_attention(et, Q, bad, V, hd, seqs, docs=docs, **call), run_attention(et, Q, K, V, hd, seqs, docs=docs, **call))
+    bad = K.clone()
+    bad[:16] = math.nan
+    near = dict(window=(n - nq - 16, 0))                 # the first sixteen keys are before it
+    assert torch.equal(run_attention(et, Q, bad, V, hd, seqs, **near, **call), run_attention(et, Q, K, V, hd, seqs, **near, **call))
+
+
+@pytest.mark.parametrize("n", [49, 65, 993])
+@pytest.mark.parametrize("nq", [1, 4, 6])
+@pytest.mark.parametrize("hd", [64, 128, 24])
+def test_tokens_over_kept_keys_of_values_beside_scores_far_below(et, hd, nq, n):
+    """A value that is not finite counts however small its key's weight is: beside 0 it is not a number."""
+    import torch
+    Q, K, V = normal(1, nq, 4 * hd, std=0.1), normal(2, n, 2 * hd, std=0.1), normal(3, n, 2 * hd)
+    Q[:, ::hd] = 30.0
+    K[:, ::hd] = 0.0
+    seqs, call = [(0, nq, 0, n, n - nq)], dict(k_start=[0], k_lens=[n], max_q=nq)
+    for first, last in ((32, 48), (n - 1, n)):
+        for value in (math.inf, math.nan):
+            far, bad = K.clone(), V.clone()
+            far[first:last, hd] = -30.0 * math.sqrt(hd)  # scores of -900 for the second K/V head's queries
+            bad[first, hd + 5] = value
+            out = run_attention(et, Q, far, bad, hd, seqs, **call)
+            expect = torch.zeros(nq, 4, hd, dtype=torch.bool, device="cuda")
+            expect[:, 2:, 5] = True
+            assert torch.equal(~torch.isfinite(out).view(nq, 4, hd), expect)

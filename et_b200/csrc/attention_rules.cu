@@ -80,6 +80,9 @@ extern "C" int et_attention_rules(void* out, const void* Q, const void* K, const
     p.scale_log2 = (float)(scale * 1.4426950408889634);
     p.cap_in = r.cap > 0.f ? (float)(2.0 * scale * 1.4426950408889634 / r.cap) : 0.f;
     p.cap_out = (float)(r.cap * 1.4426950408889634);
+    p.to_y = r.cap > 0.f ? (float)(scale / r.cap) : 0.f;
+    p.cap_near = p.to_y > 0.f ? std::fmin(kCapNear / p.to_y, 3.4e38f) : 0.f;   // (an infinite score is capped)
+    p.cap_wide = r.cap > kWideCap;
     ET_REQUIRE(std::isfinite(p.scale_log2) && std::isfinite(p.cap_in) && std::isfinite(p.cap_out), "et_attention_rules: scale and cap are too far apart");
     p.slopes = r.slopes; p.table = static_cast<const half*>(r.distance_bias); p.reach = r.distance_bias ? r.reach : 0;
     p.window_left = r.window_left < 0 || r.window_left >= kNoLimit ? kNoLimit : r.window_left;

@@ -40,6 +40,7 @@ constexpr int kShiftPitch = 800;          // bytes of one of four copies of a bl
 constexpr int kShiftBytes = 4 * kShiftPitch;
 
 enum Bias { kNoBias = 0, kSlopes = 1, kTable = 2 };
+enum Cap { kNoCap = 0, kCapped = 1, kWide = 2 };   // kWide: above kWideCap
 enum BlockFlags { kPartial = 1, kFirst = 2, kLast = 4, kEnd = 8, kMixed = 16 };   // kPartial: by place, kMixed: by document
 
 struct TcRules {
@@ -50,7 +51,6 @@ struct TcRules {
     bool sorted;              // a ragged batch of at most kMaxSorted sequences, the longest first
     bool heavy_first;         // equal lengths: late queries, which see more, first
     int* err;
-    float to_y, cap_near;     // capped: score -> score / cap, and the largest score for which cap_near2 is taken
 };
 
 struct Item {
@@ -98,11 +98,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float rcp_fast(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ float min_nan(float a, float b) {
     float d;
     asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -125,21 +120,6 @@ __device__ __forceinline__ void cap4(float& a, float& b, float& c, float& d, flo
     const float2 out2 = make_float2(cap_out, cap_out), n2 = make_float2(-2.f * cap_out, -2.f * cap_out);
     const float2 ab = fma2(mul2(inv, y), n2, out2), cd = fma2(mul2(inv, x), n2, out2);
     a = ab.x; b = ab.y; c = cd.x; d = cd.y;
-}
-// The same of two scores whose size is at most kCapNear caps: c tanh(y) = c y P(y^2), y = s / c, P the polynomial of degree 4 with the smallest relative error (1.3e-8, by
-// the exchange of extremes) for tanh(y) / y up to there: no exponential, no reciprocal. A warp takes it for a block all of whose scores are that small. (4 x 4096 tokens, cap 50, 16 heads
-// of 64: 691 us of scores of a deviation of 1, 754 by cap4; of 8, where no block is, 849 and 794; of 128: 747 and 843, 876 and 827.) to_y: score -> y, to_out: score -> log2 domain.
-constexpr float kCapNear = 0.5f;
-__device__ __forceinline__ void cap_near2(float& a, float& b, float to_y, float to_out) {
-    const float2 s = make_float2(a, b), y = mul2(s, make_float2(to_y, to_y)), t = mul2(y, y);
-    auto both = [](float x) { return make_float2(x, x); };
-    float2 p = fma2(both(0.017135007306933403f), t, both(-0.05298607423901558f));
-    p = fma2(p, t, both(0.13324779272079468f));
-    p = fma2(p, t, both(-0.3333306908607483f));
-    p = fma2(p, t, both(1.f));
-    const float2 out = mul2(mul2(s, make_float2(to_out, to_out)), p);
-    a = out.x;
-    b = out.y;
 }
 // Bits i >= from of a word (from: any whole number).
 __device__ __forceinline__ uint32_t bits_from(int from) { return from <= 0 ? ~0u : from >= 32 ? 0u : ~0u << from; }
@@ -361,12 +341,12 @@ struct Blocks {
     }
 };
 
-template <int kHD, int kBias, bool kCap>
+template <int kHD, int kBias, int kCap>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                                                                                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TcRules p) {
     using C = Cfg<kHD>;
     const bool docs = p.summary != nullptr, help = kBias == kTable || docs;
-    constexpr bool kChanged = kCap || kBias != kNoBias;   // scores are in the log2 domain before the maximum is taken
+    constexpr bool kChanged = kCap != kNoCap || kBias != kNoBias;   // scores are in the log2 domain before the maximum is taken
     const RuleParams& r = p.r;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -728,21 +708,27 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 tmem_ld32(s_addr, reinterpret_cast<uint32_t(&)[32]>(v[0]));
                 tmem_ld32(s_addr + 32, reinterpret_cast<uint32_t(&)[32]>(v[1]));
                 tmem_ld_wait(v[0], v[1]);
-                if constexpr (kCap) {
+                if constexpr (kCap != kNoCap) {
                     if (left < kBK) {   // four scores share a reciprocal: what lies behind the last key must not be not a number
 #pragma unroll
                         for (int i = 0; i < 64; ++i) v[i >> 5][i & 31] = i < left ? v[i >> 5][i & 31] : 0.f;
                     }
+                    // A warp takes the polynomial for a block all of whose scores are within half a cap: a tenth faster where scores are small, but a fifteenth slower where they are
+                    // not, for the vote. (4 x 4096 tokens, cap 50, 16 heads of 64, scores of a deviation of 1: 691 us, 754 by cap4 alone; of 8, where no block is that small, 849
+                    // and 794. Heads of 128: 747 and 843, 876 and 827.)
                     bool near = false;
-                    if constexpr (kBias == kNoBias) {   // (where there is a bias the registers are short)
+                    if constexpr (kBias == kNoBias || kCap == kWide) {   // (where there is a bias the registers are short)
                         float size[2] = {0.f, 0.f};
 #pragma unroll
                         for (int i = 0; i < 64; i += 2) size[(i >> 1) & 1] = max3(size[(i >> 1) & 1], fabsf(v[i >> 5][i & 31]), fabsf(v[i >> 5][(i & 31) + 1]));
-                        near = __all_sync(0xffffffffu, fmaxf(size[0], size[1]) <= p.cap_near);
+                        near = __all_sync(0xffffffffu, fmaxf(size[0], size[1]) <= r.cap_near);
                     }
                     if (near) {
 #pragma unroll
-                        for (int i = 0; i < 64; i += 2) cap_near2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1], p.to_y, r.scale_log2);
+                        for (int i = 0; i < 64; i += 2) cap_near2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1], r.to_y, r.scale_log2);
+                    } else if constexpr (kCap == kWide) {
+#pragma unroll
+                        for (int i = 0; i < 64; i += 2) cap_wide2(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1], r);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 64; i += 4) cap4(v[i >> 5][i & 31], v[i >> 5][(i & 31) + 1], v[i >> 5][(i & 31) + 2], v[i >> 5][(i & 31) + 3], r.cap_in, r.cap_out);
@@ -925,7 +911,7 @@ __global__ void __launch_bounds__(128) document_summary_kernel(const __grid_cons
     }
 }
 
-template <int kHD, int kBias, bool kCap>
+template <int kHD, int kBias, int kCap>
 cudaError_t launch(int grid, cudaStream_t st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcRules& p) {
     const auto kernel = attention_rules_tc_kernel<kHD, kBias, kCap>;
     static_assert(Cfg<kHD>::kHelpAt + 2 * kShiftBytes + sizeof(TcShared) + sizeof(SeqTable) + 2048 <= 233472 / kCtasPerSm, "two CTAs to an SM");
@@ -935,12 +921,14 @@ cudaError_t launch(int grid, cudaStream_t st, const CUtensorMap& tq, const CUten
     const size_t smem = Cfg<kHD>::kHelpAt + (kBias == kTable ? 2 * kShiftBytes : 0) + sizeof(TcShared) + (p.sorted ? sizeof(SeqTable) : 0) + 1024;
     return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, tq, tk, tv, p);
 }
+template <int kHD, int kBias>
+cudaError_t launch_with(int grid, cudaStream_t st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcRules& p) {
+    const auto run = p.r.cap_wide ? launch<kHD, kBias, kWide> : p.r.cap_out > 0.f ? launch<kHD, kBias, kCapped> : launch<kHD, kBias, kNoCap>;
+    return run(grid, st, tq, tk, tv, p);
+}
 template <int kHD>
 cudaError_t launch_for(int grid, cudaStream_t st, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const TcRules& p) {
-    const bool cap = p.r.cap_out > 0.f;
-    const auto run = p.r.slopes  ? (cap ? launch<kHD, kSlopes, true> : launch<kHD, kSlopes, false>)
-                     : p.r.table ? (cap ? launch<kHD, kTable, true> : launch<kHD, kTable, false>)
-                                 : (cap ? launch<kHD, kNoBias, true> : launch<kHD, kNoBias, false>);
+    const auto run = p.r.slopes ? launch_with<kHD, kSlopes> : p.r.table ? launch_with<kHD, kTable> : launch_with<kHD, kNoBias>;
     return run(grid, st, tq, tk, tv, p);
 }
 
@@ -962,8 +950,6 @@ int attention_rules_tc_launch(const RuleParams& r, void* scratch, cudaStream_t s
         !make_tmap_heads_f16(&tk, r.k, r.k_rows, r.nhead / r.group, r.head_dim, r.k_pitch, kBK) ||
         !make_tmap_heads_f16(&tv, r.v, r.k_rows, r.nhead / r.group, r.head_dim, r.v_pitch, kBK))
         return fail(ET_ERR_CUDA, "et_attention_rules: cuTensorMapEncodeTiled failed");
-    p.to_y = (float)((double)r.cap_in * 0.34657359027997264);   // ln 2 / 2
-    p.cap_near = p.to_y > 0.f ? kCapNear / p.to_y : 0.f;
     p.summary = static_cast<const int2*>(scratch);
     p.summary_blocks = (r.max_k_len + kBK - 1) / kBK;
     if (scratch) {

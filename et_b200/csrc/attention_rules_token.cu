@@ -57,14 +57,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-__device__ __forceinline__ float rcp_fast(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // kHD: 64 or 128, the head's width rounded up. kTall: more than eight rows; otherwise the lower half of the tile is empty and left out of everything but the products.
-template <int kHD, bool kTall>
+// kWide: a cap above kWideCap.
+template <int kHD, bool kTall, bool kWide>
 __global__ void __launch_bounds__(kThreads) attention_rules_token_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                                                                          const __grid_constant__ RuleParams p, int row_tiles, bool longest_first, int* err) {
     using C = Cfg<kHD>;
@@ -198,7 +193,13 @@ __global__ void __launch_bounds__(kThreads) attention_rules_token_kernel(const _
         for (int x = 0; x < kX; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[x][e] = sc[e >> 1][2 * x + (e & 1)];
-        if (p.cap_out > 0.f) {
+        if (kWide) {
+#pragma unroll
+            for (int x = 0; x < kX; ++x) {
+                cap_wide2(v[x][0], v[x][1], p);
+                cap_wide2(v[x][2], v[x][3], p);
+            }
+        } else if (p.cap_out > 0.f) {
 #pragma unroll
             for (int x = 0; x < kX; ++x)
 #pragma unroll
@@ -372,9 +373,9 @@ __global__ void __launch_bounds__(kThreads) attention_rules_token_kernel(const _
     cluster.sync();   // nobody leaves while its rows are read
 }
 
-template <int kHD, bool kTall>
+template <int kHD, bool kTall, bool kWide>
 cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const RuleParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
-    const auto kernel = attention_rules_token_kernel<kHD, kTall>;
+    const auto kernel = attention_rules_token_kernel<kHD, kTall, kWide>;
     static PerDeviceOnce once;
     cudaError_t e = once.run([&] {
         cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kHD>::kBytes);
@@ -400,6 +401,11 @@ cudaError_t launch(const CUtensorMap& tk, const CUtensorMap& tv, const RuleParam
     return cudaLaunchKernelEx(&cfg, kernel, tk, tv, p, row_tiles, longest_first, err);
 }
 
+template <int kHD, bool kTall>
+cudaError_t launch_with(const CUtensorMap& tk, const CUtensorMap& tv, const RuleParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
+    return (p.cap_wide ? launch<kHD, kTall, true> : launch<kHD, kTall, false>)(tk, tv, p, row_tiles, units, csize, err, st);
+}
+
 }  // namespace
 
 bool attention_rules_token_takes(const RuleParams& p) {
@@ -423,7 +429,7 @@ int attention_rules_token_launch(const RuleParams& p, cudaStream_t st) {
     int csize = 1;
     while (csize < kMaxCluster && (long long)csize * kWarps * kKeys < p.max_k_len && units * csize * 2 <= (csize < 8 ? 4 : 1) * sm_count()) csize *= 2;
     const bool tall = p.max_q_len * p.group > 8;
-    const auto run = p.head_dim <= 64 ? (tall ? launch<64, true> : launch<64, false>) : (tall ? launch<128, true> : launch<128, false>);
+    const auto run = p.head_dim <= 64 ? (tall ? launch_with<64, true> : launch_with<64, false>) : (tall ? launch_with<128, true> : launch_with<128, false>);
     return cuda_status(run(tk, tv, p, row_tiles, units, csize, err, st), "et_attention_rules launch");
 }
 

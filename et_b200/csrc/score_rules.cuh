@@ -21,11 +21,44 @@ struct RuleParams {
     int batch, q_tokens, k_rows, max_q_len, max_k_len;
     float scale_log2;                      // score -> log2 domain
     float cap_in, cap_out;                 // 2 log2(e) scale / cap and cap log2(e); cap_out 0: not capped
+    float to_y, cap_near;                  // capped: score -> score / cap, and the largest score for which cap_near2 is taken
+    bool cap_wide;                         // a cap above kWideCap
     const float* slopes;
     const half* table;                     // [nhead][2 reach + 1]
     int reach, window_left, window_right;  // windows: kNoLimit without one
     const int *prefix_lens, *q_docs, *k_docs;
 };
+
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// c tanh(y) = c y P(y^2), y = s / c, of two scores whose size is at most kCapNear caps: P the polynomial of degree 4 with the smallest relative error for tanh(y) / y up to
+// there (by the exchange of extremes; 2.8e-8 with its coefficients as they stand here, beside some 2e-7 that fp32 products and sums lose): no exponential, no reciprocal.
+// to_out: score -> log2 domain.
+constexpr float kCapNear = 0.5f;
+__device__ __forceinline__ void cap_near2(float& a, float& b, float to_y, float to_out) {
+    const float2 s = make_float2(a, b), y = mul2(s, make_float2(to_y, to_y)), t = mul2(y, y);
+    auto both = [](float x) { return make_float2(x, x); };
+    float2 p = fma2(both(0.017135007306933403f), t, both(-0.05298607423901558f));
+    p = fma2(p, t, both(0.13324779272079468f));
+    p = fma2(p, t, both(-0.3333306908607483f));
+    p = fma2(p, t, both(1.f));
+    const float2 out = mul2(mul2(s, make_float2(to_out, to_out)), p);
+    a = out.x;
+    b = out.y;
+}
+// Caps above kWideCap: c - 2 c / (1 + 2^x) would be off by more than a fraction of a weight's half step in fp16 (4.9e-4): 1e-4 there, everything at 1e7. Each score
+// by the polynomial where it is within half a cap; beyond, that error is one of the score's own size. (A kernel of its own, as
+// the choice for each score costs more than one for all: single tokens, 64 x 8192 keys, 97 us with both in one kernel, 94 so.)
+constexpr float kWideCap = 512.f;
+__device__ __forceinline__ void cap_wide2(float& a, float& b, const RuleParams& p) {
+    float x = a, y = b;
+    cap_near2(x, y, p.to_y, p.scale_log2);
+    a = fabsf(a) <= p.cap_near ? x : fmaf(rcp_fast(1.f + ex2_fast(a * p.cap_in)), -2.f * p.cap_out, p.cap_out);
+    b = fabsf(b) <= p.cap_near ? y : fmaf(rcp_fast(1.f + ex2_fast(b * p.cap_in)), -2.f * p.cap_out, p.cap_out);
+}
 
 // Where a sequence's queries and keys are.
 struct RuleSeq {
@@ -100,7 +133,13 @@ static __device__ __noinline__ void rules_row(const RuleParams& p, const RuleSeq
             } else {
                 for (int d = 0; d < hd; ++d) dot = fmaf(__half2float(q[d]), __half2float(kr[d]), dot);
             }
-            score = p.cap_out > 0.f ? p.cap_out - 2.f * p.cap_out / (1.f + exp2f(dot * p.cap_in)) : dot * p.scale_log2;
+            if (p.cap_wide) {
+                float none = 0.f;
+                cap_wide2(dot, none, p);
+                score = dot;
+            } else {
+                score = p.cap_out > 0.f ? p.cap_out - 2.f * p.cap_out / (1.f + exp2f(dot * p.cap_in)) : dot * p.scale_log2;
+            }
             const int away = j - qpos;
             if (p.slopes) score -= slope * fabsf((float)away);
             if (table) score = fmaf(__half2float(table[max(-p.reach, min(p.reach, away))]), kRulesLog2e, score);

@@ -797,3 +797,37 @@ def test_tokens_over_kept_keys_of_values_beside_scores_far_below(et, hd, nq, n):
             expect = torch.zeros(nq, 4, hd, dtype=torch.bool, device="cuda")
             expect[:, 2:, 5] = True
             assert torch.equal(~torch.isfinite(out).view(nq, 4, hd), expect)
+
+
+@pytest.mark.parametrize("cap", [512.0, 600.0, 1.0e4, 1.0e6, 1.0e9, 1.0e30])
+@pytest.mark.parametrize("bias", ["none", "slopes", "table"])
+@pytest.mark.parametrize("hd", [64, 128, 24])
+@pytest.mark.parametrize("nq", [1, 4, 150])
+def test_attention_of_caps_far_above_the_scores(et, nq, hd, bias, cap):
+    """Such a cap changes next to nothing: the error does not grow with it."""
+    import torch
+    n = 333
+    Q, K, V = normal(7, nq, 4 * hd, std=4.0), normal(8, n, 2 * hd), normal(9, n, 2 * hd)
+    seqs = [(0, nq, 0, n, n - nq)]
+    rules = {"slopes": torch.rand(4, device="cuda") * 0.02} if bias == "slopes" else {"table": normal(4, 4, 61)} if bias == "table" else {}
+    scores = torch.einsum("qhd,khd->hqk", Q.double().view(nq, 4, hd), K.double().view(n, 2, hd).repeat_interleave(2, 1)) * hd ** -0.5
+    assert 8 < scores.abs().max() < 32
+    out = et.attention_rules(torch.zeros_like(Q), Q, K, V, hd, k_start=dev([0]), k_lens=dev([n]), batch=1, max_q_len=nq, max_k_len=n, cap=cap, slopes=rules.get("slopes"),
+                             distance_bias=rules.get("table"))
+    et.attention_check()
+    want, _ = ol.attention(Q, K, V, hd, seqs, cap=cap, **rules)
+    # The bound without a cap, a tenth wider. The cap moves a score by s^3 / 3 c^2 <= 0.042 (s <= 32, c >= 512) and a weight, which the bound is linear in, by 4.3 %
+    # (relative to the sum of the weights, in which scores of 8 and more hardly differ, less). Its own rounding, 2^-21 of a score, is 1.6e-5 of a weight: 3.2 % of the half step 2^-11 that each
+    # has in the bound. Up to c = 512 the quotient's rounding of 2^-22 c is as much as 1.3e-4: that one is counted as the oracle does.
+    _, bound = ol.attention(Q, K, V, hd, seqs, cap=cap if cap <= 512 else 0.0, **rules)
+    ol.assert_within(out, want, 1.1 * bound, f"cap {cap}")
+
+
+@pytest.mark.parametrize("hd", [64, 128, 24])
+@pytest.mark.parametrize("nq", [1, 4, 150])
+@pytest.mark.parametrize("std", [100.0, 1000.0])
+def test_attention_of_wide_caps_and_scores_around_them(et, nq, hd, std):
+    Q, K, V = normal(7, nq, 4 * hd, std=std), normal(8, 333, 2 * hd), normal(9, 333, 2 * hd)
+    for cap in (520.0, 2000.0):
+        for rules in ({}, {"table": normal(4, 4, 61)}):
+            run_attention(et, Q, K, V, hd, [(0, nq, 0, 333, 333 - nq)], k_start=[0], k_lens=[333], cap=cap, **rules)

@@ -11,7 +11,7 @@
 // O: an item's rows are written during the next one.
 //
 // Not a number times the weight 0 is not a number: V rows behind the last key are cleared in shared memory before P V, and a row whose result is not
-// finite is computed again from the keys that it sees (rules_row). So is one whose result, a mean of values near fp16's largest, has left the range by the
+// finite is computed again from the keys that it sees (rules_row), behind the CTA's last item. So is one whose result, a mean of values near fp16's largest, has left the range by the
 // rounding of its weights.
 //
 // Every mbarrier wait is bounded; a wait that gives up sets the error word that et_attention_check reads and the CTA leaves through the common exit.
@@ -74,6 +74,15 @@ struct Cfg {
     static constexpr int kKAt = kQStages * kQTile, kVAt = kKAt + kStages * kKTile, kHelpAt = kVAt + kStages * kKTile;
 };
 
+// Rows of an item that a softmax warp computes again once it has no more items: nobody may wait for that (some 14 us a key for 32 rows).
+struct Again {
+    int b, qi0, head;
+    unsigned rows;
+};
+// A CTA takes no more items while one of these lists has no room for those that may be on their way when the loading warp looks: one in each slot, its own
+// and the next. (What is not taken starts as a CTA of its own.)
+constexpr int kMaxAgain = 16;
+static_assert(kMaxAgain >= kItemRing + 3, "a CTA's first items have room");
 struct TcShared {
     uint4 clc;
     uint64_t clc_full;
@@ -86,6 +95,8 @@ struct TcShared {
     Block block[kBlockRing];
     alignas(16) int docs[2][kBK];         // read four at a time
     uint32_t tmem_base;
+    int n_again[kSoftmaxWarps], no_more;
+    alignas(16) Again again[kSoftmaxWarps][kMaxAgain];
 };
 struct SeqTable {
     RuleSeq seq[kMaxSorted];
@@ -198,6 +209,15 @@ __device__ __forceinline__ void sort_sequences(const RuleParams& p, SeqTable* t,
     }
     if (lane == 0) t->before[0] = 0;
     __syncwarp();
+}
+
+// The rows of a list, computed again (whole warp).
+static __device__ __noinline__ void rows_again(const RuleParams& r, const Again* list, int n) {
+    for (int i = 0; i < n; ++i) {
+        const Again a = list[i];
+        const RuleSeq s = rule_seq(r, a.b);
+        for (unsigned left = a.rows; left; left &= left - 1) rules_row(r, s, a.qi0 + __ffs(left) - 1, a.head);
+    }
 }
 
 // Which queries block `blk` is (whole warp); false: it lies beyond the batch (the grid of a ragged batch has slack).
@@ -363,6 +383,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
 
     if (warp == kLoadWarp) {
         if (lane == 0) {
+            for (int i = 0; i < kSoftmaxWarps; ++i) sh->n_again[i] = 0;
+            sh->no_more = 0;
             mbar_init(&sh->clc_full, 1);
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh->q_full[i], 1); mbar_init(&sh->q_empty[i], 1);
@@ -430,7 +452,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
             ++g;
         };
         for (;;) {
-            if (lane == 0 && p.take_over) {
+            const bool take_over = p.take_over && !__any_sync(0xffffffffu, *const_cast<volatile int*>(&sh->no_more));
+            if (lane == 0 && take_over) {
                 mbar_expect_tx(&sh->clc_full, 16);
                 clc_ask(&sh->clc, &sh->clc_full);
             }
@@ -464,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                     }
                 }
             }
-            if (!p.take_over) break;
+            if (!take_over) break;
             // the answer is awaited even on the way out: nothing may be in flight towards shared memory when the CTA leaves
             const bool answered = mbar_wait(&sh->clc_full, clc_phase);
             clc_phase ^= 1u;
@@ -654,8 +677,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 sixteen(o[1], 16, c + 3);
             }
             const float largest = fmaxf(__low2float(top), __high2float(top)), sum = __low2float(top) + __high2float(top);
-            unsigned again = __ballot_sync(0xffffffffu, in && !(largest <= 65504.f && sum == sum));
-            for (; again; again &= again - 1) rules_row(r, it.seq, it.qi0 + warp * 32 + __ffs(again) - 1, it.head);
+            const unsigned again = __ballot_sync(0xffffffffu, in && !(largest <= 65504.f && sum == sum));
+            if (again && lane == 0) {
+                const int n = sh->n_again[warp]++;
+                sh->again[warp][n] = Again{it.b, it.qi0 + warp * 32, it.head, again};
+                if (n >= kMaxAgain - kItemRing - 3) sh->no_more = 1;
+            }
             arrive(ET_BAR(item_empty, done_slot));
             done_slot = -1;
             return true;
@@ -876,6 +903,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
         }
         if (!ok && lane == 0) atomicExch(p.err, 22);
         __syncwarp();
+        const int n_again = sh->n_again[warp];
+        if (n_again) rows_again(r, sh->again[warp], n_again);
     }
 #undef ET_BAR
     tc_fence_before();

@@ -831,3 +831,33 @@ def test_attention_of_wide_caps_and_scores_around_them(et, nq, hd, std):
     for cap in (520.0, 2000.0):
         for rules in ({}, {"table": normal(4, 4, 61)}):
             run_attention(et, Q, K, V, hd, [(0, nq, 0, 333, 333 - nq)], k_start=[0], k_lens=[333], cap=cap, **rules)
+
+
+def test_attention_waits_for_long_rows_that_are_computed_again(et):
+    """An infinite value in a long sequence, seen by every query: its rows take a second, CTAs have more items, and no wait gives up meanwhile."""
+    import torch
+    hd, hq, nq, n = 64, 300, 32, 60000
+    Q, K, V = normal(1, nq, hq * hd), normal(2, n, hd), normal(3, n, hd)
+    V[n // 2, 5] = math.inf
+    out = et.attention_rules(torch.zeros_like(Q), Q, K, V, hd, k_start=dev([0]), k_lens=dev([n]), batch=1, max_q_len=nq, max_k_len=n)
+    et.attention_check()
+    odd = ~torch.isfinite(out).view(nq, hq, hd)
+    assert odd[:, :, 5].all() and int(odd.sum()) == nq * hq
+    for h in (0, 299):
+        want, bound = ol.attention(Q[:, h * hd:(h + 1) * hd], K, V.where(torch.isfinite(V), 0), hd, [(0, nq, 0, n, n - nq)])
+        want[:, 5] = math.nan
+        ol.assert_within(out[:, h * hd:(h + 1) * hd], want, bound, "rows computed again")
+
+
+def test_attention_of_many_items_with_rows_computed_again(et):
+    """More such items than a CTA keeps: every short sequence has a value that is not finite, of which only some queries know."""
+    import torch
+    hd, hq, lengths = 64, 16, [40, 200] * 200
+    Q, K, V, cu, seqs = packed(3, lengths, hq, hq, hd)
+    V[torch.as_tensor(cu[:-1] + 20, device="cuda", dtype=torch.long), hd + 7] = math.nan
+    for window in ((-1, 0), (-1, -1)):
+        out = run_attention(et, Q, K, V, hd, seqs, cu=cu, window=window)
+        odd = torch.zeros(len(Q), hq, hd, dtype=torch.bool, device="cuda")
+        at = torch.cat([torch.arange(n, device="cuda") for n in lengths])
+        odd[at >= (20 if window[1] == 0 else 0), 1, 7] = True
+        assert torch.equal(torch.isnan(out.view(-1, hq, hd)), odd)

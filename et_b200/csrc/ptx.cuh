@@ -96,16 +96,13 @@ __device__ __forceinline__ bool mbar_poll_warp(uint64_t* bar, uint32_t parity) {
     return __all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity));
 }
 // ------------------------------------------------------------------ TMA
-__device__ __forceinline__ void tma_load_2d_at(uint32_t dst, const void* tmap, int x, int y, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-        "{%2, %3}], [%4];" ::"r"(dst),
-        "l"(tmap), "r"(x), "r"(y), "r"(bar)
-        : "memory");
-}
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int x, int y,
                                             uint64_t* bar) {
-    tma_load_2d_at(smem_u32(dst), tmap, x, y, smem_u32(bar));
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+        "{%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(tmap), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
 }
 __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const void* tmap, int x, int y, int z, uint32_t bar) {
     asm volatile(
@@ -117,13 +114,12 @@ __device__ __forceinline__ void tma_load_3d_at(uint32_t dst, const void* tmap, i
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int x, int y, int z, uint64_t* bar) {
     tma_load_3d_at(smem_u32(dst), tmap, x, y, z, smem_u32(bar));
 }
-__device__ __forceinline__ void tma_store_2d_at(const void* tmap, uint32_t src, int x, int y) {
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                      tmap),
-                 "r"(src), "r"(x), "r"(y)
+                 "r"(smem_u32(src)), "r"(x), "r"(y)
                  : "memory");
 }
-__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int x, int y) { tma_store_2d_at(tmap, smem_u32(src), x, y); }
 __device__ __forceinline__ void tma_store_commit() {
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }

@@ -562,8 +562,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
                 left = next_left;
                 flags = next_flags;
                 if (C::kOPlaces > 1 && (flags & kFirst)) place ^= 1;
-                // The next block's scores ahead of this one's P V; of the next item only where its Q has a place of its own (else it has just been requested).
-                const bool ahead = C::kQStages > 1 || !(flags & kLast);
+                // The next block's scores ahead of this one's P V; of the next item only where its Q has a place of its own (else it has just been requested) and where it is
+                // known already: behind an item's last block may come so many without a key that the loading warp waits for this P V, which lets go of the item's slot.
+                const bool ahead = !(flags & kLast) || (C::kQStages > 1 && mbar_test(ET_BAR(block_full, (g + 1) % kBlockRing), ((g + 1) / kBlockRing) & 1u));
                 if (ahead && !(ok = entry(g + 1) && ((next_flags & kEnd) || qk(g + 1)))) break;
                 // O += P V of block g
                 const uint32_t vs = g % C::kStages;

@@ -861,3 +861,23 @@ def test_attention_of_many_items_with_rows_computed_again(et):
         at = torch.cat([torch.arange(n, device="cuda") for n in lengths])
         odd[at >= (20 if window[1] == 0 else 0), 1, 7] = True
         assert torch.equal(torch.isnan(out.view(-1, hq, hd)), odd)
+
+
+@pytest.mark.parametrize("hq,hk,hd", [(8, 8, 64), (8, 2, 32), (8, 4, 128)])
+@pytest.mark.parametrize("why", ["lengths", "documents", "positions"])
+@pytest.mark.parametrize("batch,every", [(400, 10), (120, 4), (400, 3)])
+def test_attention_of_many_items_that_see_nothing(et, hq, hk, hd, why, batch, every):
+    """A few sequences with keys and then many without one that a query sees: CTAs take several such items in a row behind one that has blocks."""
+    r = np.random.default_rng(batch)
+    lengths = [int(n) for n in r.integers(30, 300 if batch < 200 else 130, batch)]
+    full = [b < batch // every for b in range(batch)] if every != 3 else [b % 3 == 0 for b in range(batch)]
+    Q, K, V, cu, seqs = packed(3, lengths, hq, hk, hd)
+    if why == "lengths":
+        lens = [n if f else 0 for n, f in zip(lengths, full)]
+        run_attention(et, Q, K, V, hd, [(q0, n, q0, k, 0) for (q0, n, _, _, _), k in zip(seqs, lens)], cu=cu, k_lens=lens)
+    elif why == "documents":
+        ids = np.concatenate([np.full(n, 5 if f else -1) for n, f in zip(lengths, full)])
+        run_attention(et, Q, K, V, hd, seqs, cu=cu, docs=(dev(ids), dev(ids)))
+    else:   # more queries than kept keys: those before the first key see nothing, and behind the last one is nothing
+        lens = [n if f else 1 for n, f in zip(lengths, full)]
+        run_attention(et, Q, K, V, hd, [(q0, n, q0, k, k - n) for (q0, n, _, _, _), k in zip(seqs, lens)], cu=cu, k_start=[s[0] for s in seqs], k_lens=lens, window=(-1, 0))

@@ -205,7 +205,9 @@ int et_adapter_add_by(const et_adapter_add_args* args);
 
 /* ---- attention with rules on its scores (no counterpart in the reference, whose masks are additive and shared by all heads) ----
  *   score(q, k) = cap tanh(scale Q_q . K_k / cap) + bias(k - q);   out_q = sum of softmax(score) V_k over the keys that q sees
- * A query that sees no key gets zeros; what it does not see takes no part, whatever it holds (infinities, not a number). */
+ * A query that sees no key gets zeros; what it does not see takes no part, whatever it holds (infinities, not a number). What it sees and is not a
+ * number makes its row so; such rows are computed again one by one, which is slow. Scores and sums are fp32, the weights of V fp16. Fast are heads of a
+ * multiple of 16 up to 128 in rows that start on 16 bytes; a kernel of single queries takes the others. */
 typedef struct et_score_rules {
     float scale;               /* 0: 1 / sqrt(head_dim) */
     float cap;                 /* 0: scores are not capped */

@@ -881,3 +881,20 @@ def test_attention_of_many_items_that_see_nothing(et, hq, hk, hd, why, batch, ev
     else:   # more queries than kept keys: those before the first key see nothing, and behind the last one is nothing
         lens = [n if f else 1 for n, f in zip(lengths, full)]
         run_attention(et, Q, K, V, hd, [(q0, n, q0, k, k - n) for (q0, n, _, _, _), k in zip(seqs, lens)], cu=cu, k_start=[s[0] for s in seqs], k_lens=lens, window=(-1, 0))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("batch", [400, 120])
+def test_attention_of_items_that_all_have_rows_computed_again(et, batch, hd):
+    """Every item of every CTA: a CTA's list is full before its items are at an end, and the others start by themselves."""
+    import torch
+    hq, lengths = 24, [(40, 130, 75)[b % 3] for b in range(batch)]
+    Q, K, V, cu, seqs = packed(3, lengths, hq, hq, hd)
+    rows = torch.as_tensor(cu[:-1] + 20, device="cuda", dtype=torch.long)
+    for h in range(hq):
+        V[rows, h * hd + 7] = math.nan
+    out = run_attention(et, Q, K, V, hd, seqs, cu=cu, window=(-1, 0))
+    at = torch.cat([torch.arange(n, device="cuda") for n in lengths])
+    odd = torch.zeros(len(Q), hq, hd, dtype=torch.bool, device="cuda")
+    odd[:, :, 7] = (at >= 20)[:, None]
+    assert torch.equal(torch.isnan(out.view(-1, hq, hd)), odd)

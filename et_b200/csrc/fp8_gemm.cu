@@ -1,0 +1,693 @@
+// Linear with operands in e4m3: Y[T x N] = sum over blocks of 128 k of sx[block][t] sw[n / 128][block] (X . W^T over the block) + bias, optional tanh-GELU, fp16 out.
+//
+// The scales change every 128 k, so a block's products can not go on accumulating where the last block's are: each block is summed by tcgen05 (kind::f8f6f4, both operands from
+// 128-byte-swizzled shared memory, four UMMAs of 32 k) into a place of tensor memory of its own, and the epilogue's warps add it, times its scale, to sums in
+// registers while the next block is multiplied into another place. Two kernels:
+//
+// fp8_pair_kernel, many tokens: persistent pairs of CTAs (cta_group::2), 256 tokens x kBN features to a tile, two places. A thread has a token's row of kBN / 2 columns, all of
+// one block of 128 features: one scale a block and thread. A block of 256 x 256 takes the tensor pipe 512 clocks; the two epilogue warps of a scheduler 256 of additions beside the loads.
+//
+// fp8_few_kernel, few tokens: operands exchanged, 128 features are the tile's rows and kTokens tokens its columns, so that the weight, which is what has to
+// be read, fills the tile; K split over a cluster. Each CTA sends the others their columns' parts (asynchronous stores that count towards a barrier of the receiver) and
+// adds what it gets in the order of the ranks.
+//
+// The weight does not depend on the preceding kernel: its first copies are requested before griddepcontrol.wait. Every wait is bounded; a role that gives up records a code and all
+// threads reach the common exit.
+#include <algorithm>
+#include <cstring>
+#include <new>
+#include <vector>
+#include "common.h"
+#include "ptx.cuh"
+#include "tmap.h"
+
+namespace et {
+namespace {
+
+constexpr int kBlock = 128;                       // k (and features of the weight) that share a scale; bytes of a panel's rows
+constexpr int kSmemMax = 232448;
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The address of the same shared-memory object in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_cta(uint32_t at, uint32_t rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// A copy into this CTA's shared memory that reports to a barrier of either CTA of the pair (cluster address).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_f8_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void umma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Arrives on the barrier at this address in both CTAs of the pair once every UMMA issued so far has completed.
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+// Instruction descriptor of kind::f8f6f4 with e4m3 A and B, both K-major, and fp32 D: the fields lie as those of kind::f16, and e4m3 is type 0 as f16 is there.
+__host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N) { return make_idesc_f16(M, N); }
+
+// 8 columns of the thread's lane.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+
+// tanh-GELU in fp32, one special-function operation (2^-11 of the result's larger part).
+__device__ __forceinline__ float gelu_f32(float x) {
+    const float u = x * fmaf(x * x, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
+    float t;
+    asm("tanh.approx.f32 %0, %1;" : "=f"(t) : "f"(u));
+    const float h = 0.5f * x;
+    return fmaf(h, t, h);
+}
+template <bool kGelu>
+__device__ __forceinline__ float finish(float v, float bias) {
+    v += bias;
+    return kGelu ? gelu_f32(v) : v;
+}
+
+struct Fp8Params {
+    half* Y;
+    const half* bias;                             // padded with zeros to whole tiles
+    const float *x_scales, *w_scales;             // [blocks][T], [blocks of N][blocks]
+    long long y_pitch;
+    int T, N, k_blocks, tiles_n, tiles, stages;
+    int* err;
+};
+
+// ------------------------------------------------------------------------------------------ many tokens
+constexpr int kCopyWarps = 3, kEpiWarps = 8;
+constexpr int kMmaWarp = kCopyWarps, kFirstEpi = kCopyWarps + 1;
+constexpr int kPairThreads = 32 * (kFirstEpi + kEpiWarps);
+constexpr int kXPanel = 128 * kBlock;             // of a CTA's tokens
+constexpr int kUnitCols = 32, kUnitBytes = 32 * kUnitCols * 2;
+constexpr int kMaxStages = 9;
+
+struct PairShared {
+    uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t acc_full[2], acc_empty[2];
+    uint32_t tmem_base;
+};
+
+template <int kBN, bool kGelu>
+__global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
+                                                                   const __grid_constant__ Fp8Params p) {
+    constexpr int kWPanel = kBN / 2 * kBlock, kStage = kXPanel + kWPanel;
+    constexpr int kCols = kBN / 2;                // of a thread
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ PairShared shared;
+    PairShared* const sh = &shared;
+    const int S = p.stages;
+    const uint32_t ring = smem_u32(smem), epi = ring + S * kStage;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_rank();
+    const int pair = (int)blockIdx.x >> 1, G = (int)gridDim.x >> 1;
+    const int my_tiles = (p.tiles - pair + G - 1) / G;
+    if (tid == 0) {
+        for (int i = 0; i < S; ++i) { mbar_init(&sh->full[i], 1); mbar_init(&sh->empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&sh->acc_full[i], 1); mbar_init(&sh->acc_empty[i], 2 * kEpiWarps); }
+        fence_mbar_init();
+        prefetch_tmap(&tmX);
+        prefetch_tmap(&tmW);
+    }
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(2 * kBN) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // the other CTA's barriers exist
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+    const int total = my_tiles * p.k_blocks;
+    if (warp < kCopyWarps) {
+        // ---- copies: the warps take the stages in turn (their number divides that of the stages, so that a stage always falls to the same warp)
+        auto load_w = [&](int s, int kb, int tile) {
+            const uint32_t bar = in_cta(smem_u32(&sh->full[s]), 0);
+            if (rank == 0) mbar_expect_tx(&sh->full[s], 2 * kStage);
+            tma_load_2d_pair(ring + s * kStage + kXPanel, &tmW, kb * kBlock, (tile % p.tiles_n) * kBN + (int)rank * (kBN / 2), bar);
+        };
+        auto load_x = [&](int s, int kb, int tile) {
+            tma_load_2d_pair(ring + s * kStage, &tmX, kb * kBlock, (tile / p.tiles_n) * 256 + (int)rank * 128, in_cta(smem_u32(&sh->full[s]), 0));
+        };
+        const int ahead = min(S, p.k_blocks);
+        if (lane == 0)
+            for (int i = warp; i < ahead; i += kCopyWarps) load_w(i, i, pair);
+        __syncwarp();
+        pdl_wait();
+        bool ok = true;
+        int s = warp, kb = warp, tile = pair;
+        uint32_t ph = 1;
+        for (int c = warp; c < total; c += kCopyWarps) {
+            while (kb >= p.k_blocks) { kb -= p.k_blocks; tile += G; }
+            if (s >= S) { s -= S; ph ^= 1u; }
+            if (c >= S) ok = mbar_wait(&sh->empty[s], ph);
+            if (!ok) break;
+            if (lane == 0) {
+                if (c >= ahead) load_w(s, kb, tile);
+                load_x(s, kb, tile);
+            }
+            __syncwarp();
+            kb += kCopyWarps;
+            s += kCopyWarps;
+        }
+        // (On the normal way out every copy has been consumed. A wait that gives up has lasted far longer than any copy.)
+        if (!ok && lane == 0) atomicExch(p.err, 61);
+    } else if (warp == kMmaWarp) {
+        if (rank == 0 && elect_one()) {
+            constexpr uint32_t idesc = make_idesc_e4m3(256, kBN);
+            const uint64_t x0 = make_smem_desc(ring, 16, 1024, 2), w0 = make_smem_desc(ring + kXPanel, 16, 1024, 2);
+            bool ok = true;
+            int s = 0;
+            uint32_t ph = 0;
+            for (int c = 0; c < total; ++c) {
+                const int buf = c & 1;
+                ok = mbar_wait(&sh->acc_empty[buf], ((uint32_t)(c >> 1) & 1u) ^ 1u) && mbar_wait(&sh->full[s], ph);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t at = (uint64_t)(s * kStage) >> 4;   // descriptors count 16-byte units
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) umma_f8_pair(tmem + buf * kBN, x0 + at + ks * 2, w0 + at + ks * 2, idesc, ks > 0);
+                umma_commit_pair(smem_u32(&sh->empty[s]));
+                umma_commit_pair(smem_u32(&sh->acc_full[buf]));
+                if (++s == S) { s = 0; ph ^= 1u; }
+            }
+            if (!ok) atomicExch(p.err, 62);
+        }
+        __syncwarp();
+    } else {
+        // ---- sums of this CTA's 128 tokens: a row to a thread, two warps share its columns
+        const int w = warp - kFirstEpi, q = warp & 3, h = w >> 2;
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + h * kCols;
+        const uint32_t buf_at = epi + w * kUnitBytes;
+        const uint32_t to = buf_at + lane * 64, swizzle = (lane >> 1) & 3;   // row `lane`: four 16-byte chunks under the 64-byte swizzle
+        const uint32_t empty_bar = in_cta(smem_u32(&sh->acc_empty[0]), 0);
+        const int n_blocks = (p.N + kBlock - 1) / kBlock;
+        bool ok = true;
+        pdl_wait();
+        int c = 0;
+        for (int tl = 0; tl < my_tiles && ok; ++tl) {
+            const int tile = pair + tl * G;
+            const int m0 = (tile / p.tiles_n) * 256 + (int)rank * 128 + q * 32, n0 = (tile % p.tiles_n) * kBN + h * kCols;
+            const float* sx = p.x_scales + min(m0 + lane, p.T - 1);
+            const float* sw = p.w_scales + (long long)min(n0 / kBlock, n_blocks - 1) * p.k_blocks;
+            float acc[kCols];
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+            float next_x = __ldcg(sx), next_w = __ldg(sw);
+            for (int kb = 0; kb < p.k_blocks; ++kb, ++c) {
+                const int buf = c & 1;
+                const float scale = next_x * next_w;
+                if (kb + 1 < p.k_blocks) {
+                    next_x = __ldcg(sx + (long long)(kb + 1) * p.T);
+                    next_w = __ldg(sw + kb + 1);
+                }
+                ok = mbar_wait(&sh->acc_full[buf], (uint32_t)(c >> 1) & 1u);
+                if (!ok) break;
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < kCols; i += 16) {
+                    uint32_t d[16];
+                    tmem_ld16(from + buf * kBN + i, d);
+                    tmem_ld_wait(d);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[i + j] = fmaf(__uint_as_float(d[j]), scale, acc[i + j]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (elect_one()) mbar_arrive_cluster(empty_bar + buf * 8);
+                __syncwarp();
+            }
+            if (!ok) break;
+            if (tl + 1 == my_tiles) pdl_launch_dependents();
+#pragma unroll
+            for (int u = 0; u < kCols / kUnitCols; ++u) {
+                const int col = n0 + u * kUnitCols;
+                uint4 ov[4];
+                half2* const o = reinterpret_cast<half2*>(ov);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + col) + j);
+                    const half2* const b = reinterpret_cast<const half2*>(&bv);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = __half22float2(b[i]);
+                        o[j * 4 + i] = __floats2half2_rn(finish<kGelu>(acc[u * kUnitCols + j * 8 + 2 * i], f.x), finish<kGelu>(acc[u * kUnitCols + j * 8 + 2 * i + 1], f.y));
+                    }
+                }
+                tma_store_wait_read();   // the buffer's previous store has read it
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sts128(to + ((j ^ swizzle) << 4), ov[j]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (col < p.N && m0 < p.T && elect_one()) {
+                    tma_store_2d(&tmY, smem + (buf_at - ring), col, m0);
+                    tma_store_commit();
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok && lane == 0) atomicExch(p.err, 63);
+        tma_store_wait_read();
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();   // nobody still reads this CTA's shared memory or signals its barriers
+    tc_fence_after();
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kBN) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------ few tokens
+constexpr int kFewEpi = 8, kWWarp = 8, kXWarp = 9, kFewMma = 10, kFewThreads = 11 * 32;
+constexpr int kMaxPlaces = 8;
+constexpr int kWTile = 128 * kBlock;              // 128 features of the weight
+
+struct FewShared {
+    uint64_t full[kMaxPlaces], empty[kMaxPlaces];
+    uint64_t acc_full[kMaxPlaces], acc_empty[kMaxPlaces];
+    uint64_t received;
+    uint32_t tmem_base;
+    __align__(16) float scales[kFewEpi][2][64];   // of a warp's columns, two blocks in turn
+};
+
+// Four words to the address `addr` of CTA `rank` of the cluster, which count towards the bytes that its barrier at `bar` waits for.
+__device__ __forceinline__ void st_async_cluster(uint32_t addr, uint32_t bar, uint32_t rank, const float* v) {
+    asm volatile("{\n.reg .b32 a, b;\nmapa.shared::cluster.u32 a, %0, %2;\nmapa.shared::cluster.u32 b, %1, %2;\n"
+                 "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [a], {%3,%4,%5,%6}, [b];\n}" ::"r"(addr), "r"(bar), "r"(rank), "r"(__float_as_uint(v[0])),
+                 "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3]))
+                 : "memory");
+}
+// A bounded wait like mbar_wait, for what other CTAs of the cluster have written.
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
+        uint32_t ok;
+        asm volatile("{\n.reg .pred P;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\nselp.u32 %0, 1, 0, P;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
+
+// Places of tensor memory, of kTokens columns each.
+__host__ __device__ constexpr int few_places(int tokens) { return tokens <= 64 ? 4 : 2; }
+// A CTA that waits for the others of its cluster may not have to wait for tensor memory that another cluster's CTA holds, which may wait for this one's. So each
+// takes no smaller a part of an SM's shared memory (227 KB) than of its tensor memory (512 columns): those that find a place find both.
+constexpr int kSmemPerColumn = 454;
+
+template <int kTokens, bool kGelu>
+__global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Fp8Params p,
+                                                                 int split) {
+    constexpr int kXTile = kTokens * kBlock, kStage = kWTile + kXTile;
+    constexpr int kPlaces = few_places(kTokens);
+    constexpr int kAlloc = kPlaces * kTokens;
+    constexpr int kCols = kTokens / 2;                        // of a warp
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ FewShared shared;
+    FewShared* const sh = &shared;
+    const int S = p.stages, own_cols = kTokens / split;
+    const uint32_t ring = smem_u32(smem);
+    float4* const recv = reinterpret_cast<float4*>(smem + S * kStage);   // of the other shares, this CTA's columns: [share][four columns][row]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)cluster_rank(), tile = (int)blockIdx.x / split;
+    const int n0 = (tile % p.tiles_n) * 128, t0 = (tile / p.tiles_n) * kTokens;
+    const int kb0 = (int)((long long)rank * p.k_blocks / split), kn = (int)((long long)(rank + 1) * p.k_blocks / split) - kb0;
+    if (warp == kWWarp) {
+        if (lane == 0) {
+            for (int i = 0; i < S; ++i) { mbar_init(&sh->full[i], 2); mbar_init(&sh->empty[i], 1); }
+            for (int i = 0; i < kPlaces; ++i) { mbar_init(&sh->acc_full[i], 1); mbar_init(&sh->acc_empty[i], kFewEpi); }
+            mbar_init(&sh->received, 1);
+            fence_mbar_init();
+            mbar_expect_tx(&sh->received, (uint32_t)((split - 1) * own_cols * 128 * 4));
+        }
+    } else if (warp == kFewMma) {
+        tmem_alloc(&sh->tmem_base, kAlloc);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this CTA runs and its barriers exist: its memory may be written to
+    const uint32_t tmem = sh->tmem_base;
+    bool ok = true;
+    float acc[kCols];
+#pragma unroll
+    for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
+    if (warp == kWWarp || warp == kXWarp) {
+        const bool is_x = warp == kXWarp;
+        if (is_x) pdl_wait();
+        if (lane == 0) {
+            int s = 0;
+            uint32_t ph = 1;
+            int i = 0;
+            for (; i < kn; ++i) {
+                ok = i < S || mbar_wait(&sh->empty[s], ph);
+                if (!ok) break;
+                mbar_expect_tx(&sh->full[s], is_x ? kXTile : kWTile);
+                if (is_x) tma_load_2d(smem + s * kStage + kWTile, &tmX, (kb0 + i) * kBlock, t0, &sh->full[s]);
+                else tma_load_2d(smem + s * kStage, &tmW, (kb0 + i) * kBlock, n0, &sh->full[s]);
+                if (++s == S) { s = 0; ph ^= 1u; }
+            }
+            if (!ok) {   // copies in flight land before the CTA leaves (bounded)
+                atomicExch(p.err, 64);
+                for (int j = max(i - S, 0); j < i; ++j) mbar_wait(&sh->full[j % S], (j / S) & 1);
+            }
+        }
+        __syncwarp();
+    } else if (warp == kFewMma) {
+        if (elect_one()) {
+            constexpr uint32_t idesc = make_idesc_e4m3(128, kTokens);
+            const uint64_t w0 = make_smem_desc(ring, 16, 1024, 2), x0 = make_smem_desc(ring + kWTile, 16, 1024, 2);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int i = 0; i < kn; ++i) {
+                const int place = i % kPlaces;
+                ok = (i < kPlaces || mbar_wait(&sh->acc_empty[place], (uint32_t)(i / kPlaces - 1) & 1u)) && mbar_wait(&sh->full[s], ph);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t at = (uint64_t)(s * kStage) >> 4;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) umma_f8(tmem + place * kTokens, w0 + at + ks * 2, x0 + at + ks * 2, idesc, ks > 0);
+                umma_commit(&sh->empty[s]);
+                umma_commit(&sh->acc_full[place]);
+                if (++s == S) { s = 0; ph ^= 1u; }
+            }
+            if (!ok) atomicExch(p.err, 65);
+        }
+        __syncwarp();
+    } else {
+        // ---- a feature to a thread, two warps share the tokens
+        const int q = warp & 3, h = warp >> 2;
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + h * kCols;
+        const float* const sw = p.w_scales + (long long)(n0 / kBlock) * p.k_blocks + kb0;
+        constexpr int kPer = (kCols + 31) / 32;   // columns of a lane, whose scales it fetches
+        pdl_wait();
+        auto fetch = [&](int i, float (&v)[kPer]) {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int t = t0 + h * kCols + j * 32 + lane;
+                v[j] = j * 32 + lane < kCols && t < p.T ? __ldcg(p.x_scales + (long long)(kb0 + i) * p.T + t) * __ldg(sw + i) : 0.f;
+            }
+        };
+        float next[kPer];
+        if (kn > 0) fetch(0, next);
+        for (int i = 0; i < kn; ++i) {
+            const int place = i % kPlaces;
+            float* const mine = sh->scales[warp][i & 1];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                if (j * 32 + lane < kCols) mine[j * 32 + lane] = next[j];
+            __syncwarp();
+            if (i + 1 < kn) fetch(i + 1, next);
+            ok = mbar_wait(&sh->acc_full[place], (uint32_t)(i / kPlaces) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            constexpr int kStep = kCols < 16 ? kCols : 16;
+#pragma unroll
+            for (int c = 0; c < kCols; c += kStep) {
+                uint32_t d[kStep];
+                if constexpr (kStep == 8) tmem_ld8(from + place * kTokens + c, d);
+                else tmem_ld16(from + place * kTokens + c, d);
+                tmem_ld_wait(d);
+#pragma unroll
+                for (int j = 0; j < kStep; j += 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(mine + c + j);
+                    acc[c + j] = fmaf(__uint_as_float(d[j]), f.x, acc[c + j]);
+                    acc[c + j + 1] = fmaf(__uint_as_float(d[j + 1]), f.y, acc[c + j + 1]);
+                    acc[c + j + 2] = fmaf(__uint_as_float(d[j + 2]), f.z, acc[c + j + 2]);
+                    acc[c + j + 3] = fmaf(__uint_as_float(d[j + 3]), f.w, acc[c + j + 3]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->acc_empty[place]);
+        }
+        if (!ok && lane == 0) atomicExch(p.err, 66);
+    }
+    __syncwarp();
+    pdl_launch_dependents();
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // every CTA of the cluster runs
+    bool got = true;
+    if (warp < kFewEpi) {
+        const int q = warp & 3, h = warp >> 2, row = q * 32 + lane;
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4) {
+            const int col = h * kCols + c, dst = col / own_cols, g = (col - dst * own_cols) / 4;
+            if (dst == rank) continue;   // the same for the whole warp
+            const int share = rank < dst ? rank : rank - 1;
+            st_async_cluster(smem_u32(recv + ((size_t)share * (own_cols / 4) + g) * 128 + row), smem_u32(&sh->received), dst, acc + c);
+        }
+    }
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this warp has sent everything
+    if (warp < kFewEpi) {
+        if (split > 1) got = mbar_wait_cluster(smem_u32(&sh->received), 0);
+        if (!got && lane == 0) atomicExch(p.err, 67);
+        const int q = warp & 3, h = warp >> 2, row = q * 32 + lane, n = n0 + row;
+        const float bias = __half2float(p.bias[n]);
+#pragma unroll
+        for (int c = 0; c < kCols; c += 4) {
+            const int col = h * kCols + c, dst = col / own_cols, g = (col - dst * own_cols) / 4;
+            if (dst != rank || t0 + col >= p.T) continue;
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < split; ++k) {   // in the order of the shares
+                float4 x = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                if (k != rank) x = recv[((size_t)(k < rank ? k : k - 1) * (own_cols / 4) + g) * 128 + row];
+                v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
+            }
+            if (n < p.N) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (t0 + col + j < p.T) p.Y[(long long)(t0 + col + j) * p.y_pitch + n] = __float2half_rn(finish<kGelu>(v[j], bias));
+            }
+        }
+    }
+    __syncwarp();
+    // Normally all have sent when this CTA has received. One that gave up stays until nothing is on its way to it.
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    if (!got) mbar_wait_cluster(smem_u32(&sh->received), 0);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kFewMma) tmem_dealloc(tmem, kAlloc);
+}
+
+bool make_tmap_bytes(CUtensorMap* out, const void* base, uint64_t rows, uint64_t cols, uint64_t pitch, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {pitch};
+    cuuint32_t box[2] = {kBlock, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace
+}  // namespace et
+
+struct et_fp8_weight {
+    int device = 0, K = 0, N = 0;
+    uint8_t* codes = nullptr;     // [N x K]
+    float* scales = nullptr;      // [blocks of N][blocks of K]
+    half* bias = nullptr;         // padded with zeros to a multiple of 256
+    int* err = nullptr;
+    CUtensorMap map64, map128;    // 64 and 128 rows to a copy
+};
+
+namespace et {
+namespace {
+
+struct Fp8Plan {
+    int bn;        // > 0: pairs with tiles of bn features
+    int tokens;    // few tokens: columns of a tile, and CTAs that share a tile's K
+    int split;
+};
+
+Fp8Plan fp8_plan(int T, int N, int k_blocks) {
+    Fp8Plan plan = {0, 0, 1};
+    const int tiles_n = (N + 127) / 128;
+    if (T > 256) {
+        const int pairs = sm_count() / 2, m = (T + 255) / 256;
+        plan.bn = m * ((N + 255) / 256) >= pairs ? 256 : 128;
+        return plan;
+    }
+    plan.tokens = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+    const int tiles = tiles_n * ((T + plan.tokens - 1) / plan.tokens);
+    while (plan.split < 8 && plan.split * 2 <= k_blocks && plan.tokens / (plan.split * 2) >= 4 && tiles * plan.split * 2 <= sm_count()) plan.split *= 2;
+    return plan;
+}
+
+template <int kBN, bool kGelu>
+cudaError_t launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& ty, Fp8Params p, cudaStream_t st) {
+    constexpr int kStage = kXPanel + kBN / 2 * kBlock;
+    const auto kernel = fp8_pair_kernel<kBN, kGelu>;
+    static PerDeviceOnce once;
+    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - 1024); });
+    if (e != cudaSuccess) return e;
+    p.tiles_n = (p.N + kBN - 1) / kBN;
+    p.tiles = (p.T + 255) / 256 * p.tiles_n;
+    p.stages = std::min(kMaxStages, (kSmemMax - 2048 - kEpiWarps * kUnitBytes) / kStage) / kCopyWarps * kCopyWarps;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * std::min(p.tiles, sm_count() / 2)));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = (size_t)p.stages * kStage + kEpiWarps * kUnitBytes + 1024;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, ty, p);
+}
+
+template <int kTokens, bool kGelu>
+cudaError_t launch_few(const CUtensorMap& tx, const CUtensorMap& tw, Fp8Params p, int split, cudaStream_t st) {
+    constexpr int kStage = kWTile + kTokens * kBlock;
+    const auto kernel = fp8_few_kernel<kTokens, kGelu>;
+    static PerDeviceOnce once;
+    const int max_smem = kSmemMax - ((int)sizeof(FewShared) + 1023) / 1024 * 1024;
+    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, max_smem); });
+    if (e != cudaSuccess) return e;
+    p.tiles_n = (p.N + 127) / 128;
+    p.tiles = (p.T + kTokens - 1) / kTokens * p.tiles_n;
+    const int recv = (split - 1) * (kTokens / split) * 128 * 4;
+    p.stages = std::min({kMaxPlaces, (max_smem - 1024 - recv) / kStage, (p.k_blocks + split - 1) / split});
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.tiles * split));
+    cfg.blockDim = dim3(kFewThreads);
+    cfg.dynamicSmemBytes = (size_t)std::max(p.stages * kStage + recv + 1024, few_places(kTokens) * kTokens * kSmemPerColumn);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, p, split);
+}
+
+template <bool kGelu>
+int fp8_run(const et_fp8_weight* w, const Fp8Params& p, const Fp8Plan& plan, const void* x, long long x_pitch, cudaStream_t st) {
+    CUtensorMap tx, ty;
+    const int x_rows = plan.bn ? 128 : plan.tokens;
+    if (!make_tmap_bytes(&tx, x, (uint64_t)p.T, (uint64_t)w->K, (uint64_t)x_pitch, (uint32_t)x_rows)) return fail(ET_ERR_CUDA, "et_fp8_linear: cuTensorMapEncodeTiled failed");
+    cudaError_t e;
+    if (plan.bn) {
+        if (!make_tmap_2d_f16(&ty, p.Y, (uint64_t)p.T, (uint64_t)p.N, (uint64_t)p.y_pitch, 32, kUnitCols, 64)) return fail(ET_ERR_CUDA, "et_fp8_linear: cuTensorMapEncodeTiled failed");
+        e = plan.bn == 256 ? launch_pair<256, kGelu>(tx, w->map128, ty, p, st) : launch_pair<128, kGelu>(tx, w->map64, ty, p, st);
+    } else {
+        e = plan.tokens == 16   ? launch_few<16, kGelu>(tx, w->map128, p, plan.split, st)
+            : plan.tokens == 32 ? launch_few<32, kGelu>(tx, w->map128, p, plan.split, st)
+            : plan.tokens == 64 ? launch_few<64, kGelu>(tx, w->map128, p, plan.split, st)
+                                : launch_few<128, kGelu>(tx, w->map128, p, plan.split, st);
+    }
+    return cuda_status(e, "et_fp8_linear launch");
+}
+
+}  // namespace
+}  // namespace et
+
+extern "C" int et_fp8_weight_destroy(et_fp8_weight* w) {
+    if (!w) return ET_OK;
+    cudaFree(w->codes);
+    cudaFree(w->scales);
+    cudaFree(w->bias);
+    cudaFree(w->err);
+    delete w;
+    return ET_OK;
+}
+
+extern "C" int et_fp8_weight_create(et_fp8_weight** out, int in_feat, int out_feat, const void* codes_host, const float* scales_host, const void* bias_host) {
+    using namespace et;
+    ET_REQUIRE(out, "et_fp8_weight_create: null output");
+    *out = nullptr;
+    ET_REQUIRE(in_feat > 0 && out_feat > 0 && in_feat % 16 == 0 && out_feat % 16 == 0, "et_fp8_weight_create: in_feat and out_feat must be positive multiples of 16");
+    ET_REQUIRE(codes_host && scales_host, "et_fp8_weight_create: null pointer");
+    auto* w = new (std::nothrow) et_fp8_weight;
+    if (!w) return fail(ET_ERR_CUDA, "et_fp8_weight_create: out of host memory");
+    w->K = in_feat;
+    w->N = out_feat;
+    const size_t bytes = (size_t)in_feat * out_feat, n_scales = (size_t)((in_feat + kBlock - 1) / kBlock) * ((out_feat + kBlock - 1) / kBlock), n_bias = ((size_t)out_feat + 255) / 256 * 256;
+    cudaError_t e = cudaGetDevice(&w->device);
+    if (e == cudaSuccess) e = cudaMalloc(&w->codes, bytes);
+    if (e == cudaSuccess) e = cudaMalloc(&w->scales, n_scales * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&w->bias, n_bias * sizeof(half));
+    if (e == cudaSuccess) e = cudaMalloc(&w->err, sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(w->bias, 0, n_bias * sizeof(half));
+    if (e == cudaSuccess) e = cudaMemset(w->err, 0, sizeof(int));
+    if (e == cudaSuccess) e = cudaMemcpy(w->codes, codes_host, bytes, cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaMemcpy(w->scales, scales_host, n_scales * sizeof(float), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess && bias_host) e = cudaMemcpy(w->bias, bias_host, (size_t)out_feat * sizeof(half), cudaMemcpyHostToDevice);
+    if (e == cudaSuccess) e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) {
+        et_fp8_weight_destroy(w);
+        return cuda_status(e, "et_fp8_weight_create");
+    }
+    if (!make_tmap_bytes(&w->map64, w->codes, (uint64_t)out_feat, (uint64_t)in_feat, (uint64_t)in_feat, 64) ||
+        !make_tmap_bytes(&w->map128, w->codes, (uint64_t)out_feat, (uint64_t)in_feat, (uint64_t)in_feat, 128)) {
+        et_fp8_weight_destroy(w);
+        return fail(ET_ERR_CUDA, "et_fp8_weight_create: cuTensorMapEncodeTiled failed");
+    }
+    *out = w;
+    return ET_OK;
+}
+
+extern "C" int et_fp8_weight_check(const et_fp8_weight* w, int* code) {
+    using namespace et;
+    ET_REQUIRE(w && code, "et_fp8_weight_check: null pointer");
+    *code = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpy(code, w->err, sizeof(int), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess && *code) e = cudaMemset(w->err, 0, sizeof(int));
+    if (e != cudaSuccess) return cuda_status(e, "et_fp8_weight_check");
+    if (*code) {
+        set_error("8-bit linear: device wait %d gave up", *code);
+        return ET_ERR_DEVICE_TIMEOUT;
+    }
+    return ET_OK;
+}
+
+extern "C" int et_fp8_linear(const et_fp8_linear_args* a) {
+    using namespace et;
+    ET_REQUIRE(a && a->weight, "et_fp8_linear: null weight");
+    const et_fp8_weight* const w = a->weight;
+    ET_REQUIRE(a->tokens >= 0, "et_fp8_linear: negative size");
+    if (a->tokens == 0) return ET_OK;
+    ET_REQUIRE(a->y && a->x && a->x_scales, "et_fp8_linear: null pointer");
+    const long long y_pitch = a->tokens == 1 ? (w->N + 7) / 8 * 8 : a->y_pitch, x_pitch = a->tokens == 1 ? w->K : a->x_pitch;
+    ET_REQUIRE(y_pitch >= w->N && x_pitch >= w->K, "et_fp8_linear: pitch below the width");
+    ET_REQUIRE(aligned16(a->x) && aligned16(a->y) && x_pitch % 16 == 0 && y_pitch % 8 == 0, "et_fp8_linear: rows must start on 16 bytes");
+    int dev = -1;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return cuda_status(e, "et_fp8_linear");
+    ET_REQUIRE(dev == w->device, "et_fp8_linear: the weight belongs to another device");
+    Fp8Params p = {};
+    p.Y = static_cast<half*>(a->y); p.bias = w->bias; p.x_scales = a->x_scales; p.w_scales = w->scales;
+    p.y_pitch = y_pitch; p.T = a->tokens; p.N = w->N; p.k_blocks = (w->K + kBlock - 1) / kBlock; p.err = w->err;
+    const Fp8Plan plan = fp8_plan(a->tokens, w->N, p.k_blocks);
+    return (a->gelu ? fp8_run<true> : fp8_run<false>)(w, p, plan, a->x, x_pitch, static_cast<cudaStream_t>(a->stream));
+}

@@ -18,6 +18,7 @@ __all__ = [
     "encoder_batch_buffer_size", "KIND_TILE", "KIND_PRUNE", "KIND_LENGTH", "KIND_PRUNE_QKV",
     "Model", "attention_check", "prune_dense_to_tiles", "select_rows_magnitude", "compact_rows", "set_tuning_goal",
     "set_attention_scores_fp32", "attention_scores_fp32", "rotary_axes", "AdapterBank", "attention_rules", "attention_rules_scratch_size",
+    "skip_rmsnorm", "quantise_rows", "Fp8Weight", "kv_cache_write", "kv_cache_read", "attention_tree",
 ]
 
 _i = ctypes.c_int
@@ -31,6 +32,7 @@ _SIGNATURES = {
     "et_qk_scores": "pppiiip", "et_attention_sharedqk": "ppppiiip", "et_attention_static_scores": "pppppiiip",
     "et_attention_batch": "ppppiippppippiiiiiip", "et_encoder_run": "pppp", "et_encoder_run_batch": "pppppipsp",
     "et_model_run_batch": "pppppip", "et_rotary_axes_by": "p", "et_adapter_add_by": "p", "et_attention_rules_by": "p",
+    "et_skip_rmsnorm": "p", "et_quantise_rows": "p", "et_fp8_linear": "p", "et_kv_cache_write": "p", "et_kv_cache_read": "p", "et_attention_tree": "p",
 }
 
 
@@ -454,6 +456,190 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
         0 if prefix_lens is None else _array("prefix_lens", prefix_lens, i32, device, batch),
         0 if q_docs is None else _array("q_docs", q_docs, i32, device, tokens), 0 if k_docs is None else _array("k_docs", k_docs, i32, device, k_rows),
         out_pitch, q_pitch, k_pitch, v_pitch, nhead, nhead_kv, head_dim, batch, tokens, k_rows, max_q_len or tokens, max_k_len or k_rows))
+    if rc:
+        check(rc)
+    return out
+
+
+# ---------------------------------------------------------------------------------- layers in 8 bits
+# et_skip_rmsnorm_args, et_quantise_rows_args, et_fp8_linear_args, et_kv_cache_args and et_attention_tree_args as they lie in memory
+_rmsnorm_args, _quantise_args, _fp8_args, _cache_args, _tree_args = (struct.Struct(f).pack for f in ("@7P6if0P", "@4P4i0P", "@5P4i0P", "@6P7i0P", "@9P12if0P"))
+_kept8 = None
+
+
+def _torch_kept8():
+    """(e4m3, uint8, int8, int64) of torch."""
+    global _kept8
+    if _kept8 is None:
+        import torch
+        _kept8 = (torch.float8_e4m3fn, torch.uint8, torch.int8, torch.int64)
+    return _kept8
+
+
+def _rows(name, t, dtypes, shape, device):
+    """(address, pitch) of rows with neighbouring elements that may be slices of wider ones."""
+    if t.dtype in dtypes and t.get_device() == device and t.shape == shape:
+        pitch, step = t.stride()
+        if shape[0] <= 1:
+            pitch = shape[1]
+        if step == 1 or shape[1] == 1:
+            return t.data_ptr(), pitch
+    raise ValueError(f"{name}: {tuple(shape)} of {' or '.join(str(d) for d in dtypes)} on the current CUDA device ({device}) with neighbouring elements expected, "
+                     f"not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _row_scales(scales, rows, width, f32, device):
+    if scales.dtype is not f32 or scales.get_device() != device or scales.shape != ((width + 127) // 128, rows) or not scales.is_contiguous():
+        raise ValueError(f"scales: contiguous float32 {((width + 127) // 128, rows)} on the current CUDA device ({device}) expected, not {scales.dtype} {tuple(scales.shape)} on {scales.device}")
+    return scales.data_ptr()
+
+
+def skip_rmsnorm(out, x, skip, gamma, residual=None, scales=None, eps=1e-6, stream=None):
+    """h = x + skip (skip may be None), out = h / sqrt(mean(h^2) + eps) * gamma for rows [rows, width] of float16, residual = h where it is given. Without scales
+    out is float16; with scales float32 [ceil(width / 128), rows] it is e4m3 (or uint8), a scale for each 128 features of a row. Rows may be slices of wider ones; residual
+    (and a float16 out) may be x or skip. Returns out."""
+    current, stream_of, f16, _, f32 = _kept or _torch_kept()
+    e4m3, u8, _, _ = _kept8 or _torch_kept8()
+    device = current()
+    shape = x.shape
+    rows, width = shape
+    x_at, x_pitch = _rows("x", x, (f16,), shape, device)
+    skip_at = skip_pitch = residual_at = residual_pitch = scales_at = 0
+    if skip is not None:
+        skip_at, skip_pitch = _rows("skip", skip, (f16,), shape, device)
+    if residual is not None:
+        residual_at, residual_pitch = _rows("residual", residual, (f16,), shape, device)
+    if scales is not None:
+        scales_at = _row_scales(scales, rows, width, f32, device)
+    out_at, out_pitch = _rows("out", out, (f16,) if scales is None else (e4m3, u8), shape, device)
+    rc = (_entries or _lib()).et_skip_rmsnorm(_rmsnorm_args(
+        out_at, x_at, skip_at, _array("gamma", gamma, f16, device, width), residual_at, scales_at, stream_of(device) if stream is None else stream.cuda_stream,
+        out_pitch, x_pitch, skip_pitch, residual_pitch, rows, width, eps))
+    if rc:
+        check(rc)
+    return out
+
+
+def quantise_rows(out, scales, x, stream=None):
+    """Rows of float16 x [rows, width] as e4m3 (or uint8) out with a scale for each 128 features of a row in scales float32 [ceil(width / 128), rows]. Returns (out, scales)."""
+    current, stream_of, f16, _, f32 = _kept or _torch_kept()
+    e4m3, u8, _, _ = _kept8 or _torch_kept8()
+    device = current()
+    shape = x.shape
+    rows, width = shape
+    x_at, x_pitch = _rows("x", x, (f16,), shape, device)
+    out_at, out_pitch = _rows("out", out, (e4m3, u8), shape, device)
+    rc = (_entries or _lib()).et_quantise_rows(_quantise_args(
+        out_at, _row_scales(scales, rows, width, f32, device), x_at, stream_of(device) if stream is None else stream.cuda_stream, out_pitch, x_pitch, rows, width))
+    if rc:
+        check(rc)
+    return out, scales
+
+
+class Fp8Weight:
+    """Linear with operands in e4m3: codes uint8 [out_feat, in_feat] (the bytes of e4m3) and scales float32 [ceil(out_feat / 128), ceil(in_feat / 128)], host arrays."""
+
+    def __init__(self, in_feat, out_feat, codes, scales, bias=None, is_gelu=False):
+        self.in_feat, self.out_feat, self.is_gelu = in_feat, out_feat, is_gelu
+        self._h = ctypes.c_void_p(0)
+        codes, scales = np.ascontiguousarray(codes), np.ascontiguousarray(scales, dtype=np.float32)
+        bias = None if bias is None else np.ascontiguousarray(bias, dtype=np.float16)
+        blocks = ((out_feat + 127) // 128, (in_feat + 127) // 128)
+        if codes.dtype != np.uint8 or codes.shape != (out_feat, in_feat) or scales.shape != blocks or (bias is not None and bias.shape != (out_feat,)):
+            raise ValueError(f"codes uint8 {(out_feat, in_feat)}, scales {blocks} and bias {(out_feat,)} expected, not {codes.dtype} {codes.shape}, {scales.shape}"
+                             + ("" if bias is None else f" and {bias.shape}"))
+        check(lib().et_fp8_weight_create(ctypes.byref(self._h), _i(in_feat), _i(out_feat), ptr(codes), ptr(scales), ptr(bias)))
+
+    def run(self, out, x, x_scales, gelu=None, stream=None):
+        """out [tokens, out_feat] float16 = x . W^T + bias (then tanh-GELU), x [tokens, in_feat] e4m3 (or uint8) with x_scales float32 [ceil(in_feat / 128), tokens]; rows
+        may be slices of wider ones."""
+        current, stream_of, f16, _, f32 = _kept or _torch_kept()
+        e4m3, u8, _, _ = _kept8 or _torch_kept8()
+        device = current()
+        tokens = x.shape[0]
+        x_at, x_pitch = _rows("x", x, (e4m3, u8), (tokens, self.in_feat), device)
+        out_at, out_pitch = _rows("out", out, (f16,), (tokens, self.out_feat), device)
+        rc = (_entries or _lib()).et_fp8_linear(_fp8_args(
+            self._h.value or 0, out_at, x_at, _row_scales(x_scales, tokens, self.in_feat, f32, device), stream_of(device) if stream is None else stream.cuda_stream,
+            out_pitch, x_pitch, tokens, 1 if (self.is_gelu if gelu is None else gelu) else 0))
+        if rc:
+            check(rc)
+        return out
+
+    def check(self):
+        """Raises EtError (ET_ERR_DEVICE_TIMEOUT) if a device-side wait of one of the weight's launches gave up."""
+        code = _i(0)
+        check(lib().et_fp8_weight_check(self._h, ctypes.byref(code)))
+
+    def close(self):
+        if self._h:
+            lib().et_fp8_weight_destroy(self._h)
+            self._h = ctypes.c_void_p(0)
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def _cache(codes, scales, i8, f32, device):
+    """(pages, heads, rows of a page, head_dim) of a cache."""
+    shape = codes.shape
+    if (codes.dtype is not i8 or scales.dtype is not f32 or codes.get_device() != device or scales.get_device() != device or len(shape) != 5 or shape[1] != 2
+            or scales.shape != shape[:4] or not codes.is_contiguous() or not scales.is_contiguous()):
+        raise ValueError(f"contiguous int8 codes [pages, 2, heads, page, head_dim] and float32 scales [pages, 2, heads, page] on the current CUDA device ({device}) expected, "
+                         f"not {codes.dtype} {tuple(codes.shape)} on {codes.device} and {scales.dtype} {tuple(scales.shape)} on {scales.device}")
+    return shape[0], shape[2], shape[3], shape[4]
+
+
+def _cache_call(entry, codes, scales, k, v, slots, stream):
+    current, stream_of, f16, i32, f32 = _kept or _torch_kept()
+    _, _, i8, _ = _kept8 or _torch_kept8()
+    device = current()
+    pages, heads, page, head_dim = _cache(codes, scales, i8, f32, device)
+    shape = (k.shape[0], heads * head_dim)
+    k_at, k_pitch = _rows("k", k, (f16,), shape, device)
+    v_at, v_pitch = _rows("v", v, (f16,), shape, device)
+    rc = entry(_cache_args(codes.data_ptr(), scales.data_ptr(), k_at, v_at, _array("slots", slots, i32, device, shape[0]),
+                           stream_of(device) if stream is None else stream.cuda_stream, k_pitch, v_pitch, shape[0], pages, heads, page, head_dim))
+    if rc:
+        check(rc)
+
+
+def kv_cache_write(codes, scales, k, v, slots, stream=None):
+    """Quantises rows of k and v [tokens, heads * head_dim] float16 into a cache: codes int8 [pages, 2, heads, page, head_dim], scales float32 [pages, 2, heads, page]. Row t
+    goes to slots[t] (int32: page number * page + row; below 0: nowhere); slots differ. Returns (codes, scales)."""
+    _cache_call((_entries or _lib()).et_kv_cache_write, codes, scales, k, v, slots, stream)
+    return codes, scales
+
+
+def kv_cache_read(k, v, codes, scales, slots, stream=None):
+    """Rows of a cache as float16: k and v [tokens, heads * head_dim], row t from slots[t] (below 0: left as it is). Returns (k, v)."""
+    _cache_call((_entries or _lib()).et_kv_cache_read, codes, scales, k, v, slots, stream)
+    return k, v
+
+
+def attention_tree(out, q, codes, scales, table, k_lens, tree=None, cu_seqlens=None, max_q_len=0, max_k_len=0, scale=0.0, stream=None):
+    """Attention of drafted tokens q [tokens, heads * head_dim] float16 over a cache (as kv_cache_write leaves it): table int32 [batch, pages of the longest], k_lens int32 [batch]
+    keys, the drafted tokens' own the last of them. A token sees the keys before those and the drafted ones whose bit is set in tree int64 [tokens] (None: those up to
+    itself). cu_seqlens int32 [batch + 1], or None: max_q_len tokens each. max_q_len (0: 1 without cu_seqlens, 64 with it) and max_k_len (0: all that the table has)."""
+    current, stream_of, f16, i32, f32 = _kept or _torch_kept()
+    _, _, i8, i64 = _kept8 or _torch_kept8()
+    device = current()
+    pages, heads, page, head_dim = _cache(codes, scales, i8, f32, device)
+    shape = q.shape
+    tokens, width = shape
+    if not head_dim or not heads or width % head_dim:
+        raise ValueError(f"q: whole heads of {head_dim} expected, not rows of {width}")
+    q_at, q_pitch = _rows("q", q, (f16,), shape, device)
+    out_at, out_pitch = _rows("out", out, (f16,), shape, device)
+    batch, most = _matrix("table", table, i32, device)
+    rc = (_entries or _lib()).et_attention_tree(_tree_args(
+        out_at, q_at, codes.data_ptr(), scales.data_ptr(), table.data_ptr(), _array("k_lens", k_lens, i32, device, batch),
+        0 if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), 0 if tree is None else _array("tree", tree, i64, device, tokens),
+        stream_of(device) if stream is None else stream.cuda_stream, out_pitch, q_pitch, width // head_dim, heads, head_dim, batch, tokens,
+        max_q_len or (1 if cu_seqlens is None else 64), max_k_len or most * page, pages, page, most, scale))
     if rc:
         check(rc)
     return out

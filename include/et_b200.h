@@ -244,6 +244,69 @@ typedef struct et_attention_rules_args {
 } et_attention_rules_args;
 int et_attention_rules_by(const et_attention_rules_args* args);
 
+/* ---- rows in 8 bits (no counterpart in the reference, which knows fp16 alone) ----
+ * Root-mean-square norm with the residual's addition: h = x + skip, out = h / sqrt(mean(h^2) + eps) * gamma. x, skip (NULL: nothing is added), gamma [width] and
+ * residual (NULL, or receives h) are fp16, the arithmetic fp32. scales NULL: out is fp16. scales [ceil(width / 128)][rows] fp32: out is e4m3 (one byte), a scale for
+ * each 128 features of a row, the largest size among them / 448; out times scale stands for the value. Rows may be slices of wider ones
+ * (pitches in elements). residual and an fp16 out may lie where x or skip lies, with the same pitch; any other overlap is the caller's error. width 1 to 32768, eps above 0 and at
+ * most 1. Fast are widths of a multiple of 8 up to 16384 in rows that start on 16 bytes (codes: on 8). Values that are not finite make codes or scales that are not numbers. */
+typedef struct et_skip_rmsnorm_args {
+    void* out; const void* x; const void* skip; const void* gamma; void* residual; float* scales; void* stream;
+    int out_pitch, x_pitch, skip_pitch, residual_pitch, rows, width;
+    float eps;
+} et_skip_rmsnorm_args;
+int et_skip_rmsnorm(const et_skip_rmsnorm_args* args);
+/* The same without the norm: rows of fp16 brought to e4m3 with scales, the input of a linear that no norm precedes. */
+typedef struct et_quantise_rows_args {
+    void* out; float* scales; const void* x; void* stream;
+    int out_pitch, x_pitch, rows, width;
+} et_quantise_rows_args;
+int et_quantise_rows(const et_quantise_rows_args* args);
+
+/* ---- linear with operands in e4m3 (no counterpart in the reference) ----
+ * Y[tokens x out_feat] = X . W^T + bias, tanh-GELU when gelu != 0, in fp16, of values that are code times scale: X [tokens x in_feat] e4m3 with x_scales
+ * [ceil(in_feat / 128)][tokens] (et_skip_rmsnorm, et_quantise_rows), W [out_feat x in_feat] e4m3 with scales [ceil(out_feat / 128)][ceil(in_feat / 128)], one for each 128 x 128 block. A weight is
+ * made from HOST arrays, which are copied (bias fp16 or NULL), on the current device; synchronises it. in_feat and out_feat are multiples of 16. Products and sums in
+ * fp32. Rows start on 16 bytes (pitch of X a multiple of 16, of Y of 8). Y overlaps X in nothing. */
+typedef struct et_fp8_weight et_fp8_weight;
+int et_fp8_weight_create(et_fp8_weight** out, int in_feat, int out_feat, const void* codes_host, const float* scales_host, const void* bias_host);
+int et_fp8_weight_destroy(et_fp8_weight* w);
+typedef struct et_fp8_linear_args {
+    const et_fp8_weight* weight; void* y; const void* x; const float* x_scales; void* stream;
+    int y_pitch, x_pitch, tokens, gelu;
+} et_fp8_linear_args;
+int et_fp8_linear(const et_fp8_linear_args* args);
+/* Reads and clears the weight's device error word, as et_tile_weight_check. */
+int et_fp8_weight_check(const et_fp8_weight* w, int* code);
+
+/* ---- a cache of keys and values in int8 pages (no counterpart in the reference, which keeps nothing between calls) ----
+ * codes [pages][2][heads][page][head_dim] int8 (K, then V) and scales [pages][2][heads][page] fp32, for each row of a head the largest size / 127: code times scale is the value.
+ * A slot is page number x page + row. et_kv_cache_write: rows t of K and V [tokens x heads * head_dim] fp16 go to slots[t], code = value / scale to the
+ * nearest (ties to even). et_kv_cache_read: rows of the cache come back to K and V. A slot that there is not (below 0: padding) is passed over: nothing is written, and rows of
+ * K and V that are read to stay as they are. Slots of one write differ: of two rows for one place any mixture may stay. head_dim a multiple of 16 up to 256, page a multiple of 16, codes start on
+ * 16 bytes; rows of K and V may be slices of wider ones, fast where they start on 16 bytes. A row with a value that is not finite becomes a row that is not a number. */
+typedef struct et_kv_cache_args {
+    void* codes; float* scales; void* k; void* v; const int* slots; void* stream;
+    int k_pitch, v_pitch, tokens, pages, heads, page, head_dim;
+} et_kv_cache_args;
+int et_kv_cache_write(const et_kv_cache_args* args);
+int et_kv_cache_read(const et_kv_cache_args* args);
+
+/* ---- attention of drafted tokens over that cache (no counterpart in the reference) ----
+ *   out_q = sum of softmax(scale q . k) v over the keys that q sees, of values that are code times scale
+ * q and out [q_tokens x nhead * head_dim] fp16, nhead a multiple of nhead_kv (query head h reads K/V head h / (nhead / nhead_kv)). Sequence b has the drafted tokens of rows
+ * cu_seqlens[b] .. cu_seqlens[b + 1] (device, batch + 1 ints; NULL: max_q_len each), at most max_q_len of them, at most 64. Its keys are k_lens[b] rows of the pages
+ * table[b][0], table[b][1], .. (device, [batch][table_width]), those of the n drafted tokens themselves (written before the call) the last n. A token sees all keys before those, and of them the ones whose
+ * bit is set in tree[row] (device, q_tokens 64-bit words: bit j is the sequence's j-th drafted token; its own bit counts like any other), or, with tree NULL, those up to itself: single tokens, and chains. A token that sees no key
+ * gets zeros. Keys beyond max_k_len, the table, or in a page that there is not, are not seen. Rows of out in no sequence are left as they are. scale 0: 1 / sqrt(head_dim).
+ * Scores and sums are fp32, the weights times the values' scales fp16. Rows of q and out start on 16 bytes; out overlaps q in nothing. */
+typedef struct et_attention_tree_args {
+    void* out; const void* q; const void* codes; const float* scales; const int* table; const int* k_lens; const int* cu_seqlens; const int64_t* tree; void* stream;
+    int out_pitch, q_pitch, nhead, nhead_kv, head_dim, batch, q_tokens, max_q_len, max_k_len, pages, page, table_width;
+    float scale;
+} et_attention_tree_args;
+int et_attention_tree(const et_attention_tree_args* args);
+
 /* ---- pruned-format generators (host) ----------------------------------------------------------
  * Seeded and reproducible. bernoulli == 0 keeps exactly floor(total*(1-sparsity)) tiles (a block-row's
  * tiles in draw order); otherwise each tile is kept with probability 1-sparsity (ascending offsets).

@@ -4,8 +4,10 @@
 // 128-byte-swizzled shared memory, four UMMAs of 32 k) into a place of tensor memory of its own, and the epilogue's warps add it, times its scale, to sums in
 // registers while the next block is multiplied into another place. Two kernels:
 //
-// fp8_pair_kernel, many tokens: persistent pairs of CTAs (cta_group::2), 256 tokens x kBN features to a tile, two places. A thread has a token's row of kBN / 2 columns, all of
-// one block of 128 features: one scale a block and thread. A block of 256 x 256 takes the tensor pipe 512 clocks; the two epilogue warps of a scheduler 256 of additions beside the loads.
+// fp8_pair_kernel, many tokens: persistent pairs of CTAs (cta_group::2), 256 tokens x kBN features to a tile. A thread has a token's row of kBN / 2 columns. 16384 x 4096 -> 4096:
+// 248 us (2.2e15 operations a second), with GELU 257. Of the ~900 clocks a block of 256 x 256 takes (UMMAs: 512) copies alone would take ~800 (the way from L2), sums and hand-overs
+// alone ~850. Tried, with and without the others' work: one warp that issues all UMMAs 244 / 253 us, four of them 248 / 256, sixteen warps that sum 255 / 266, eight with one
+// load from tensor memory at a time 260 / 275.
 //
 // fp8_few_kernel, few tokens: operands exchanged, 128 features are the tile's rows and kTokens tokens its columns, so that the weight, which is what has to
 // be read, fills the tile; K split over a cluster. Each CTA sends the others their columns' parts (asynchronous stores that count towards a barrier of the receiver) and
@@ -20,6 +22,7 @@
 #include "common.h"
 #include "ptx.cuh"
 #include "tmap.h"
+#include "vec_math.cuh"
 
 namespace et {
 namespace {
@@ -39,7 +42,9 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t at, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Arrives at a barrier of another CTA of the cluster. Relaxed: what was read from tensor memory is in registers by then, and nothing in shared or global memory
+// is handed over. (A release waits for the thread's loads of the next scales: a block of 128 k took 2120 clocks instead of 600.)
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // A copy into this CTA's shared memory that reports to a barrier of either CTA of the pair (cluster address).
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, int x, int y, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(tmap), "r"(x), "r"(y), "r"(bar)
@@ -75,10 +80,7 @@ __device__ __forceinline__ float gelu_f32(float x) {
     return fmaf(h, t, h);
 }
 template <bool kGelu>
-__device__ __forceinline__ float finish(float v, float bias) {
-    v += bias;
-    return kGelu ? gelu_f32(v) : v;
-}
+__device__ __forceinline__ float finish(float v) { return kGelu ? gelu_f32(v) : v; }
 
 struct Fp8Params {
     half* Y;
@@ -90,43 +92,60 @@ struct Fp8Params {
 };
 
 // ------------------------------------------------------------------------------------------ many tokens
-constexpr int kCopyWarps = 3, kEpiWarps = 8;
-constexpr int kMmaWarp = kCopyWarps, kFirstEpi = kCopyWarps + 1;
+// Warps: 0 copies X, 1 copies W, 2 and 3 issue UMMAs, 4 to 11 sum.
+constexpr int kXCopy = 0, kFirstMma = 2, kFirstEpi = 4, kEpiWarps = 8;
+// Registers of a thread: launched with 168, the roles' warpgroup gives some to the sums' two. (With 168 for all the scales on their way were spilled, that is waited for.)
+constexpr int kRoleRegs = 40, kSumRegs = 232;
+static_assert(kRoleRegs + 2 * kSumRegs <= 3 * 168, "the block's registers at launch");
 constexpr int kPairThreads = 32 * (kFirstEpi + kEpiWarps);
 constexpr int kXPanel = 128 * kBlock;             // of a CTA's tokens
 constexpr int kUnitCols = 32, kUnitBytes = 32 * kUnitCols * 2;
-constexpr int kMaxStages = 9;
+constexpr int kMaxStages = 8;
+
+template <int kBN>
+struct PairCfg {
+    static constexpr int kWPanel = kBN / 2 * kBlock, kStage = kXPanel + kWPanel;
+    static constexpr int kCols = kBN / 2;                        // of a thread
+    // Tensor memory: tiles of 256 take all of it with two places, each in two halves that are multiplied, added and freed by themselves: a half's round (256 clocks of
+    // UMMAs, some 500 of hand-overs, the additions) fits into the 1024 clocks that it may take. Tiles of 128 have four places.
+    static constexpr int kHalves = kBN == 256 ? 2 : 1;
+    static constexpr int kSlots = 512 / kBN * kHalves, kSlotCols = kBN / kHalves;
+    static_assert(kSlots == 4, "two to each warp that issues");
+    static constexpr int kOut = kEpiWarps * (kCols / kUnitCols) * kUnitBytes;   // a tile's results, on their way out while the next tile is summed
+    static constexpr int kStages = kBN == 256 ? 5 : 8;
+    static_assert(kHalves == 2 || kStages % 2 == 0, "a stage always falls to the same warp that issues");   // (a parity wait needs a waiter that has seen the phase before)
+    static constexpr int kBytes = kStages * kStage + kOut + 1024;
+};
 
 struct PairShared {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2];
+    uint64_t acc_full[4], acc_empty[4];
     uint32_t tmem_base;
 };
 
 template <int kBN, bool kGelu>
 __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
                                                                    const __grid_constant__ Fp8Params p) {
-    constexpr int kWPanel = kBN / 2 * kBlock, kStage = kXPanel + kWPanel;
-    constexpr int kCols = kBN / 2;                // of a thread
+    using C = PairCfg<kBN>;
+    constexpr int S = C::kStages, kStage = C::kStage, kCols = C::kCols;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ PairShared shared;
     PairShared* const sh = &shared;
-    const int S = p.stages;
     const uint32_t ring = smem_u32(smem), epi = ring + S * kStage;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_rank();
     const int pair = (int)blockIdx.x >> 1, G = (int)gridDim.x >> 1;
     const int my_tiles = (p.tiles - pair + G - 1) / G;
     if (tid == 0) {
-        for (int i = 0; i < S; ++i) { mbar_init(&sh->full[i], 1); mbar_init(&sh->empty[i], 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(&sh->acc_full[i], 1); mbar_init(&sh->acc_empty[i], 2 * kEpiWarps); }
+        for (int i = 0; i < S; ++i) { mbar_init(&sh->full[i], 1); mbar_init(&sh->empty[i], C::kHalves); }
+        for (int i = 0; i < C::kSlots; ++i) { mbar_init(&sh->acc_full[i], 1); mbar_init(&sh->acc_empty[i], 2 * kEpiWarps / C::kHalves); }
         fence_mbar_init();
         prefetch_tmap(&tmX);
         prefetch_tmap(&tmW);
     }
-    if (warp == kMmaWarp) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh->tmem_base)), "r"(2 * kBN) : "memory");
+    if (warp == kFirstMma) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sh->tmem_base)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -135,133 +154,169 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
     tc_fence_after();
     const uint32_t tmem = sh->tmem_base;
     const int total = my_tiles * p.k_blocks;
-    if (warp < kCopyWarps) {
-        // ---- copies: the warps take the stages in turn (their number divides that of the stages, so that a stage always falls to the same warp)
-        auto load_w = [&](int s, int kb, int tile) {
-            const uint32_t bar = in_cta(smem_u32(&sh->full[s]), 0);
-            if (rank == 0) mbar_expect_tx(&sh->full[s], 2 * kStage);
-            tma_load_2d_pair(ring + s * kStage + kXPanel, &tmW, kb * kBlock, (tile % p.tiles_n) * kBN + (int)rank * (kBN / 2), bar);
-        };
-        auto load_x = [&](int s, int kb, int tile) {
-            tma_load_2d_pair(ring + s * kStage, &tmX, kb * kBlock, (tile / p.tiles_n) * 256 + (int)rank * 128, in_cta(smem_u32(&sh->full[s]), 0));
-        };
-        const int ahead = min(S, p.k_blocks);
-        if (lane == 0)
-            for (int i = warp; i < ahead; i += kCopyWarps) load_w(i, i, pair);
-        __syncwarp();
-        pdl_wait();
-        bool ok = true;
-        int s = warp, kb = warp, tile = pair;
-        uint32_t ph = 1;
-        for (int c = warp; c < total; c += kCopyWarps) {
-            while (kb >= p.k_blocks) { kb -= p.k_blocks; tile += G; }
-            if (s >= S) { s -= S; ph ^= 1u; }
-            if (c >= S) ok = mbar_wait(&sh->empty[s], ph);
-            if (!ok) break;
+    if (warp < kFirstEpi) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRoleRegs));
+        if (warp < kFirstMma) {
+            // ---- copies; both CTAs' report to the first one's barriers
+            const bool is_x = warp == kXCopy;
+            if (is_x) pdl_wait();
             if (lane == 0) {
-                if (c >= ahead) load_w(s, kb, tile);
-                load_x(s, kb, tile);
+                bool ok = true;
+                int s = 0, kb = 0, tile = pair;
+                uint32_t ph = 1;
+                for (int c = 0; c < total; ++c) {
+                    ok = mbar_wait_at(smem_u32(&sh->empty[s]), ph);
+                    if (!ok) break;
+                    const uint32_t bar = in_cta(smem_u32(&sh->full[s]), 0);
+                    if (is_x) {
+                        tma_load_2d_pair(ring + s * kStage, &tmX, kb * kBlock, (tile / p.tiles_n) * 256 + (int)rank * 128, bar);
+                    } else {
+                        if (rank == 0) mbar_expect_tx(&sh->full[s], 2 * kStage);
+                        tma_load_2d_pair(ring + s * kStage + kXPanel, &tmW, kb * kBlock, (tile % p.tiles_n) * kBN + (int)rank * (kBN / 2), bar);
+                    }
+                    if (++kb == p.k_blocks) { kb = 0; tile += G; }
+                    if (++s == S) { s = 0; ph ^= 1u; }
+                }
+                // (On the normal way out every copy has been consumed. A wait that gives up has lasted far longer than any copy.)
+                if (!ok) atomicExch(p.err, 61);
             }
             __syncwarp();
-            kb += kCopyWarps;
-            s += kCopyWarps;
-        }
-        // (On the normal way out every copy has been consumed. A wait that gives up has lasted far longer than any copy.)
-        if (!ok && lane == 0) atomicExch(p.err, 61);
-    } else if (warp == kMmaWarp) {
-        if (rank == 0 && elect_one()) {
-            constexpr uint32_t idesc = make_idesc_e4m3(256, kBN);
-            const uint64_t x0 = make_smem_desc(ring, 16, 1024, 2), w0 = make_smem_desc(ring + kXPanel, 16, 1024, 2);
-            bool ok = true;
-            int s = 0;
-            uint32_t ph = 0;
-            for (int c = 0; c < total; ++c) {
-                const int buf = c & 1;
-                ok = mbar_wait(&sh->acc_empty[buf], ((uint32_t)(c >> 1) & 1u) ^ 1u) && mbar_wait(&sh->full[s], ph);
-                if (!ok) break;
-                tc_fence_after();
-                const uint64_t at = (uint64_t)(s * kStage) >> 4;   // descriptors count 16-byte units
+        } else if (rank == 0) {
+            // ---- UMMAs of the pair, by two warps: either has a half of each block, or (tiles of 128) every other block
+            if (elect_one()) {
+                constexpr uint32_t idesc = make_idesc_e4m3(256, C::kSlotCols);
+                constexpr int kStep = 3 - C::kHalves;
+                const int m = warp - kFirstMma;
+                // (half h: rows h * 64 .. of the weight's panel in either CTA, columns of the first CTA's and then of the second's)
+                const uint64_t x0 = make_smem_desc(ring, 16, 1024, 2), w0 = make_smem_desc(ring + kXPanel + (C::kHalves == 2 ? m * (kBN / 4 * kBlock) : 0), 16, 1024, 2);
+                const uint32_t full = smem_u32(&sh->full[0]), empty = smem_u32(&sh->empty[0]), acc_full = smem_u32(&sh->acc_full[0]), acc_empty = smem_u32(&sh->acc_empty[0]);
+                bool ok = true;
+                int s = C::kHalves == 2 ? 0 : m, slot = m;
+                uint32_t ph = 0, slot_ph = 1;
+                for (int c = s; c < total; c += kStep) {
+                    ok = mbar_wait_at(acc_empty + slot * 8, slot_ph) && mbar_wait_at(full + s * 8, ph);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t at = (uint64_t)(s * kStage) >> 4;   // descriptors count 16-byte units
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) umma_f8_pair(tmem + buf * kBN, x0 + at + ks * 2, w0 + at + ks * 2, idesc, ks > 0);
-                umma_commit_pair(smem_u32(&sh->empty[s]));
-                umma_commit_pair(smem_u32(&sh->acc_full[buf]));
-                if (++s == S) { s = 0; ph ^= 1u; }
+                    for (int ks = 0; ks < 4; ++ks) umma_f8_pair(tmem + slot * C::kSlotCols, x0 + at + ks * 2, w0 + at + ks * 2, idesc, ks > 0);
+                    umma_commit_pair(acc_full + slot * 8);
+                    umma_commit_pair(empty + s * 8);
+                    slot += 2;
+                    if (slot >= 4) { slot -= 4; slot_ph ^= 1u; }
+                    s += kStep;
+                    if (s >= S) { s -= S; ph ^= 1u; }
+                }
+                if (!ok) atomicExch(p.err, 62);
             }
-            if (!ok) atomicExch(p.err, 62);
+            __syncwarp();
         }
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegs));
         // ---- sums of this CTA's 128 tokens: a row to a thread, two warps share its columns
         const int w = warp - kFirstEpi, q = warp & 3, h = w >> 2;
-        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + h * kCols;
-        const uint32_t buf_at = epi + w * kUnitBytes;
+        const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (C::kHalves == 2 ? 0 : h * kCols);
+        const uint32_t buf_at = epi + w * (kCols / kUnitCols) * kUnitBytes;
         const uint32_t to = buf_at + lane * 64, swizzle = (lane >> 1) & 3;   // row `lane`: four 16-byte chunks under the 64-byte swizzle
         const uint32_t empty_bar = in_cta(smem_u32(&sh->acc_empty[0]), 0);
         const int n_blocks = (p.N + kBlock - 1) / kBlock;
         bool ok = true;
         pdl_wait();
-        int c = 0;
+        auto row_scales = [&](int tile) { return p.x_scales + min((tile / p.tiles_n) * 256 + (int)rank * 128 + q * 32 + lane, p.T - 1); };
+        // The token's scales are requested two blocks ahead: of even blocks, of odd ones.
+        float even = __ldcg(row_scales(pair)), odd = p.k_blocks > 1 ? __ldcg(row_scales(pair) + p.T) : 0.f;
+        int slot = C::kHalves == 2 ? h : 0;
+        uint32_t slot_ph = 0;
         for (int tl = 0; tl < my_tiles && ok; ++tl) {
             const int tile = pair + tl * G;
-            const int m0 = (tile / p.tiles_n) * 256 + (int)rank * 128 + q * 32, n0 = (tile % p.tiles_n) * kBN + h * kCols;
-            const float* sx = p.x_scales + min(m0 + lane, p.T - 1);
-            const float* sw = p.w_scales + (long long)min(n0 / kBlock, n_blocks - 1) * p.k_blocks;
-            float acc[kCols];
+            const int m0 = (tile / p.tiles_n) * 256 + (int)rank * 128 + q * 32, n0 = (tile % p.tiles_n) * kBN;
+            // Columns of the thread, 32 at a time: of half h of a tile of 256 the features h 64 .. and 128 + h 64 .. (64 each), else h 64 ...
+            auto column = [&](int u) { return n0 + h * 64 + (u < 2 ? u * kUnitCols : 128 + (u - 2) * kUnitCols); };
+            const float* const sx = row_scales(tile);
+            // the scales of the weight for the first and for the last 64 columns
+            const float* const sw0 = p.w_scales + (long long)(n0 / kBlock) * p.k_blocks;
+            const float* const sw1 = p.w_scales + (long long)min(n0 / kBlock + 1, n_blocks - 1) * p.k_blocks;
+            float next0 = __ldg(sw0), next1 = C::kHalves == 2 ? __ldg(sw1) : 0.f;
+            float acc[kCols];   // from the bias on (padded with zeros to a multiple of 256)
 #pragma unroll
-            for (int i = 0; i < kCols; ++i) acc[i] = 0.f;
-            float next_x = __ldcg(sx), next_w = __ldg(sw);
-            for (int kb = 0; kb < p.k_blocks; ++kb, ++c) {
-                const int buf = c & 1;
-                const float scale = next_x * next_w;
-                if (kb + 1 < p.k_blocks) {
-                    next_x = __ldcg(sx + (long long)(kb + 1) * p.T);
-                    next_w = __ldg(sw + kb + 1);
+            for (int i = 0; i < kCols; i += 8) {
+                const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + column(i / kUnitCols) + i % kUnitCols));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = __half22float2(reinterpret_cast<const half2*>(&bv)[j]);
+                    acc[i + 2 * j] = f.x;
+                    acc[i + 2 * j + 1] = f.y;
                 }
-                ok = mbar_wait(&sh->acc_full[buf], (uint32_t)(c >> 1) & 1u);
-                if (!ok) break;
+            }
+            auto add_block = [&](int kb, float& token) {
+                const float scale0 = token * next0, scale1 = token * next1;
+                if (kb + 2 < p.k_blocks) token = __ldcg(sx + (long long)(kb + 2) * p.T);
+                if (kb + 1 < p.k_blocks) {
+                    next0 = __ldg(sw0 + kb + 1);
+                    if (C::kHalves == 2) next1 = __ldg(sw1 + kb + 1);
+                }
+                if (!mbar_wait(&sh->acc_full[slot], slot_ph)) return false;
                 tc_fence_after();
+                // the next 16 columns are on their way while 16 are added
+                uint32_t d[2][16];
+                tmem_ld16(from + slot * C::kSlotCols, d[0]);
 #pragma unroll
                 for (int i = 0; i < kCols; i += 16) {
-                    uint32_t d[16];
-                    tmem_ld16(from + buf * kBN + i, d);
-                    tmem_ld_wait(d);
+                    tmem_ld_wait(d[(i >> 4) & 1]);
+                    if (i + 16 < kCols) {
+                        tmem_ld16(from + slot * C::kSlotCols + i + 16, d[(i >> 4 & 1) ^ 1]);
+                    } else {   // the slot may be overwritten
+                        tc_fence_before();
+                        __syncwarp();
+                        if (elect_one()) mbar_arrive_cluster(empty_bar + slot * 8);
+                    }
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[i + j] = fmaf(__uint_as_float(d[j]), scale, acc[i + j]);
+                    for (int j = 0; j < 16; j += 2) {
+                        const float f = C::kHalves == 2 && i >= 64 ? scale1 : scale0;
+                        const float2 r = fma2(make_float2(__uint_as_float(d[(i >> 4) & 1][j]), __uint_as_float(d[(i >> 4) & 1][j + 1])), make_float2(f, f), make_float2(acc[i + j], acc[i + j + 1]));
+                        acc[i + j] = r.x;
+                        acc[i + j + 1] = r.y;
+                    }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (elect_one()) mbar_arrive_cluster(empty_bar + buf * 8);
-                __syncwarp();
+                slot += C::kHalves;
+                if (slot >= C::kSlots) {
+                    slot -= C::kSlots;
+                    slot_ph ^= 1u;
+                }
+                return true;
+            };
+            for (int kb = 0; kb < p.k_blocks && ok; kb += 2) {
+                ok = add_block(kb, even);
+                if (ok && kb + 1 < p.k_blocks) ok = add_block(kb + 1, odd);
+            }
+            if (tl + 1 < my_tiles) {
+                even = __ldcg(row_scales(tile + G));
+                if (p.k_blocks > 1) odd = __ldcg(row_scales(tile + G) + p.T);
             }
             if (!ok) break;
             if (tl + 1 == my_tiles) pdl_launch_dependents();
+            tma_store_wait_read();   // the stores of the tile before have read the buffers
+            __syncwarp();
 #pragma unroll
             for (int u = 0; u < kCols / kUnitCols; ++u) {
-                const int col = n0 + u * kUnitCols;
-                uint4 ov[4];
-                half2* const o = reinterpret_cast<half2*>(ov);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint4 bv = __ldg(reinterpret_cast<const uint4*>(p.bias + col) + j);
-                    const half2* const b = reinterpret_cast<const half2*>(&bv);
+                    uint4 ov;
+                    half2* const o = reinterpret_cast<half2*>(&ov);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = __half22float2(b[i]);
-                        o[j * 4 + i] = __floats2half2_rn(finish<kGelu>(acc[u * kUnitCols + j * 8 + 2 * i], f.x), finish<kGelu>(acc[u * kUnitCols + j * 8 + 2 * i + 1], f.y));
-                    }
+                    for (int i = 0; i < 4; ++i) o[i] = __floats2half2_rn(finish<kGelu>(acc[u * kUnitCols + j * 8 + 2 * i]), finish<kGelu>(acc[u * kUnitCols + j * 8 + 2 * i + 1]));
+                    sts128(to + u * kUnitBytes + ((j ^ swizzle) << 4), ov);
                 }
-                tma_store_wait_read();   // the buffer's previous store has read it
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sts128(to + ((j ^ swizzle) << 4), ov[j]);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (col < p.N && m0 < p.T && elect_one()) {
-                    tma_store_2d(&tmY, smem + (buf_at - ring), col, m0);
-                    tma_store_commit();
-                }
-                __syncwarp();
             }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (m0 < p.T && elect_one()) {
+#pragma unroll
+                for (int u = 0; u < kCols / kUnitCols; ++u)
+                    if (column(u) < p.N) tma_store_2d(&tmY, smem + (buf_at - ring) + u * kUnitBytes, column(u), m0);
+                tma_store_commit();
+            }
+            __syncwarp();
         }
         if (!ok && lane == 0) atomicExch(p.err, 63);
         tma_store_wait_read();
@@ -271,7 +326,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
     __syncthreads();
     cluster_sync();   // nobody still reads this CTA's shared memory or signals its barriers
     tc_fence_after();
-    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kBN) : "memory");
+    if (warp == kFirstMma) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------ few tokens
@@ -475,7 +530,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
             if (n < p.N) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (t0 + col + j < p.T) p.Y[(long long)(t0 + col + j) * p.y_pitch + n] = __float2half_rn(finish<kGelu>(v[j], bias));
+                    if (t0 + col + j < p.T) p.Y[(long long)(t0 + col + j) * p.y_pitch + n] = __float2half_rn(finish<kGelu>(v[j] + bias));
             }
         }
     }
@@ -538,18 +593,16 @@ Fp8Plan fp8_plan(int T, int N, int k_blocks) {
 
 template <int kBN, bool kGelu>
 cudaError_t launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& ty, Fp8Params p, cudaStream_t st) {
-    constexpr int kStage = kXPanel + kBN / 2 * kBlock;
     const auto kernel = fp8_pair_kernel<kBN, kGelu>;
     static PerDeviceOnce once;
-    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax - 1024); });
+    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<kBN>::kBytes); });
     if (e != cudaSuccess) return e;
     p.tiles_n = (p.N + kBN - 1) / kBN;
     p.tiles = (p.T + 255) / 256 * p.tiles_n;
-    p.stages = std::min(kMaxStages, (kSmemMax - 2048 - kEpiWarps * kUnitBytes) / kStage) / kCopyWarps * kCopyWarps;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(2 * std::min(p.tiles, sm_count() / 2)));
     cfg.blockDim = dim3(kPairThreads);
-    cfg.dynamicSmemBytes = (size_t)p.stages * kStage + kEpiWarps * kUnitBytes + 1024;
+    cfg.dynamicSmemBytes = PairCfg<kBN>::kBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -8,7 +8,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libet_b200.so")
 SOURCES = ["error.cu", "layernorm.cu", "softmax.cu", "tile_gemm.cu", "attention.cu", "attention_tc.cu", "dense_gemm.cu", "resident_gemm.cu", "formats.cu",
            "encoder.cu", "api.cu", "rotary.cu", "adapter.cu", "adapter_tc.cu", "attention_rules.cu", "attention_rules_tc.cu", "attention_rules_token.cu",
-           "rmsnorm.cu", "fp8_gemm.cu", "kv_cache.cu", "attention_tree.cu"]
+           "rmsnorm.cu", "fp8_gemm.cu", "kv_cache.cu", "attention_tree.cu", "attention_tree_tc.cu"]
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
          "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall", "-shared"]
 

@@ -415,7 +415,7 @@ extern "C" int et_attention_tree(const et_attention_tree_args* a) {
     p.batch = a->batch; p.q_tokens = a->q_tokens; p.max_q_len = a->max_q_len; p.max_k_len = a->max_k_len;
     p.pages = a->pages; p.page = a->page; p.table_width = a->table_width;
     p.scale_log2 = (a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale) * 1.4426950408889634f;
-    return attention_tree_launch(p, static_cast<cudaStream_t>(a->stream));
+    return (attention_tree_tc_takes(p) ? attention_tree_tc_launch : attention_tree_launch)(p, static_cast<cudaStream_t>(a->stream));
 }
 
 namespace et {

@@ -1,0 +1,464 @@
+// Attention of drafted tokens over a cache of int8 codes, many rows: a CTA has up to 128 of the rows (queries x query heads) of a K/V head, so that both products go to tcgen05 and a
+// code is converted once for all of them.
+//
+// Blocks of 64 keys. Four warps fetch the codes (cp.async, each thread into a place that only it reads, a block or two ahead) and write them as halves where the tensor cores read them (rows of 64
+// features, 128-byte swizzle; V as it lies, features are its N). Q lies in tensor memory as the first product's A operand, the scores beside it, and the weights where the
+// scores were, as the second product's A operand. A thread has a row: scale of the key, mask, weight times the value's scale, a running reference that moves when
+// it has to (then O is rescaled in tensor memory). Two CTAs share an SM: while one waits for its products the other takes exponentials. A cluster shares a sequence's keys; its CTAs' rows are joined
+// through distributed shared memory in a fixed order.
+#include <cooperative_groups.h>
+#include "attention.h"
+#include "attention_tree.cuh"
+#include "attention_tree.h"
+#include "common.h"
+#include "ptx.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace et {
+namespace {
+
+constexpr int kKeys = 64;                 // of a block
+constexpr int kRows = 128;                // of a CTA
+constexpr int kSoftmaxWarps = 4, kConvertWarps = 4, kThreads = 8 * 32;   // (two CTAs to an SM with 128 registers a thread)
+constexpr int kMaxCluster = 8;
+constexpr int kScaleStages = 4;
+constexpr float kRescaleStep = 8.f;       // log2 units
+constexpr uint32_t kTmemCols = 256;
+
+template <int kHD>
+struct Cfg {
+    static constexpr int kPanel = kKeys * 128, kTile = kHD / 64 * kPanel;       // halves of a block of K or V
+    static constexpr int kChunks = kKeys * kHD / 16 / 128;                      // 16 codes each, of a thread, of K and of V
+    static constexpr int kRaw = 2 * kChunks * 2048 + 512;                       // a block's codes and scales as they come
+    static constexpr int kRawStages = kHD == 64 ? 4 : 2;
+    static constexpr uint32_t kQCol = 0, kSCol = kHD / 2, kOCol = kSCol + kKeys;
+    static_assert(kOCol + kHD <= kTmemCols, "");
+    static constexpr int kKAt = 0, kVAt = 2 * kTile, kRawAt = 4 * kTile;
+    static constexpr int kScaleAt = kRawAt + kRawStages * kRaw;                 // [stage][key: score factor, value's scale, its logarithm][64]
+    static constexpr int kPartAt = kScaleAt + kScaleStages * 3 * kKeys * 4;     // [reference, sum][128]
+    // Half of an SM's shared memory for half of its tensor memory: a CTA that finds one finds the other, and none waits for columns that another cluster holds.
+    static constexpr int kBytes = 113664;
+    static_assert(kPartAt + 2 * kRows * 4 + 1024 <= kBytes && kTmemCols == 256, "");
+    static_assert(kRows * kHD * 4 <= 4 * kTile, "O in 32 bits fits where the blocks were");
+};
+
+struct Shared {
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_ready, s_full, p_ready, o_done;
+    uint32_t good[kScaleStages];          // a bit for each 16 keys of a block: their page is there
+    uint32_t tmem_base;
+};
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t no_infinity(uint32_t two) {
+    const uint32_t lo = (two & 0x7fffu) == 0x7c00u ? 0x7fffu : two & 0xffffu, hi = (two & 0x7fff0000u) == 0x7c000000u ? 0x7fff0000u : two & 0xffff0000u;
+    return lo | hi;
+}
+template <int kSize>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int real) {
+    if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+    const uint4 v = lds128(a);
+    return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+}
+
+template <int kHD>
+__global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __grid_constant__ TreeParams p, int row_tiles, bool longest_first, int* err) {
+    using C = Cfg<kHD>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ Shared shared;
+    Shared* const sh = &shared;
+    const uint32_t at = smem_u32(smem);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int csize = cluster.num_blocks(), crank = cluster.block_rank();
+    int unit = blockIdx.x / csize;        // sequence, K/V head, tile of rows
+    const int tile = unit % row_tiles;
+    unit /= row_tiles;
+    const int n_kv = p.nhead / p.group, kv_head = unit % n_kv;
+    int b = unit / n_kv;
+    pdl_wait();
+    if (longest_first) {   // the b-th sequence in order of length: the one that has b longer (or as long and earlier) ones
+        __shared__ int lens[kThreads], found;
+        const int len = tid < p.batch ? p.k_lens[tid] : 0;
+        lens[tid] = len;
+        __syncthreads();
+        int before = 0;
+        for (int j = 0; j < p.batch; ++j) before += lens[j] > len || (lens[j] == len && j < tid) ? 1 : 0;
+        if (tid < p.batch && before == b) found = tid;
+        __syncthreads();
+        b = found;
+    }
+    const TreeSeq s = tree_seq(p, b);
+    const int rows = min(s.qlen * p.group - tile * kRows, kRows), hd = p.head_dim;
+    if (rows <= 0) return;                // the same for the whole cluster
+    const int n_blocks = (s.klen + kKeys - 1) / kKeys, mine = n_blocks > crank ? (n_blocks - crank + csize - 1) / csize : 0;   // blocks crank, crank + csize, ..
+    if (warp == kSoftmaxWarps) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh->k_full[i], kConvertWarps);
+                mbar_init(&sh->v_full[i], kConvertWarps);
+                mbar_init(&sh->k_empty[i], 1);
+                mbar_init(&sh->v_empty[i], 1);
+            }
+            mbar_init(&sh->q_ready, kSoftmaxWarps);
+            mbar_init(&sh->s_full, 1);
+            mbar_init(&sh->p_ready, kSoftmaxWarps);
+            mbar_init(&sh->o_done, 1);
+            fence_mbar_init();
+        }
+        __syncwarp();
+        tmem_alloc(&sh->tmem_base, kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem_base;
+    pdl_launch_dependents();
+    bool ok = true;
+    float top = -INFINITY, sum = 0.f;
+    if (warp >= kSoftmaxWarps) {
+        // ---- codes to halves
+        const int c = tid - kSoftmaxWarps * 32;                       // 0 to 127
+        constexpr int kPerKey = kHD / 16;                             // chunks of a key
+        const int key_c = c / kPerKey, f = (c % kPerKey) * 16;        // of the thread's first chunk; the others are 128 / kPerKey keys apart
+        const int key_s = c & 63, side_s = c >> 6;                    // whose scale it brings
+        const int* const table = p.table + (long long)b * p.table_width;
+        const uint32_t raw = at + C::kRawAt;
+        auto page_of = [&](int key) {                                 // page of a key, -1: none
+            if (key >= s.klen) return -1;
+            const int id = __ldg(table + key / p.page);
+            return id < p.pages ? id : -1;
+        };
+        auto row_of = [&](int key, int id, int side) { return (((long long)id * 2 + side) * n_kv + kv_head) * p.page + key % p.page; };
+        auto fetch = [&](int j) {
+            if (j < mine) {
+                const int key0 = (crank + j * csize) * kKeys;
+                const uint32_t to = raw + (j % C::kRawStages) * C::kRaw + c * 16;
+#pragma unroll
+                for (int n = 0; n < C::kChunks; ++n) {
+                    const int key = key0 + key_c + n * (128 / kPerKey), id = page_of(key & ~15);   // (16 keys of a block lie in one page)
+                    const bool good = id >= 0 && f < hd;
+                    const long long k_row = row_of(key, max(id, 0), 0), v_row = k_row + (long long)n_kv * p.page;
+                    copy_async<16>(to + n * 2048, good ? p.codes + k_row * hd + f : p.codes, good ? 16 : 0);
+                    copy_async<16>(to + (C::kChunks + n) * 2048, good ? p.codes + v_row * hd + f : p.codes, good ? 16 : 0);
+                }
+                const int key = key0 + key_s, id = page_of(key);
+                copy_async<4>(raw + (j % C::kRawStages) * C::kRaw + 2 * C::kChunks * 2048 + c * 4, id >= 0 ? p.scales + row_of(key, id, side_s) : p.scales, id >= 0 ? 4 : 0);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        // 16 codes of the thread as halves at 16 bytes 2 f / 16 and the next of the key's row. (Every second thread of eight that write at once takes the second 16 bytes first:
+        // rows of two panels lie on the same banks.)
+        auto convert = [&](uint32_t from, uint32_t tile_at, int key) {
+            const uint4 w = lds128(from);
+            const uint32_t u[4] = {codes_biased(w.x), codes_biased(w.y), codes_biased(w.z), codes_biased(w.w)};
+            uint4 h[2];
+            h[0] = make_uint4(codes_to_half2<0>(u[0]), codes_to_half2<1>(u[0]), codes_to_half2<0>(u[1]), codes_to_half2<1>(u[1]));
+            h[1] = make_uint4(codes_to_half2<0>(u[2]), codes_to_half2<1>(u[2]), codes_to_half2<0>(u[3]), codes_to_half2<1>(u[3]));
+            const uint32_t line = tile_at + (f >> 6) * C::kPanel + key * 128;
+            const int chunk = (f & 63) >> 3, swap = kHD == 128 ? f >> 6 : 0;
+            sts128(line + (((chunk + swap) ^ (key & 7)) << 4), swap ? h[1] : h[0]);
+            sts128(line + (((chunk + 1 - swap) ^ (key & 7)) << 4), swap ? h[0] : h[1]);
+        };
+        for (int n = 0; n < C::kRawStages - 1; ++n) fetch(n);
+        for (int j = 0; j < mine; ++j) {
+            fetch(j + C::kRawStages - 1);   // (the thread has read that place a turn ago)
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::kRawStages - 1) : "memory");
+            const int st = j & 1, key0 = (crank + j * csize) * kKeys;
+            const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u, from = raw + (j % C::kRawStages) * C::kRaw;
+            ok = mbar_wait(&sh->k_empty[st], ph);
+            if (!ok) break;
+#pragma unroll
+            for (int n = 0; n < C::kChunks; ++n) convert(from + (n * 128 + c) * 16, at + C::kKAt + st * C::kTile, key_c + n * (128 / kPerKey));
+            // Scales go to the places of block j - 4, whose scores are done with: those of block j - 2 have been multiplied, behind the weights of block j - 3.
+            const float scale = __uint_as_float(lds32(from + 2 * C::kChunks * 2048 + c * 4));
+            const bool real = key0 + key_s < s.klen;   // (behind the last key anything may lie)
+            float* const to = reinterpret_cast<float*>(smem + C::kScaleAt) + (j % kScaleStages) * 3 * kKeys + key_s;
+            if (side_s == 0) {
+                to[0] = real ? scale * p.scale_log2 : 0.f;
+            } else {
+                to[kKeys] = real ? scale : 0.f;
+                to[2 * kKeys] = log2_of_scale(real ? scale : 0.f);
+            }
+            if (c == 0) {
+                uint32_t good = 0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) good |= (page_of(key0 + n * 16) >= 0 ? 1u : 0u) << n;
+                sh->good[j % kScaleStages] = good;
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->k_full[st]);
+            ok = mbar_wait(&sh->v_empty[st], ph);
+            if (!ok) break;
+#pragma unroll
+            for (int n = 0; n < C::kChunks; ++n) convert(from + ((C::kChunks + n) * 128 + c) * 16, at + C::kVAt + st * C::kTile, key_c + n * (128 / kPerKey));
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->v_full[st]);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok && lane == 0) atomicExch(err, 26);
+    } else {
+        // ---- a row to a thread
+        const uint32_t mine_at = tmem + ((uint32_t)warp << 21);       // the warp's lanes of tensor memory
+        const bool real = tid < rows;
+        const int r = tile * kRows + (real ? tid : 0), i = r / p.group;
+        const unsigned long long bits = tree_bits(p, s, i);
+        if (mine > 0) {
+            const half* const q = p.q + (s.q0 + i) * p.q_pitch + (long long)(kv_head * p.group + r % p.group) * hd;
+#pragma unroll
+            for (int n = 0; n < kHD / 32; ++n) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int f = n * 32 + e * 8;
+                    const uint4 v = real && f < hd ? *reinterpret_cast<const uint4*>(q + f) : make_uint4(0u, 0u, 0u, 0u);
+                    w[4 * e] = no_infinity(v.x);
+                    w[4 * e + 1] = no_infinity(v.y);
+                    w[4 * e + 2] = no_infinity(v.z);
+                    w[4 * e + 3] = no_infinity(v.w);
+                }
+                tmem_store16(mine_at + C::kQCol + n * 16, w);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->q_ready);
+        }
+        // The first warp issues the UMMAs too: everybody waits for them anyway.
+        const uint32_t idesc_qk = make_idesc_f16(128, kKeys), idesc_pv = make_idesc_f16(128, hd, false, true);
+        const uint64_t k_desc = make_smem_desc(at + C::kKAt, 16, 1024, 2), v_desc = make_smem_desc(at + C::kVAt, C::kPanel, 1024, 2);
+        auto scores_of = [&](int j) {   // (where the weights of the block before lie, which are read by then: UMMAs of a thread run in order)
+            if (!mbar_wait(&sh->k_full[j & 1], (uint32_t)(j >> 1) & 1u)) return false;
+            tc_fence_after();
+            const uint64_t kd = k_desc + (j & 1) * (C::kTile >> 4);
+            for (int ks = 0; ks < hd / 16; ++ks) umma_f16_ts(tmem + C::kSCol, tmem + C::kQCol + ks * 8, kd + ((ks >> 2) * C::kPanel + (ks & 3) * 32) / 16, idesc_qk, ks > 0);
+            umma_commit(&sh->k_empty[j & 1]);
+            umma_commit(&sh->s_full);
+            return true;
+        };
+        if (warp == 0 && mine > 0) {
+            if (elect_one()) ok = mbar_wait(&sh->q_ready, 0) && scores_of(0);
+            __syncwarp();
+        }
+        for (int j = 0; j < mine; ++j) {
+            const int key0 = (crank + j * csize) * kKeys;
+            ok = mbar_wait(&sh->k_full[j & 1], (uint32_t)(j >> 1) & 1u) && mbar_wait(&sh->s_full, (uint32_t)j & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t raw[2][32];
+            tmem_ld32(mine_at + C::kSCol, raw[0]);
+            tmem_ld32(mine_at + C::kSCol + 32, raw[1]);
+            tmem_ld_wait(raw[0], raw[1]);
+            const uint32_t scales = at + C::kScaleAt + (j % kScaleStages) * 3 * kKeys * 4;
+            // what the row sees of the block
+            const uint32_t good = sh->good[j % kScaleStages];
+            const bool masked = key0 + kKeys > s.kept || key0 + kKeys > s.klen || good != 15u;
+            unsigned long long seen = ~0ull;
+            if (masked) {
+                const int d = key0 - s.kept;   // place of the first key among the drafted tokens
+                seen = d >= 64 ? 0ull : d >= 0 ? bits >> d : d > -64 ? (bits << -d) | ((1ull << -d) - 1ull) : ~0ull;
+                const int left = s.klen - key0;
+                if (left < 64) seen &= (1ull << left) - 1ull;
+                if (good != 15u)
+                    for (int n = 0; n < 4; ++n)
+                        if (!((good >> n) & 1u)) seen &= ~(0xffffull << (n * 16));
+            }
+            float most = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < kKeys; e += 4) {
+                const float4 ks = lds_f4(scales + e * 4), lv = lds_f4(scales + (2 * kKeys + e) * 4);
+                uint32_t* const x = &raw[e >> 5][e & 31];
+                const float2 a = fma2(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), make_float2(ks.x, ks.y), make_float2(0.f, 0.f));
+                const float2 c = fma2(make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])), make_float2(ks.z, ks.w), make_float2(0.f, 0.f));
+                float v[4] = {a.x, a.y, c.x, c.y};
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (!((seen >> (e + k)) & 1ull)) v[k] = -INFINITY;
+                }
+                most = max3(most, v[0] + lv.x, v[1] + lv.y);
+                most = max3(most, v[2] + lv.z, v[3] + lv.w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = __float_as_uint(v[k]);
+            }
+            const bool grow = most > top + kRescaleStep;   // also true for the first finite score of a row
+            if (__any_sync(0xffffffffu, grow)) {
+                const float keep = grow ? (top == -INFINITY ? 0.f : ex2_fast(top - most)) : 1.f;
+                if (grow) top = most;
+                sum *= keep;
+                if (j > 0) {   // (these scores were multiplied behind the weights of the block before: O is at rest)
+                    for (int n = 0; n < hd; n += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(mine_at + C::kOCol + n, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                        tmem_store16(mine_at + C::kOCol + n, o);
+                    }
+                }
+            }
+            const float shift = top == -INFINITY ? 0.f : -top;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 vs = lds_f4(scales + (kKeys + h * 32 + e) * 4);
+                    const float2 shift2 = make_float2(shift, shift);
+                    float2 a = add2(make_float2(__uint_as_float(raw[h][e]), __uint_as_float(raw[h][e + 1])), shift2);
+                    float2 c = add2(make_float2(__uint_as_float(raw[h][e + 2]), __uint_as_float(raw[h][e + 3])), shift2);
+                    a.x = ex2_fast(a.x);
+                    a.y = ex2_fast(a.y);
+                    c.x = ex2_fast(c.x);
+                    c.y = ex2_fast(c.y);
+                    const float2 t = add2(a, c);
+                    sum += t.x + t.y;
+                    a = mul2(a, make_float2(vs.x, vs.y));
+                    c = mul2(c, make_float2(vs.z, vs.w));
+                    if (masked) {   // (what is not seen may have any scale)
+                        const uint32_t m = (uint32_t)(seen >> (h * 32 + e));
+                        if (!(m & 1u)) a.x = 0.f;
+                        if (!(m & 2u)) a.y = 0.f;
+                        if (!(m & 4u)) c.x = 0.f;
+                        if (!(m & 8u)) c.y = 0.f;
+                    }
+                    w[e / 2] = pack2(a.x, a.y);
+                    w[e / 2 + 1] = pack2(c.x, c.y);
+                }
+                tmem_store16(mine_at + C::kSCol + h * 16, w);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->p_ready);
+            if (warp == 0) {
+                if (elect_one()) {
+                    ok = mbar_wait(&sh->p_ready, (uint32_t)j & 1u) && mbar_wait(&sh->v_full[j & 1], (uint32_t)(j >> 1) & 1u);
+                    if (ok) {
+                        tc_fence_after();
+                        const uint64_t vd = v_desc + (j & 1) * (C::kTile >> 4);
+#pragma unroll
+                        for (int ks = 0; ks < kKeys / 16; ++ks) umma_f16_ts(tmem + C::kOCol, tmem + C::kSCol + ks * 8, vd + ks * (2048 / 16), idesc_pv, j > 0 || ks > 0);
+                        umma_commit(&sh->v_empty[j & 1]);
+                        if (j + 1 == mine) umma_commit(&sh->o_done);
+                        else ok = scores_of(j + 1);
+                    }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
+        }
+        // O goes to shared memory where the blocks were: [row][features], 16 bytes c of a row at c ^ row, so that rows lie on different banks
+        if (ok && mine > 0) ok = mbar_wait(&sh->o_done, 0);
+        if (!ok && lane == 0) atomicExch(err, 27);
+    }
+    __syncwarp();
+    __syncthreads();   // (whoever gave up: the converting warps write no more)
+    if (warp < kSoftmaxWarps) {
+        tc_fence_after();
+        float* const part = reinterpret_cast<float*>(smem + C::kPartAt);
+        // (scores that are not numbers leave no reference: any finite one makes the part count below)
+        part[tid] = sum == sum ? top : 0.f;
+        part[kRows + tid] = sum;
+        if (mine > 0) {
+            const uint32_t from = tmem + ((uint32_t)warp << 21) + C::kOCol;
+#pragma unroll
+            for (int n = 0; n < kHD; n += 16) {
+                uint32_t o[16];
+                tmem_ld16(from + n, o);
+                tmem_ld_wait(o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    sts128(at + tid * kHD * 4 + (((n / 4 + k) ^ (tid & (kHD / 4 - 1))) << 4), make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+            }
+        }
+    }
+    tc_fence_before();
+    cluster.sync();
+    tc_fence_after();
+    if (warp == kSoftmaxWarps) tmem_dealloc(tmem, kTmemCols);
+    // ---- the CTAs' rows are joined: a row to kHD / 4 lanes
+    constexpr int kLanes = kHD / 4, kGroups = kThreads / kLanes;
+    for (int r = crank + csize * (tid / kLanes); r < rows; r += csize * kGroups) {
+        const int chunk = tid % kLanes;
+        float part_m[kMaxCluster], m = -INFINITY, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) part_m[k] = k < csize ? reinterpret_cast<const float*>(cluster.map_shared_rank(smem, k) + C::kPartAt)[r] : -INFINITY;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) m = fmaxf(m, part_m[k]);
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            if (part_m[k] != -INFINITY) {   // (a part that has seen nothing has no reference)
+                const uint8_t* const other = cluster.map_shared_rank(smem, k);
+                const float f = ex2_fast(part_m[k] - m);
+                const float4 o = *reinterpret_cast<const float4*>(other + r * kHD * 4 + ((chunk ^ (r & (kHD / 4 - 1))) << 4));
+                l = fmaf(f, reinterpret_cast<const float*>(other + C::kPartAt)[kRows + r], l);
+                v.x = fmaf(f, o.x, v.x);
+                v.y = fmaf(f, o.y, v.y);
+                v.z = fmaf(f, o.z, v.z);
+                v.w = fmaf(f, o.w, v.w);
+            }
+        }
+        if (chunk * 4 < hd) {
+            const float inv = 1.f / l;
+            const bool none = l == 0.f;
+            const int row = tile * kRows + r, i = row / p.group, h = kv_head * p.group + row % p.group;
+            const uint2 z = none ? make_uint2(0u, 0u) : make_uint2(pack2(v.x * inv, v.y * inv), pack2(v.z * inv, v.w * inv));
+            *reinterpret_cast<uint2*>(p.out + (s.q0 + i) * p.out_pitch + (long long)h * hd + chunk * 4) = z;
+        }
+    }
+    cluster.sync();   // nobody leaves while its rows are read
+}
+
+template <int kHD>
+cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
+    const auto kernel = attention_tree_tc_kernel<kHD>;
+    static PerDeviceOnce once;
+    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kHD>::kBytes); });
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * csize));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<kHD>::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)csize;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const bool longest_first = p.batch <= kThreads && units * csize > 2 * sm_count();
+    return cudaLaunchKernelEx(&cfg, kernel, p, row_tiles, longest_first, err);
+}
+
+}  // namespace
+
+bool attention_tree_tc_takes(const TreeParams& p) { return p.head_dim <= 128 && p.max_q_len * p.group >= 32 && p.max_k_len >= 64; }
+
+int attention_tree_tc_launch(const TreeParams& p, cudaStream_t st) {
+    const int row_tiles = (p.max_q_len * p.group + kRows - 1) / kRows;
+    const long long units = (long long)p.batch * (p.nhead / p.group) * row_tiles;
+    if (units * kMaxCluster > 0x7fffffff) return fail(ET_ERR_INVALID, "et_attention_tree: too large");
+    int* err = nullptr;
+    const int rc = attn_err_address(&err);
+    if (rc) return rc;
+    int csize = 1;
+    while (csize < kMaxCluster && csize * kKeys * 2 <= p.max_k_len && units * csize <= 4 * sm_count()) csize *= 2;
+    return cuda_status((p.head_dim <= 64 ? launch<64> : launch<128>)(p, row_tiles, units, csize, err, st), "et_attention_tree launch");
+}
+
+}  // namespace et

@@ -299,7 +299,8 @@ int et_kv_cache_read(const et_kv_cache_args* args);
  * table[b][0], table[b][1], .. (device, [batch][table_width]), those of the n drafted tokens themselves (written before the call) the last n. A token sees all keys before those, and of them the ones whose
  * bit is set in tree[row] (device, q_tokens 64-bit words: bit j is the sequence's j-th drafted token; its own bit counts like any other), or, with tree NULL, those up to itself: single tokens, and chains. A token that sees no key
  * gets zeros. Keys beyond max_k_len, the table, or in a page that there is not, are not seen. Rows of out in no sequence are left as they are. scale 0: 1 / sqrt(head_dim).
- * Scores and sums are fp32, the weights times the values' scales fp16. Rows of q and out start on 16 bytes; out overlaps q in nothing. */
+ * Scores and sums are fp32, the weights times the values' scales fp16. Rows of q and out start on 16 bytes; out overlaps q in nothing. The first call on a device looks up
+ * the device's error word (et_attention_check): make it before a stream capture. */
 typedef struct et_attention_tree_args {
     void* out; const void* q; const void* codes; const float* scales; const int* table; const int* k_lens; const int* cu_seqlens; const int64_t* tree; void* stream;
     int out_pitch, q_pitch, nhead, nhead_kv, head_dim, batch, q_tokens, max_q_len, max_k_len, pages, page, table_width;

@@ -7,6 +7,7 @@
 // it has to (then O is rescaled in tensor memory). Two CTAs share an SM: while one waits for its products the other takes exponentials. A cluster shares a sequence's keys; its CTAs' rows are joined
 // through distributed shared memory in a fixed order.
 #include <cooperative_groups.h>
+#include <type_traits>
 #include "attention.h"
 #include "attention_tree.cuh"
 #include "attention_tree.h"
@@ -45,7 +46,7 @@ struct Cfg {
 
 struct Shared {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_ready, s_full, p_ready, o_done;
+    uint64_t scales_full[kScaleStages], q_ready, s_full, p_ready, o_done;
     uint32_t good[kScaleStages];          // a bit for each 16 keys of a block: their page is there
     uint32_t tmem_base;
 };
@@ -108,6 +109,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 mbar_init(&sh->k_empty[i], 1);
                 mbar_init(&sh->v_empty[i], 1);
             }
+            for (int i = 0; i < kScaleStages; ++i) mbar_init(&sh->scales_full[i], kConvertWarps);
             mbar_init(&sh->q_ready, kSoftmaxWarps);
             mbar_init(&sh->s_full, 1);
             mbar_init(&sh->p_ready, kSoftmaxWarps);
@@ -133,26 +135,38 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         const int key_s = c & 63, side_s = c >> 6;                    // whose scale it brings
         const int* const table = p.table + (long long)b * p.table_width;
         const uint32_t raw = at + C::kRawAt;
-        auto page_of = [&](int key) {                                 // page of a key, -1: none
-            if (key >= s.klen) return -1;
-            const int id = __ldg(table + key / p.page);
-            return id < p.pages ? id : -1;
+        const long long v_from_k = (long long)n_kv * p.page, v_codes = v_from_k * hd;   // from a key's K to its V
+        const int in_piece = (key_c & 15) * hd + f;
+        // The four 16 keys of a block, each in one page, a lane each (over and over): the page's number is requested a block before it is needed.
+        int piece_id = -1, piece_off = 0;
+        auto look_up = [&](int j) {
+            const int key = (crank + j * csize) * kKeys + (lane & 3) * 16;
+            piece_id = -1;
+            if (j < mine && key < s.klen) {
+                const int n = key / p.page;
+                piece_id = __ldg(table + n);
+                piece_off = key - n * p.page;
+            }
         };
-        auto row_of = [&](int key, int id, int side) { return (((long long)id * 2 + side) * n_kv + kv_head) * p.page + key % p.page; };
-        auto fetch = [&](int j) {
+        uint32_t good_bits = 0;                                       // of eight blocks, four bits each
+        auto fetch = [&](int j) {                                     // block j, whose pages have been looked up
+            const bool there = piece_id >= 0 && piece_id < p.pages;
+            const long long row = there ? ((long long)piece_id * 2 * n_kv + kv_head) * p.page + piece_off : -1, start = row * hd;   // its first row, and its codes
+            look_up(j + 1);
+            const uint32_t good = __ballot_sync(0xffffffffu, there) & 15u;
+            good_bits = (good_bits & ~(15u << (4 * (j & 7)))) | good << (4 * (j & 7));
             if (j < mine) {
-                const int key0 = (crank + j * csize) * kKeys;
                 const uint32_t to = raw + (j % C::kRawStages) * C::kRaw + c * 16;
 #pragma unroll
                 for (int n = 0; n < C::kChunks; ++n) {
-                    const int key = key0 + key_c + n * (128 / kPerKey), id = page_of(key & ~15);   // (16 keys of a block lie in one page)
-                    const bool good = id >= 0 && f < hd;
-                    const long long k_row = row_of(key, max(id, 0), 0), v_row = k_row + (long long)n_kv * p.page;
-                    copy_async<16>(to + n * 2048, good ? p.codes + k_row * hd + f : p.codes, good ? 16 : 0);
-                    copy_async<16>(to + (C::kChunks + n) * 2048, good ? p.codes + v_row * hd + f : p.codes, good ? 16 : 0);
+                    const long long first = __shfl_sync(0xffffffffu, start, (key_c >> 4) + n * (8 / kPerKey));
+                    const bool real = first >= 0 && f < hd;
+                    const int8_t* const k = p.codes + (real ? first + in_piece : 0);
+                    copy_async<16>(to + n * 2048, k, real ? 16 : 0);
+                    copy_async<16>(to + (C::kChunks + n) * 2048, real ? k + v_codes : k, real ? 16 : 0);
                 }
-                const int key = key0 + key_s, id = page_of(key);
-                copy_async<4>(raw + (j % C::kRawStages) * C::kRaw + 2 * C::kChunks * 2048 + c * 4, id >= 0 ? p.scales + row_of(key, id, side_s) : p.scales, id >= 0 ? 4 : 0);
+                const long long first = __shfl_sync(0xffffffffu, row, key_s >> 4);
+                copy_async<4>(raw + (j % C::kRawStages) * C::kRaw + 2 * C::kChunks * 2048 + c * 4, p.scales + (first >= 0 ? first + (key_s & 15) + side_s * v_from_k : 0), first >= 0 ? 4 : 0);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -169,6 +183,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             sts128(line + (((chunk + swap) ^ (key & 7)) << 4), swap ? h[1] : h[0]);
             sts128(line + (((chunk + 1 - swap) ^ (key & 7)) << 4), swap ? h[0] : h[1]);
         };
+        look_up(0);
         for (int n = 0; n < C::kRawStages - 1; ++n) fetch(n);
         for (int j = 0; j < mine; ++j) {
             fetch(j + C::kRawStages - 1);   // (the thread has read that place a turn ago)
@@ -189,15 +204,13 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 to[kKeys] = real ? scale : 0.f;
                 to[2 * kKeys] = log2_of_scale(real ? scale : 0.f);
             }
-            if (c == 0) {
-                uint32_t good = 0;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) good |= (page_of(key0 + n * 16) >= 0 ? 1u : 0u) << n;
-                sh->good[j % kScaleStages] = good;
-            }
+            if (c == 0) sh->good[j % kScaleStages] = (good_bits >> (4 * (j & 7))) & 15u;
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh->k_full[st]);
+            if (lane == 0) {
+                mbar_arrive(&sh->scales_full[j % kScaleStages]);
+                mbar_arrive(&sh->k_full[st]);
+            }
             ok = mbar_wait(&sh->v_empty[st], ph);
             if (!ok) break;
 #pragma unroll
@@ -253,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         }
         for (int j = 0; j < mine; ++j) {
             const int key0 = (crank + j * csize) * kKeys;
-            ok = mbar_wait(&sh->k_full[j & 1], (uint32_t)(j >> 1) & 1u) && mbar_wait(&sh->s_full, (uint32_t)j & 1u);
+            // (Not for k_full: the place may be full of block j + 2 before this warp looks, and the phases of two blocks look alike. The scales of block j + 4 wait for this one's weights.)
+            ok = mbar_wait(&sh->scales_full[j % kScaleStages], (uint32_t)(j / kScaleStages) & 1u) && mbar_wait(&sh->s_full, (uint32_t)j & 1u);
             if (!ok) break;
             tc_fence_after();
             uint32_t raw[2][32];
@@ -263,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             const uint32_t scales = at + C::kScaleAt + (j % kScaleStages) * 3 * kKeys * 4;
             // what the row sees of the block
             const uint32_t good = sh->good[j % kScaleStages];
-            const bool masked = key0 + kKeys > s.kept || key0 + kKeys > s.klen || good != 15u;
+            const bool masked = key0 + kKeys > s.kept || key0 + kKeys > s.klen || good != 15u;   // the same for the whole CTA
             unsigned long long seen = ~0ull;
             if (masked) {
                 const int d = key0 - s.kept;   // place of the first key among the drafted tokens
@@ -275,23 +289,27 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                         if (!((good >> n) & 1u)) seen &= ~(0xffffull << (n * 16));
             }
             float most = -INFINITY;
+            auto two = [](const uint32_t* x) { return make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])); };
+            // (with and without masks by themselves: a branch at every four keys kept the others' loads behind it, 2200 clocks for 700)
+            auto largest = [&](auto with_masks) {
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int e = 0; e < kKeys; e += 4) {
-                const float4 ks = lds_f4(scales + e * 4), lv = lds_f4(scales + (2 * kKeys + e) * 4);
-                uint32_t* const x = &raw[e >> 5][e & 31];
-                const float2 a = fma2(make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])), make_float2(ks.x, ks.y), make_float2(0.f, 0.f));
-                const float2 c = fma2(make_float2(__uint_as_float(x[2]), __uint_as_float(x[3])), make_float2(ks.z, ks.w), make_float2(0.f, 0.f));
-                float v[4] = {a.x, a.y, c.x, c.y};
-                if (masked) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (!((seen >> (e + k)) & 1ull)) v[k] = -INFINITY;
+                for (int e = 0; e < kKeys; e += 4) {
+                    const float4 ks = lds_f4(scales + e * 4), lv = lds_f4(scales + (2 * kKeys + e) * 4);
+                    float2 a = fma2(two(&raw[e >> 5][e & 31]), make_float2(ks.x, ks.y), make_float2(lv.x, lv.y)), c = fma2(two(&raw[e >> 5][e & 31] + 2), make_float2(ks.z, ks.w), make_float2(lv.z, lv.w));
+                    if constexpr (with_masks) {
+                        const uint32_t m = (uint32_t)(seen >> e);
+                        if (!(m & 1u)) a.x = -INFINITY;
+                        if (!(m & 2u)) a.y = -INFINITY;
+                        if (!(m & 4u)) c.x = -INFINITY;
+                        if (!(m & 8u)) c.y = -INFINITY;
+                    }
+                    m4[(e >> 1) & 3] = max3(m4[(e >> 1) & 3], a.x, a.y);
+                    m4[((e >> 1) & 3) + 1] = max3(m4[((e >> 1) & 3) + 1], c.x, c.y);
                 }
-                most = max3(most, v[0] + lv.x, v[1] + lv.y);
-                most = max3(most, v[2] + lv.z, v[3] + lv.w);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = __float_as_uint(v[k]);
-            }
+                return fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
+            };
+            most = masked ? largest(std::true_type()) : largest(std::false_type());
             const bool grow = most > top + kRescaleStep;   // also true for the first finite score of a row
             if (__any_sync(0xffffffffu, grow)) {
                 const float keep = grow ? (top == -INFINITY ? 0.f : ex2_fast(top - most)) : 1.f;
@@ -309,35 +327,38 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 }
             }
             const float shift = top == -INFINITY ? 0.f : -top;
+            auto weights = [&](auto with_masks) {
+                float2 sums = make_float2(0.f, 0.f);
+                const float2 shift2 = make_float2(shift, shift);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[16];
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t w[16];
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    const float4 vs = lds_f4(scales + (kKeys + h * 32 + e) * 4);
-                    const float2 shift2 = make_float2(shift, shift);
-                    float2 a = add2(make_float2(__uint_as_float(raw[h][e]), __uint_as_float(raw[h][e + 1])), shift2);
-                    float2 c = add2(make_float2(__uint_as_float(raw[h][e + 2]), __uint_as_float(raw[h][e + 3])), shift2);
-                    a.x = ex2_fast(a.x);
-                    a.y = ex2_fast(a.y);
-                    c.x = ex2_fast(c.x);
-                    c.y = ex2_fast(c.y);
-                    const float2 t = add2(a, c);
-                    sum += t.x + t.y;
-                    a = mul2(a, make_float2(vs.x, vs.y));
-                    c = mul2(c, make_float2(vs.z, vs.w));
-                    if (masked) {   // (what is not seen may have any scale)
-                        const uint32_t m = (uint32_t)(seen >> (h * 32 + e));
-                        if (!(m & 1u)) a.x = 0.f;
-                        if (!(m & 2u)) a.y = 0.f;
-                        if (!(m & 4u)) c.x = 0.f;
-                        if (!(m & 8u)) c.y = 0.f;
+                    for (int e = 0; e < 32; e += 4) {
+                        const float4 ks = lds_f4(scales + (h * 32 + e) * 4), vs = lds_f4(scales + (kKeys + h * 32 + e) * 4);
+                        float2 a = fma2(two(&raw[h][e]), make_float2(ks.x, ks.y), shift2), c = fma2(two(&raw[h][e] + 2), make_float2(ks.z, ks.w), shift2);
+                        a.x = ex2_fast(a.x);
+                        a.y = ex2_fast(a.y);
+                        c.x = ex2_fast(c.x);
+                        c.y = ex2_fast(c.y);
+                        float2 x = mul2(a, make_float2(vs.x, vs.y)), y = mul2(c, make_float2(vs.z, vs.w));
+                        if constexpr (with_masks) {   // (what is not seen may have any scale)
+                            const uint32_t m = (uint32_t)(seen >> (h * 32 + e));
+                            if (!(m & 1u)) a.x = x.x = 0.f;
+                            if (!(m & 2u)) a.y = x.y = 0.f;
+                            if (!(m & 4u)) c.x = y.x = 0.f;
+                            if (!(m & 8u)) c.y = y.y = 0.f;
+                        }
+                        sums = add2(sums, add2(a, c));
+                        w[e / 2] = pack2(x.x, x.y);
+                        w[e / 2 + 1] = pack2(y.x, y.y);
                     }
-                    w[e / 2] = pack2(a.x, a.y);
-                    w[e / 2 + 1] = pack2(c.x, c.y);
+                    tmem_store16(mine_at + C::kSCol + h * 16, w);
                 }
-                tmem_store16(mine_at + C::kSCol + h * 16, w);
-            }
+                sum += sums.x + sums.y;
+            };
+            if (masked) weights(std::true_type());
+            else weights(std::false_type());
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();

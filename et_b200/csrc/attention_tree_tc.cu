@@ -23,7 +23,7 @@ constexpr int kKeys = 64;                 // of a block
 constexpr int kRows = 128;                // of a CTA
 constexpr int kSoftmaxWarps = 4, kConvertWarps = 4, kThreads = 8 * 32;   // (two CTAs to an SM with 128 registers a thread)
 constexpr int kMaxCluster = 8;
-constexpr int kScaleStages = 4;
+constexpr int kScaleStages = 4, kScaleBytes = kKeys * (4 + 4 + 2);
 constexpr float kRescaleStep = 8.f;       // log2 units
 constexpr uint32_t kTmemCols = 256;
 
@@ -36,8 +36,8 @@ struct Cfg {
     static constexpr uint32_t kQCol = 0, kSCol = kHD / 2, kOCol = kSCol + kKeys;
     static_assert(kOCol + kHD <= kTmemCols, "");
     static constexpr int kKAt = 0, kVAt = 2 * kTile, kRawAt = 4 * kTile;
-    static constexpr int kScaleAt = kRawAt + kRawStages * kRaw;                 // [stage][key: score factor, value's scale, its logarithm][64]
-    static constexpr int kPartAt = kScaleAt + kScaleStages * 3 * kKeys * 4;     // [reference, sum][128]
+    static constexpr int kScaleAt = kRawAt + kRawStages * kRaw;                 // [stage]: of 64 keys score factors, values' scales, their logarithms as fp16
+    static constexpr int kPartAt = kScaleAt + kScaleStages * kScaleBytes;     // [reference, sum][128]
     // Half of an SM's shared memory for half of its tensor memory: a CTA that finds one finds the other, and none waits for columns that another cluster holds.
     static constexpr int kBytes = 113664;
     static_assert(kPartAt + 2 * kRows * 4 + 1024 <= kBytes && kTmemCols == 256, "");
@@ -63,6 +63,10 @@ template <int kSize>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from, int real) {
     if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
     else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
+}
+// Two halves added to two fp32 values.
+__device__ __forceinline__ void add_halves(uint32_t h, float a, float b, float& x, float& y) {
+    asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\nadd.rn.f32.f16 %0, l, %3;\nadd.rn.f32.f16 %1, h, %4;\n}" : "=f"(x), "=f"(y) : "r"(h), "f"(a), "f"(b));
 }
 __device__ __forceinline__ float4 lds_f4(uint32_t a) {
     const uint4 v = lds128(a);
@@ -100,6 +104,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
     const TreeSeq s = tree_seq(p, b);
     const int rows = min(s.qlen * p.group - tile * kRows, kRows), hd = p.head_dim;
     if (rows <= 0) return;                // the same for the whole cluster
+    const int row_warps = (rows + 31) / 32;   // the other softmax warps have no row: their lanes of tensor memory hold anything, which no row sees
     const int n_blocks = (s.klen + kKeys - 1) / kKeys, mine = n_blocks > crank ? (n_blocks - crank + csize - 1) / csize : 0;   // blocks crank, crank + csize, ..
     if (warp == kSoftmaxWarps) {
         if (lane == 0) {
@@ -110,9 +115,9 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 mbar_init(&sh->v_empty[i], 1);
             }
             for (int i = 0; i < kScaleStages; ++i) mbar_init(&sh->scales_full[i], kConvertWarps);
-            mbar_init(&sh->q_ready, kSoftmaxWarps);
+            mbar_init(&sh->q_ready, row_warps);
             mbar_init(&sh->s_full, 1);
-            mbar_init(&sh->p_ready, kSoftmaxWarps);
+            mbar_init(&sh->p_ready, row_warps);
             mbar_init(&sh->o_done, 1);
             fence_mbar_init();
         }
@@ -197,12 +202,12 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             // Scales go to the places of block j - 4, whose scores are done with: those of block j - 2 have been multiplied, behind the weights of block j - 3.
             const float scale = __uint_as_float(lds32(from + 2 * C::kChunks * 2048 + c * 4));
             const bool real = key0 + key_s < s.klen;   // (behind the last key anything may lie)
-            float* const to = reinterpret_cast<float*>(smem + C::kScaleAt) + (j % kScaleStages) * 3 * kKeys + key_s;
+            uint8_t* const to = smem + C::kScaleAt + (j % kScaleStages) * kScaleBytes;
             if (side_s == 0) {
-                to[0] = real ? scale * p.scale_log2 : 0.f;
+                reinterpret_cast<float*>(to)[key_s] = real ? scale * p.scale_log2 : 0.f;
             } else {
-                to[kKeys] = real ? scale : 0.f;
-                to[2 * kKeys] = log2_of_scale(real ? scale : 0.f);
+                reinterpret_cast<float*>(to)[kKeys + key_s] = real ? scale : 0.f;
+                reinterpret_cast<half*>(to + 8 * kKeys)[key_s] = __float2half_rn(log2_of_scale(real ? scale : 0.f));   // (for the reference alone)
             }
             if (c == 0) sh->good[j % kScaleStages] = (good_bits >> (4 * (j & 7))) & 15u;
             fence_proxy_async_smem();
@@ -221,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (!ok && lane == 0) atomicExch(err, 26);
-    } else {
+    } else if (warp < row_warps) {
         // ---- a row to a thread
         const uint32_t mine_at = tmem + ((uint32_t)warp << 21);       // the warp's lanes of tensor memory
         const bool real = tid < rows;
@@ -274,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             tmem_ld32(mine_at + C::kSCol, raw[0]);
             tmem_ld32(mine_at + C::kSCol + 32, raw[1]);
             tmem_ld_wait(raw[0], raw[1]);
-            const uint32_t scales = at + C::kScaleAt + (j % kScaleStages) * 3 * kKeys * 4;
+            const uint32_t scales = at + C::kScaleAt + (j % kScaleStages) * kScaleBytes;
             // what the row sees of the block
             const uint32_t good = sh->good[j % kScaleStages];
             const bool masked = key0 + kKeys > s.kept || key0 + kKeys > s.klen || good != 15u;   // the same for the whole CTA
@@ -294,18 +299,27 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             auto largest = [&](auto with_masks) {
                 float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < kKeys; e += 4) {
-                    const float4 ks = lds_f4(scales + e * 4), lv = lds_f4(scales + (2 * kKeys + e) * 4);
-                    float2 a = fma2(two(&raw[e >> 5][e & 31]), make_float2(ks.x, ks.y), make_float2(lv.x, lv.y)), c = fma2(two(&raw[e >> 5][e & 31] + 2), make_float2(ks.z, ks.w), make_float2(lv.z, lv.w));
-                    if constexpr (with_masks) {
-                        const uint32_t m = (uint32_t)(seen >> e);
-                        if (!(m & 1u)) a.x = -INFINITY;
-                        if (!(m & 2u)) a.y = -INFINITY;
-                        if (!(m & 4u)) c.x = -INFINITY;
-                        if (!(m & 8u)) c.y = -INFINITY;
+                for (int e = 0; e < kKeys; e += 8) {
+                    const uint4 lv8 = lds128(scales + 8 * kKeys + e * 2);
+                    const uint32_t lv[4] = {lv8.x, lv8.y, lv8.z, lv8.w};
+#pragma unroll
+                    for (int k = 0; k < 8; k += 4) {
+                        const float4 ks = lds_f4(scales + (e + k) * 4);
+                        uint32_t* const x = &raw[e >> 5][(e & 31) + k];
+                        const float2 a = mul2(two(x), make_float2(ks.x, ks.y)), c = mul2(two(x + 2), make_float2(ks.z, ks.w));
+                        float v[4] = {a.x, a.y, c.x, c.y}, t[4];
+                        if constexpr (with_masks) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (!((seen >> (e + k + i)) & 1ull)) v[i] = -INFINITY;
+                        }
+                        add_halves(lv[k / 2], v[0], v[1], t[0], t[1]);
+                        add_halves(lv[k / 2 + 1], v[2], v[3], t[2], t[3]);
+                        m4[k / 2] = max3(m4[k / 2], t[0], t[1]);
+                        m4[k / 2 + 1] = max3(m4[k / 2 + 1], t[2], t[3]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = __float_as_uint(v[i]);
                     }
-                    m4[(e >> 1) & 3] = max3(m4[(e >> 1) & 3], a.x, a.y);
-                    m4[((e >> 1) & 3) + 1] = max3(m4[((e >> 1) & 3) + 1], c.x, c.y);
                 }
                 return fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
             };
@@ -335,8 +349,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                     uint32_t w[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 4) {
-                        const float4 ks = lds_f4(scales + (h * 32 + e) * 4), vs = lds_f4(scales + (kKeys + h * 32 + e) * 4);
-                        float2 a = fma2(two(&raw[h][e]), make_float2(ks.x, ks.y), shift2), c = fma2(two(&raw[h][e] + 2), make_float2(ks.z, ks.w), shift2);
+                        const float4 vs = lds_f4(scales + (kKeys + h * 32 + e) * 4);
+                        float2 a = add2(two(&raw[h][e]), shift2), c = add2(two(&raw[h][e] + 2), shift2);
                         a.x = ex2_fast(a.x);
                         a.y = ex2_fast(a.y);
                         c.x = ex2_fast(c.x);
@@ -344,10 +358,10 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                         float2 x = mul2(a, make_float2(vs.x, vs.y)), y = mul2(c, make_float2(vs.z, vs.w));
                         if constexpr (with_masks) {   // (what is not seen may have any scale)
                             const uint32_t m = (uint32_t)(seen >> (h * 32 + e));
-                            if (!(m & 1u)) a.x = x.x = 0.f;
-                            if (!(m & 2u)) a.y = x.y = 0.f;
-                            if (!(m & 4u)) c.x = y.x = 0.f;
-                            if (!(m & 8u)) c.y = y.y = 0.f;
+                            if (!(m & 1u)) x.x = 0.f;
+                            if (!(m & 2u)) x.y = 0.f;
+                            if (!(m & 4u)) y.x = 0.f;
+                            if (!(m & 8u)) y.y = 0.f;
                         }
                         sums = add2(sums, add2(a, c));
                         w[e / 2] = pack2(x.x, x.y);

@@ -1,7 +1,8 @@
 // A cache of keys and values in int8, in pages: rows of K and V quantised as they are written (a scale for each row and head: its largest size / 127), and rows read back.
 //
-// codes [pages][K, V][heads][page rows][head_dim], scales [pages][K, V][heads][page rows]: a page of a head is one piece. A group of neighbouring lanes has a
-// row of a head, 8 features to a lane, so that fp16 rows go as 16 bytes a lane and codes as 8; heads of a token lie side by side in a warp. Bound by memory: 3 bytes a feature.
+// codes [pages][K, V][heads][page rows][head_dim], scales [pages][K, V][heads][page rows]: a page of a head is one piece. Neighbouring lanes have a
+// row of a head, 16 features each: 16 bytes of codes, 32 of fp16. Heads of a token lie side by side in a block, whose threads take the same row of several tokens at once. Bound by memory: 3 bytes a feature.
+#include <algorithm>
 #include "common.h"
 #include "ptx.cuh"
 #include "vec_math.cuh"
@@ -9,8 +10,10 @@
 namespace et {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRowsInFlight = 4;
+// 27 thousand rows of 16 heads of 128 read back, with one, two, four, eight tokens of a thread in flight: 31.7, 28.3, 38.7, 46.5 us, written (8192 tokens) 13.9, 13.3,
+// 13.5, 17.4, blocks of 256 threads 30.3 and 13.3; few tokens with one and two 2.25 and 2.86.
+constexpr int kThreads = 128;
+constexpr int kBlockRows = 4;    // of a token, at most, in a block
 
 struct CacheParams {
     int8_t* codes;
@@ -18,25 +21,33 @@ struct CacheParams {
     half *k, *v;                 // read by the write, written by the read
     const int* slots;
     long long k_pitch, v_pitch, n_slots;
-    long long items;             // tokens x K, V x heads
-    int heads, head_dim, page;
+    int tokens, heads, head_dim, page;
+    int lanes;                   // of a row, a power of two
+    int block_rows, block_tokens;   // rows of a token, and tokens, side by side in a block
 };
 
-// Row (token, side, head) with number i, in which heads of a token's K and then of its V are neighbours.
-struct CacheRow {
-    half* x;
-    long long at;                // among the cache's rows; below 0: no place
+// What a thread works on: 16 features of row (side, head) of tokens first, first + step, ..
+struct CachePlace {
+    bool in;
+    int at, row, first, step;
 };
-__device__ __forceinline__ CacheRow cache_row(const CacheParams& p, long long i) {
-    const int per_token = 2 * p.heads;
-    const long long token = i / per_token;
-    const int r = (int)(i - token * per_token), side = r >= p.heads, head = r - side * p.heads;
-    const int slot = p.slots[token];
-    CacheRow c;
-    c.x = (side ? p.v + token * p.v_pitch : p.k + token * p.k_pitch) + head * p.head_dim;
-    const int page = slot / p.page;
-    c.at = slot < 0 || slot >= p.n_slots ? -1 : ((long long)page * per_token + r) * p.page + (slot - page * p.page);
+__device__ __forceinline__ CachePlace cache_place(const CacheParams& p, int tokens) {
+    const int g = threadIdx.x / p.lanes, t = g / p.block_rows;
+    CachePlace c;
+    c.at = (threadIdx.x & (p.lanes - 1)) * 16;
+    c.row = blockIdx.y * p.block_rows + g - t * p.block_rows;
+    c.first = blockIdx.x * (p.block_tokens * tokens) + t;
+    c.step = p.block_tokens;
+    c.in = t < p.block_tokens && c.row < 2 * p.heads;
     return c;
+}
+// Where a token's row lies among the cache's rows; below 0: no place.
+__device__ __forceinline__ long long cache_row(const CacheParams& p, int token, int row) {
+    const int slot = p.slots[token], page = slot / p.page;
+    return slot < 0 || slot >= p.n_slots ? -1 : ((long long)page * (2 * p.heads) + row) * p.page + (slot - page * p.page);
+}
+__device__ __forceinline__ half* token_row(const CacheParams& p, int token, int row) {
+    return row >= p.heads ? p.v + token * p.v_pitch + (row - p.heads) * p.head_dim : p.k + token * p.k_pitch + row * p.head_dim;
 }
 
 // fp16 rows in whole 16 bytes, or elements one by one.
@@ -60,86 +71,97 @@ __device__ __forceinline__ void store8(half* x, const uint4& v) {
     }
 }
 
-// lanes: of a group, a power of two. code = x / scale to the nearest, of two equally near the even one; x / scale is corrected by what its product with the scale
-// leaves, so that it is the rounded quotient.
-template <bool kVec>
-__global__ void __launch_bounds__(kThreads) cache_write_kernel(const __grid_constant__ CacheParams p, int lanes) {
-    const int at = (threadIdx.x & (lanes - 1)) * 8, groups = kThreads / lanes;
-    const long long first = (long long)blockIdx.x * groups * kRowsInFlight + threadIdx.x / lanes;
+// code = x / scale to the nearest, of two equally near the even one; x / scale is corrected by what its product with the scale leaves, so that it is the
+// rounded quotient. The code comes out of the low bits of 1.5 2^23 + x / scale, to which the addition rounds it.
+// kTokens: of a thread, all requested at once.
+template <bool kVec, int kTokens>
+__global__ void __launch_bounds__(kThreads) cache_write_kernel(const __grid_constant__ CacheParams p) {
+    const CachePlace c = cache_place(p, kTokens);
+    const bool features = c.at < p.head_dim;
     pdl_wait();
     pdl_launch_dependents();
-    uint4 x[kRowsInFlight];
-    long long to[kRowsInFlight];
+    uint4 x[kTokens][2];
+    long long to[kTokens];
 #pragma unroll
-    for (int n = 0; n < kRowsInFlight; ++n) {
-        const long long i = first + n * groups;
-        x[n] = make_uint4(0u, 0u, 0u, 0u);
+    for (int n = 0; n < kTokens; ++n) {
+        const int token = c.first + n * c.step;
+        x[n][0] = x[n][1] = make_uint4(0u, 0u, 0u, 0u);
         to[n] = -1;
-        if (i < p.items) {
-            const CacheRow c = cache_row(p, i);
-            to[n] = c.at;
-            if (c.at >= 0 && at < p.head_dim) x[n] = load8<kVec>(c.x + at);
+        if (c.in && token < p.tokens) {
+            to[n] = cache_row(p, token, c.row);
+            if (features) {   // (read whether it has a place or not: both are on their way at once)
+                const half* const from = token_row(p, token, c.row) + c.at;
+                x[n][0] = load8<kVec>(from);
+                x[n][1] = load8<kVec>(from + 8);
+            }
         }
     }
 #pragma unroll
-    for (int n = 0; n < kRowsInFlight; ++n) {
-        float f[8], top = 0.f;
+    for (int n = 0; n < kTokens; ++n) {
+        float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 v = __half22float2(reinterpret_cast<const half2*>(&x[n])[i]);
-            f[2 * i] = v.x;
-            f[2 * i + 1] = v.y;
+        for (int i = 0; i < 8; ++i) {
+            const float2 v = __half22float2(reinterpret_cast<const half2*>(x[n])[i]);
             top = max_nan(top, max_nan(fabsf(v.x), fabsf(v.y)));
         }
-        for (int o = lanes >> 1; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = p.lanes >> 1; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (to[n] < 0) continue;
         const float scale = top / 127.f, inverse = scale > 0.f ? 1.f / scale : 0.f;
-        if (at < p.head_dim) {
-            uint32_t w[2] = {0u, 0u};
+        if (features) {
+            uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float q = f[i] * inverse;
-                w[i >> 2] |= (uint32_t)(uint8_t)(int8_t)__float2int_rn(fmaf(fmaf(-q, scale, f[i]), inverse, q)) << (8 * (i & 3));
+            for (int i = 0; i < 4; ++i) {
+                uint32_t b[4];
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {
+                    const float2 v = __half22float2(reinterpret_cast<const half2*>(x[n])[i * 2 + k / 2]);
+                    const float q0 = v.x * inverse, q1 = v.y * inverse;
+                    const float r0 = fmaf(fmaf(-q0, scale, v.x), inverse, q0), r1 = fmaf(fmaf(-q1, scale, v.y), inverse, q1);
+                    b[k] = __float_as_uint(r0 + 12582912.f);
+                    b[k + 1] = __float_as_uint(r1 + 12582912.f);
+                }
+                w[i] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
             }
-            *reinterpret_cast<uint2*>(p.codes + to[n] * p.head_dim + at) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint4*>(p.codes + to[n] * p.head_dim + c.at) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        if (at == 0) p.scales[to[n]] = scale;
+        if (c.at == 0) p.scales[to[n]] = scale - scale == 0.f ? scale : __int_as_float(0x7fffffff);   // (infinite: all of the row is not a number)
     }
 }
 
-template <bool kVec>
-__global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ CacheParams p, int lanes) {
-    const int at = (threadIdx.x & (lanes - 1)) * 8, groups = kThreads / lanes;
-    const long long first = (long long)blockIdx.x * groups * kRowsInFlight + threadIdx.x / lanes;
+template <bool kVec, int kTokens>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const __grid_constant__ CacheParams p) {
+    const CachePlace c = cache_place(p, kTokens);
+    if (!c.in || c.at >= p.head_dim) return;
     pdl_wait();
     pdl_launch_dependents();
-    uint2 c[kRowsInFlight];
-    float scale[kRowsInFlight];
-    half* to[kRowsInFlight];
+    uint4 w[kTokens];
+    float scale[kTokens];
+    bool there[kTokens];
 #pragma unroll
-    for (int n = 0; n < kRowsInFlight; ++n) {
-        const long long i = first + n * groups;
-        to[n] = nullptr;
-        if (i < p.items && at < p.head_dim) {
-            const CacheRow r = cache_row(p, i);
-            if (r.at >= 0) {
-                to[n] = r.x + at;
-                c[n] = *reinterpret_cast<const uint2*>(p.codes + r.at * p.head_dim + at);
-                scale[n] = p.scales[r.at];
-            }
+    for (int n = 0; n < kTokens; ++n) {
+        const int token = c.first + n * c.step;
+        const long long row = token < p.tokens ? cache_row(p, token, c.row) : -1;
+        there[n] = row >= 0;
+        if (there[n]) {
+            w[n] = *reinterpret_cast<const uint4*>(p.codes + row * p.head_dim + c.at);
+            scale[n] = p.scales[row];
         }
     }
 #pragma unroll
-    for (int n = 0; n < kRowsInFlight; ++n) {
-        if (!to[n]) continue;
-        uint4 v;
-        half2* const h = reinterpret_cast<half2*>(&v);
+    for (int n = 0; n < kTokens; ++n) {
+        if (!there[n]) continue;
+        const uint32_t u[4] = {w[n].x ^ 0x80808080u, w[n].y ^ 0x80808080u, w[n].z ^ 0x80808080u, w[n].w ^ 0x80808080u};
+        uint4 v[2];
+        half2* const h = reinterpret_cast<half2*>(v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t w = (i < 2 ? c[n].x : c[n].y) >> (16 * (i & 1));
-            h[i] = __floats2half2_rn((float)(int8_t)w * scale[n], (float)(int8_t)(w >> 8) * scale[n]);
+        for (int i = 0; i < 8; ++i) {   // the byte + 128 as the low bits of 2^23
+            const float lo = __uint_as_float(__byte_perm(u[i / 2], 0x4b000000u, i & 1 ? 0x7442 : 0x7440)) - 8388736.f;
+            const float hi = __uint_as_float(__byte_perm(u[i / 2], 0x4b000000u, i & 1 ? 0x7443 : 0x7441)) - 8388736.f;
+            h[i] = __floats2half2_rn(lo * scale[n], hi * scale[n]);
         }
-        store8<kVec>(to[n], v);
+        half* const to = token_row(p, c.first + n * c.step, c.row) + c.at;
+        store8<kVec>(to, v[0]);
+        store8<kVec>(to + 8, v[1]);
     }
 }
 
@@ -154,6 +176,7 @@ int cache_run(const et_kv_cache_args* a, bool write, const char* where) {
     if (a->heads < 1 || a->heads > 65535) return bad("heads must be 1 to 65535");
     if (a->head_dim < 16 || a->head_dim > 256 || a->head_dim % 16) return bad("head_dim must be a multiple of 16 up to 256");
     if (a->page < 16 || a->page % 16) return bad("the rows of a page must be a multiple of 16");
+    if (a->tokens > 0x7ff00000) return bad("too many rows");
     if ((long long)a->pages * a->page > 0x7fffffff) return bad("more places than 32 bits number");
     if (a->tokens == 0) return ET_OK;
     if (!a->codes || !a->scales || !a->k || !a->v || !a->slots) return bad("null pointer");
@@ -164,15 +187,22 @@ int cache_run(const et_kv_cache_args* a, bool write, const char* where) {
     p.codes = static_cast<int8_t*>(a->codes); p.scales = a->scales;
     p.k = static_cast<half*>(a->k); p.v = static_cast<half*>(a->v); p.slots = a->slots;
     p.k_pitch = a->k_pitch; p.v_pitch = a->v_pitch; p.n_slots = (long long)a->pages * a->page;
-    p.items = (long long)a->tokens * 2 * a->heads;
-    p.heads = a->heads; p.head_dim = a->head_dim; p.page = a->page;
+    p.tokens = a->tokens; p.heads = a->heads; p.head_dim = a->head_dim; p.page = a->page;
     const bool vec = aligned16(a->k) && aligned16(a->v) && (a->tokens == 1 || ((a->k_pitch | a->v_pitch) & 7) == 0);
-    int lanes = 2;
-    while (lanes * 8 < a->head_dim) lanes *= 2;
-    const long long rows = (long long)kThreads / lanes * kRowsInFlight, blocks = (p.items + rows - 1) / rows;
-    if (blocks > 0x7fffffff) return bad("too many rows");
-    const auto kernel = write ? (vec ? cache_write_kernel<true> : cache_write_kernel<false>) : (vec ? cache_read_kernel<true> : cache_read_kernel<false>);
-    return cuda_status(launch_pdl(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, static_cast<cudaStream_t>(a->stream), p, lanes), where);
+    p.lanes = 1;
+    while (p.lanes * 16 < a->head_dim) p.lanes *= 2;
+    const int groups = kThreads / p.lanes, rows = 2 * a->heads;
+    p.block_rows = std::min(std::min(groups, rows), kBlockRows);
+    p.block_tokens = groups / p.block_rows;
+    // Two tokens to a thread where that leaves the SMs their blocks.
+    const unsigned grid_y = (unsigned)((rows + p.block_rows - 1) / p.block_rows);
+    const long long blocks = (a->tokens + (long long)p.block_tokens - 1) / p.block_tokens;
+    const int in_flight = blocks * grid_y >= 16LL * sm_count() ? 2 : 1;
+    const dim3 grid((unsigned)((blocks + in_flight - 1) / in_flight), grid_y);
+    static void (*const kernels[2][2][2])(CacheParams) = {{{cache_read_kernel<false, 1>, cache_read_kernel<false, 2>}, {cache_read_kernel<true, 1>, cache_read_kernel<true, 2>}},
+                                                          {{cache_write_kernel<false, 1>, cache_write_kernel<false, 2>}, {cache_write_kernel<true, 1>, cache_write_kernel<true, 2>}}};
+    const auto kernel = kernels[write][vec][in_flight - 1];
+    return cuda_status(launch_pdl(kernel, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(a->stream), p), where);
 }
 
 }  // namespace

@@ -1,8 +1,9 @@
 // Attention of drafted tokens (a tree of up to 64, or single tokens) over keys and values kept in int8 pages: softmax(scale q . k) v over the keys kept before and, of the drafted
 // tokens' own, those whose bit is set. Bound by reading the codes once where there are few rows.
 //
-// The queries and query heads of a K/V head are rows, 16 to a tile of mma.sync m16n8k16. Codes become halves exactly (three operations for four), the key's scale multiplies the
-// score, the value's scale the weight. Which features a step of the first product takes, and which the columns of the second are, is free: a lane has 16 neighbouring codes of a key
+// The queries and query heads of a K/V head are rows, eight to a tile of mma.sync m16n8k16: 16 keys x 8 rows of scores, then 16 features x 8 rows of O, so that no part of a tile is empty (with the
+// rows as the tile's 16, which four query heads fill to a quarter, twice the products). Codes become halves exactly (three operations for four), the key's scale multiplies the
+// score, the value's scale the weight. Which features a step of the first product takes, and which the rows of the second are, is free: a lane has 16 neighbouring codes of a key
 // of K, and for V of four keys the codes of kHD / 8 neighbouring features, so both come by wide loads, each lane's into a place of shared memory that only it reads
 // (cp.async, no barrier). A cluster of CTAs shares a sequence's keys, its warps take blocks of 16 in turn with a reference, sum and O of their own, joined in shared
 // and then distributed shared memory in a fixed order: no workspace, one launch, the same bits every time.
@@ -21,23 +22,24 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kKeys = 16;                 // of a block
-constexpr int kRows = 16;                 // of a tile
 constexpr int kMaxCluster = 16;
 constexpr float kRescaleStep = 8.f;       // log2 units
 
-template <int kHD>
+template <int kHD, int kX>
 struct Cfg {
+    static constexpr int kRows = 8 * kX;                         // of a CTA
     static constexpr int kFeat = kHD / 8;                        // features of V that a lane has
     static constexpr int kKLoads = 2 * (kHD / 64);               // of 16 bytes: two keys
     static constexpr int kVLoads = 4 * (kHD >= 128 ? kHD / 128 : 1);   // four keys, of 16 bytes (of 8 in heads of 64)
     static constexpr int kVBytes = kHD >= 128 ? 16 : 8;
-    static constexpr int kStages = kHD == 64 ? 5 : kHD == 128 ? 4 : 3;
-    // of a warp's stage: [load][lane]
-    static constexpr int kVAt = kKLoads * 512, kScaleAt = kVAt + kVLoads * 32 * kVBytes, kStage = kScaleAt + 4 * 32 * 8;
+    static constexpr int kStages = kHD == 64 ? 5 : 3;
+    // of a warp's stage: [load][lane], and the scales of 16 keys of K and of V
+    static constexpr int kVAt = kKLoads * 512, kScaleAt = kVAt + kVLoads * 32 * kVBytes, kStage = kScaleAt + 128;
     static constexpr int kRing = kStages * kStage;
-    static constexpr int kJoin = kWarps * (kRows * kHD + 2 * kRows) * 4;
-    static constexpr int kSumAt = kWarps * kRing > kJoin ? kWarps * kRing : kJoin;   // this CTA's rows: [kRows][kHD] floats, then references and sums
-    static constexpr int kBytes = kSumAt + (kRows * kHD + 2 * kRows) * 4;
+    static constexpr int kLine = kHD + 4;                        // of a row of O in shared memory, in floats: lanes write to different banks
+    static constexpr int kJoin = kWarps * (kRows * kLine + 2 * kRows) * 4;
+    static constexpr int kSumAt = kWarps * kRing > kJoin ? kWarps * kRing : kJoin;   // this CTA's rows: [kRows][kLine] floats, then references and sums
+    static constexpr int kBytes = kSumAt + (kRows * kLine + 2 * kRows) * 4;
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -53,12 +55,18 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <int kSize>
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from, int real) {
     if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(from), "r"(real), "n"(kSize) : "memory");
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
     return v;
+}
+// An 8 x 8 matrix of halves, two neighbours of row lane / 4 in each lane, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 // An infinite feature of a query makes its row not a number, as it does in 0 times infinity and in infinity - infinity.
 __device__ __forceinline__ uint32_t no_infinity(uint32_t two) {
@@ -66,11 +74,11 @@ __device__ __forceinline__ uint32_t no_infinity(uint32_t two) {
     return lo | hi;
 }
 
-// kHD: 64, 128 or 256, the head's width rounded up. kTall: more than eight rows; otherwise the lower half of the tile is empty and left out of everything but the products.
-template <int kHD, bool kTall>
-__global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_constant__ TreeParams p, int row_tiles, bool longest_first) {
-    using C = Cfg<kHD>;
-    constexpr int kX = kTall ? 2 : 1;     // rows of a lane: g and g + 8
+// kHD: 64, 128 or 256, the head's width rounded up. kX: tiles of eight rows.
+template <int kHD, int kX>
+__global__ void __launch_bounds__(kThreads, kHD == 256 || kX == 2 ? 1 : 4) attention_tree_kernel(const __grid_constant__ TreeParams p, int row_tiles, bool longest_first) {
+    using C = Cfg<kHD, kX>;
+    constexpr int kRows = C::kRows;
     extern __shared__ __align__(128) uint8_t smem[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     cg::cluster_group cluster = cg::this_cluster();
@@ -101,90 +109,116 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
     const int stride = csize * kWarps, mine = crank * kWarps + warp;
     const int* const table = p.table + (long long)b * p.table_width;
     const uint32_t ring = smem_u32(smem) + warp * C::kRing;
-    auto page_of = [&](int i) {
-        const int id = i < n_blocks ? __ldg(table + i * kKeys / p.page) : -1;
-        return id < p.pages ? id : -1;
+    // Where a block's 16 keys are, which lie in one page: its number is requested a block before it is needed. Blocks are looked up in turn (no division).
+    int page_id = -1, page_off = 0, next_n = mine * kKeys / p.page, next_off = mine * kKeys - next_n * p.page, next_i = mine;
+    const int step_n = stride * kKeys / p.page, step_off = stride * kKeys - step_n * p.page;
+    auto look_up = [&]() {
+        page_id = -1;
+        if (next_i < n_blocks) {
+            page_id = __ldg(table + next_n);
+            page_off = next_off;
+            next_i += stride;
+            next_n += step_n;
+            next_off += step_off;
+            if (next_off >= p.page) {
+                next_off -= p.page;
+                ++next_n;
+            }
+        }
     };
-    // Block i, which lies in page id: the lane's codes and scales.
-    auto fetch = [&](int i, int id, int stage) {
+    const long long v_rows = (long long)n_kv * p.page, page_rows = 2 * v_rows;   // from a key's K to its V; of a page
+    const long long page_codes = page_rows * hd;
+    // What the lane reads of a block (nothing behind the head's last feature), from the block's first code on: of K key g and 16 features in each 64, of V key 2t.
+    const int k_lane = g * hd + (t * 16 < hd ? t * 16 : 0), v_lane = 2 * t * hd + (g * C::kFeat < hd ? g * C::kFeat : 0);
+    const int8_t* const codes_k = p.codes + (long long)kv_head * p.page * hd + k_lane;
+    const int8_t* const codes_v = p.codes + (long long)kv_head * p.page * hd + v_rows * hd + v_lane;
+    const float* const scales_at = p.scales + (long long)kv_head * p.page + (lane >> 4) * v_rows + (lane & 15);
+    // The block that has been looked up: the lane's codes and a scale. Whether its page is there.
+    auto fetch = [&](int i, int stage) {
+        const bool there = page_id >= 0 && page_id < p.pages;
         if (i < n_blocks) {
             const uint32_t to = ring + stage * C::kStage + lane * 16;
-            const bool good = id >= 0;
-            const long long row_k = ((long long)max(id, 0) * 2 * n_kv + kv_head) * p.page + (i * kKeys) % p.page, row_v = row_k + (long long)n_kv * p.page;
-            const int8_t* const k = p.codes + row_k * hd;
-            const int8_t* const v = p.codes + row_v * hd;
+            const int id = there ? page_id : 0;
+            const long long from = id * page_codes + page_off * hd;
+            const int8_t* const k = codes_k + from;
+            const int8_t* const v = codes_v + from;
 #pragma unroll
             for (int n = 0; n < C::kKLoads; ++n) {
-                const int f = (n >> 1) * 64 + t * 16;
-                copy_async<16>(to + n * 512, f < hd ? k + ((n & 1) * 8 + g) * hd + f : k, good && f < hd ? 16 : 0);
+                const bool in = there && (n >> 1) * 64 + t * 16 < hd;
+                copy_async<16>(to + n * 512, k + (n & 1) * 8 * hd + (in ? (n >> 1) * 64 : 0), in ? 16 : 0);
             }
 #pragma unroll
             for (int n = 0; n < C::kVLoads; ++n) {
-                const int key = 2 * t + (n & 1) + ((n >> 1) & 1) * 8, f = g * C::kFeat + (n >> 2) * 16;
-                copy_async<C::kVBytes>(ring + stage * C::kStage + C::kVAt + (n * 32 + lane) * C::kVBytes, f < hd ? v + key * hd + f : v, good && f < hd ? C::kVBytes : 0);
+                const bool in = there && g * C::kFeat + (n >> 2) * 16 < hd;
+                copy_async<C::kVBytes>(to + C::kVAt - lane * (16 - C::kVBytes) + n * 32 * C::kVBytes, v + ((n & 1) + ((n >> 1) & 1) * 8) * hd + (in ? (n >> 2) * 16 : 0), in ? C::kVBytes : 0);
             }
-#pragma unroll
-            for (int n = 0; n < 4; ++n)
-                copy_async<8>(ring + stage * C::kStage + C::kScaleAt + (n * 32 + lane) * 8, p.scales + (n < 2 ? row_k : row_v) + (n & 1) * 8 + 2 * t, good ? 8 : 0);
+            copy_async<4>(to + C::kScaleAt - lane * 12, scales_at + (id * page_rows + page_off), there ? 4 : 0);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
+        return there;
     };
-    int id_next = -1, ids[C::kStages];    // of the blocks on their way
+    uint32_t there_bits = 0;              // of the blocks on their way, by stage
+    look_up();
 #pragma unroll
-    for (int n = 0; n < C::kStages - 1; ++n) ids[n] = page_of(mine + n * stride);
-    id_next = page_of(mine + (C::kStages - 1) * stride);
-#pragma unroll
-    for (int n = 0; n < C::kStages - 1; ++n) fetch(mine + n * stride, ids[n], n);
-    // the lane's rows
-    unsigned long long bits[kX];
-    bool real[kX];
-    uint32_t qf[kHD / 16][2 * kX];
+    for (int n = 0; n < C::kStages - 1; ++n) {
+        if (fetch(mine + n * stride, n)) there_bits |= 1u << n;
+        look_up();
+    }
+    // the lane's rows: in scores 8x + 2t and 8x + 2t + 1, as an operand 8x + g
+    unsigned long long bits[kX][2];
+    uint32_t qf[kX][kHD / 16][2];
 #pragma unroll
     for (int x = 0; x < kX; ++x) {
-        real[x] = g + 8 * x < rows;
-        const int r = tile * kRows + (real[x] ? g + 8 * x : 0), i = r / p.group, head = kv_head * p.group + r % p.group;
-        bits[x] = tree_bits(p, s, i);
-        const half* const q = p.q + (s.q0 + i) * p.q_pitch + (long long)head * hd;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) bits[x][e] = tree_bits(p, s, (tile * kRows + min(8 * x + 2 * t + e, rows - 1)) / p.group);
+        const bool real = 8 * x + g < rows;
+        const int r = tile * kRows + (real ? 8 * x + g : 0);
+        const half* const q = p.q + (s.q0 + r / p.group) * p.q_pitch + (long long)(kv_head * p.group + r % p.group) * hd;
 #pragma unroll
         for (int n = 0; n < kHD / 64; ++n) {   // 16 features of the lane in each 64, four to a step
             const int f = n * 64 + t * 16;
             uint4 a = make_uint4(0u, 0u, 0u, 0u), c = a;
-            if (f < hd && real[x]) {
+            if (f < hd && real) {
                 a = *reinterpret_cast<const uint4*>(q + f);
                 c = *reinterpret_cast<const uint4*>(q + f + 8);
             }
             const uint32_t w[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                qf[n * 4 + k][2 * x] = no_infinity(w[2 * k]);
-                qf[n * 4 + k][2 * x + 1] = no_infinity(w[2 * k + 1]);
+                qf[x][n * 4 + k][0] = no_infinity(w[2 * k]);
+                qf[x][n * 4 + k][1] = no_infinity(w[2 * k + 1]);
             }
         }
     }
-    float o[C::kFeat][4];
-#pragma unroll
-    for (int n = 0; n < C::kFeat; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-    float top[kX], sum[kX];
+    float o[kX][C::kFeat / 2][4];         // features 2i and 2i + 1 of the lane's, rows 2t and 2t + 1
+    float top[kX][2], sum[kX][2];
 #pragma unroll
     for (int x = 0; x < kX; ++x) {
-        top[x] = -INFINITY;
-        sum[x] = 0.f;
+#pragma unroll
+        for (int n = 0; n < C::kFeat / 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[x][n][i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            top[x][e] = -INFINITY;
+            sum[x][e] = 0.f;
+        }
     }
     int stage = 0, fill = C::kStages - 1;
     for (int i = mine; i < n_blocks; i += stride) {
-        fetch(i + (C::kStages - 1) * stride, id_next, fill);   // (the lane has read that stage a turn ago)
-        id_next = page_of(i + C::kStages * stride);
+        const bool next_there = fetch(i + (C::kStages - 1) * stride, fill);   // (the stage was left at the end of the turn before)
+        there_bits = (there_bits & ~(1u << fill)) | (next_there ? 1u : 0u) << fill;
+        look_up();
         asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+        __syncwarp();                     // (the scales come by all lanes)
         const uint32_t at = ring + stage * C::kStage;
         const int key0 = i * kKeys;
-        // ---- scores: the lane has keys 2t, 2t + 1, 2t + 8, 2t + 9 of its rows
-        float sc[2][4];
+        // ---- scores: the lane has keys g and g + 8 of its rows
+        float v[kX][4], v2[kX][4];        // key g: rows 2t, 2t + 1; key g + 8 (every other step, so that a product does not wait for the one before)
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int x = 0; x < kX; ++x)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
+            for (int e = 0; e < 4; ++e) v[x][e] = v2[x][e] = 0.f;
 #pragma unroll
         for (int n = 0; n < kHD / 64; ++n) {
             const uint4 k0 = lds128(at + (2 * n * 32 + lane) * 16), k1 = lds128(at + ((2 * n + 1) * 32 + lane) * 16);
@@ -192,121 +226,144 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t u0 = codes_biased(w0[k]), u1 = codes_biased(w1[k]);
-                const uint32_t(&a)[2 * kX] = qf[n * 4 + k];
-                const uint32_t a1 = kTall ? a[2 * kX - 2] : 0u, a3 = kTall ? a[2 * kX - 1] : 0u;
-                mma_16816(sc[0], a[0], a1, a[1], a3, codes_to_half2<0>(u0), codes_to_half2<1>(u0));
-                mma_16816(sc[1], a[0], a1, a[1], a3, codes_to_half2<0>(u1), codes_to_half2<1>(u1));
+                const uint32_t a0 = codes_to_half2<0>(u0), a1 = codes_to_half2<0>(u1), a2 = codes_to_half2<1>(u0), a3 = codes_to_half2<1>(u1);
+#pragma unroll
+                for (int x = 0; x < kX; ++x) mma_16816(k & 1 ? v2[x] : v[x], a0, a1, a2, a3, qf[x][n * 4 + k][0], qf[x][n * 4 + k][1]);
             }
         }
-        float ks[4], vs[4], lv[4];
+        float ks[2], vs[2], lv[2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const uint2 a = lds64(at + C::kScaleAt + (n * 32 + lane) * 8), c = lds64(at + C::kScaleAt + ((n + 2) * 32 + lane) * 8);
-            ks[2 * n] = __uint_as_float(a.x) * p.scale_log2;
-            ks[2 * n + 1] = __uint_as_float(a.y) * p.scale_log2;
-            vs[2 * n] = __uint_as_float(c.x);
-            vs[2 * n + 1] = __uint_as_float(c.y);
+        for (int e = 0; e < 2; ++e) {
+            ks[e] = __uint_as_float(lds32(at + C::kScaleAt + (g + 8 * e) * 4)) * p.scale_log2;
+            vs[e] = __uint_as_float(lds32(at + C::kScaleAt + 64 + (g + 8 * e) * 4));
+            lv[e] = log2_of_scale(vs[e]);
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) lv[e] = log2_of_scale(vs[e]);
-        float v[kX][4], scale[kX][4];
+        float scale[kX][4];
 #pragma unroll
         for (int x = 0; x < kX; ++x)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[x][e] = sc[e >> 1][2 * x + (e & 1)] * ks[e];
-                scale[x][e] = vs[e];
+                v[x][e] = (v[x][e] + v2[x][e]) * ks[e >> 1];
+                scale[x][e] = vs[e >> 1];
             }
         // masks, where not every row sees every key of the block
-        const bool no_page = __ldg(table + key0 / p.page) < 0 || __ldg(table + key0 / p.page) >= p.pages;
-        if (key0 + kKeys > s.kept || key0 + kKeys > s.klen || no_page) {
+        const bool there = (there_bits >> stage) & 1u;
+        if (key0 + kKeys > s.kept || key0 + kKeys > s.klen || !there) {
 #pragma unroll
             for (int x = 0; x < kX; ++x)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (no_page || !tree_sees(s, bits[x], key0 + (e >> 1) * 8 + 2 * t + (e & 1))) {   // (what is not seen may have any scale)
+                    if (!there || !tree_sees(s, bits[x][e & 1], key0 + g + (e >> 1) * 8)) {   // (what is not seen may have any scale)
                         v[x][e] = -INFINITY;
                         scale[x][e] = 0.f;
                     }
         }
-        float most[kX];
         bool grow = false;
+        float most[kX][2];
 #pragma unroll
-        for (int x = 0; x < kX; ++x) {
-            most[x] = fmaxf(fmaxf(v[x][0] + lv[0], v[x][1] + lv[1]), fmaxf(v[x][2] + lv[2], v[x][3] + lv[3]));
-            most[x] = fmaxf(most[x], __shfl_xor_sync(0xffffffffu, most[x], 1));
-            most[x] = fmaxf(most[x], __shfl_xor_sync(0xffffffffu, most[x], 2));
-            grow = grow || most[x] > top[x] + kRescaleStep;   // also true for the first finite score of a row
-        }
+        for (int x = 0; x < kX; ++x)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                most[x][e] = fmaxf(v[x][e] + lv[0], v[x][e + 2] + lv[1]);
+                grow = grow || most[x][e] > top[x][e] + kRescaleStep;   // also true for the first finite score of a row
+            }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-            for (int x = 0; x < kX; ++x) {
-                if (most[x] > top[x] + kRescaleStep) {
-                    const float keep = top[x] == -INFINITY ? 0.f : ex2_fast(top[x] - most[x]);
-                    top[x] = most[x];
-                    sum[x] *= keep;
+            for (int x = 0; x < kX; ++x)
 #pragma unroll
-                    for (int n = 0; n < C::kFeat; ++n) {
-                        o[n][2 * x] *= keep;
-                        o[n][2 * x + 1] *= keep;
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) most[x][e] = fmaxf(most[x][e], __shfl_xor_sync(0xffffffffu, most[x][e], d));
+                    if (most[x][e] > top[x][e] + kRescaleStep) {
+                        const float keep = top[x][e] == -INFINITY ? 0.f : ex2_fast(top[x][e] - most[x][e]);
+                        top[x][e] = most[x][e];
+                        sum[x][e] *= keep;
+#pragma unroll
+                        for (int n = 0; n < C::kFeat / 2; ++n) {
+                            o[x][n][e] *= keep;
+                            o[x][n][e + 2] *= keep;
+                        }
                     }
+                }
+        }
+        uint32_t w[kX][2];                // weights as an operand: of row g keys 2t, 2t + 1, then 2t + 8, 2t + 9
+#pragma unroll
+        for (int x = 0; x < kX; ++x) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float m = top[x][e & 1];
+                v[x][e] = ex2_fast(v[x][e] - (m == -INFINITY ? 0.f : m));
+                sum[x][e & 1] += v[x][e];
+                v[x][e] *= scale[x][e];
+            }
+            w[x][0] = transposed(pack2(v[x][0], v[x][1]));
+            w[x][1] = transposed(pack2(v[x][2], v[x][3]));
+        }
+        // ---- O: rows m and m + 8 of the product's tile are features 2i and 2i + 1 of lane m's
+#pragma unroll
+        for (int h = 0; h < C::kFeat / (C::kVBytes == 16 ? 16 : 8); ++h) {
+            uint32_t u[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t from = at + C::kVAt + ((h * 4 + k) * 32 + lane) * C::kVBytes;
+                if constexpr (C::kVBytes == 16) {
+                    const uint4 q = lds128(from);
+                    u[k][0] = codes_biased(q.x);
+                    u[k][1] = codes_biased(q.y);
+                    u[k][2] = codes_biased(q.z);
+                    u[k][3] = codes_biased(q.w);
+                } else {
+                    const uint2 q = lds64(from);
+                    u[k][0] = codes_biased(q.x);
+                    u[k][1] = codes_biased(q.y);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < C::kVBytes / 4; ++c) {   // four features
+                const uint32_t lo0 = __byte_perm(u[0][c], u[1][c], 0x5140), hi0 = __byte_perm(u[0][c], u[1][c], 0x7362);
+                const uint32_t lo1 = __byte_perm(u[2][c], u[3][c], 0x5140), hi1 = __byte_perm(u[2][c], u[3][c], 0x7362);
+                const int n = h * 8 + 2 * c;
+#pragma unroll
+                for (int x = 0; x < kX; ++x) {
+                    mma_16816(o[x][n], codes_to_half2<0>(lo0), codes_to_half2<1>(lo0), codes_to_half2<0>(lo1), codes_to_half2<1>(lo1), w[x][0], w[x][1]);
+                    mma_16816(o[x][n + 1], codes_to_half2<0>(hi0), codes_to_half2<1>(hi0), codes_to_half2<0>(hi1), codes_to_half2<1>(hi1), w[x][0], w[x][1]);
                 }
             }
         }
-        uint32_t w[2 * kX];   // weights: keys 2t, 2t + 1, then 2t + 8, 2t + 9 of a row
-#pragma unroll
-        for (int x = 0; x < kX; ++x) {
-            const float shift = top[x] == -INFINITY ? 0.f : top[x];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[x][e] = ex2_fast(v[x][e] - shift);
-                sum[x] += v[x][e];
-                v[x][e] *= scale[x][e];
-            }
-            w[2 * x] = pack2(v[x][0], v[x][1]);
-            w[2 * x + 1] = pack2(v[x][2], v[x][3]);
-        }
-        const uint32_t w1 = kTall ? w[2 * kX - 2] : 0u, w3 = kTall ? w[2 * kX - 1] : 0u;
-        // ---- O: step j of the lane's features is a tile of eight columns, column n the feature n kFeat + j
-#pragma unroll
-        for (int c = 0; c < C::kFeat / 4; ++c) {   // four features
-            uint32_t u[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) u[k] = codes_biased(lds32(at + C::kVAt + (((c >> 2) * 4 + k) * 32 + lane) * C::kVBytes + (c & 3) * 4));
-            const uint32_t lo0 = __byte_perm(u[0], u[1], 0x5140), hi0 = __byte_perm(u[0], u[1], 0x7362), lo1 = __byte_perm(u[2], u[3], 0x5140), hi1 = __byte_perm(u[2], u[3], 0x7362);
-            mma_16816(o[4 * c], w[0], w1, w[1], w3, codes_to_half2<0>(lo0), codes_to_half2<0>(lo1));
-            mma_16816(o[4 * c + 1], w[0], w1, w[1], w3, codes_to_half2<1>(lo0), codes_to_half2<1>(lo1));
-            mma_16816(o[4 * c + 2], w[0], w1, w[1], w3, codes_to_half2<0>(hi0), codes_to_half2<0>(hi1));
-            mma_16816(o[4 * c + 3], w[0], w1, w[1], w3, codes_to_half2<1>(hi0), codes_to_half2<1>(hi1));
-        }
+        __syncwarp();                     // the stage has been read
         stage = stage + 1 == C::kStages ? 0 : stage + 1;
         fill = fill + 1 == C::kStages ? 0 : fill + 1;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     // ---- the warps' rows are joined, then the CTAs'
 #pragma unroll
-    for (int x = 0; x < kX; ++x) {
-        sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 1);
-        sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 2);
-    }
+    for (int x = 0; x < kX; ++x)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) sum[x][e] += __shfl_xor_sync(0xffffffffu, sum[x][e], d);
     __syncthreads();
-    float* const warp_o = reinterpret_cast<float*>(smem);                      // [kWarps][kRows][kHD], features in the order of the columns
-    float* const warp_ms = warp_o + kWarps * kRows * kHD;                      // [kWarps][2][kRows]
-    float* const cta_o = reinterpret_cast<float*>(smem + C::kSumAt);           // [kRows][kHD]
-    float* const cta_ms = cta_o + kRows * kHD;                                 // [2][kRows]
+    float* const warp_o = reinterpret_cast<float*>(smem);                      // [kWarps][kRows][kLine], feature n of lane m's in column (n / 2) 16 + (n % 2) 8 + m
+    float* const warp_ms = warp_o + kWarps * kRows * C::kLine;                 // [kWarps][2][kRows]
+    float* const cta_o = reinterpret_cast<float*>(smem + C::kSumAt);           // [kRows][kLine]
+    float* const cta_ms = cta_o + kRows * C::kLine;                            // [2][kRows]
 #pragma unroll
-    for (int n = 0; n < C::kFeat; ++n)
+    for (int x = 0; x < kX; ++x)
 #pragma unroll
-        for (int x = 0; x < kX; ++x)
-            if (real[x]) *reinterpret_cast<float2*>(warp_o + (warp * kRows + g + 8 * x) * kHD + n * 8 + 2 * t) = make_float2(o[n][2 * x], o[n][2 * x + 1]);
-    if (t == 0) {
+        for (int e = 0; e < 2; ++e) {
+            const int r = 8 * x + 2 * t + e;
+            float* const line = warp_o + (warp * kRows + r) * C::kLine + g;
 #pragma unroll
-        for (int x = 0; x < kX; ++x) {
-            // (scores that are not numbers leave no reference: any finite one makes the part count below)
-            warp_ms[warp * 2 * kRows + g + 8 * x] = sum[x] == sum[x] ? top[x] : 0.f;
-            warp_ms[warp * 2 * kRows + kRows + g + 8 * x] = sum[x];
+            for (int n = 0; n < C::kFeat / 2; ++n) {
+                line[n * 16] = o[x][n][e];
+                line[n * 16 + 8] = o[x][n][e + 2];
+            }
+            if (g == 0) {
+                // (scores that are not numbers leave no reference: any finite one makes the part count below)
+                warp_ms[warp * 2 * kRows + r] = sum[x][e] == sum[x][e] ? top[x][e] : 0.f;
+                warp_ms[warp * 2 * kRows + kRows + r] = sum[x][e];
+            }
         }
-    }
     __syncthreads();
     auto saw = [](float m) { return m != -INFINITY; };   // (a part that has seen nothing has no reference)
     for (int e = threadIdx.x; e < rows * kHD; e += kThreads) {
@@ -319,11 +376,11 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
             const float part = warp_ms[w * 2 * kRows + r];
             if (saw(part)) {
                 const float f = ex2_fast(part - m);
-                v = fmaf(f, warp_o[(w * kRows + r) * kHD + c], v);
+                v = fmaf(f, warp_o[(w * kRows + r) * C::kLine + c], v);
                 l = fmaf(f, warp_ms[w * 2 * kRows + kRows + r], l);
             }
         }
-        cta_o[r * kHD + c] = v;
+        cta_o[r * C::kLine + c] = v;
         if (c == 0) {
             cta_ms[r] = m;
             cta_ms[kRows + r] = l;
@@ -338,13 +395,13 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < kMaxCluster; ++k) m = fmaxf(m, part_m[k]);
         for (int f = threadIdx.x; f < hd; f += kThreads) {
-            const int c = f % C::kFeat * 8 + f / C::kFeat;
+            const int n = f % C::kFeat, c = n / 2 * 16 + n % 2 * 8 + f / C::kFeat;
             float l = 0.f, v = 0.f;
 #pragma unroll
             for (int k = 0; k < kMaxCluster; ++k) {
                 if (saw(part_m[k])) {
                     const float x = ex2_fast(part_m[k] - m);
-                    v = fmaf(x, cluster.map_shared_rank(cta_o, k)[r * kHD + c], v);
+                    v = fmaf(x, cluster.map_shared_rank(cta_o, k)[r * C::kLine + c], v);
                     l = fmaf(x, cluster.map_shared_rank(cta_ms, k)[kRows + r], l);
                 }
             }
@@ -355,12 +412,12 @@ __global__ void __launch_bounds__(kThreads) attention_tree_kernel(const __grid_c
     cluster.sync();   // nobody leaves while its rows are read
 }
 
-template <int kHD, bool kTall>
+template <int kHD, int kX>
 cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, cudaStream_t st) {
-    const auto kernel = attention_tree_kernel<kHD, kTall>;
+    const auto kernel = attention_tree_kernel<kHD, kX>;
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] {
-        cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kHD>::kBytes);
+        cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kHD, kX>::kBytes);
         if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         return x;
     });
@@ -368,7 +425,7 @@ cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csiz
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * csize));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Cfg<kHD>::kBytes;
+    cfg.dynamicSmemBytes = Cfg<kHD, kX>::kBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -421,17 +478,17 @@ extern "C" int et_attention_tree(const et_attention_tree_args* a) {
 namespace et {
 
 int attention_tree_launch(const TreeParams& p, cudaStream_t st) {
-    const int row_tiles = (p.max_q_len * p.group + kRows - 1) / kRows;
+    const int all_rows = p.max_q_len * p.group, tiles = all_rows > 8 ? 2 : 1, row_tiles = (all_rows + 8 * tiles - 1) / (8 * tiles);
     const long long units = (long long)p.batch * (p.nhead / p.group) * row_tiles;
     if (units * kMaxCluster > 0x7fffffff) return fail(ET_ERR_INVALID, "et_attention_tree: too large");
-    // CTAs that share a sequence's keys: as many as give each warp a block, up to four CTAs to an SM; more than eight to a cluster (which not every
+    // CTAs that share a sequence's keys: as many as give each warp a block, up to eight CTAs to an SM (64 sequences of up to 8192 keys, 16 heads of 128 over 4, with clusters of two, four, eight:
+    // 109, 69, 84 us; two of eight warps to a CTA 67); more than eight to a cluster (which not every
     // place on the chip can hold at once) only where the SMs would not all have one.
     int csize = 1;
-    while (csize < kMaxCluster && (long long)csize * kWarps * kKeys < p.max_k_len && units * csize * 2 <= (csize < 8 ? 4 : 1) * sm_count()) csize *= 2;
-    const bool tall = p.max_q_len * p.group > 8;
-    const auto run = p.head_dim <= 64    ? (tall ? launch<64, true> : launch<64, false>)
-                     : p.head_dim <= 128 ? (tall ? launch<128, true> : launch<128, false>)
-                                         : (tall ? launch<256, true> : launch<256, false>);
+    while (csize < kMaxCluster && (long long)csize * kWarps * kKeys < p.max_k_len && units * csize * 2 <= (csize < 8 ? 8 : 1) * sm_count()) csize *= 2;
+    const auto run = p.head_dim <= 64    ? (tiles == 2 ? launch<64, 2> : launch<64, 1>)
+                     : p.head_dim <= 128 ? (tiles == 2 ? launch<128, 2> : launch<128, 1>)
+                                         : (tiles == 2 ? launch<256, 2> : launch<256, 1>);
     return cuda_status(run(p, row_tiles, units, csize, st), "et_attention_tree launch");
 }
 

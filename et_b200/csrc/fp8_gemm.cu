@@ -332,6 +332,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
 // ------------------------------------------------------------------------------------------ few tokens
 constexpr int kFewEpi = 8, kWWarp = 8, kXWarp = 9, kFewMma = 10, kFewThreads = 11 * 32;
 constexpr int kMaxPlaces = 8;
+constexpr int kScaleBlocks = 16;                  // blocks whose scales are fetched at once
 constexpr int kWTile = 128 * kBlock;              // 128 features of the weight
 
 struct FewShared {
@@ -339,7 +340,7 @@ struct FewShared {
     uint64_t acc_full[kMaxPlaces], acc_empty[kMaxPlaces];
     uint64_t received;
     uint32_t tmem_base;
-    __align__(16) float scales[kFewEpi][2][64];   // of a warp's columns, two blocks in turn
+    __align__(16) float scales[kScaleBlocks * 128];   // of the tokens and of the weight, multiplied: [block][token]
 };
 
 // Four words to the address `addr` of CTA `rank` of the cluster, which count towards the bytes that its barrier at `bar` waits for.
@@ -349,6 +350,7 @@ __device__ __forceinline__ void st_async_cluster(uint32_t addr, uint32_t bar, ui
                  "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3]))
                  : "memory");
 }
+__device__ __forceinline__ void few_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewEpi) : "memory"); }
 // A bounded wait like mbar_wait, for what other CTAs of the cluster have written.
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
 #pragma unroll 1
@@ -368,7 +370,7 @@ constexpr int kSmemPerColumn = 454;
 
 template <int kTokens, bool kGelu>
 __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ Fp8Params p,
-                                                                 int split) {
+                                                                 int log_split) {
     constexpr int kXTile = kTokens * kBlock, kStage = kWTile + kXTile;
     constexpr int kPlaces = few_places(kTokens);
     constexpr int kAlloc = kPlaces * kTokens;
@@ -377,9 +379,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
     uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     __shared__ FewShared shared;
     FewShared* const sh = &shared;
-    const int S = p.stages, own_cols = kTokens / split;
+    const int S = p.stages, split = 1 << log_split, own_cols = kTokens >> log_split, log_own = 31 - __clz(own_cols);
     const uint32_t ring = smem_u32(smem);
-    float4* const recv = reinterpret_cast<float4*>(smem + S * kStage);   // of the other shares, this CTA's columns: [share][four columns][row]
+    float4* const recv = reinterpret_cast<float4*>(smem + S * kStage);   // of each share, this CTA's columns: [share][four columns][row]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)cluster_rank(), tile = (int)blockIdx.x / split;
     const int n0 = (tile % p.tiles_n) * 128, t0 = (tile / p.tiles_n) * kTokens;
@@ -452,25 +454,20 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
         const int q = warp & 3, h = warp >> 2;
         const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + h * kCols;
         const float* const sw = p.w_scales + (long long)(n0 / kBlock) * p.k_blocks + kb0;
-        constexpr int kPer = (kCols + 31) / 32;   // columns of a lane, whose scales it fetches
         pdl_wait();
-        auto fetch = [&](int i, float (&v)[kPer]) {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int t = t0 + h * kCols + j * 32 + lane;
-                v[j] = j * 32 + lane < kCols && t < p.T ? __ldcg(p.x_scales + (long long)(kb0 + i) * p.T + t) * __ldg(sw + i) : 0.f;
-            }
-        };
-        float next[kPer];
-        if (kn > 0) fetch(0, next);
         for (int i = 0; i < kn; ++i) {
             const int place = i % kPlaces;
-            float* const mine = sh->scales[warp][i & 1];
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (j * 32 + lane < kCols) mine[j * 32 + lane] = next[j];
-            __syncwarp();
-            if (i + 1 < kn) fetch(i + 1, next);
+            const float* const mine = sh->scales + (i % kScaleBlocks) * kTokens + h * kCols;
+            if (i % kScaleBlocks == 0) {
+                if (i > 0) few_barrier();   // (the scales before have been read)
+                const int n = min(kScaleBlocks, kn - i) * kTokens;
+#pragma unroll 4
+                for (int e = tid; e < n; e += 32 * kFewEpi) {
+                    const int kb = i + e / kTokens, t = t0 + e % kTokens;
+                    sh->scales[e] = t < p.T ? __ldcg(p.x_scales + (long long)(kb0 + kb) * p.T + t) * __ldg(sw + kb) : 0.f;
+                }
+                few_barrier();
+            }
             ok = mbar_wait(&sh->acc_full[place], (uint32_t)(i / kPlaces) & 1u);
             if (!ok) break;
             tc_fence_after();
@@ -501,36 +498,37 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
     asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // every CTA of the cluster runs
     bool got = true;
     if (warp < kFewEpi) {
-        const int q = warp & 3, h = warp >> 2, row = q * 32 + lane;
+        const int row = (warp & 3) * 32 + lane, h = warp >> 2;
 #pragma unroll
         for (int c = 0; c < kCols; c += 4) {
-            const int col = h * kCols + c, dst = col / own_cols, g = (col - dst * own_cols) / 4;
-            if (dst == rank) continue;   // the same for the whole warp
-            const int share = rank < dst ? rank : rank - 1;
-            st_async_cluster(smem_u32(recv + ((size_t)share * (own_cols / 4) + g) * 128 + row), smem_u32(&sh->received), dst, acc + c);
+            const int col = h * kCols + c, dst = col >> log_own;
+            float4* const to = recv + (rank * (own_cols / 4) + ((col & (own_cols - 1)) >> 2)) * 128 + row;
+            if (dst == rank) *to = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);   // (the same for the whole warp)
+            else st_async_cluster(smem_u32(to), smem_u32(&sh->received), dst, acc + c);
         }
     }
     __syncwarp();
     asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this warp has sent everything
     if (warp < kFewEpi) {
+        few_barrier();
         if (split > 1) got = mbar_wait_cluster(smem_u32(&sh->received), 0);
         if (!got && lane == 0) atomicExch(p.err, 67);
-        const int q = warp & 3, h = warp >> 2, row = q * 32 + lane, n = n0 + row;
+        const int row = tid & 127, n = n0 + row;
         const float bias = __half2float(p.bias[n]);
-#pragma unroll
-        for (int c = 0; c < kCols; c += 4) {
-            const int col = h * kCols + c, dst = col / own_cols, g = (col - dst * own_cols) / 4;
-            if (dst != rank || t0 + col >= p.T) continue;
+        half* y = p.Y + (long long)(t0 + rank * own_cols) * p.y_pitch + n;
+        for (int g = tid >> 7; g < own_cols / 4; g += kFewEpi / 4) {
+            const int t = t0 + rank * own_cols + g * 4;
+            if (t >= p.T) break;
+            const float4* const from = recv + g * 128 + row;
             float v[4] = {0.f, 0.f, 0.f, 0.f};
             for (int k = 0; k < split; ++k) {   // in the order of the shares
-                float4 x = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-                if (k != rank) x = recv[((size_t)(k < rank ? k : k - 1) * (own_cols / 4) + g) * 128 + row];
+                const float4 x = from[k * (own_cols / 4) * 128];
                 v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
             }
             if (n < p.N) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (t0 + col + j < p.T) p.Y[(long long)(t0 + col + j) * p.y_pitch + n] = __float2half_rn(finish<kGelu>(v[j] + bias));
+                    if (t + j < p.T) y[(g * 4 + j) * p.y_pitch] = __float2half_rn(finish<kGelu>(v[j] + bias));
             }
         }
     }
@@ -574,11 +572,11 @@ namespace {
 struct Fp8Plan {
     int bn;        // > 0: pairs with tiles of bn features
     int tokens;    // few tokens: columns of a tile, and CTAs that share a tile's K
-    int split;
+    int log_split;
 };
 
 Fp8Plan fp8_plan(int T, int N, int k_blocks) {
-    Fp8Plan plan = {0, 0, 1};
+    Fp8Plan plan = {0, 0, 0};
     const int tiles_n = (N + 127) / 128;
     if (T > 256) {
         const int pairs = sm_count() / 2, m = (T + 255) / 256;
@@ -587,7 +585,7 @@ Fp8Plan fp8_plan(int T, int N, int k_blocks) {
     }
     plan.tokens = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
     const int tiles = tiles_n * ((T + plan.tokens - 1) / plan.tokens);
-    while (plan.split < 8 && plan.split * 2 <= k_blocks && plan.tokens / (plan.split * 2) >= 4 && tiles * plan.split * 2 <= sm_count()) plan.split *= 2;
+    while (plan.log_split < 3 && (2 << plan.log_split) <= k_blocks && (plan.tokens >> plan.log_split) >= 8 && (tiles << plan.log_split) * 2 <= sm_count()) ++plan.log_split;
     return plan;
 }
 
@@ -616,7 +614,8 @@ cudaError_t launch_pair(const CUtensorMap& tx, const CUtensorMap& tw, const CUte
 }
 
 template <int kTokens, bool kGelu>
-cudaError_t launch_few(const CUtensorMap& tx, const CUtensorMap& tw, Fp8Params p, int split, cudaStream_t st) {
+cudaError_t launch_few(const CUtensorMap& tx, const CUtensorMap& tw, Fp8Params p, int log_split, cudaStream_t st) {
+    const int split = 1 << log_split;
     constexpr int kStage = kWTile + kTokens * kBlock;
     const auto kernel = fp8_few_kernel<kTokens, kGelu>;
     static PerDeviceOnce once;
@@ -625,7 +624,7 @@ cudaError_t launch_few(const CUtensorMap& tx, const CUtensorMap& tw, Fp8Params p
     if (e != cudaSuccess) return e;
     p.tiles_n = (p.N + 127) / 128;
     p.tiles = (p.T + kTokens - 1) / kTokens * p.tiles_n;
-    const int recv = (split - 1) * (kTokens / split) * 128 * 4;
+    const int recv = kTokens * 128 * 4;   // of all shares, the CTA's columns
     p.stages = std::min({kMaxPlaces, (max_smem - 1024 - recv) / kStage, (p.k_blocks + split - 1) / split});
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(p.tiles * split));
@@ -640,7 +639,7 @@ cudaError_t launch_few(const CUtensorMap& tx, const CUtensorMap& tw, Fp8Params p
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, p, split);
+    return cudaLaunchKernelEx(&cfg, kernel, tx, tw, p, log_split);
 }
 
 template <bool kGelu>
@@ -653,10 +652,10 @@ int fp8_run(const et_fp8_weight* w, const Fp8Params& p, const Fp8Plan& plan, con
         if (!make_tmap_2d_f16(&ty, p.Y, (uint64_t)p.T, (uint64_t)p.N, (uint64_t)p.y_pitch, 32, kUnitCols, 64)) return fail(ET_ERR_CUDA, "et_fp8_linear: cuTensorMapEncodeTiled failed");
         e = plan.bn == 256 ? launch_pair<256, kGelu>(tx, w->map128, ty, p, st) : launch_pair<128, kGelu>(tx, w->map64, ty, p, st);
     } else {
-        e = plan.tokens == 16   ? launch_few<16, kGelu>(tx, w->map128, p, plan.split, st)
-            : plan.tokens == 32 ? launch_few<32, kGelu>(tx, w->map128, p, plan.split, st)
-            : plan.tokens == 64 ? launch_few<64, kGelu>(tx, w->map128, p, plan.split, st)
-                                : launch_few<128, kGelu>(tx, w->map128, p, plan.split, st);
+        e = plan.tokens == 16   ? launch_few<16, kGelu>(tx, w->map128, p, plan.log_split, st)
+            : plan.tokens == 32 ? launch_few<32, kGelu>(tx, w->map128, p, plan.log_split, st)
+            : plan.tokens == 64 ? launch_few<64, kGelu>(tx, w->map128, p, plan.log_split, st)
+                                : launch_few<128, kGelu>(tx, w->map128, p, plan.log_split, st);
     }
     return cuda_status(e, "et_fp8_linear launch");
 }

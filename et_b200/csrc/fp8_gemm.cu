@@ -575,18 +575,33 @@ struct Fp8Plan {
     int log_split;
 };
 
+// Clocks of a launch, fitted to 790 launches of 1 to 1700 tokens, seven shapes and every plan: the plan taken takes 0.8 % longer than the fastest in the mean, 18 % at most. A few-token
+// CTA's block costs its hand-overs or its copies (26 clocks a KB), a tile at its end 65 clocks a token (exchange and stores).
+// (64 x 4096 -> 4096, tiles of 64, four CTAs to a tile's K 6.7 us, of 16 10.9, pairs 14.2; 512 tokens pairs 15.4, tiles of 128 17.9.)
 Fp8Plan fp8_plan(int T, int N, int k_blocks) {
-    Fp8Plan plan = {0, 0, 0};
-    const int tiles_n = (N + 127) / 128;
-    if (T > 256) {
-        const int pairs = sm_count() / 2, m = (T + 255) / 256;
-        plan.bn = m * ((N + 255) / 256) >= pairs ? 256 : 128;
-        return plan;
+    Fp8Plan best = {0, 0, 0};
+    double least = 1e30;
+    auto take = [&](const Fp8Plan& plan, double cost) {
+        if (cost < least) {
+            least = cost;
+            best = plan;
+        }
+    };
+    auto waves = [](long long n, long long at_once) { return (double)((n + at_once - 1) / at_once); };
+    for (int bn : {128, 256}) {
+        const double w = waves((T + 255LL) / 256 * ((N + bn - 1) / bn), sm_count() / 2);
+        take({bn, 0, 0}, 4100.0 + w * (k_blocks * (bn == 128 ? 670.0 : 790.0) + 12.4 * bn));
     }
-    plan.tokens = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
-    const int tiles = tiles_n * ((T + plan.tokens - 1) / plan.tokens);
-    while (plan.log_split < 3 && (2 << plan.log_split) <= k_blocks && (plan.tokens >> plan.log_split) >= 8 && (tiles << plan.log_split) * 2 <= sm_count()) ++plan.log_split;
-    return plan;
+    if (T > 4096) return best;
+    for (int tokens : {16, 32, 64, 128})
+        for (int log_split = 0; log_split < 4 && (1 << log_split) <= k_blocks && (tokens >> log_split) >= 4; ++log_split) {
+            // CTAs of clusters that run at once: clusters do not straddle the groups of 16 to 20 SMs
+            const int at_once = log_split == 3 ? 14 * 8 : log_split == 2 ? 33 * 4 : sm_count();
+            const double w = waves((N + 127LL) / 128 * ((T + tokens - 1) / tokens) << log_split, at_once);
+            const int blocks = (k_blocks + (1 << log_split) - 1) >> log_split;
+            take({0, tokens, log_split}, 2950.0 + w * (blocks * std::max(577.0, 0.0257 * (kWTile + tokens * kBlock)) + 65.0 * tokens) + (w - 1) * 500.0);
+        }
+    return best;
 }
 
 template <int kBN, bool kGelu>

@@ -468,50 +468,50 @@ _kept8 = None
 
 
 def _torch_kept8():
-    """(e4m3, uint8, int8, int64) of torch."""
+    """(float16, float32, (float16,), (e4m3, uint8), int8, int64, lookups of the current device and of its stream)."""
     global _kept8
     if _kept8 is None:
         import torch
-        _kept8 = (torch.float8_e4m3fn, torch.uint8, torch.int8, torch.int64)
+        current, stream_of, f16, _, f32 = _torch_kept()
+        _kept8 = (f16, f32, (f16,), (torch.float8_e4m3fn, torch.uint8), torch.int8, torch.int64, current, stream_of)
     return _kept8
 
 
 def _rows(name, t, dtypes, shape, device):
     """(address, pitch) of rows with neighbouring elements that may be slices of wider ones."""
     if t.dtype in dtypes and t.get_device() == device and t.shape == shape:
+        if t.is_contiguous():
+            return t.data_ptr(), shape[1]
         pitch, step = t.stride()
-        if shape[0] <= 1:
-            pitch = shape[1]
         if step == 1 or shape[1] == 1:
-            return t.data_ptr(), pitch
+            return t.data_ptr(), pitch if shape[0] > 1 else shape[1]
     raise ValueError(f"{name}: {tuple(shape)} of {' or '.join(str(d) for d in dtypes)} on the current CUDA device ({device}) with neighbouring elements expected, "
                      f"not {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
 def _row_scales(scales, rows, width, f32, device):
-    if scales.dtype is not f32 or scales.get_device() != device or scales.shape != ((width + 127) // 128, rows) or not scales.is_contiguous():
-        raise ValueError(f"scales: contiguous float32 {((width + 127) // 128, rows)} on the current CUDA device ({device}) expected, not {scales.dtype} {tuple(scales.shape)} on {scales.device}")
-    return scales.data_ptr()
+    if scales.dtype is f32 and scales.get_device() == device and scales.shape == ((width + 127) // 128, rows) and scales.is_contiguous():
+        return scales.data_ptr()
+    raise ValueError(f"scales: contiguous float32 {((width + 127) // 128, rows)} on the current CUDA device ({device}) expected, not {scales.dtype} {tuple(scales.shape)} on {scales.device}")
 
 
 def skip_rmsnorm(out, x, skip, gamma, residual=None, scales=None, eps=1e-6, stream=None):
     """h = x + skip (skip may be None), out = h / sqrt(mean(h^2) + eps) * gamma for rows [rows, width] of float16, residual = h where it is given. Without scales
     out is float16; with scales float32 [ceil(width / 128), rows] it is e4m3 (or uint8), a scale for each 128 features of a row. Rows may be slices of wider ones; residual
     (and a float16 out) may be x or skip. Returns out."""
-    current, stream_of, f16, _, f32 = _kept or _torch_kept()
-    e4m3, u8, _, _ = _kept8 or _torch_kept8()
+    f16, f32, f16s, e4m3s, _, _, current, stream_of = _kept8 or _torch_kept8()
     device = current()
     shape = x.shape
     rows, width = shape
-    x_at, x_pitch = _rows("x", x, (f16,), shape, device)
-    skip_at = skip_pitch = residual_at = residual_pitch = scales_at = 0
-    if skip is not None:
-        skip_at, skip_pitch = _rows("skip", skip, (f16,), shape, device)
-    if residual is not None:
-        residual_at, residual_pitch = _rows("residual", residual, (f16,), shape, device)
-    if scales is not None:
+    x_at, x_pitch = _rows("x", x, f16s, shape, device)
+    skip_at, skip_pitch = (0, 0) if skip is None else _rows("skip", skip, f16s, shape, device)
+    residual_at, residual_pitch = (0, 0) if residual is None else _rows("residual", residual, f16s, shape, device)
+    if scales is None:
+        scales_at = 0
+        out_at, out_pitch = _rows("out", out, f16s, shape, device)
+    else:
         scales_at = _row_scales(scales, rows, width, f32, device)
-    out_at, out_pitch = _rows("out", out, (f16,) if scales is None else (e4m3, u8), shape, device)
+        out_at, out_pitch = _rows("out", out, e4m3s, shape, device)
     rc = (_entries or _lib()).et_skip_rmsnorm(_rmsnorm_args(
         out_at, x_at, skip_at, _array("gamma", gamma, f16, device, width), residual_at, scales_at, stream_of(device) if stream is None else stream.cuda_stream,
         out_pitch, x_pitch, skip_pitch, residual_pitch, rows, width, eps))
@@ -522,13 +522,12 @@ def skip_rmsnorm(out, x, skip, gamma, residual=None, scales=None, eps=1e-6, stre
 
 def quantise_rows(out, scales, x, stream=None):
     """Rows of float16 x [rows, width] as e4m3 (or uint8) out with a scale for each 128 features of a row in scales float32 [ceil(width / 128), rows]. Returns (out, scales)."""
-    current, stream_of, f16, _, f32 = _kept or _torch_kept()
-    e4m3, u8, _, _ = _kept8 or _torch_kept8()
+    _, f32, f16s, e4m3s, _, _, current, stream_of = _kept8 or _torch_kept8()
     device = current()
     shape = x.shape
     rows, width = shape
-    x_at, x_pitch = _rows("x", x, (f16,), shape, device)
-    out_at, out_pitch = _rows("out", out, (e4m3, u8), shape, device)
+    x_at, x_pitch = _rows("x", x, f16s, shape, device)
+    out_at, out_pitch = _rows("out", out, e4m3s, shape, device)
     rc = (_entries or _lib()).et_quantise_rows(_quantise_args(
         out_at, _row_scales(scales, rows, width, f32, device), x_at, stream_of(device) if stream is None else stream.cuda_stream, out_pitch, x_pitch, rows, width))
     if rc:
@@ -553,12 +552,11 @@ class Fp8Weight:
     def run(self, out, x, x_scales, gelu=None, stream=None):
         """out [tokens, out_feat] float16 = x . W^T + bias (then tanh-GELU), x [tokens, in_feat] e4m3 (or uint8) with x_scales float32 [ceil(in_feat / 128), tokens]; rows
         may be slices of wider ones."""
-        current, stream_of, f16, _, f32 = _kept or _torch_kept()
-        e4m3, u8, _, _ = _kept8 or _torch_kept8()
+        _, f32, f16s, e4m3s, _, _, current, stream_of = _kept8 or _torch_kept8()
         device = current()
         tokens = x.shape[0]
-        x_at, x_pitch = _rows("x", x, (e4m3, u8), (tokens, self.in_feat), device)
-        out_at, out_pitch = _rows("out", out, (f16,), (tokens, self.out_feat), device)
+        x_at, x_pitch = _rows("x", x, e4m3s, (tokens, self.in_feat), device)
+        out_at, out_pitch = _rows("out", out, f16s, (tokens, self.out_feat), device)
         rc = (_entries or _lib()).et_fp8_linear(_fp8_args(
             self._h.value or 0, out_at, x_at, _row_scales(x_scales, tokens, self.in_feat, f32, device), stream_of(device) if stream is None else stream.cuda_stream,
             out_pitch, x_pitch, tokens, 1 if (self.is_gelu if gelu is None else gelu) else 0))
@@ -586,22 +584,22 @@ class Fp8Weight:
 def _cache(codes, scales, i8, f32, device):
     """(pages, heads, rows of a page, head_dim) of a cache."""
     shape = codes.shape
-    if (codes.dtype is not i8 or scales.dtype is not f32 or codes.get_device() != device or scales.get_device() != device or len(shape) != 5 or shape[1] != 2
-            or scales.shape != shape[:4] or not codes.is_contiguous() or not scales.is_contiguous()):
-        raise ValueError(f"contiguous int8 codes [pages, 2, heads, page, head_dim] and float32 scales [pages, 2, heads, page] on the current CUDA device ({device}) expected, "
-                         f"not {codes.dtype} {tuple(codes.shape)} on {codes.device} and {scales.dtype} {tuple(scales.shape)} on {scales.device}")
-    return shape[0], shape[2], shape[3], shape[4]
+    if (codes.dtype is i8 and scales.dtype is f32 and codes.get_device() == device and scales.get_device() == device and len(shape) == 5 and shape[1] == 2
+            and scales.shape == shape[:4] and codes.is_contiguous() and scales.is_contiguous()):
+        pages, _, heads, page, head_dim = shape
+        return pages, heads, page, head_dim
+    raise ValueError(f"contiguous int8 codes [pages, 2, heads, page, head_dim] and float32 scales [pages, 2, heads, page] on the current CUDA device ({device}) expected, "
+                     f"not {codes.dtype} {tuple(codes.shape)} on {codes.device} and {scales.dtype} {tuple(scales.shape)} on {scales.device}")
 
 
 def _cache_call(entry, codes, scales, k, v, slots, stream):
-    current, stream_of, f16, i32, f32 = _kept or _torch_kept()
-    _, _, i8, _ = _kept8 or _torch_kept8()
+    f16, f32, f16s, _, i8, _, current, stream_of = _kept8 or _torch_kept8()
     device = current()
     pages, heads, page, head_dim = _cache(codes, scales, i8, f32, device)
     shape = (k.shape[0], heads * head_dim)
-    k_at, k_pitch = _rows("k", k, (f16,), shape, device)
-    v_at, v_pitch = _rows("v", v, (f16,), shape, device)
-    rc = entry(_cache_args(codes.data_ptr(), scales.data_ptr(), k_at, v_at, _array("slots", slots, i32, device, shape[0]),
+    k_at, k_pitch = _rows("k", k, f16s, shape, device)
+    v_at, v_pitch = _rows("v", v, f16s, shape, device)
+    rc = entry(_cache_args(codes.data_ptr(), scales.data_ptr(), k_at, v_at, _array("slots", slots, (_kept or _torch_kept())[3], device, shape[0]),
                            stream_of(device) if stream is None else stream.cuda_stream, k_pitch, v_pitch, shape[0], pages, heads, page, head_dim))
     if rc:
         check(rc)
@@ -624,16 +622,16 @@ def attention_tree(out, q, codes, scales, table, k_lens, tree=None, cu_seqlens=N
     """Attention of drafted tokens q [tokens, heads * head_dim] float16 over a cache (as kv_cache_write leaves it): table int32 [batch, pages of the longest], k_lens int32 [batch]
     keys, the drafted tokens' own the last of them. A token sees the keys before those and the drafted ones whose bit is set in tree int64 [tokens] (None: those up to
     itself). cu_seqlens int32 [batch + 1], or None: max_q_len tokens each. max_q_len (0: 1 without cu_seqlens, 64 with it) and max_k_len (0: all that the table has)."""
-    current, stream_of, f16, i32, f32 = _kept or _torch_kept()
-    _, _, i8, i64 = _kept8 or _torch_kept8()
+    f16, f32, f16s, _, i8, i64, current, stream_of = _kept8 or _torch_kept8()
+    i32 = (_kept or _torch_kept())[3]
     device = current()
     pages, heads, page, head_dim = _cache(codes, scales, i8, f32, device)
     shape = q.shape
     tokens, width = shape
     if not head_dim or not heads or width % head_dim:
         raise ValueError(f"q: whole heads of {head_dim} expected, not rows of {width}")
-    q_at, q_pitch = _rows("q", q, (f16,), shape, device)
-    out_at, out_pitch = _rows("out", out, (f16,), shape, device)
+    q_at, q_pitch = _rows("q", q, f16s, shape, device)
+    out_at, out_pitch = _rows("out", out, f16s, shape, device)
     batch, most = _matrix("table", table, i32, device)
     rc = (_entries or _lib()).et_attention_tree(_tree_args(
         out_at, q_at, codes.data_ptr(), scales.data_ptr(), table.data_ptr(), _array("k_lens", k_lens, i32, device, batch),

@@ -453,7 +453,7 @@ extern "C" int et_attention_tree(const et_attention_tree_args* a) {
     ET_REQUIRE(a->max_q_len <= 64, "et_attention_tree: at most 64 drafted tokens to a sequence");
     ET_REQUIRE(a->scale >= 0.f && a->scale < INFINITY, "et_attention_tree: scale must be a finite number, 0 for 1 / sqrt(head_dim)");
     ET_REQUIRE((long long)a->nhead * a->head_dim <= 0x7fffffff && (long long)a->nhead / a->nhead_kv * a->max_q_len <= 0x7fffff && (long long)a->batch * a->max_q_len <= 0x7fffffff &&
-                   a->max_k_len <= 0x7fffffff - 64,
+                   a->max_k_len <= 0x7ff00000,
                "et_attention_tree: too large");
     if (a->batch == 0 || a->q_tokens == 0 || a->max_q_len == 0) return ET_OK;
     ET_REQUIRE(a->out && a->q && a->k_lens, "et_attention_tree: null pointer");

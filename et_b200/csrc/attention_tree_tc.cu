@@ -141,23 +141,32 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         const int* const table = p.table + (long long)b * p.table_width;
         const uint32_t raw = at + C::kRawAt;
         const long long v_from_k = (long long)n_kv * p.page, v_codes = v_from_k * hd;   // from a key's K to its V
-        const int in_piece = (key_c & 15) * hd + f;
-        // The four 16 keys of a block, each in one page, a lane each (over and over): the page's number is requested a block before it is needed.
-        int piece_id = -1, piece_off = 0;
-        auto look_up = [&](int j) {
-            const int key = (crank + j * csize) * kKeys + (lane & 3) * 16;
+        const long long page_rows = 2 * v_from_k, page_codes = page_rows * hd;
+        // what the thread reads of a block, from the head's first row in a page on
+        const int8_t* const codes_at = p.codes + (long long)kv_head * p.page * hd + (key_c & 15) * hd + (f < hd ? f : 0);
+        const float* const scales_at = p.scales + (long long)kv_head * p.page + (key_s & 15) + side_s * v_from_k;
+        // The four 16 keys of a block, each in one page, a lane each (over and over): the page's number is requested a block before it is needed, places in turn (no division).
+        int piece_key = crank * kKeys + (lane & 3) * 16, piece_n = piece_key / p.page, next_off = piece_key - piece_n * p.page, piece_id = -1, piece_off = 0;
+        const int step = csize * kKeys, step_n = step / p.page, step_off = step - step_n * p.page;
+        auto look_up = [&]() {                                        // the next block
             piece_id = -1;
-            if (j < mine && key < s.klen) {
-                const int n = key / p.page;
-                piece_id = __ldg(table + n);
-                piece_off = key - n * p.page;
+            if (piece_key < s.klen) {
+                piece_id = __ldg(table + piece_n);
+                piece_off = next_off;
+                piece_key += step;
+                piece_n += step_n;
+                next_off += step_off;
+                if (next_off >= p.page) {
+                    next_off -= p.page;
+                    ++piece_n;
+                }
             }
         };
         uint32_t good_bits = 0;                                       // of eight blocks, four bits each
         auto fetch = [&](int j) {                                     // block j, whose pages have been looked up
             const bool there = piece_id >= 0 && piece_id < p.pages;
-            const long long row = there ? ((long long)piece_id * 2 * n_kv + kv_head) * p.page + piece_off : -1, start = row * hd;   // its first row, and its codes
-            look_up(j + 1);
+            const long long start = there ? piece_id * page_codes + piece_off * hd : -1, row = there ? piece_id * page_rows + piece_off : -1;
+            look_up();
             const uint32_t good = __ballot_sync(0xffffffffu, there) & 15u;
             good_bits = (good_bits & ~(15u << (4 * (j & 7)))) | good << (4 * (j & 7));
             if (j < mine) {
@@ -165,13 +174,13 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
 #pragma unroll
                 for (int n = 0; n < C::kChunks; ++n) {
                     const long long first = __shfl_sync(0xffffffffu, start, (key_c >> 4) + n * (8 / kPerKey));
-                    const bool real = first >= 0 && f < hd;
-                    const int8_t* const k = p.codes + (real ? first + in_piece : 0);
-                    copy_async<16>(to + n * 2048, k, real ? 16 : 0);
-                    copy_async<16>(to + (C::kChunks + n) * 2048, real ? k + v_codes : k, real ? 16 : 0);
+                    const int size = first >= 0 && f < hd ? 16 : 0;
+                    const int8_t* const k = codes_at + (first >= 0 ? first : 0);
+                    copy_async<16>(to + n * 2048, k, size);
+                    copy_async<16>(to + (C::kChunks + n) * 2048, k + v_codes, size);
                 }
                 const long long first = __shfl_sync(0xffffffffu, row, key_s >> 4);
-                copy_async<4>(raw + (j % C::kRawStages) * C::kRaw + 2 * C::kChunks * 2048 + c * 4, p.scales + (first >= 0 ? first + (key_s & 15) + side_s * v_from_k : 0), first >= 0 ? 4 : 0);
+                copy_async<4>(raw + (j % C::kRawStages) * C::kRaw + 2 * C::kChunks * 2048 + c * 4, scales_at + (first >= 0 ? first : 0), first >= 0 ? 4 : 0);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -188,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             sts128(line + (((chunk + swap) ^ (key & 7)) << 4), swap ? h[1] : h[0]);
             sts128(line + (((chunk + 1 - swap) ^ (key & 7)) << 4), swap ? h[0] : h[1]);
         };
-        look_up(0);
+        look_up();
         for (int n = 0; n < C::kRawStages - 1; ++n) fetch(n);
         for (int j = 0; j < mine; ++j) {
             fetch(j + C::kRawStages - 1);   // (the thread has read that place a turn ago)

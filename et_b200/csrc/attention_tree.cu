@@ -9,6 +9,7 @@
 // and then distributed shared memory in a fixed order: no workspace, one launch, the same bits every time.
 //
 // Scores, references and sums are fp32; the weights times the values' scales go to the second product as fp16 (half a step of 2^-11 of a weight).
+#include <algorithm>
 #include <cooperative_groups.h>
 #include "attention_tree.cuh"
 #include "attention_tree.h"
@@ -472,20 +473,28 @@ extern "C" int et_attention_tree(const et_attention_tree_args* a) {
     p.batch = a->batch; p.q_tokens = a->q_tokens; p.max_q_len = a->max_q_len; p.max_k_len = a->max_k_len;
     p.pages = a->pages; p.page = a->page; p.table_width = a->table_width;
     p.scale_log2 = (a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale) * 1.4426950408889634f;
-    return (attention_tree_tc_takes(p) ? attention_tree_tc_launch : attention_tree_launch)(p, static_cast<cudaStream_t>(a->stream));
+    const TreePlan few = attention_tree_plan(p), many = attention_tree_tc_plan(p);
+    return many.us < few.us ? attention_tree_tc_launch(p, many.csize, static_cast<cudaStream_t>(a->stream)) : attention_tree_launch(p, few.csize, static_cast<cudaStream_t>(a->stream));
 }
 
 namespace et {
 
-int attention_tree_launch(const TreeParams& p, cudaStream_t st) {
+TreePlan attention_tree_plan(const TreeParams& p) {
+    const int rows = p.max_q_len * p.group, tiles = rows > 8 ? 2 : 1;
+    const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + 8 * tiles - 1) / (8 * tiles));
+    const int blocks = std::max(1, (p.max_k_len + kKeys - 1) / kKeys);
+    const bool wide = p.head_dim > 64;
+    const double sm = sm_count() * (p.head_dim > 128 ? 1 : wide && tiles == 2 ? 3 : 4);
+    const double places[5] = {sm, sm, sm * (wide ? 0.91 : 0.86), sm * (wide ? 0.90 : 0.87), sm * (wide ? 0.74 : 0.5)};
+    // (heads above 128: twice a head of 128)
+    const double f = p.head_dim > 128 ? 2.0 : 1.0, second = tiles == 2 ? (wide ? 0.18 : 0.23) : 0.0;
+    return tree_plan(units, blocks, kWarps, 4, sm_count(), f * ((wide ? 0.53 : 0.30) + second), f * ((wide ? 1.17 : 0.80) + second), wide ? 11.1 : 6.8, wide ? 0.0 : 1.8, wide ? 0.0 : 0.09, places);
+}
+
+int attention_tree_launch(const TreeParams& p, int csize, cudaStream_t st) {
     const int all_rows = p.max_q_len * p.group, tiles = all_rows > 8 ? 2 : 1, row_tiles = (all_rows + 8 * tiles - 1) / (8 * tiles);
     const long long units = (long long)p.batch * (p.nhead / p.group) * row_tiles;
     if (units * kMaxCluster > 0x7fffffff) return fail(ET_ERR_INVALID, "et_attention_tree: too large");
-    // CTAs that share a sequence's keys: as many as give each warp a block, up to eight CTAs to an SM (64 sequences of up to 8192 keys, 16 heads of 128 over 4, with clusters of two, four, eight:
-    // 109, 69, 84 us; two of eight warps to a CTA 67); more than eight to a cluster (which not every
-    // place on the chip can hold at once) only where the SMs would not all have one.
-    int csize = 1;
-    while (csize < kMaxCluster && (long long)csize * kWarps * kKeys < p.max_k_len && units * csize * 2 <= (csize < 8 ? 8 : 1) * sm_count()) csize *= 2;
     const auto run = p.head_dim <= 64    ? (tiles == 2 ? launch<64, 2> : launch<64, 1>)
                      : p.head_dim <= 128 ? (tiles == 2 ? launch<128, 2> : launch<128, 1>)
                                          : (tiles == 2 ? launch<256, 2> : launch<256, 1>);

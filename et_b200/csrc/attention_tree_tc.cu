@@ -6,6 +6,11 @@
 // scores were, as the second product's A operand. A thread has a row: scale of the key, mask, weight times the value's scale, a running reference that moves when
 // it has to (then O is rescaled in tensor memory). Two CTAs share an SM: while one waits for its products the other takes exponentials. A cluster shares a sequence's keys; its CTAs' rows are joined
 // through distributed shared memory in a fixed order.
+//
+// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 154 us; codes read once 36. No unit is full (shared-memory pipe 41 %, ALU 37 %, issue slots 39 %, tensor pipe 25 %):
+// a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3400 clocks with two CTAs to an SM. Tried: two places for scores, Q in
+// shared memory (as tensor memory is full then), a warp of its own that issues UMMAs, registers handed over: 174 us, with codes fetched into registers 168 to 178 (operands from
+// shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182.
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "attention.h"
@@ -22,7 +27,7 @@ namespace {
 constexpr int kKeys = 64;                 // of a block
 constexpr int kRows = 128;                // of a CTA
 constexpr int kSoftmaxWarps = 4, kConvertWarps = 4, kThreads = 8 * 32;   // (two CTAs to an SM with 128 registers a thread)
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 16;
 constexpr int kScaleStages = 4, kScaleBytes = kKeys * (4 + 4 + 2);
 constexpr float kRescaleStep = 8.f;       // log2 units
 constexpr uint32_t kTmemCols = 256;
@@ -470,7 +475,11 @@ template <int kHD>
 cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
     const auto kernel = attention_tree_tc_kernel<kHD>;
     static PerDeviceOnce once;
-    const cudaError_t e = once.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kHD>::kBytes); });
+    const cudaError_t e = once.run([&] {
+        cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kHD>::kBytes);
+        if (x == cudaSuccess) x = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        return x;
+    });
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * csize));
@@ -491,17 +500,23 @@ cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csiz
 
 }  // namespace
 
-bool attention_tree_tc_takes(const TreeParams& p) { return p.head_dim <= 128 && p.max_q_len * p.group >= 32 && p.max_k_len >= 64; }
+TreePlan attention_tree_tc_plan(const TreeParams& p) {
+    if (p.head_dim > 128 || p.max_k_len < 1) return {1e30, 1};
+    const int rows = p.max_q_len * p.group;
+    const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + kRows - 1) / kRows);
+    const bool wide = p.head_dim > 64;
+    const double sm = 2.0 * sm_count(), part = (rows < kRows ? rows : kRows) / (double)kRows * (wide ? 0.61 : 0.25);   // of the rows
+    const double places[5] = {sm, sm, sm * (wide ? 0.89 : 0.93), sm * 0.86, sm * 0.54};
+    return tree_plan(units, (p.max_k_len + kKeys - 1) / kKeys, 1, 4, sm_count(), (wide ? 1.18 : 1.12) + part, (wide ? 1.36 : 1.08) + part, wide ? 8.2 : 8.1, wide ? 2.0 : 0.0, wide ? 0.1 : 0.0, places);
+}
 
-int attention_tree_tc_launch(const TreeParams& p, cudaStream_t st) {
+int attention_tree_tc_launch(const TreeParams& p, int csize, cudaStream_t st) {
     const int row_tiles = (p.max_q_len * p.group + kRows - 1) / kRows;
     const long long units = (long long)p.batch * (p.nhead / p.group) * row_tiles;
     if (units * kMaxCluster > 0x7fffffff) return fail(ET_ERR_INVALID, "et_attention_tree: too large");
     int* err = nullptr;
     const int rc = attn_err_address(&err);
     if (rc) return rc;
-    int csize = 1;
-    while (csize < kMaxCluster && csize * kKeys * 2 <= p.max_k_len && units * csize <= 4 * sm_count()) csize *= 2;
     return cuda_status((p.head_dim <= 64 ? launch<64> : launch<128>)(p, row_tiles, units, csize, err, st), "et_attention_tree launch");
 }
 

@@ -77,7 +77,7 @@ __device__ __forceinline__ uint32_t no_infinity(uint32_t two) {
 
 // kHD: 64, 128 or 256, the head's width rounded up. kX: tiles of eight rows.
 template <int kHD, int kX>
-__global__ void __launch_bounds__(kThreads, kHD == 256 || kX == 2 ? 1 : 4) attention_tree_kernel(const __grid_constant__ TreeParams p, int row_tiles, bool longest_first) {
+__global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) attention_tree_kernel(const __grid_constant__ TreeParams p, int row_tiles, bool longest_first) {
     using C = Cfg<kHD, kX>;
     constexpr int kRows = C::kRows;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -366,7 +366,6 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 || kX == 2 ? 1 : 4) atten
             }
         }
     __syncthreads();
-    auto saw = [](float m) { return m != -INFINITY; };   // (a part that has seen nothing has no reference)
     for (int e = threadIdx.x; e < rows * kHD; e += kThreads) {
         const int r = e / kHD, c = e % kHD;
         float m = -INFINITY, l = 0.f, v = 0.f;
@@ -375,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 || kX == 2 ? 1 : 4) atten
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const float part = warp_ms[w * 2 * kRows + r];
-            if (saw(part)) {
+            if (tree_saw(part)) {
                 const float f = ex2_fast(part - m);
                 v = fmaf(f, warp_o[(w * kRows + r) * C::kLine + c], v);
                 l = fmaf(f, warp_ms[w * 2 * kRows + kRows + r], l);
@@ -400,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 || kX == 2 ? 1 : 4) atten
             float l = 0.f, v = 0.f;
 #pragma unroll
             for (int k = 0; k < kMaxCluster; ++k) {
-                if (saw(part_m[k])) {
+                if (tree_saw(part_m[k])) {
                     const float x = ex2_fast(part_m[k] - m);
                     v = fmaf(x, cluster.map_shared_rank(cta_o, k)[r * C::kLine + c], v);
                     l = fmaf(x, cluster.map_shared_rank(cta_ms, k)[kRows + r], l);
@@ -482,13 +481,14 @@ namespace et {
 TreePlan attention_tree_plan(const TreeParams& p) {
     const int rows = p.max_q_len * p.group, tiles = rows > 8 ? 2 : 1;
     const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + 8 * tiles - 1) / (8 * tiles));
-    const int blocks = std::max(1, (p.max_k_len + kKeys - 1) / kKeys);
-    const bool wide = p.head_dim > 64;
-    const double sm = sm_count() * (p.head_dim > 128 ? 1 : wide && tiles == 2 ? 3 : 4);
-    const double places[5] = {sm, sm, sm * (wide ? 0.91 : 0.86), sm * (wide ? 0.90 : 0.87), sm * (wide ? 0.74 : 0.5)};
-    // (heads above 128: twice a head of 128)
-    const double f = p.head_dim > 128 ? 2.0 : 1.0, second = tiles == 2 ? (wide ? 0.18 : 0.23) : 0.0;
-    return tree_plan(units, blocks, kWarps, 4, sm_count(), f * ((wide ? 0.53 : 0.30) + second), f * ((wide ? 1.17 : 0.80) + second), wide ? 11.1 : 6.8, wide ? 0.0 : 1.8, wide ? 0.0 : 0.09, places);
+    const int turns = std::max(1, (p.max_k_len + kKeys * kWarps - 1) / (kKeys * kWarps));
+    const double sm = sm_count();
+    static const TreeCosts costs[2][2] = {{{0.39, 1.05, 5.6, 2.3, 4.0, {1.0, 1.1, 1.1}, 0.0}, {0.46, 0.92, 8.4, 1.7, 3.0, {1.1, 1.1, 1.1}, 0.0}},
+                                          {{0.61, 2.00, 5.9, 3.3, 4.0, {1.1, 1.1, 0.48}, 0.0}, {0.89, 1.47, 9.4, 3.3, 3.0, {1.1, 1.1, 1.1}, 0.0}}};
+    TreeCosts c = costs[p.head_dim > 64][tiles - 1];
+    if (p.head_dim > 128) c = {2 * c.alone, 2 * c.shared, c.start, c.start_shared, tiles == 2 ? 1.0 : 2.0, {1.0, 1.0, 0.44}, 0.0};   // (not fitted: twice a head of 128)
+    c.places *= sm;
+    return tree_plan(units, turns, sm_count(), c);
 }
 
 int attention_tree_launch(const TreeParams& p, int csize, cudaStream_t st) {

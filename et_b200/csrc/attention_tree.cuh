@@ -69,4 +69,7 @@ __device__ __forceinline__ float log2_of_scale(float s) {
     return y;
 }
 
+// A part of a row's sums counts if it has a reference (its scores may not be numbers: it is given one then); a part without one has seen nothing.
+__device__ __forceinline__ bool tree_saw(float reference) { return reference != -INFINITY; }
+
 }  // namespace et

@@ -5,9 +5,9 @@
 
 namespace et {
 
-// How CTAs share a sequence's keys, and what a launch takes in microseconds by a model fitted to 6500 launches (1 to 64 sequences of 200 to 16000 keys, 1 to 256 rows of a K/V head, heads
-// of 64, 96 and 128, every cluster): the kernel and the cluster taken so cost 4.5 % over the fastest in the mean (with rules of thumb, tcgen05 from 32 rows on and clusters that fill the SMs, it
-// was 26 %).
+// How CTAs share a sequence's keys, and what a launch takes in microseconds by a model fitted to 6200 launches (1 to 128 sequences of 200 to 16000 keys, all alike or ragged, 1 to 256 rows of
+// a K/V head, heads of 64, 96 and 128, every cluster): the kernel and the cluster taken so cost 4 % over the fastest in the mean, 25 % at the 95th percentile (with rules of thumb, tcgen05
+// from 32 rows on and clusters that fill the SMs, 26 and 100 %).
 struct TreePlan {
     double us;
     int csize;
@@ -18,21 +18,26 @@ int attention_tree_launch(const TreeParams& p, int csize, cudaStream_t st);
 TreePlan attention_tree_tc_plan(const TreeParams& p);
 int attention_tree_tc_launch(const TreeParams& p, int csize, cudaStream_t st);
 
-// units: clusters; blocks: of a sequence's keys, those of a CTA's share taking `alone` each, or `shared` where all places are taken; start: of a CTA; places: CTAs that run at once, by log2 of the
-// cluster's size.
-inline TreePlan tree_plan(long long units, int blocks, int per_turn, int max_log, int sms, double alone, double shared, double start, double fixed, double per_doubling, const double (&places)[5]) {
+// What the model says of one kernel: a turn (a CTA's blocks of keys that its warps take at once) takes `alone` or, where all places are taken, `shared`, and `rows` for what it has of them; a CTA
+// starts and ends in `start`, and up to `start_shared` more. places: CTAs that run at once, and the part of them that clusters of 4, 8, 16 find.
+struct TreeCosts {
+    double alone, shared, start, start_shared, places, part[3], rows;
+};
+// units: clusters; turns: of a sequence that one CTA has alone.
+inline TreePlan tree_plan(long long units, int turns, int sms, const TreeCosts& c) {
     TreePlan best = {1e30, 1};
-    for (int log = 0; log <= max_log; ++log) {
+    for (int log = 0; log <= 4; ++log) {
         const int csize = 1 << log;
-        if (log > 0 && (csize * per_turn >= 2 * blocks || (log == 4 && units * csize > sms))) break;   // (clusters of 16 find few places)
-        const double turns = (blocks + csize * per_turn - 1) / (csize * per_turn), load = units * csize / places[log];
-        double us = turns * alone + start;
-        if (load > 1.0) {
-            const double whole = (double)(long long)(load + 0.999999), many = 0.5 * (whole + load) * (turns * shared + start);
-            if (many > us) us = many;
-        }
-        us += fixed + per_doubling * log;
-        if (us < best.us) best = {us, csize};
+        if (log > 0 && (csize >= 2 * turns || (log == 4 && units * csize > sms))) break;   // (clusters of 16 find few places)
+        const double n = (turns + csize - 1) / csize, load = units * csize / (c.places * (log < 2 ? 1.0 : c.part[log - 2]));
+        auto least = [](double a, double b) { return a < b ? a : b; };
+        auto most = [](double a, double b) { return a > b ? a : b; };
+        const double start = c.start + c.start_shared * least(load, 1.0), waves = load > 1.0 ? 0.5 * (double)(long long)(load + 0.999999) + 0.5 * load : 1.0;
+        // sequences all as long as the longest, and ragged ones, half as long in the mean, the longest first
+        const double alike = waves * (n * (most(c.alone, c.shared * least(load, 1.0)) + c.rows) + start);
+        const double ragged = most(n * (most(c.alone, c.shared * least(0.92 * load, 1.0)) + c.rows) + start, load * (0.55 * n * (c.shared + c.rows) + start));
+        const double us = 0.25 * alike + 0.75 * ragged;
+        if (us < 1.02 * best.us) best = {us, csize};   // (as good: the larger cluster, for ragged ones)
     }
     return best;
 }

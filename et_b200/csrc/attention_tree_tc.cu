@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         for (int k = 0; k < kMaxCluster; ++k) m = fmaxf(m, part_m[k]);
 #pragma unroll
         for (int k = 0; k < kMaxCluster; ++k) {
-            if (part_m[k] != -INFINITY) {   // (a part that has seen nothing has no reference)
+            if (tree_saw(part_m[k])) {   // (a part that has seen nothing has no reference)
                 const uint8_t* const other = cluster.map_shared_rank(smem, k);
                 const float f = ex2_fast(part_m[k] - m);
                 const float4 o = *reinterpret_cast<const float4*>(other + r * kHD * 4 + ((chunk ^ (r & (kHD / 4 - 1))) << 4));
@@ -504,10 +504,9 @@ TreePlan attention_tree_tc_plan(const TreeParams& p) {
     if (p.head_dim > 128 || p.max_k_len < 1) return {1e30, 1};
     const int rows = p.max_q_len * p.group;
     const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + kRows - 1) / kRows);
-    const bool wide = p.head_dim > 64;
-    const double sm = 2.0 * sm_count(), part = (rows < kRows ? rows : kRows) / (double)kRows * (wide ? 0.61 : 0.25);   // of the rows
-    const double places[5] = {sm, sm, sm * (wide ? 0.89 : 0.93), sm * 0.86, sm * 0.54};
-    return tree_plan(units, (p.max_k_len + kKeys - 1) / kKeys, 1, 4, sm_count(), (wide ? 1.18 : 1.12) + part, (wide ? 1.36 : 1.08) + part, wide ? 8.2 : 8.1, wide ? 2.0 : 0.0, wide ? 0.1 : 0.0, places);
+    const double part = (rows < kRows ? rows : kRows) / (double)kRows, places = 2.0 * sm_count();
+    const TreeCosts narrow = {1.13, 1.44, 7.2, 3.7, places, {1.0, 1.0, 0.86}, 0.22 * part}, wide = {1.19, 1.84, 8.0, 5.3, places, {1.1, 1.1, 0.60}, 0.44 * part};
+    return tree_plan(units, (p.max_k_len + kKeys - 1) / kKeys, sm_count(), p.head_dim > 64 ? wide : narrow);
 }
 
 int attention_tree_tc_launch(const TreeParams& p, int csize, cudaStream_t st) {

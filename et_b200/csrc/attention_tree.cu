@@ -443,8 +443,10 @@ cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csiz
 }  // namespace
 }  // namespace et
 
-extern "C" int et_attention_tree(const et_attention_tree_args* a) {
-    using namespace et;
+namespace et {
+namespace {
+// kernel: 0 few rows, 1 many rows, below 0 the one that the model says, with its cluster.
+int tree_run(const et_attention_tree_args* a, int kernel, int csize) {
     ET_REQUIRE(a, "et_attention_tree: null pointer");
     ET_REQUIRE(a->batch >= 0 && a->q_tokens >= 0 && a->max_q_len >= 0 && a->max_k_len >= 0 && a->pages >= 0 && a->table_width >= 0, "et_attention_tree: negative size");
     ET_REQUIRE(a->nhead_kv > 0 && a->nhead > 0 && a->nhead % a->nhead_kv == 0, "et_attention_tree: nhead must be a multiple of nhead_kv");
@@ -472,8 +474,20 @@ extern "C" int et_attention_tree(const et_attention_tree_args* a) {
     p.batch = a->batch; p.q_tokens = a->q_tokens; p.max_q_len = a->max_q_len; p.max_k_len = a->max_k_len;
     p.pages = a->pages; p.page = a->page; p.table_width = a->table_width;
     p.scale_log2 = (a->scale == 0.f ? 1.f / sqrtf((float)a->head_dim) : a->scale) * 1.4426950408889634f;
+    const cudaStream_t st = static_cast<cudaStream_t>(a->stream);
+    if (kernel == 0) return attention_tree_launch(p, csize, st);
+    if (kernel == 1) return attention_tree_tc_launch(p, csize, st);
     const TreePlan few = attention_tree_plan(p), many = attention_tree_tc_plan(p);
-    return many.us < few.us ? attention_tree_tc_launch(p, many.csize, static_cast<cudaStream_t>(a->stream)) : attention_tree_launch(p, few.csize, static_cast<cudaStream_t>(a->stream));
+    return many.us < few.us ? attention_tree_tc_launch(p, many.csize, st) : attention_tree_launch(p, few.csize, st);
+}
+}  // namespace
+}  // namespace et
+
+extern "C" int et_attention_tree(const et_attention_tree_args* a) { return et::tree_run(a, -1, 1); }
+// Not part of the public header: one of the kernels with a cluster of 1 to 16, for tests that reach each of them.
+extern "C" int et_debug_attention_tree(const et_attention_tree_args* a, int kernel, int log_csize) {
+    if (!a || kernel < 0 || kernel > 1 || log_csize < 0 || log_csize > 4 || (kernel == 1 && a->head_dim > 128)) return et::fail(ET_ERR_INVALID, "et_debug_attention_tree: no such kernel");
+    return et::tree_run(a, kernel, 1 << log_csize);
 }
 
 namespace et {

@@ -257,23 +257,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
                 }
                 if (!mbar_wait(&sh->acc_full[slot], slot_ph)) return false;
                 tc_fence_after();
-                // the next 16 columns are on their way while 16 are added
-                uint32_t d[2][16];
-                tmem_ld16(from + slot * C::kSlotCols, d[0]);
 #pragma unroll
-                for (int i = 0; i < kCols; i += 16) {
-                    tmem_ld_wait(d[(i >> 4) & 1]);
-                    if (i + 16 < kCols) {
-                        tmem_ld16(from + slot * C::kSlotCols + i + 16, d[(i >> 4 & 1) ^ 1]);
-                    } else {   // the slot may be overwritten
+                for (int i = 0; i < kCols; i += 32) {
+                    uint32_t lo[16], hi[16];
+                    tmem_ld16(from + slot * C::kSlotCols + i, lo);
+                    tmem_ld16(from + slot * C::kSlotCols + i + 16, hi);
+                    tmem_ld_wait(lo, hi);
+                    if (i + 32 == kCols) {   // the slot may be overwritten
                         tc_fence_before();
                         __syncwarp();
                         if (elect_one()) mbar_arrive_cluster(empty_bar + slot * 8);
                     }
+                    const float f = C::kHalves == 2 && i >= 64 ? scale1 : scale0;
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float f = C::kHalves == 2 && i >= 64 ? scale1 : scale0;
-                        const float2 r = fma2(make_float2(__uint_as_float(d[(i >> 4) & 1][j]), __uint_as_float(d[(i >> 4) & 1][j + 1])), make_float2(f, f), make_float2(acc[i + j], acc[i + j + 1]));
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 d = j < 16 ? make_float2(__uint_as_float(lo[j]), __uint_as_float(lo[j + 1])) : make_float2(__uint_as_float(hi[j - 16]), __uint_as_float(hi[j - 15]));
+                        const float2 r = fma2(d, make_float2(f, f), make_float2(acc[i + j], acc[i + j + 1]));
                         acc[i + j] = r.x;
                         acc[i + j + 1] = r.y;
                     }
@@ -742,7 +741,7 @@ extern "C" int et_fp8_linear(const et_fp8_linear_args* a) {
     using namespace et;
     ET_REQUIRE(a && a->weight, "et_fp8_linear: null weight");
     const et_fp8_weight* const w = a->weight;
-    ET_REQUIRE(a->tokens >= 0, "et_fp8_linear: negative size");
+    ET_REQUIRE(a->tokens >= 0 && a->tokens <= 0x7ff00000, "et_fp8_linear: negative size, or more tokens than 32 bits number");
     if (a->tokens == 0) return ET_OK;
     ET_REQUIRE(a->y && a->x && a->x_scales, "et_fp8_linear: null pointer");
     const long long y_pitch = a->tokens == 1 ? (w->N + 7) / 8 * 8 : a->y_pitch, x_pitch = a->tokens == 1 ? w->K : a->x_pitch;

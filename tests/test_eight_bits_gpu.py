@@ -403,6 +403,51 @@ def test_trees(et, hq, hk, hd, drafts):
     check_tree(out, q, cache, counts, tree)
 
 
+def run_kernel(et, kernel, log_csize, out, q, cache, tree, cu, most, max_k_len=0):
+    """attention_tree by one of its kernels (0: few rows, 1: many) with clusters of 2^log_csize."""
+    import ctypes
+    from et_b200 import ops
+    p = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    batch, width = cache.table.shape
+    packed = ops._tree_args(p(out), p(q), p(cache.codes), p(cache.scales), p(cache.table), p(cache.k_lens), p(cu), p(tree), torch.cuda.current_stream().cuda_stream,
+                            out.stride(0), q.stride(0), q.shape[1] // cache.hd, cache.hk, cache.hd, batch, q.shape[0], most, max_k_len or width * cache.page, cache.pages, cache.page, width, 0.0)
+    et.check(et.lib().et_debug_attention_tree(ctypes.create_string_buffer(packed, len(packed)), kernel, log_csize))
+
+
+@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("log_csize", [0, 1, 2, 3, 4])
+@pytest.mark.parametrize("hq,hk,hd,most", [(2, 2, 16, 5), (6, 2, 32, 21), (8, 1, 48, 17), (4, 4, 64, 40), (8, 2, 80, 9), (4, 1, 96, 64), (3, 3, 112, 1), (8, 2, 128, 33), (2, 1, 256, 20)])
+def test_each_kernel_with_every_cluster(et, kernel, log_csize, hq, hk, hd, most):
+    if kernel == 1 and hd > 128:
+        return
+    counts = [most, 1, 0, (most + 1) // 2, most]
+    lengths = [700 + most, 1, 40, most, 2 * most + 63]
+    cache = Cache(lengths, hk, hd, 48, seed=hd)
+    cache.table[4, 0] = -7
+    q, tree = queries(counts + [2], hq, hd) * 2, random_tree(counts + [2], 2)
+    out = torch.full_like(q, 9.0)
+    run_kernel(et, kernel, log_csize, out, q, cache, tree, starts(counts), most)
+    assert (out[sum(counts):] == 9).all()
+    check_tree(out[:sum(counts)], q[:sum(counts)], cache, counts, tree[:sum(counts)])
+    again = torch.zeros_like(q)
+    run_kernel(et, kernel, log_csize, again, q, cache, tree, starts(counts), most)
+    assert torch.equal(again[:sum(counts)], out[:sum(counts)])
+    # what is not seen, in this kernel and cluster: anything, and a value that is not finite for those that see it
+    used = torch.zeros(cache.pages, cache.page, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(lengths):
+        at = torch.arange(n, device="cuda")
+        ids = cache.table[b, at // 48].long()
+        used[ids.clamp(0), at % 48] |= ids >= 0
+    cache.scales.masked_fill_(~used[:, None, None], float("nan"))
+    run_kernel(et, kernel, log_csize, again, q, cache, tree, starts(counts), most)
+    assert torch.equal(again[:sum(counts)], out[:sum(counts)])
+    page = int(cache.table[0, 10])     # key 500 of the first sequence, which all its tokens see
+    cache.scales[page, 1, :, 500 - 480] = float("inf")
+    run_kernel(et, kernel, log_csize, again, q, cache, tree, starts(counts), most)
+    assert not again[:most].isfinite().any() and torch.equal(again[most:sum(counts)], out[most:sum(counts)])
+    et.attention_check()
+
+
 @pytest.mark.parametrize("hq,hk,hd", [(12, 12, 64), (16, 4, 128), (8, 1, 80)])
 @pytest.mark.parametrize("tree", [True, False])
 def test_ragged(et, hq, hk, hd, tree):

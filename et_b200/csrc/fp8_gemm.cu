@@ -5,9 +5,9 @@
 // registers while the next block is multiplied into another place. Two kernels:
 //
 // fp8_pair_kernel, many tokens: persistent pairs of CTAs (cta_group::2), 256 tokens x kBN features to a tile. A thread has a token's row of kBN / 2 columns. 16384 x 4096 -> 4096:
-// 248 us (2.2e15 operations a second), with GELU 257. Of the ~900 clocks a block of 256 x 256 takes (UMMAs: 512) copies alone would take ~800 (the way from L2), sums and hand-overs
-// alone ~850. Tried, with and without the others' work: one warp that issues all UMMAs 244 / 253 us, four of them 248 / 256, sixteen warps that sum 255 / 266, eight with one
-// load from tensor memory at a time 260 / 275.
+// 244 us (2.2e15 operations a second), with GELU 254 (on random codes and for a quarter of a second 305: power). Of the ~900 clocks a block of 256 x 256 takes (UMMAs: 512) copies alone would take ~800 (the way from L2), sums and hand-overs
+// alone ~850. Tried: one warp that issues all UMMAs 244 / 253 us, four of them 248 / 256, sixteen warps that sum 255 / 266, eight with one
+// load from tensor memory at a time 260 / 275, waits by one lane of a warp 267, scales read behind the wait 269.
 //
 // fp8_few_kernel, few tokens: operands exchanged, 128 features are the tile's rows and kTokens tokens its columns, so that the weight, which is what has to
 // be read, fills the tile; K split over a cluster. Each CTA sends the others their columns' parts (asynchronous stores that count towards a barrier of the receiver) and
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
         const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (C::kHalves == 2 ? 0 : h * kCols);
         const uint32_t buf_at = epi + w * (kCols / kUnitCols) * kUnitBytes;
         const uint32_t to = buf_at + lane * 64, swizzle = (lane >> 1) & 3;   // row `lane`: four 16-byte chunks under the 64-byte swizzle
-        const uint32_t empty_bar = in_cta(smem_u32(&sh->acc_empty[0]), 0);
+        const uint32_t empty_bar = in_cta(smem_u32(&sh->acc_empty[0]), 0), acc_full = smem_u32(&sh->acc_full[0]);
         const int n_blocks = (p.N + kBlock - 1) / kBlock;
         bool ok = true;
         pdl_wait();
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
                     next0 = __ldg(sw0 + kb + 1);
                     if (C::kHalves == 2) next1 = __ldg(sw1 + kb + 1);
                 }
-                if (!mbar_wait(&sh->acc_full[slot], slot_ph)) return false;
+                if (!mbar_wait_at(acc_full + slot * 8, slot_ph)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < kCols; i += 32) {
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
                 }
                 few_barrier();
             }
-            ok = mbar_wait(&sh->acc_full[place], (uint32_t)(i / kPlaces) & 1u);
+            ok = mbar_wait_at(smem_u32(&sh->acc_full[place]), (uint32_t)(i / kPlaces) & 1u);
             if (!ok) break;
             tc_fence_after();
             constexpr int kStep = kCols < 16 ? kCols : 16;

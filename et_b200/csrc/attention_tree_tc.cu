@@ -9,7 +9,7 @@
 //
 // 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 154 us; codes read once 36. No unit is full (shared-memory pipe 41 %, ALU 37 %, issue slots 39 %, tensor pipe 25 %):
 // a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3400 clocks with two CTAs to an SM. Tried: two places for scores, Q in
-// shared memory (as tensor memory is full then), a warp of its own that issues UMMAs, registers handed over: 174 us, with codes fetched into registers 168 to 178 (operands from
+// shared memory (as tensor memory is full then), a warp of its own that issues UMMAs, registers handed over: 174 us (with Q in tensor memory and one place for scores 163), with codes fetched into registers 168 to 178 (operands from
 // shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182.
 #include <cooperative_groups.h>
 #include <type_traits>

@@ -465,6 +465,24 @@ def attention_rules(out, Q, K, V, head_dim, cu_seqlens=None, k_start=None, k_len
 # et_skip_rmsnorm_args, et_quantise_rows_args, et_fp8_linear_args, et_kv_cache_args and et_attention_tree_args as they lie in memory
 _rmsnorm_args, _quantise_args, _fp8_args, _cache_args, _tree_args = (struct.Struct(f).pack for f in ("@7P6if0P", "@4P4i0P", "@5P4i0P", "@6P7i0P", "@9P12if0P"))
 _kept8 = None
+_fast = None
+
+
+def _load_fast():
+    """The module that checks and packs the arguments of these calls in C++ (binding.cpp), or False where it has not been built: then, and where it does not take what it is given, the
+    checks below do it, which name what is wrong."""
+    global _fast
+    if _fast is None:
+        try:
+            import torch  # noqa: F401  (its libraries are loaded first)
+            from . import _binding
+        except ImportError:
+            _fast = False
+            return _fast
+        _binding.bind(*(ctypes.cast(lib()[name], ctypes.c_void_p).value for name in (
+            "et_skip_rmsnorm", "et_quantise_rows", "et_fp8_linear", "et_kv_cache_write", "et_kv_cache_read", "et_attention_tree")))
+        _fast = _binding
+    return _fast
 
 
 def _torch_kept8():
@@ -499,6 +517,13 @@ def skip_rmsnorm(out, x, skip, gamma, residual=None, scales=None, eps=1e-6, stre
     """h = x + skip (skip may be None), out = h / sqrt(mean(h^2) + eps) * gamma for rows [rows, width] of float16, residual = h where it is given. Without scales
     out is float16; with scales float32 [ceil(width / 128), rows] it is e4m3 (or uint8), a scale for each 128 features of a row. Rows may be slices of wider ones; residual
     (and a float16 out) may be x or skip. Returns out."""
+    fast = _fast if _fast is not None else _load_fast()
+    if fast:
+        rc = fast.skip_rmsnorm(out, x, skip, gamma, residual, scales, eps, None if stream is None else stream.cuda_stream)
+        if rc == 0:
+            return out
+        if rc > 0:
+            check(rc)
     f16, f32, f16s, e4m3s, _, _, current, stream_of = _kept8 or _torch_kept8()
     device = current()
     shape = x.shape
@@ -522,6 +547,13 @@ def skip_rmsnorm(out, x, skip, gamma, residual=None, scales=None, eps=1e-6, stre
 
 def quantise_rows(out, scales, x, stream=None):
     """Rows of float16 x [rows, width] as e4m3 (or uint8) out with a scale for each 128 features of a row in scales float32 [ceil(width / 128), rows]. Returns (out, scales)."""
+    fast = _fast if _fast is not None else _load_fast()
+    if fast:
+        rc = fast.quantise_rows(out, scales, x, None if stream is None else stream.cuda_stream)
+        if rc == 0:
+            return out, scales
+        if rc > 0:
+            check(rc)
     _, f32, f16s, e4m3s, _, _, current, stream_of = _kept8 or _torch_kept8()
     device = current()
     shape = x.shape
@@ -552,6 +584,14 @@ class Fp8Weight:
     def run(self, out, x, x_scales, gelu=None, stream=None):
         """out [tokens, out_feat] float16 = x . W^T + bias (then tanh-GELU), x [tokens, in_feat] e4m3 (or uint8) with x_scales float32 [ceil(in_feat / 128), tokens]; rows
         may be slices of wider ones."""
+        fast = _fast if _fast is not None else _load_fast()
+        if fast:
+            rc = fast.fp8_linear(self._h.value or 0, self.in_feat, self.out_feat, 1 if (self.is_gelu if gelu is None else gelu) else 0, out, x, x_scales,
+                                 None if stream is None else stream.cuda_stream)
+            if rc == 0:
+                return out
+            if rc > 0:
+                check(rc)
         _, f32, f16s, e4m3s, _, _, current, stream_of = _kept8 or _torch_kept8()
         device = current()
         tokens = x.shape[0]
@@ -592,7 +632,16 @@ def _cache(codes, scales, i8, f32, device):
                      f"not {codes.dtype} {tuple(codes.shape)} on {codes.device} and {scales.dtype} {tuple(scales.shape)} on {scales.device}")
 
 
-def _cache_call(entry, codes, scales, k, v, slots, stream):
+def _cache_call(write, codes, scales, k, v, slots, stream):
+    fast = _fast if _fast is not None else _load_fast()
+    if fast:
+        rc = fast.kv_cache(write, codes, scales, k, v, slots, None if stream is None else stream.cuda_stream)
+        if rc == 0:
+            return
+        if rc > 0:
+            check(rc)
+    entries = _entries or _lib()
+    entry = entries.et_kv_cache_write if write else entries.et_kv_cache_read
     f16, f32, f16s, _, i8, _, current, stream_of = _kept8 or _torch_kept8()
     device = current()
     pages, heads, page, head_dim = _cache(codes, scales, i8, f32, device)
@@ -608,13 +657,13 @@ def _cache_call(entry, codes, scales, k, v, slots, stream):
 def kv_cache_write(codes, scales, k, v, slots, stream=None):
     """Quantises rows of k and v [tokens, heads * head_dim] float16 into a cache: codes int8 [pages, 2, heads, page, head_dim], scales float32 [pages, 2, heads, page]. Row t
     goes to slots[t] (int32: page number * page + row; below 0: nowhere); slots differ. Returns (codes, scales)."""
-    _cache_call((_entries or _lib()).et_kv_cache_write, codes, scales, k, v, slots, stream)
+    _cache_call(True, codes, scales, k, v, slots, stream)
     return codes, scales
 
 
 def kv_cache_read(k, v, codes, scales, slots, stream=None):
     """Rows of a cache as float16: k and v [tokens, heads * head_dim], row t from slots[t] (below 0: left as it is). Returns (k, v)."""
-    _cache_call((_entries or _lib()).et_kv_cache_read, codes, scales, k, v, slots, stream)
+    _cache_call(False, codes, scales, k, v, slots, stream)
     return k, v
 
 
@@ -622,6 +671,13 @@ def attention_tree(out, q, codes, scales, table, k_lens, tree=None, cu_seqlens=N
     """Attention of drafted tokens q [tokens, heads * head_dim] float16 over a cache (as kv_cache_write leaves it): table int32 [batch, pages of the longest], k_lens int32 [batch]
     keys, the drafted tokens' own the last of them. A token sees the keys before those and the drafted ones whose bit is set in tree int64 [tokens] (None: those up to
     itself). cu_seqlens int32 [batch + 1], or None: max_q_len tokens each. max_q_len (0: 1 without cu_seqlens, 64 with it) and max_k_len (0: all that the table has)."""
+    fast = _fast if _fast is not None else _load_fast()
+    if fast:
+        rc = fast.attention_tree(out, q, codes, scales, table, k_lens, tree, cu_seqlens, max_q_len, max_k_len, scale, None if stream is None else stream.cuda_stream)
+        if rc == 0:
+            return out
+        if rc > 0:
+            check(rc)
     f16, f32, f16s, _, i8, i64, current, stream_of = _kept8 or _torch_kept8()
     i32 = (_kept or _torch_kept())[3]
     device = current()

@@ -17,6 +17,20 @@ def et():
     return et_b200
 
 
+def test_arguments_are_checked_and_packed_in_cpp(et):
+    from et_b200 import ops
+    assert ops._load_fast(), "et_b200/_binding.so is missing: run `python et_b200/build.py`"
+
+
+@pytest.fixture(params=["checked in C++", "checked in Python"])
+def both_ways(request, et, monkeypatch):
+    """What a call gives does not depend on who looks at its arguments."""
+    from et_b200 import ops
+    ops._load_fast()
+    if request.param == "checked in Python":
+        monkeypatch.setattr(ops, "_fast", False)
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
@@ -88,7 +102,7 @@ def test_norm(et, rows, width, pitch, shift, codes, skipped):
 @pytest.mark.parametrize("place", ["x", "skip"])
 @pytest.mark.parametrize("codes", [True, False])
 @pytest.mark.parametrize("width", [1024, 4096, 100])
-def test_norm_in_place(et, place, codes, width):
+def test_norm_in_place(both_ways, et, place, codes, width):
     g = gen(width)
     x, skip, gamma = normal(g, 9, width).half(), normal(g, 9, width).half(), normal(g, width).half()
     fresh, scales = torch.zeros_like(x), (torch.zeros(blocks(width), 9, device="cuda") if codes else None)
@@ -104,7 +118,7 @@ def test_norm_in_place(et, place, codes, width):
 
 
 @pytest.mark.parametrize("rows,width,pitch", [(1, 16, 16), (5, 127, 127), (64, 1024, 1024), (1000, 768, 776), (3, 16400, 16400), (2, 8192, 8192)])
-def test_quantise(et, rows, width, pitch):
+def test_quantise(both_ways, et, rows, width, pitch):
     g = gen(width)
     x = rows_of((normal(g, rows, width) * torch.exp(2 * normal(g, width))).half(), pitch)
     x[0, :64] = 0
@@ -175,7 +189,7 @@ def test_linear(et, k, n, tokens):
 
 @pytest.mark.parametrize("tokens", [1, 40, 100, 300, 5000])
 @pytest.mark.parametrize("bias", [True, False])
-def test_linear_gelu(et, tokens, bias):
+def test_linear_gelu(both_ways, et, tokens, bias):
     lin = Linear(et, 768, 528, bias=bias, gelu=True)
     x, s = lin.inputs(tokens)
     out = torch.zeros(tokens, 528, dtype=torch.float16, device="cuda")
@@ -196,7 +210,7 @@ def test_linear_large(et, k, n, tokens):
 
 
 @pytest.mark.parametrize("tokens", [1, 50, 400])
-def test_linear_of_slices(et, tokens):
+def test_linear_of_slices(both_ways, et, tokens):
     lin = Linear(et, 272, 176)
     x, s = lin.inputs(tokens)
     wide = torch.full((tokens, 200), 3.0, dtype=torch.float16, device="cuda")
@@ -220,7 +234,7 @@ def test_linear_rows_do_not_mix(et):
         assert out[3].isnan().all() and not out[4].isfinite().any() and torch.equal(out[rest], clean[rest])
 
 
-def test_linear_refuses(et):
+def test_linear_refuses(both_ways, et):
     lin = Linear(et, 64, 64)
     x, s = lin.inputs(4)
     out = torch.zeros(4, 64, dtype=torch.float16, device="cuda")
@@ -246,7 +260,7 @@ def quantised(x):
 
 @pytest.mark.parametrize("heads,hd,page,pages,tokens,shift,extra", [(1, 16, 16, 2, 1, 0, 0), (2, 64, 16, 40, 77, 0, 0), (3, 80, 32, 9, 100, 8, 64), (4, 128, 64, 30, 1000, 0, 0), (12, 64, 16, 70, 500, 0, 768),
                                                                     (1, 256, 48, 5, 33, 0, 0), (5, 96, 128, 3, 64, 0, 3), (2, 32, 16, 9, 20, 1, 0)])
-def test_cache(et, heads, hd, page, pages, tokens, shift, extra):
+def test_cache(both_ways, et, heads, hd, page, pages, tokens, shift, extra):
     g = gen(heads * hd)
     width = heads * hd
     rows = lambda: rows_of((normal(g, tokens, width) * torch.exp(normal(g, tokens, 1))).half(), width + extra, shift)  # noqa: E731
@@ -450,7 +464,7 @@ def test_each_kernel_with_every_cluster(et, kernel, log_csize, hq, hk, hd, most)
 
 @pytest.mark.parametrize("hq,hk,hd", [(12, 12, 64), (16, 4, 128), (8, 1, 80)])
 @pytest.mark.parametrize("tree", [True, False])
-def test_ragged(et, hq, hk, hd, tree):
+def test_ragged(both_ways, et, hq, hk, hd, tree):
     counts = [5, 0, 1, 40, 64, 3, 17]
     lengths = [200, 30, 1, 41, 64, 2000, 90]
     cache = Cache(lengths, hk, hd, 16, seed=3)
@@ -564,7 +578,7 @@ def test_pages_that_there_are_not(et, drafts, hq, hk, hd):
 
 
 @pytest.mark.parametrize("drafts", [1, 40])
-def test_keys_beyond_a_limit(et, drafts):
+def test_keys_beyond_a_limit(both_ways, et, drafts):
     lengths, counts = [300, 200], [drafts, drafts]
     cache = Cache(lengths, 2, 64, 16, seed=8)
     q = queries(counts, 8, 64)
@@ -588,7 +602,7 @@ def test_queries_that_are_not_finite(et, drafts, hq, hk, hd):
     assert out[0, :3 * hd].isnan().all() and torch.equal(out[0, 3 * hd:], clean[0, 3 * hd:]) and torch.equal(out[1:], clean[1:])
 
 
-def test_tree_of_slices(et):
+def test_tree_of_slices(both_ways, et):
     for drafts, hq, hk, hd in ((1, 4, 4, 64), (5, 8, 2, 128), (40, 8, 2, 128)):
         counts = [drafts] * 3
         cache = Cache([64, 65, 400], hk, hd, 16, seed=8)
@@ -622,7 +636,7 @@ def test_offsets_beyond_32_bits(et):
         check_tree(out, q, cache, [drafts])
 
 
-def test_tree_refuses(et):
+def test_tree_refuses(both_ways, et):
     cache = Cache([64, 65], 2, 64, 16)
     q = queries([2, 2], 4, 64)
     out = torch.zeros_like(q)
@@ -689,7 +703,7 @@ class Layer:
         return torch.cat([o[0] for o in outs]), torch.cat([o[1] for o in outs])
 
 
-def test_a_layer_of_them_together(et):
+def test_a_layer_of_them_together(both_ways, et):
     """A prompt goes in a token at a time into the cache, then a tree of drafted tokens: against the layer without roundings. Codes of e4m3 are off by 2^-4 at most, by some 2^-5.5 in the mean square;
     three linears behind one another, each with both operands' roundings averaged over its products, leave a few percent of the results' size."""
     layer = Layer(et)
@@ -773,3 +787,34 @@ def test_two_streams_at_once(et):
         assert torch.equal(b["f"], want[0]) and torch.equal(b["h"], want[1])
         for w in (layer.qkv, layer.o, layer.ffn):
             w.handle.check()
+
+
+def test_norm_refuses(both_ways, et):
+    x, gamma = torch.zeros(4, 256, dtype=torch.float16, device="cuda"), torch.ones(256, dtype=torch.float16, device="cuda")
+    codes, scales = torch.zeros(4, 256, dtype=torch.uint8, device="cuda"), torch.zeros(2, 4, device="cuda")
+    et.skip_rmsnorm(codes, x, None, gamma, scales=scales)
+    for args in [(x, x.float(), None, gamma), (x[:3], x, None, gamma), (codes, x, None, gamma), (x, x, x[:, :128], gamma), (x, x, None, gamma[:128]), (x, x, None, gamma.float()), (x, x.t(), None, gamma),
+                 (x, x.cpu(), None, gamma)]:
+        with pytest.raises(ValueError):
+            et.skip_rmsnorm(*args)
+    for bad in (scales.t(), scales[:1], scales.half()):
+        with pytest.raises(ValueError):
+            et.skip_rmsnorm(codes, x, None, gamma, scales=bad)
+        with pytest.raises(ValueError):
+            et.quantise_rows(codes, bad, x)
+    with pytest.raises(et.EtError):
+        et.skip_rmsnorm(x.clone(), x, None, gamma, eps=0.0)
+    out = x.clone()
+    with pytest.raises(et.EtError):
+        et.skip_rmsnorm(out, x, None, gamma, residual=out)
+
+
+def test_cache_refuses_tensors(both_ways, et):
+    codes, scales = torch.zeros(2, 2, 3, 16, 32, dtype=torch.int8, device="cuda"), torch.zeros(2, 2, 3, 16, device="cuda")
+    k, slots = torch.zeros(5, 96, dtype=torch.float16, device="cuda"), torch.arange(5, dtype=torch.int32, device="cuda")
+    et.kv_cache_write(codes, scales, k, k, slots)
+    for args in [(codes.view(torch.uint8), scales, k, k, slots), (codes, scales.half(), k, k, slots), (codes, scales[:1], k, k, slots), (codes, scales, k[:, :64], k, slots), (codes, scales, k, k[:4], slots),
+                 (codes, scales, k, k, slots.long()), (codes, scales, k, k, slots[:4]), (codes.transpose(3, 4), scales, k, k, slots), (codes, scales, k.cpu(), k, slots)]:
+        for call in (lambda c, s, a, b, i: et.kv_cache_write(c, s, a, b, i), lambda c, s, a, b, i: et.kv_cache_read(a, b, c, s, i)):
+            with pytest.raises(ValueError):
+                call(*args)

@@ -117,6 +117,16 @@ struct Call {
     }
 };
 
+// Calls the C ABI without Python's lock: a launch waits where the device's queue is full, for as long as what is queued takes.
+template <typename Args>
+PyObject* run(int (*entry)(const Args*), const Args& a) {
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = entry(&a);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 constexpr at::ScalarType kE4m3 = at::ScalarType::Float8_e4m3fn;
 PyObject* unsuitable() { return PyLong_FromLong(-1); }
 
@@ -137,7 +147,7 @@ PyObject* skip_rmsnorm(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.stream = c.stream;
     a.rows = (int)rows;
     a.width = (int)width;
-    return c.ok ? PyLong_FromLong(entries.skip_rmsnorm(&a)) : unsuitable();
+    return c.ok ? run(entries.skip_rmsnorm, a) : unsuitable();
 }
 
 // (out, scales, x, stream)
@@ -153,7 +163,7 @@ PyObject* quantise_rows(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.stream = c.stream;
     a.rows = (int)rows;
     a.width = (int)width;
-    return c.ok ? PyLong_FromLong(entries.quantise_rows(&a)) : unsuitable();
+    return c.ok ? run(entries.quantise_rows, a) : unsuitable();
 }
 
 // (weight, in_feat, out_feat, gelu, out, x, x_scales, stream)
@@ -172,7 +182,7 @@ PyObject* fp8_linear(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.stream = c.stream;
     a.tokens = (int)tokens;
     a.gelu = c.number(o[3]);
-    return c.ok ? PyLong_FromLong(entries.fp8_linear(&a)) : unsuitable();
+    return c.ok ? run(entries.fp8_linear, a) : unsuitable();
 }
 
 // (write, codes, scales, k, v, slots, stream)
@@ -195,7 +205,7 @@ PyObject* kv_cache(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.stream = c.stream;
     a.tokens = (int)tokens;
     const bool write = o[0] == Py_True;
-    return c.ok ? PyLong_FromLong((write ? entries.cache_write : entries.cache_read)(&a)) : unsuitable();
+    return c.ok ? run(write ? entries.cache_write : entries.cache_read, a) : unsuitable();
 }
 
 // (out, q, codes, scales, table, k_lens, tree, cu_seqlens, max_q_len, max_k_len, scale, stream)
@@ -234,7 +244,7 @@ PyObject* attention_tree(PyObject*, PyObject* const* o, Py_ssize_t n) {
         a.max_k_len = (int)(most * page);
     }
     a.scale = c.real(o[10]);
-    return c.ok ? PyLong_FromLong(entries.attention_tree(&a)) : unsuitable();
+    return c.ok ? run(entries.attention_tree, a) : unsuitable();
 }
 
 // Addresses of the C ABI's functions, in the order of Entries.

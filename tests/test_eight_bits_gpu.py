@@ -818,3 +818,32 @@ def test_cache_refuses_tensors(both_ways, et):
         for call in (lambda c, s, a, b, i: et.kv_cache_write(c, s, a, b, i), lambda c, s, a, b, i: et.kv_cache_read(a, b, c, s, i)):
             with pytest.raises(ValueError):
                 call(*args)
+
+
+def test_other_threads_run_while_a_launch_waits(both_ways, et):
+    """A launch that waits for room in the device's queue does not hold Python's lock."""
+    import threading
+    import time
+    x = torch.zeros(1, 128, dtype=torch.float16, device="cuda")
+    out, scales = torch.zeros(1, 128, dtype=torch.uint8, device="cuda"), torch.zeros(1, 1, device="cuda")
+    et.quantise_rows(out, scales, x)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    begin = time.perf_counter()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(2_000_000_000)      # a second or so
+
+    def launches():
+        for _ in range(4000):                 # more than the queue takes
+            et.quantise_rows(out, scales, x, stream=stream)
+
+    thread = threading.Thread(target=launches)
+    thread.start()
+    last, longest = time.perf_counter(), 0.0
+    while thread.is_alive():
+        time.sleep(0.001)
+        now = time.perf_counter()
+        longest, last = max(longest, now - last), now
+    torch.cuda.synchronize()
+    took = time.perf_counter() - begin
+    assert longest < 0.5 * took, f"this thread stood still for {longest:.2f} of {took:.2f} s"

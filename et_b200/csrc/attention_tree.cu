@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
         if (i < n_blocks) {
             const uint32_t to = ring + stage * C::kStage + lane * 16;
             const int id = there ? page_id : 0;
-            const long long from = id * page_codes + page_off * hd;
+            const long long from = id * page_codes + (long long)page_off * hd;
             const int8_t* const k = codes_k + from;
             const int8_t* const v = codes_v + from;
 #pragma unroll

@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         uint32_t good_bits = 0;                                       // of eight blocks, four bits each
         auto fetch = [&](int j) {                                     // block j, whose pages have been looked up
             const bool there = piece_id >= 0 && piece_id < p.pages;
-            const long long start = there ? piece_id * page_codes + piece_off * hd : -1, row = there ? piece_id * page_rows + piece_off : -1;
+            const long long start = there ? piece_id * page_codes + (long long)piece_off * hd : -1, row = there ? piece_id * page_rows + piece_off : -1;
             look_up();
             const uint32_t good = __ballot_sync(0xffffffffu, there) & 15u;
             good_bits = (good_bits & ~(15u << (4 * (j & 7)))) | good << (4 * (j & 7));

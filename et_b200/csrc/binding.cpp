@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <algorithm>
 #include <climits>
 #include "../../include/et_b200.h"
 
@@ -127,6 +128,7 @@ PyObject* run(int (*entry)(const Args*), const Args& a) {
     return PyLong_FromLong(rc);
 }
 
+constexpr int64_t kMostKeys = 0x7ff00000;   // that et_attention_tree takes
 constexpr at::ScalarType kE4m3 = at::ScalarType::Float8_e4m3fn;
 PyObject* unsuitable() { return PyLong_FromLong(-1); }
 
@@ -239,10 +241,7 @@ PyObject* attention_tree(PyObject*, PyObject* const* o, Py_ssize_t n) {
     a.max_q_len = c.number(o[8]);
     a.max_k_len = c.number(o[9]);
     if (a.max_q_len == 0) a.max_q_len = o[7] == Py_None ? 1 : 64;
-    if (a.max_k_len == 0) {
-        if (most * page > INT_MAX) return unsuitable();
-        a.max_k_len = (int)(most * page);
-    }
+    if (a.max_k_len == 0) a.max_k_len = (int)std::min<int64_t>(most * page, kMostKeys);
     a.scale = c.real(o[10]);
     return c.ok ? run(entries.attention_tree, a) : unsuitable();
 }

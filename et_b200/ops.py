@@ -693,7 +693,7 @@ def attention_tree(out, q, codes, scales, table, k_lens, tree=None, cu_seqlens=N
         out_at, q_at, codes.data_ptr(), scales.data_ptr(), table.data_ptr(), _array("k_lens", k_lens, i32, device, batch),
         0 if cu_seqlens is None else _array("cu_seqlens", cu_seqlens, i32, device, batch + 1), 0 if tree is None else _array("tree", tree, i64, device, tokens),
         stream_of(device) if stream is None else stream.cuda_stream, out_pitch, q_pitch, width // head_dim, heads, head_dim, batch, tokens,
-        max_q_len or (1 if cu_seqlens is None else 64), max_k_len or most * page, pages, page, most, scale))
+        max_q_len or (1 if cu_seqlens is None else 64), max_k_len or min(most * page, 0x7ff00000), pages, page, most, scale))
     if rc:
         check(rc)
     return out

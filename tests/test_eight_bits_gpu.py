@@ -636,6 +636,27 @@ def test_offsets_beyond_32_bits(et):
         check_tree(out, q, cache, [drafts])
 
 
+@pytest.mark.parametrize("drafts", [1, 48])
+def test_pages_of_more_than_31_bits(both_ways, et, drafts):
+    """One page of 16 million keys: the last ones lie beyond 2^31 codes of their page. The others' scores are 160 below these, so that their weights are 0 even in fp32."""
+    hd, group, page, n = 128, 4, (1 << 24) + 64, 64
+    codes = torch.zeros(1, 2, 1, page, hd, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(1, 2, 1, page, device="cuda")
+    k, v = (4 + 0.05 * normal(gen(1), n, hd)).half(), normal(gen(2), n, hd).half()
+    et.kv_cache_write(codes, scales, k, v, (page - n + torch.arange(n, device="cuda")).int())
+    last = Cache([n], 1, hd, n, spare=0)
+    last.codes.copy_(codes[:, :, :, page - n:])
+    last.scales.copy_(scales[:, :, :, page - n:])
+    k2, v2 = torch.zeros_like(k), torch.zeros_like(v)
+    et.kv_cache_read(k2, v2, codes, scales, (page - n + torch.arange(n, device="cuda")).int())
+    assert (k2 - k).abs().max() < 0.03 and (v2 - v).abs().max() < 0.03 and codes[:, :, :, :page - n].count_nonzero() == 0
+    q = (4 + 0.05 * normal(gen(3), drafts, group * hd)).half()
+    out = torch.zeros_like(q)
+    table = torch.zeros(1, 128, dtype=torch.int32, device="cuda")   # (of more keys than 31 bits count)
+    et.attention_tree(out, q, codes, scales, table, torch.tensor([page], dtype=torch.int32, device="cuda"), max_q_len=drafts)
+    check_tree(out, q, last, [drafts])
+
+
 def test_tree_refuses(both_ways, et):
     cache = Cache([64, 65], 2, 64, 16)
     q = queries([2, 2], 4, 64)

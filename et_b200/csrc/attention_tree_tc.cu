@@ -7,10 +7,11 @@
 // it has to (then O is rescaled in tensor memory). Two CTAs share an SM: while one waits for its products the other takes exponentials. A cluster shares a sequence's keys; its CTAs' rows are joined
 // through distributed shared memory in a fixed order.
 //
-// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 154 us; codes read once 36. No unit is full (shared-memory pipe 41 %, ALU 37 %, issue slots 39 %, tensor pipe 25 %):
-// a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3400 clocks with two CTAs to an SM. Tried: two places for scores, Q in
-// shared memory (as tensor memory is full then), a warp of its own that issues UMMAs, registers handed over: 174 us (with Q in tensor memory and one place for scores 163), with codes fetched into registers 168 to 178 (operands from
-// shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182.
+// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 153 us (158 with the scores' UMMAs in a loop that is not unrolled); codes read once 36. No unit is full
+// (shared-memory pipe 41 %, ALU 37 %, issue slots 39 %, tensor pipe 25 %): a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3300 clocks
+// with two CTAs to an SM. Tried: scores in halves of 32 keys, one multiplied while the other is weighed, by a warp of its own that issues UMMAs 165 (20 of them to a block instead of 12, some 45
+// clocks of the issuing thread each); two places for scores, Q in shared memory (as tensor memory is full then), such a warp, registers handed over 174 (with Q in tensor memory and one place 163),
+// with codes fetched into registers 168 to 178 (operands from shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182.
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "attention.h"
@@ -274,7 +275,9 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             if (!mbar_wait(&sh->k_full[j & 1], (uint32_t)(j >> 1) & 1u)) return false;
             tc_fence_after();
             const uint64_t kd = k_desc + (j & 1) * (C::kTile >> 4);
-            for (int ks = 0; ks < hd / 16; ++ks) umma_f16_ts(tmem + C::kSCol, tmem + C::kQCol + ks * 8, kd + ((ks >> 2) * C::kPanel + (ks & 3) * 32) / 16, idesc_qk, ks > 0);
+#pragma unroll
+            for (int ks = 0; ks < kHD / 16; ++ks)
+                if (ks * 16 < hd) umma_f16_ts(tmem + C::kSCol, tmem + C::kQCol + ks * 8, kd + ((ks >> 2) * C::kPanel + (ks & 3) * 32) / 16, idesc_qk, ks > 0);
             umma_commit(&sh->k_empty[j & 1]);
             umma_commit(&sh->s_full);
             return true;

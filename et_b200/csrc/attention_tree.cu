@@ -3,18 +3,23 @@
 //
 // The queries and query heads of a K/V head are rows, eight to a tile of mma.sync m16n8k16: 16 keys x 8 rows of scores, then 16 features x 8 rows of O, so that no part of a tile is empty (with the
 // rows as the tile's 16, which four query heads fill to a quarter, twice the products). Codes become halves exactly (three operations for four), the key's scale multiplies the
-// score, the value's scale the weight. Which features a step of the first product takes, and which the rows of the second are, is free: a lane has 16 neighbouring codes of a key
-// of K, and for V of four keys the codes of kHD / 8 neighbouring features, so both come by wide loads, each lane's into a place of shared memory that only it reads
-// (cp.async, no barrier). A cluster of CTAs shares a sequence's keys, its warps take blocks of 16 in turn with a reference, sum and O of their own, joined in shared
-// and then distributed shared memory in a fixed order: no workspace, one launch, the same bits every time.
+// score, the value's scale the weight. A block of 16 keys of a head lies in one page: K and V of it come by one TMA copy (16 x 128 bytes each, swizzled; heads of 256 by two) and their scales by
+// two small ones, a block or two ahead, into a ring that each warp has for itself (a lane's own pieces by cp.async, 60 instructions of all lanes to a block: 69 us where this takes 58, below).
+// Which features a step of the first product takes, and which the rows of the second are, is free: a lane has 16 neighbouring codes of a key of K, and for V of four keys the codes of 16 (8)
+// neighbouring features, by wide loads without bank conflicts. A cluster of CTAs shares a sequence's keys, its warps take blocks of 16 in turn with a reference, sum and O of their own,
+// joined in shared and then distributed shared memory in a fixed order: no workspace, one launch, the same bits every time.
+//
+// 64 sequences of up to 8192 keys, single tokens of 16 heads of 128 over 4: 58 us; codes read once 42.
 //
 // Scores, references and sums are fp32; the weights times the values' scales go to the second product as fp16 (half a step of 2^-11 of a weight).
 #include <algorithm>
 #include <cooperative_groups.h>
+#include "attention.h"
 #include "attention_tree.cuh"
 #include "attention_tree.h"
 #include "common.h"
 #include "ptx.cuh"
+#include "tmap.h"
 
 namespace cg = cooperative_groups;
 
@@ -30,17 +35,16 @@ template <int kHD, int kX>
 struct Cfg {
     static constexpr int kRows = 8 * kX;                         // of a CTA
     static constexpr int kFeat = kHD / 8;                        // features of V that a lane has
-    static constexpr int kKLoads = 2 * (kHD / 64);               // of 16 bytes: two keys
-    static constexpr int kVLoads = 4 * (kHD >= 128 ? kHD / 128 : 1);   // four keys, of 16 bytes (of 8 in heads of 64)
-    static constexpr int kVBytes = kHD >= 128 ? 16 : 8;
+    static constexpr int kRowBytes = kHD == 64 ? 64 : 128, kPanels = kHD / kRowBytes;   // of a key in shared memory, under a swizzle as wide
+    static constexpr int kSide = kKeys * kRowBytes;              // of K or V in a panel
     static constexpr int kStages = kHD == 64 ? 5 : 3;
-    // of a warp's stage: [load][lane], and the scales of 16 keys of K and of V
-    static constexpr int kVAt = kKLoads * 512, kScaleAt = kVAt + kVLoads * 32 * kVBytes, kStage = kScaleAt + 128;
-    static constexpr int kRing = kStages * kStage;
+    static constexpr int kStage = 2 * kPanels * kSide;           // of a warp: [panel][K, V][key]
+    static constexpr int kRing = kStages * kStage, kScaleAt = kWarps * kRing;           // then [warp][stage]: the scales of 16 keys of K and of V
+    static constexpr int kCopies = kScaleAt + kWarps * kStages * 128;
     static constexpr int kLine = kHD + 4;                        // of a row of O in shared memory, in floats: lanes write to different banks
     static constexpr int kJoin = kWarps * (kRows * kLine + 2 * kRows) * 4;
-    static constexpr int kSumAt = kWarps * kRing > kJoin ? kWarps * kRing : kJoin;   // this CTA's rows: [kRows][kLine] floats, then references and sums
-    static constexpr int kBytes = kSumAt + (kRows * kLine + 2 * kRows) * 4;
+    static constexpr int kSumAt = kCopies > kJoin ? kCopies : kJoin;   // this CTA's rows: [kRows][kLine] floats, then references and sums
+    static constexpr int kBytes = kSumAt + (kRows * kLine + 2 * kRows) * 4 + 1024;
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -52,11 +56,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// `size` bytes, of which `real` are read and the others are zeros.
-template <int kSize>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int real) {
-    if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(from), "r"(real), "n"(kSize) : "memory");
+// 16 keys of a head in a page, as far as a panel has their features, of K and of V.
+__device__ __forceinline__ void load_keys(uint32_t to, const void* tmap, int feature, int row, int head, int page_side, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(tmap), "r"(feature), "r"(row), "r"(head),
+                 "r"(page_side), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void load_scales(uint32_t to, const void* from, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 64, [%2];" ::"r"(to), "l"(from), "r"(bar) : "memory");
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 v;
@@ -77,10 +84,13 @@ __device__ __forceinline__ uint32_t no_infinity(uint32_t two) {
 
 // kHD: 64, 128 or 256, the head's width rounded up. kX: tiles of eight rows.
 template <int kHD, int kX>
-__global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) attention_tree_kernel(const __grid_constant__ TreeParams p, int row_tiles, bool longest_first) {
+__global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) attention_tree_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ TreeParams p, int row_tiles, bool longest_first,
+                                                                                                      int* err) {
     using C = Cfg<kHD, kX>;
     constexpr int kRows = C::kRows;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t bars[kWarps][C::kStages];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     cg::cluster_group cluster = cg::this_cluster();
     const int csize = cluster.num_blocks(), crank = cluster.block_rank();
@@ -90,6 +100,12 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
     unit /= row_tiles;
     const int n_kv = p.nhead / p.group, kv_head = unit % n_kv;
     int b = unit / n_kv;
+    if (lane == 0) {
+        for (int i = 0; i < C::kStages; ++i) mbar_init(&bars[warp][i], 1);
+        fence_mbar_init();
+        prefetch_tmap(&codes);
+    }
+    __syncwarp();
     pdl_wait();
     pdl_launch_dependents();
     if (longest_first) {   // the b-th sequence in order of length: the one that has b longer (or as long and earlier) ones
@@ -109,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
     const int n_blocks = (s.klen + kKeys - 1) / kKeys;
     const int stride = csize * kWarps, mine = crank * kWarps + warp;
     const int* const table = p.table + (long long)b * p.table_width;
-    const uint32_t ring = smem_u32(smem) + warp * C::kRing;
+    const uint32_t ring = smem_u32(smem) + warp * C::kRing, scales_ring = smem_u32(smem) + C::kScaleAt + warp * C::kStages * 128, bar0 = smem_u32(&bars[warp][0]);
     // Where a block's 16 keys are, which lie in one page: its number is requested a block before it is needed. Blocks are looked up in turn (no division).
     int page_id = -1, page_off = 0, next_n = mine * kKeys / p.page, next_off = mine * kKeys - next_n * p.page, next_i = mine;
     const int step_n = stride * kKeys / p.page, step_off = stride * kKeys - step_n * p.page;
@@ -127,35 +143,21 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
             }
         }
     };
-    const long long v_rows = (long long)n_kv * p.page, page_rows = 2 * v_rows;   // from a key's K to its V; of a page
-    const long long page_codes = page_rows * hd;
-    // What the lane reads of a block (nothing behind the head's last feature), from the block's first code on: of K key g and 16 features in each 64, of V key 2t.
-    const int k_lane = g * hd + (t * 16 < hd ? t * 16 : 0), v_lane = 2 * t * hd + (g * C::kFeat < hd ? g * C::kFeat : 0);
-    const int8_t* const codes_k = p.codes + (long long)kv_head * p.page * hd + k_lane;
-    const int8_t* const codes_v = p.codes + (long long)kv_head * p.page * hd + v_rows * hd + v_lane;
-    const float* const scales_at = p.scales + (long long)kv_head * p.page + (lane >> 4) * v_rows + (lane & 15);
-    // The block that has been looked up: the lane's codes and a scale. Whether its page is there.
+    const long long v_rows = (long long)n_kv * p.page;   // from a key's K to its V
+    const float* const scales_at = p.scales + (long long)kv_head * p.page;
+    // The block that has been looked up: its codes and scales. Whether its page is there.
     auto fetch = [&](int i, int stage) {
-        const bool there = page_id >= 0 && page_id < p.pages;
-        if (i < n_blocks) {
-            const uint32_t to = ring + stage * C::kStage + lane * 16;
-            const int id = there ? page_id : 0;
-            const long long from = id * page_codes + (long long)page_off * hd;
-            const int8_t* const k = codes_k + from;
-            const int8_t* const v = codes_v + from;
+        const bool there = i < n_blocks && page_id >= 0 && page_id < p.pages;
+        if (there && elect_one()) {
+            const uint32_t bar = bar0 + stage * 8, to = ring + stage * C::kStage;
+            mbar_expect_tx_at(bar, C::kStage + 128);
 #pragma unroll
-            for (int n = 0; n < C::kKLoads; ++n) {
-                const bool in = there && (n >> 1) * 64 + t * 16 < hd;
-                copy_async<16>(to + n * 512, k + (n & 1) * 8 * hd + (in ? (n >> 1) * 64 : 0), in ? 16 : 0);
-            }
-#pragma unroll
-            for (int n = 0; n < C::kVLoads; ++n) {
-                const bool in = there && g * C::kFeat + (n >> 2) * 16 < hd;
-                copy_async<C::kVBytes>(to + C::kVAt - lane * (16 - C::kVBytes) + n * 32 * C::kVBytes, v + ((n & 1) + ((n >> 1) & 1) * 8) * hd + (in ? (n >> 2) * 16 : 0), in ? C::kVBytes : 0);
-            }
-            copy_async<4>(to + C::kScaleAt - lane * 12, scales_at + (id * page_rows + page_off), there ? 4 : 0);
+            for (int n = 0; n < C::kPanels; ++n) load_keys(to + n * 2 * C::kSide, &codes, n * 128, page_off, kv_head, 2 * page_id, bar);
+            const float* const from = scales_at + page_id * 2 * v_rows + page_off;
+            load_scales(scales_ring + stage * 128, from, bar);
+            load_scales(scales_ring + stage * 128 + 64, from + v_rows, bar);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        __syncwarp();
         return there;
     };
     uint32_t there_bits = 0;              // of the blocks on their way, by stage
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
         const half* const q = p.q + (s.q0 + r / p.group) * p.q_pitch + (long long)(kv_head * p.group + r % p.group) * hd;
 #pragma unroll
         for (int n = 0; n < kHD / 64; ++n) {   // 16 features of the lane in each 64, four to a step
-            const int f = n * 64 + t * 16;
+            const int f = kHD == 64 ? t * 16 : n / 2 * 128 + t * 32 + n % 2 * 16;   // (of a panel: such that neighbouring lanes' pieces of K lie in different banks)
             uint4 a = make_uint4(0u, 0u, 0u, 0u), c = a;
             if (f < hd && real) {
                 a = *reinterpret_cast<const uint4*>(q + f);
@@ -205,14 +207,22 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
             sum[x][e] = 0.f;
         }
     }
+    bool ok = true;
+    uint32_t phases = 0;                  // of the stages' barriers
     int stage = 0, fill = C::kStages - 1;
     for (int i = mine; i < n_blocks; i += stride) {
         const bool next_there = fetch(i + (C::kStages - 1) * stride, fill);   // (the stage was left at the end of the turn before)
         there_bits = (there_bits & ~(1u << fill)) | (next_there ? 1u : 0u) << fill;
         look_up();
-        asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
-        __syncwarp();                     // (the scales come by all lanes)
-        const uint32_t at = ring + stage * C::kStage;
+        fill = fill + 1 == C::kStages ? 0 : fill + 1;
+        const int turn = stage;
+        stage = stage + 1 == C::kStages ? 0 : stage + 1;
+        if (!((there_bits >> turn) & 1u)) continue;   // keys in a page that there is not: nobody sees them
+        ok = mbar_wait_at(bar0 + turn * 8, (phases >> turn) & 1u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        phases ^= 1u << turn;
+        const uint32_t at = ring + turn * C::kStage, scales = scales_ring + turn * 128;
         const int key0 = i * kKeys;
         // ---- scores: the lane has keys g and g + 8 of its rows
         float v[kX][4], v2[kX][4];        // key g: rows 2t, 2t + 1; key g + 8 (every other step, so that a product does not wait for the one before)
@@ -222,7 +232,9 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
             for (int e = 0; e < 4; ++e) v[x][e] = v2[x][e] = 0.f;
 #pragma unroll
         for (int n = 0; n < kHD / 64; ++n) {
-            const uint4 k0 = lds128(at + (2 * n * 32 + lane) * 16), k1 = lds128(at + ((2 * n + 1) * 32 + lane) * 16);
+            // keys g and g + 8, whose rows' chunks lie in the same order
+            const uint32_t k_at = kHD == 64 ? at + g * 64 + ((t ^ (g >> 1 & 3)) << 4) : at + n / 2 * 2 * C::kSide + g * 128 + (((2 * t + n % 2) ^ g) << 4);
+            const uint4 k0 = lds128(k_at), k1 = lds128(k_at + 8 * C::kRowBytes);
             const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -235,8 +247,8 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
         float ks[2], vs[2], lv[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            ks[e] = __uint_as_float(lds32(at + C::kScaleAt + (g + 8 * e) * 4)) * p.scale_log2;
-            vs[e] = __uint_as_float(lds32(at + C::kScaleAt + 64 + (g + 8 * e) * 4));
+            ks[e] = __uint_as_float(lds32(scales + (g + 8 * e) * 4)) * p.scale_log2;
+            vs[e] = __uint_as_float(lds32(scales + 64 + (g + 8 * e) * 4));
             lv[e] = log2_of_scale(vs[e]);
         }
         float scale[kX][4];
@@ -248,13 +260,12 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
                 scale[x][e] = vs[e >> 1];
             }
         // masks, where not every row sees every key of the block
-        const bool there = (there_bits >> stage) & 1u;
-        if (key0 + kKeys > s.kept || key0 + kKeys > s.klen || !there) {
+        if (key0 + kKeys > s.kept || key0 + kKeys > s.klen) {
 #pragma unroll
             for (int x = 0; x < kX; ++x)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (!there || !tree_sees(s, bits[x][e & 1], key0 + g + (e >> 1) * 8)) {   // (what is not seen may have any scale)
+                    if (!tree_sees(s, bits[x][e & 1], key0 + g + (e >> 1) * 8)) {   // (what is not seen may have any scale)
                         v[x][e] = -INFINITY;
                         scale[x][e] = 0.f;
                     }
@@ -302,12 +313,13 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
         }
         // ---- O: rows m and m + 8 of the product's tile are features 2i and 2i + 1 of lane m's
 #pragma unroll
-        for (int h = 0; h < C::kFeat / (C::kVBytes == 16 ? 16 : 8); ++h) {
+        for (int h = 0; h < C::kPanels; ++h) {
             uint32_t u[4][4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const uint32_t from = at + C::kVAt + ((h * 4 + k) * 32 + lane) * C::kVBytes;
-                if constexpr (C::kVBytes == 16) {
+                const int key = 2 * t + (k & 1) + (k >> 1) * 8;
+                const uint32_t from = at + h * 2 * C::kSide + C::kSide + key * C::kRowBytes + (kHD == 64 ? ((g >> 1) ^ (key >> 1 & 3)) * 16 + (g & 1) * 8 : (g ^ (key & 7)) * 16);
+                if constexpr (kHD > 64) {
                     const uint4 q = lds128(from);
                     u[k][0] = codes_biased(q.x);
                     u[k][1] = codes_biased(q.y);
@@ -320,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
                 }
             }
 #pragma unroll
-            for (int c = 0; c < C::kVBytes / 4; ++c) {   // four features
+            for (int c = 0; c < (kHD == 64 ? 2 : 4); ++c) {   // four features
                 const uint32_t lo0 = __byte_perm(u[0][c], u[1][c], 0x5140), hi0 = __byte_perm(u[0][c], u[1][c], 0x7362);
                 const uint32_t lo1 = __byte_perm(u[2][c], u[3][c], 0x5140), hi1 = __byte_perm(u[2][c], u[3][c], 0x7362);
                 const int n = h * 8 + 2 * c;
@@ -332,10 +344,15 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
             }
         }
         __syncwarp();                     // the stage has been read
-        stage = stage + 1 == C::kStages ? 0 : stage + 1;
-        fill = fill + 1 == C::kStages ? 0 : fill + 1;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok) {   // (what was requested lands before the CTA leaves, bounded)
+        if (lane == 0) {
+            atomicExch(err, 28);
+            for (int n = 0; n < C::kStages; ++n)
+                if ((there_bits >> n) & 1u) mbar_wait_at(bar0 + n * 8, (phases >> n) & 1u);
+        }
+        __syncwarp();
+    }
     // ---- the warps' rows are joined, then the CTAs'
 #pragma unroll
     for (int x = 0; x < kX; ++x)
@@ -395,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
 #pragma unroll
         for (int k = 0; k < kMaxCluster; ++k) m = fmaxf(m, part_m[k]);
         for (int f = threadIdx.x; f < hd; f += kThreads) {
-            const int n = f % C::kFeat, c = n / 2 * 16 + n % 2 * 8 + f / C::kFeat;
+            const int n = kHD == 64 ? f % 8 : f / 128 * 16 + f % 16, c = n / 2 * 16 + n % 2 * 8 + (kHD == 64 ? f / 8 : f % 128 / 16);
             float l = 0.f, v = 0.f;
 #pragma unroll
             for (int k = 0; k < kMaxCluster; ++k) {
@@ -412,8 +429,23 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
     cluster.sync();   // nobody leaves while its rows are read
 }
 
+// The cache as [page and side][head][row][feature].
+bool make_tmap_codes(CUtensorMap* out, const TreeParams& p, int row_bytes) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const uint64_t hd = (uint64_t)p.head_dim, heads = (uint64_t)(p.nhead / p.group);
+    cuuint64_t dims[4] = {hd, (cuuint64_t)p.page, heads, 2 * (cuuint64_t)p.pages};
+    cuuint64_t strides[3] = {hd, hd * p.page, hd * p.page * heads};
+    cuuint32_t box[4] = {(cuuint32_t)row_bytes, kKeys, 1, 2};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(p.codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int kHD, int kX>
-cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, cudaStream_t st) {
+cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
+    CUtensorMap codes = {};
+    if (p.pages > 0 && p.codes && !make_tmap_codes(&codes, p, Cfg<kHD, kX>::kRowBytes)) return cudaErrorInvalidValue;
     const auto kernel = attention_tree_kernel<kHD, kX>;
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] {
@@ -437,7 +469,7 @@ cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csiz
     cfg.numAttrs = 2;
     // What outlasts a wave of CTAs is taken longest first, so that short sequences are left for the end.
     const bool longest_first = p.batch <= kThreads && units * csize > 2 * sm_count();
-    return cudaLaunchKernelEx(&cfg, kernel, p, row_tiles, longest_first);
+    return cudaLaunchKernelEx(&cfg, kernel, codes, p, row_tiles, longest_first, err);
 }
 
 }  // namespace
@@ -509,10 +541,13 @@ int attention_tree_launch(const TreeParams& p, int csize, cudaStream_t st) {
     const int all_rows = p.max_q_len * p.group, tiles = all_rows > 8 ? 2 : 1, row_tiles = (all_rows + 8 * tiles - 1) / (8 * tiles);
     const long long units = (long long)p.batch * (p.nhead / p.group) * row_tiles;
     if (units * kMaxCluster > 0x7fffffff) return fail(ET_ERR_INVALID, "et_attention_tree: too large");
+    int* err = nullptr;
+    const int rc = attn_err_address(&err);
+    if (rc) return rc;
     const auto run = p.head_dim <= 64    ? (tiles == 2 ? launch<64, 2> : launch<64, 1>)
                      : p.head_dim <= 128 ? (tiles == 2 ? launch<128, 2> : launch<128, 1>)
                                          : (tiles == 2 ? launch<256, 2> : launch<256, 1>);
-    return cuda_status(run(p, row_tiles, units, csize, st), "et_attention_tree launch");
+    return cuda_status(run(p, row_tiles, units, csize, err, st), "et_attention_tree launch");
 }
 
 }  // namespace et

@@ -3,8 +3,9 @@
 //
 // The queries and query heads of a K/V head are rows, eight to a tile of mma.sync m16n8k16: 16 keys x 8 rows of scores, then 16 features x 8 rows of O, so that no part of a tile is empty (with the
 // rows as the tile's 16, which four query heads fill to a quarter, twice the products). Codes become halves exactly (three operations for four), the key's scale multiplies the
-// score, the value's scale the weight. A block of 16 keys of a head lies in one page: K and V of it come by one TMA copy (16 x 128 bytes each, swizzled; heads of 256 by two) and their scales by
-// two small ones, a block or two ahead, into a ring that each warp has for itself (a lane's own pieces by cp.async, 60 instructions of all lanes to a block: 69 us where this takes 58, below).
+// score, the value's scale the weight. A block of 16 keys of a head lies in one page: K and V of it come by one TMA copy (16 x 128 bytes each, swizzled; heads of 256 by two),
+// a block or two ahead, into a ring that each warp has for itself. (Each lane's pieces by cp.async, 60 instructions of all lanes to a block, took 69 us where this takes 58, below; heads of up to 64,
+// whose copies are half as large, are 6 to 9 % faster that way and have it.)
 // Which features a step of the first product takes, and which the rows of the second are, is free: a lane has 16 neighbouring codes of a key of K, and for V of four keys the codes of 16 (8)
 // neighbouring features, by wide loads without bank conflicts. A cluster of CTAs shares a sequence's keys, its warps take blocks of 16 in turn with a reference, sum and O of their own,
 // joined in shared and then distributed shared memory in a fixed order: no workspace, one launch, the same bits every time.
@@ -35,16 +36,17 @@ template <int kHD, int kX>
 struct Cfg {
     static constexpr int kRows = 8 * kX;                         // of a CTA
     static constexpr int kFeat = kHD / 8;                        // features of V that a lane has
-    static constexpr int kRowBytes = kHD == 64 ? 64 : 128, kPanels = kHD / kRowBytes;   // of a key in shared memory, under a swizzle as wide
-    static constexpr int kSide = kKeys * kRowBytes;              // of K or V in a panel
-    static constexpr int kStages = kHD == 64 ? 5 : 3;
-    static constexpr int kStage = 2 * kPanels * kSide;           // of a warp: [panel][K, V][key]
+    static constexpr bool kTma = kHD > 64;
+    static constexpr int kPanels = kTma ? kHD / 128 : 1;         // of 128 bytes of a key in shared memory, swizzled
+    static constexpr int kSide = kKeys * (kTma ? 128 : 64);      // of K or V in a panel
+    static constexpr int kStages = kTma ? 3 : 5;
+    static constexpr int kStage = 2 * kPanels * kSide;           // of a warp: [panel][K, V][key], or [copy][lane]: two of 16 bytes of K, four of 8 of V
     static constexpr int kRing = kStages * kStage, kScaleAt = kWarps * kRing;           // then [warp][stage]: the scales of 16 keys of K and of V
     static constexpr int kCopies = kScaleAt + kWarps * kStages * 128;
     static constexpr int kLine = kHD + 4;                        // of a row of O in shared memory, in floats: lanes write to different banks
     static constexpr int kJoin = kWarps * (kRows * kLine + 2 * kRows) * 4;
     static constexpr int kSumAt = kCopies > kJoin ? kCopies : kJoin;   // this CTA's rows: [kRows][kLine] floats, then references and sums
-    static constexpr int kBytes = kSumAt + (kRows * kLine + 2 * kRows) * 4 + 1024;
+    static constexpr int kBytes = kSumAt + (kRows * kLine + 2 * kRows) * 4 + (kTma ? 1024 : 0);
 };
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -62,8 +64,10 @@ __device__ __forceinline__ void load_keys(uint32_t to, const void* tmap, int fea
                  "r"(page_side), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ void load_scales(uint32_t to, const void* from, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 64, [%2];" ::"r"(to), "l"(from), "r"(bar) : "memory");
+template <int kSize>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+    if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kSize) : "memory");
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 v;
@@ -89,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
     using C = Cfg<kHD, kX>;
     constexpr int kRows = C::kRows;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t* const smem = C::kTma ? (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023) : smem_raw;
     __shared__ uint64_t bars[kWarps][C::kStages];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     cg::cluster_group cluster = cg::this_cluster();
@@ -100,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
     unit /= row_tiles;
     const int n_kv = p.nhead / p.group, kv_head = unit % n_kv;
     int b = unit / n_kv;
-    if (lane == 0) {
+    if (C::kTma && lane == 0) {
         for (int i = 0; i < C::kStages; ++i) mbar_init(&bars[warp][i], 1);
         fence_mbar_init();
         prefetch_tmap(&codes);
@@ -108,18 +112,8 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
     __syncwarp();
     pdl_wait();
     pdl_launch_dependents();
-    if (longest_first) {   // the b-th sequence in order of length: the one that has b longer (or as long and earlier) ones
-        __shared__ int lens[kThreads], found;
-        const int i = threadIdx.x, len = i < p.batch ? p.k_lens[i] : 0;
-        lens[i] = len;
-        __syncthreads();
-        int before = 0;
-        for (int j = 0; j < p.batch; ++j) before += lens[j] > len || (lens[j] == len && j < i) ? 1 : 0;
-        if (i < p.batch && before == b) found = i;
-        __syncthreads();
-        b = found;
-    }
-    const TreeSeq s = tree_seq(p, b);
+    const int len = longest_first ? nth_longest<kThreads>(p, b) : p.k_lens[b];
+    const TreeSeq s = tree_seq(p, b, len);
     const int rows = min(s.qlen * p.group - tile * kRows, kRows);
     if (rows <= 0) return;                // the same for the whole cluster
     const int n_blocks = (s.klen + kKeys - 1) / kKeys;
@@ -144,20 +138,38 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
         }
     };
     const long long v_rows = (long long)n_kv * p.page;   // from a key's K to its V
-    const float* const scales_at = p.scales + (long long)kv_head * p.page;
+    const float* const scales_at = p.scales + (long long)kv_head * p.page + (lane >> 4) * v_rows + (lane & 15);
+    // What the lane reads of a block in heads of up to 64 (nothing behind the head's last feature), from the head's first row in a page on: of K key g and 16 features, of V key 2t and 8.
+    const long long page_codes = 2 * v_rows * hd;
+    const int8_t* const codes_k = p.codes + (long long)kv_head * p.page * hd + g * hd + t * 16;
+    const int8_t* const codes_v = p.codes + (long long)kv_head * p.page * hd + v_rows * hd + 2 * t * hd + g * 8;
     // The block that has been looked up: its codes and scales. Whether its page is there.
     auto fetch = [&](int i, int stage) {
         const bool there = i < n_blocks && page_id >= 0 && page_id < p.pages;
-        if (there && elect_one()) {
-            const uint32_t bar = bar0 + stage * 8, to = ring + stage * C::kStage;
-            mbar_expect_tx_at(bar, C::kStage + 128);
+        if (there) {
+            const uint32_t to = ring + stage * C::kStage;
+            copy_async<4>(scales_ring + stage * 128 + lane * 4, scales_at + (page_id * 2 * v_rows + page_off));
+            if constexpr (C::kTma) {
+                if (elect_one()) {
+                    const uint32_t bar = bar0 + stage * 8;
+                    mbar_expect_tx_at(bar, C::kStage);
 #pragma unroll
-            for (int n = 0; n < C::kPanels; ++n) load_keys(to + n * 2 * C::kSide, &codes, n * 128, page_off, kv_head, 2 * page_id, bar);
-            const float* const from = scales_at + page_id * 2 * v_rows + page_off;
-            load_scales(scales_ring + stage * 128, from, bar);
-            load_scales(scales_ring + stage * 128 + 64, from + v_rows, bar);
+                    for (int n = 0; n < C::kPanels; ++n) load_keys(to + n * 2 * C::kSide, &codes, n * 128, page_off, kv_head, 2 * page_id, bar);
+                }
+                __syncwarp();
+            } else {
+                const long long from = page_id * page_codes + (long long)page_off * hd;
+                if (t * 16 < hd) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) copy_async<16>(to + n * 512 + lane * 16, codes_k + from + n * 8 * hd);
+                }
+                if (g * 8 < hd) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) copy_async<8>(to + C::kSide + n * 256 + lane * 8, codes_v + from + ((n & 1) + (n >> 1) * 8) * hd);
+                }
+            }
         }
-        __syncwarp();
+        asm volatile("cp.async.commit_group;" ::: "memory");
         return there;
     };
     uint32_t there_bits = 0;              // of the blocks on their way, by stage
@@ -218,10 +230,14 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
         const int turn = stage;
         stage = stage + 1 == C::kStages ? 0 : stage + 1;
         if (!((there_bits >> turn) & 1u)) continue;   // keys in a page that there is not: nobody sees them
-        ok = mbar_wait_at(bar0 + turn * 8, (phases >> turn) & 1u);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        phases ^= 1u << turn;
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::kStages - 1) : "memory");
+        if constexpr (C::kTma) {
+            ok = mbar_wait_at(bar0 + turn * 8, (phases >> turn) & 1u);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            phases ^= 1u << turn;
+        }
+        __syncwarp();                     // (the scales come by all lanes)
         const uint32_t at = ring + turn * C::kStage, scales = scales_ring + turn * 128;
         const int key0 = i * kKeys;
         // ---- scores: the lane has keys g and g + 8 of its rows
@@ -233,8 +249,8 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
 #pragma unroll
         for (int n = 0; n < kHD / 64; ++n) {
             // keys g and g + 8, whose rows' chunks lie in the same order
-            const uint32_t k_at = kHD == 64 ? at + g * 64 + ((t ^ (g >> 1 & 3)) << 4) : at + n / 2 * 2 * C::kSide + g * 128 + (((2 * t + n % 2) ^ g) << 4);
-            const uint4 k0 = lds128(k_at), k1 = lds128(k_at + 8 * C::kRowBytes);
+            const uint32_t k_at = C::kTma ? at + n / 2 * 2 * C::kSide + g * 128 + (((2 * t + n % 2) ^ g) << 4) : at + lane * 16;
+            const uint4 k0 = lds128(k_at), k1 = lds128(k_at + C::kSide / 2);
             const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -317,16 +333,16 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
             uint32_t u[4][4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int key = 2 * t + (k & 1) + (k >> 1) * 8;
-                const uint32_t from = at + h * 2 * C::kSide + C::kSide + key * C::kRowBytes + (kHD == 64 ? ((g >> 1) ^ (key >> 1 & 3)) * 16 + (g & 1) * 8 : (g ^ (key & 7)) * 16);
-                if constexpr (kHD > 64) {
+                if constexpr (C::kTma) {
+                    const int key = 2 * t + (k & 1) + (k >> 1) * 8;
+                    const uint32_t from = at + h * 2 * C::kSide + C::kSide + key * 128 + ((g ^ (key & 7)) << 4);
                     const uint4 q = lds128(from);
                     u[k][0] = codes_biased(q.x);
                     u[k][1] = codes_biased(q.y);
                     u[k][2] = codes_biased(q.z);
                     u[k][3] = codes_biased(q.w);
                 } else {
-                    const uint2 q = lds64(from);
+                    const uint2 q = lds64(at + C::kSide + k * 256 + lane * 8);
                     u[k][0] = codes_biased(q.x);
                     u[k][1] = codes_biased(q.y);
                 }
@@ -345,7 +361,8 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
         }
         __syncwarp();                     // the stage has been read
     }
-    if (!ok) {   // (what was requested lands before the CTA leaves, bounded)
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (C::kTma && !ok) {   // (what was requested lands before the CTA leaves, bounded)
         if (lane == 0) {
             atomicExch(err, 28);
             for (int n = 0; n < C::kStages; ++n)
@@ -430,22 +447,22 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
 }
 
 // The cache as [page and side][head][row][feature].
-bool make_tmap_codes(CUtensorMap* out, const TreeParams& p, int row_bytes) {
+bool make_tmap_codes(CUtensorMap* out, const TreeParams& p) {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) return false;
     const uint64_t hd = (uint64_t)p.head_dim, heads = (uint64_t)(p.nhead / p.group);
     cuuint64_t dims[4] = {hd, (cuuint64_t)p.page, heads, 2 * (cuuint64_t)p.pages};
     cuuint64_t strides[3] = {hd, hd * p.page, hd * p.page * heads};
-    cuuint32_t box[4] = {(cuuint32_t)row_bytes, kKeys, 1, 2};
+    cuuint32_t box[4] = {128, kKeys, 1, 2};
     cuuint32_t estr[4] = {1, 1, 1, 1};
     return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(p.codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              row_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int kHD, int kX>
 cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
     CUtensorMap codes = {};
-    if (p.pages > 0 && p.codes && !make_tmap_codes(&codes, p, Cfg<kHD, kX>::kRowBytes)) return cudaErrorInvalidValue;
+    if (Cfg<kHD, kX>::kTma && p.pages > 0 && p.codes && !make_tmap_codes(&codes, p)) return cudaErrorInvalidValue;
     const auto kernel = attention_tree_kernel<kHD, kX>;
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] {
@@ -529,8 +546,8 @@ TreePlan attention_tree_plan(const TreeParams& p) {
     const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + 8 * tiles - 1) / (8 * tiles));
     const int turns = std::max(1, (p.max_k_len + kKeys * kWarps - 1) / (kKeys * kWarps));
     const double sm = sm_count();
-    static const TreeCosts costs[2][2] = {{{0.39, 1.05, 5.6, 2.3, 4.0, {1.0, 1.1, 1.1}, 0.0}, {0.46, 0.92, 8.4, 1.7, 3.0, {1.1, 1.1, 1.1}, 0.0}},
-                                          {{0.61, 2.00, 5.9, 3.3, 4.0, {1.1, 1.1, 0.48}, 0.0}, {0.89, 1.47, 9.4, 3.3, 3.0, {1.1, 1.1, 1.1}, 0.0}}};
+    static const TreeCosts costs[2][2] = {{{0.40, 1.04, 5.5, 2.4, 4.0, {1.0, 1.1, 1.1}, 0.0}, {0.50, 0.93, 8.3, 1.8, 3.0, {1.1, 1.1, 1.1}, 0.0}},
+                                          {{0.67, 1.77, 5.5, 3.6, 4.0, {1.1, 1.1, 0.51}, 0.0}, {0.94, 1.37, 9.2, 3.9, 3.0, {1.1, 1.1, 1.1}, 0.0}}};
     TreeCosts c = costs[p.head_dim > 64][tiles - 1];
     if (p.head_dim > 128) c = {2 * c.alone, 2 * c.shared, c.start, c.start_shared, tiles == 2 ? 1.0 : 2.0, {1.0, 1.0, 0.44}, 0.0};   // (not fitted: twice a head of 128)
     c.places *= sm;

@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <climits>
 #include <cstdint>
 #include "vec_math.cuh"
 
@@ -27,7 +28,32 @@ struct TreeSeq {
     int kept;                              // keys before the drafted ones (below 0: there are fewer keys than tokens)
 };
 
-__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
+// The b-th sequence in order of length (the one that has b longer, or as long and earlier, ones) becomes b; its keys. By a block of at least as many threads as there are sequences.
+template <int kThreads>
+__device__ __forceinline__ int nth_longest(const TreeParams& p, int& b) {
+    __shared__ __align__(16) int lens[kThreads];
+    __shared__ int found[2];
+    const int i = threadIdx.x, len = i < p.batch ? p.k_lens[i] : INT_MIN;
+    lens[i] = len;
+    __syncthreads();
+    if (i < p.batch) {
+        int before = 0;
+        for (int j = 0; j < p.batch; j += 4) {
+            const int4 l = *reinterpret_cast<const int4*>(lens + j);
+            before += (l.x > len || (l.x == len && j < i)) + (l.y > len || (l.y == len && j + 1 < i)) + (l.z > len || (l.z == len && j + 2 < i)) + (l.w > len || (l.w == len && j + 3 < i));
+        }
+        if (before == b) {
+            found[0] = i;
+            found[1] = len;
+        }
+    }
+    __syncthreads();
+    b = found[0];
+    return found[1];
+}
+
+// keys: k_lens[b]
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b, int keys) {
     TreeSeq s;
     if (p.cu_seqlens) {
         s.q0 = p.cu_seqlens[b];
@@ -37,7 +63,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int b) {
         s.qlen = p.max_q_len;
     }
     s.qlen = s.q0 < 0 ? 0 : max(0, min(s.qlen, min(p.max_q_len, p.q_tokens - s.q0)));
-    const int len = max(0, p.k_lens[b]);
+    const int len = max(0, keys);
     s.kept = len - s.qlen;
     s.klen = (int)min((long long)min(len, p.max_k_len), (long long)p.table_width * p.page);
     return s;

@@ -7,7 +7,7 @@
 // it has to (then O is rescaled in tensor memory). Two CTAs share an SM: while one waits for its products the other takes exponentials. A cluster shares a sequence's keys; its CTAs' rows are joined
 // through distributed shared memory in a fixed order.
 //
-// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 153 us (158 with the scores' UMMAs in a loop that is not unrolled); codes read once 36. No unit is full
+// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 150 us (155 with the scores' UMMAs in a loop that is not unrolled); codes read once 36. No unit is full
 // (shared-memory pipe 41 %, ALU 37 %, issue slots 39 %, tensor pipe 25 %): a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3300 clocks
 // with two CTAs to an SM. Tried: scores in halves of 32 keys, one multiplied while the other is weighed, by a warp of its own that issues UMMAs 165 (20 of them to a block instead of 12, some 45
 // clocks of the issuing thread each); two places for scores, Q in shared memory (as tensor memory is full then), such a warp, registers handed over 174 (with Q in tensor memory and one place 163),
@@ -96,18 +96,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
     const int n_kv = p.nhead / p.group, kv_head = unit % n_kv;
     int b = unit / n_kv;
     pdl_wait();
-    if (longest_first) {   // the b-th sequence in order of length: the one that has b longer (or as long and earlier) ones
-        __shared__ int lens[kThreads], found;
-        const int len = tid < p.batch ? p.k_lens[tid] : 0;
-        lens[tid] = len;
-        __syncthreads();
-        int before = 0;
-        for (int j = 0; j < p.batch; ++j) before += lens[j] > len || (lens[j] == len && j < tid) ? 1 : 0;
-        if (tid < p.batch && before == b) found = tid;
-        __syncthreads();
-        b = found;
-    }
-    const TreeSeq s = tree_seq(p, b);
+    const int len = longest_first ? nth_longest<kThreads>(p, b) : p.k_lens[b];
+    const TreeSeq s = tree_seq(p, b, len);
     const int rows = min(s.qlen * p.group - tile * kRows, kRows), hd = p.head_dim;
     if (rows <= 0) return;                // the same for the whole cluster
     const int row_warps = (rows + 31) / 32;   // the other softmax warps have no row: their lanes of tensor memory hold anything, which no row sees
@@ -508,7 +498,7 @@ TreePlan attention_tree_tc_plan(const TreeParams& p) {
     const int rows = p.max_q_len * p.group;
     const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + kRows - 1) / kRows);
     const double part = (rows < kRows ? rows : kRows) / (double)kRows, places = 2.0 * sm_count();
-    const TreeCosts narrow = {1.13, 1.44, 7.2, 3.7, places, {1.0, 1.0, 0.86}, 0.22 * part}, wide = {1.19, 1.84, 8.0, 5.3, places, {1.1, 1.1, 0.60}, 0.44 * part};
+    const TreeCosts narrow = {1.06, 1.38, 7.2, 3.5, places, {1.0, 1.0, 0.88}, 0.21 * part}, wide = {1.13, 1.76, 8.0, 5.1, places, {1.1, 1.1, 0.60}, 0.45 * part};
     return tree_plan(units, (p.max_k_len + kKeys - 1) / kKeys, sm_count(), p.head_dim > 64 ? wide : narrow);
 }
 

@@ -20,7 +20,6 @@
 #include "attention_tree.h"
 #include "common.h"
 #include "ptx.cuh"
-#include "tmap.h"
 
 namespace cg = cooperative_groups;
 
@@ -57,17 +56,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     const half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
-}
-// 16 keys of a head in a page, as far as a panel has their features, of K and of V.
-__device__ __forceinline__ void load_keys(uint32_t to, const void* tmap, int feature, int row, int head, int page_side, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(tmap), "r"(feature), "r"(row), "r"(head),
-                 "r"(page_side), "r"(bar)
-                 : "memory");
-}
-template <int kSize>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
-    if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kSize) : "memory");
 }
 __device__ __forceinline__ uint2 lds64(uint32_t a) {
     uint2 v;
@@ -446,23 +434,10 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
     cluster.sync();   // nobody leaves while its rows are read
 }
 
-// The cache as [page and side][head][row][feature].
-bool make_tmap_codes(CUtensorMap* out, const TreeParams& p) {
-    EncodeTiledFn fn = encode_tiled_fn();
-    if (!fn) return false;
-    const uint64_t hd = (uint64_t)p.head_dim, heads = (uint64_t)(p.nhead / p.group);
-    cuuint64_t dims[4] = {hd, (cuuint64_t)p.page, heads, 2 * (cuuint64_t)p.pages};
-    cuuint64_t strides[3] = {hd, hd * p.page, hd * p.page * heads};
-    cuuint32_t box[4] = {128, kKeys, 1, 2};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(p.codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int kHD, int kX>
 cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
     CUtensorMap codes = {};
-    if (Cfg<kHD, kX>::kTma && p.pages > 0 && p.codes && !make_tmap_codes(&codes, p)) return cudaErrorInvalidValue;
+    if (Cfg<kHD, kX>::kTma && p.pages > 0 && p.codes && !make_tmap_codes(&codes, p, true)) return cudaErrorInvalidValue;
     const auto kernel = attention_tree_kernel<kHD, kX>;
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] {

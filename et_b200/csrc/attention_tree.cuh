@@ -77,6 +77,18 @@ __device__ __forceinline__ bool tree_sees(const TreeSeq& s, unsigned long long b
     return key < s.klen && (place < 0 || (place < 64 && ((bits >> place) & 1ull)));
 }
 
+// 16 keys of a head in a page, as far as a panel has their features, of K and of V.
+__device__ __forceinline__ void load_keys(uint32_t to, const void* tmap, int feature, int row, int head, int page_side, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(tmap), "r"(feature), "r"(row), "r"(head),
+                 "r"(page_side), "r"(bar)
+                 : "memory");
+}
+template <int kSize>
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from) {
+    if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kSize) : "memory");
+}
+
 // Codes become halves without a conversion: the byte + 128 as the low bits of 1024 is 1024 + byte + 128 in fp16, exactly, from which 1152 is taken.
 __device__ __forceinline__ uint32_t codes_biased(uint32_t four) { return four ^ 0x80808080u; }
 template <int kHigh>

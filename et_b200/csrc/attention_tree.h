@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda_runtime.h>
 #include "attention_tree.cuh"
+#include "tmap.h"
 
 namespace et {
 
@@ -40,6 +41,19 @@ inline TreePlan tree_plan(long long units, int turns, int sms, const TreeCosts& 
         if (us < 1.02 * best.us) best = {us, csize};   // (as good: the larger cluster, for ragged ones)
     }
     return best;
+}
+
+// The cache as [page and side][head][row][feature]; a copy brings 128 features of 16 keys, of K and then of V.
+inline bool make_tmap_codes(CUtensorMap* out, const TreeParams& p, bool swizzled) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return false;
+    const uint64_t hd = (uint64_t)p.head_dim, heads = (uint64_t)(p.nhead / p.group);
+    cuuint64_t dims[4] = {hd, (cuuint64_t)p.page, heads, 2 * (cuuint64_t)p.pages};
+    cuuint64_t strides[3] = {hd, hd * p.page, hd * p.page * heads};
+    cuuint32_t box[4] = {128, 16, 1, 2};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<int8_t*>(p.codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace et

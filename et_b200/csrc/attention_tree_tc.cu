@@ -1,14 +1,14 @@
 // Attention of drafted tokens over a cache of int8 codes, many rows: a CTA has up to 128 of the rows (queries x query heads) of a K/V head, so that both products go to tcgen05 and a
 // code is converted once for all of them.
 //
-// Blocks of 64 keys. Four warps fetch the codes (cp.async, each thread into a place that only it reads, a block or two ahead) and write them as halves where the tensor cores read them (rows of 64
-// features, 128-byte swizzle; V as it lies, features are its N). Q lies in tensor memory as the first product's A operand, the scores beside it, and the weights where the
+// Blocks of 64 keys. Four warps have 16 keys of a block each, which lie in one page: they fetch the codes (one TMA copy; heads of up to 64, whose copies are half as large, by cp.async) into a place of
+// their own, a block or more ahead, and write them as halves where the tensor cores read them (rows of 64 features, 128-byte swizzle; V as it lies, features are its N). Q lies in tensor memory as the first product's A operand, the scores beside it, and the weights where the
 // scores were, as the second product's A operand. A thread has a row: scale of the key, mask, weight times the value's scale, a running reference that moves when
 // it has to (then O is rescaled in tensor memory). Two CTAs share an SM: while one waits for its products the other takes exponentials. A cluster shares a sequence's keys; its CTAs' rows are joined
 // through distributed shared memory in a fixed order.
 //
-// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 150 us (155 with the scores' UMMAs in a loop that is not unrolled); codes read once 36. No unit is full
-// (shared-memory pipe 41 %, ALU 37 %, issue slots 39 %, tensor pipe 25 %): a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3300 clocks
+// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 146 us (150 with codes by cp.async, 155 with the scores' UMMAs in a loop that is not unrolled besides); codes read once 36. No unit is full
+// (shared-memory pipe 41 %, ALU 37 %, issue slots 39 %, tensor pipe 25 %): a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3200 clocks
 // with two CTAs to an SM. Tried: scores in halves of 32 keys, one multiplied while the other is weighed, by a warp of its own that issues UMMAs 165 (20 of them to a block instead of 12, some 45
 // clocks of the issuing thread each); two places for scores, Q in shared memory (as tensor memory is full then), such a warp, registers handed over 174 (with Q in tensor memory and one place 163),
 // with codes fetched into registers 168 to 178 (operands from shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182.
@@ -37,12 +37,13 @@ template <int kHD>
 struct Cfg {
     static constexpr int kPanel = kKeys * 128, kTile = kHD / 64 * kPanel;       // halves of a block of K or V
     static constexpr int kChunks = kKeys * kHD / 16 / 128;                      // 16 codes each, of a thread, of K and of V
-    static constexpr int kRaw = 2 * kChunks * 2048 + 512;                       // a block's codes and scales as they come
+    static constexpr bool kTma = kHD > 64;
+    static constexpr int kPiece = 2 * 16 * kHD;                                 // codes of 16 keys, of K and of V
     static constexpr int kRawStages = kHD == 64 ? 4 : 2;
     static constexpr uint32_t kQCol = 0, kSCol = kHD / 2, kOCol = kSCol + kKeys;
     static_assert(kOCol + kHD <= kTmemCols, "");
     static constexpr int kKAt = 0, kVAt = 2 * kTile, kRawAt = 4 * kTile;
-    static constexpr int kScaleAt = kRawAt + kRawStages * kRaw;                 // [stage]: of 64 keys score factors, values' scales, their logarithms as fp16
+    static constexpr int kScaleAt = kRawAt + kRawStages * kConvertWarps * (kPiece + 128);                 // [stage]: of 64 keys score factors, values' scales, their logarithms as fp16
     static constexpr int kPartAt = kScaleAt + kScaleStages * kScaleBytes;     // [reference, sum][128]
     // Half of an SM's shared memory for half of its tensor memory: a CTA that finds one finds the other, and none waits for columns that another cluster holds.
     static constexpr int kBytes = 113664;
@@ -52,8 +53,9 @@ struct Cfg {
 
 struct Shared {
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t raw_full[kConvertWarps][4];
     uint64_t scales_full[kScaleStages], q_ready, s_full, p_ready, o_done;
-    uint32_t good[kScaleStages];          // a bit for each 16 keys of a block: their page is there
+    uint32_t good[kScaleStages];          // a byte for each 16 keys of a block: 1 if their page is there
     uint32_t tmem_base;
 };
 
@@ -65,11 +67,6 @@ __device__ __forceinline__ uint32_t no_infinity(uint32_t two) {
     const uint32_t lo = (two & 0x7fffu) == 0x7c00u ? 0x7fffu : two & 0xffffu, hi = (two & 0x7fff0000u) == 0x7c000000u ? 0x7fff0000u : two & 0xffff0000u;
     return lo | hi;
 }
-template <int kSize>
-__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int real) {
-    if constexpr (kSize == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real) : "memory");
-}
 // Two halves added to two fp32 values.
 __device__ __forceinline__ void add_halves(uint32_t h, float a, float b, float& x, float& y) {
     asm("{\n.reg .b16 l, h;\nmov.b32 {l, h}, %2;\nadd.rn.f32.f16 %0, l, %3;\nadd.rn.f32.f16 %1, h, %4;\n}" : "=f"(x), "=f"(y) : "r"(h), "f"(a), "f"(b));
@@ -80,7 +77,7 @@ __device__ __forceinline__ float4 lds_f4(uint32_t a) {
 }
 
 template <int kHD>
-__global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __grid_constant__ TreeParams p, int row_tiles, bool longest_first, int* err) {
+__global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ TreeParams p, int row_tiles, bool longest_first, int* err) {
     using C = Cfg<kHD>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -111,11 +108,14 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 mbar_init(&sh->v_empty[i], 1);
             }
             for (int i = 0; i < kScaleStages; ++i) mbar_init(&sh->scales_full[i], kConvertWarps);
+            if (C::kTma)
+                for (int i = 0; i < kConvertWarps * C::kRawStages; ++i) mbar_init(&sh->raw_full[i / C::kRawStages][i % C::kRawStages], 1);
             mbar_init(&sh->q_ready, row_warps);
             mbar_init(&sh->s_full, 1);
             mbar_init(&sh->p_ready, row_warps);
             mbar_init(&sh->o_done, 1);
             fence_mbar_init();
+            if (C::kTma) prefetch_tmap(&codes);
         }
         __syncwarp();
         tmem_alloc(&sh->tmem_base, kTmemCols);
@@ -129,20 +129,18 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
     bool ok = true;
     float top = -INFINITY, sum = 0.f;
     if (warp >= kSoftmaxWarps) {
-        // ---- codes to halves
-        const int c = tid - kSoftmaxWarps * 32;                       // 0 to 127
-        constexpr int kPerKey = kHD / 16;                             // chunks of a key
-        const int key_c = c / kPerKey, f = (c % kPerKey) * 16;        // of the thread's first chunk; the others are 128 / kPerKey keys apart
-        const int key_s = c & 63, side_s = c >> 6;                    // whose scale it brings
+        // ---- codes to halves: a warp has 16 keys of a block, which lie in one page
+        const int w = warp - kSoftmaxWarps;
+        constexpr int kPerKey = kHD / 16, kPass = 32 / kPerKey;       // lanes, of 16 codes each, to a key; keys at once
+        const int key_c = lane / kPerKey, f = (lane % kPerKey) * 16, key_s = w * 16 + (lane & 15), side_s = lane >> 4;   // (whose scale it brings)
         const int* const table = p.table + (long long)b * p.table_width;
-        const uint32_t raw = at + C::kRawAt;
-        const long long v_from_k = (long long)n_kv * p.page, v_codes = v_from_k * hd;   // from a key's K to its V
-        const long long page_rows = 2 * v_from_k, page_codes = page_rows * hd;
-        // what the thread reads of a block, from the head's first row in a page on
-        const int8_t* const codes_at = p.codes + (long long)kv_head * p.page * hd + (key_c & 15) * hd + (f < hd ? f : 0);
-        const float* const scales_at = p.scales + (long long)kv_head * p.page + (key_s & 15) + side_s * v_from_k;
-        // The four 16 keys of a block, each in one page, a lane each (over and over): the page's number is requested a block before it is needed, places in turn (no division).
-        int piece_key = crank * kKeys + (lane & 3) * 16, piece_n = piece_key / p.page, next_off = piece_key - piece_n * p.page, piece_id = -1, piece_off = 0;
+        const uint32_t raw = at + C::kRawAt + w * C::kRawStages * C::kPiece, raw_scales = at + C::kRawAt + kConvertWarps * C::kRawStages * C::kPiece + w * C::kRawStages * 128;
+        const long long v_rows = (long long)n_kv * p.page, page_rows = 2 * v_rows;   // from a key's K to its V; of a page
+        // what the lane reads of a block, from the head's first row in a page on (codes in heads of up to 64)
+        const int8_t* const codes_at = p.codes + (long long)kv_head * p.page * hd + key_c * hd + f;
+        const float* const scales_at = p.scales + (long long)kv_head * p.page + side_s * v_rows + (lane & 15);
+        // The page's number is requested a block before it is needed, places in turn (no division).
+        int piece_key = crank * kKeys + w * 16, piece_n = piece_key / p.page, next_off = piece_key - piece_n * p.page, piece_id = -1, piece_off = 0;
         const int step = csize * kKeys, step_n = step / p.page, step_off = step - step_n * p.page;
         auto look_up = [&]() {                                        // the next block
             piece_id = -1;
@@ -158,26 +156,31 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 }
             }
         };
-        uint32_t good_bits = 0;                                       // of eight blocks, four bits each
-        auto fetch = [&](int j) {                                     // block j, whose pages have been looked up
-            const bool there = piece_id >= 0 && piece_id < p.pages;
-            const long long start = there ? piece_id * page_codes + (long long)piece_off * hd : -1, row = there ? piece_id * page_rows + piece_off : -1;
-            look_up();
-            const uint32_t good = __ballot_sync(0xffffffffu, there) & 15u;
-            good_bits = (good_bits & ~(15u << (4 * (j & 7)))) | good << (4 * (j & 7));
-            if (j < mine) {
-                const uint32_t to = raw + (j % C::kRawStages) * C::kRaw + c * 16;
+        uint32_t there_bits = 0, phases = 0;                          // of the places: their page is there; phases of their barriers
+        auto fetch = [&](int j) {                                     // block j, whose page has been looked up
+            const bool there = j < mine && piece_id >= 0 && piece_id < p.pages;
+            const int place = j % C::kRawStages;
+            there_bits = (there_bits & ~(1u << place)) | (there ? 1u : 0u) << place;
+            if (there) {
+                const uint32_t to = raw + place * C::kPiece;
+                copy_async<4>(raw_scales + place * 128 + lane * 4, scales_at + (piece_id * page_rows + piece_off));
+                if constexpr (C::kTma) {
+                    if (elect_one()) {
+                        const uint32_t bar = smem_u32(&sh->raw_full[w][place]);
+                        mbar_expect_tx_at(bar, C::kPiece);
+                        load_keys(to, &codes, 0, piece_off, kv_head, 2 * piece_id, bar);
+                    }
+                    __syncwarp();
+                } else if (f < hd) {
+                    const int8_t* const k = codes_at + (piece_id * page_rows + piece_off) * hd;
 #pragma unroll
-                for (int n = 0; n < C::kChunks; ++n) {
-                    const long long first = __shfl_sync(0xffffffffu, start, (key_c >> 4) + n * (8 / kPerKey));
-                    const int size = first >= 0 && f < hd ? 16 : 0;
-                    const int8_t* const k = codes_at + (first >= 0 ? first : 0);
-                    copy_async<16>(to + n * 2048, k, size);
-                    copy_async<16>(to + (C::kChunks + n) * 2048, k + v_codes, size);
+                    for (int n = 0; n < C::kChunks; ++n) {
+                        copy_async<16>(to + n * 512 + lane * 16, k + n * kPass * hd);
+                        copy_async<16>(to + C::kPiece / 2 + n * 512 + lane * 16, k + (v_rows + n * kPass) * hd);
+                    }
                 }
-                const long long first = __shfl_sync(0xffffffffu, row, key_s >> 4);
-                copy_async<4>(raw + (j % C::kRawStages) * C::kRaw + 2 * C::kChunks * 2048 + c * 4, scales_at + (first >= 0 ? first : 0), first >= 0 ? 4 : 0);
             }
+            look_up();
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         // 16 codes of the thread as halves at 16 bytes 2 f / 16 and the next of the key's row. (Every second thread of eight that write at once takes the second 16 bytes first:
@@ -196,17 +199,24 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         look_up();
         for (int n = 0; n < C::kRawStages - 1; ++n) fetch(n);
         for (int j = 0; j < mine; ++j) {
-            fetch(j + C::kRawStages - 1);   // (the thread has read that place a turn ago)
+            fetch(j + C::kRawStages - 1);   // (the warp has read that place a turn ago)
+            const int st = j & 1, key0 = (crank + j * csize) * kKeys, place = j % C::kRawStages;
+            const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u, from = raw + place * C::kPiece + lane * 16;
+            const bool there = (there_bits >> place) & 1u;            // (where not, any codes are converted, which no row sees)
             asm volatile("cp.async.wait_group %0;" ::"n"(C::kRawStages - 1) : "memory");
-            const int st = j & 1, key0 = (crank + j * csize) * kKeys;
-            const uint32_t ph = ((uint32_t)(j >> 1) & 1u) ^ 1u, from = raw + (j % C::kRawStages) * C::kRaw;
+            if (C::kTma && there) {
+                ok = mbar_wait(&sh->raw_full[w][place], (phases >> place) & 1u);
+                if (!ok) break;
+                phases ^= 1u << place;
+                there_bits &= ~(1u << place);
+            }
             ok = mbar_wait(&sh->k_empty[st], ph);
             if (!ok) break;
 #pragma unroll
-            for (int n = 0; n < C::kChunks; ++n) convert(from + (n * 128 + c) * 16, at + C::kKAt + st * C::kTile, key_c + n * (128 / kPerKey));
+            for (int n = 0; n < C::kChunks; ++n) convert(from + n * 512, at + C::kKAt + st * C::kTile, w * 16 + key_c + n * kPass);
             // Scales go to the places of block j - 4, whose scores are done with: those of block j - 2 have been multiplied, behind the weights of block j - 3.
-            const float scale = __uint_as_float(lds32(from + 2 * C::kChunks * 2048 + c * 4));
-            const bool real = key0 + key_s < s.klen;   // (behind the last key anything may lie)
+            const float scale = __uint_as_float(lds32(raw_scales + place * 128 + lane * 4));
+            const bool real = there && key0 + key_s < s.klen;   // (behind the last key anything may lie)
             uint8_t* const to = smem + C::kScaleAt + (j % kScaleStages) * kScaleBytes;
             if (side_s == 0) {
                 reinterpret_cast<float*>(to)[key_s] = real ? scale * p.scale_log2 : 0.f;
@@ -214,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 reinterpret_cast<float*>(to)[kKeys + key_s] = real ? scale : 0.f;
                 reinterpret_cast<half*>(to + 8 * kKeys)[key_s] = __float2half_rn(log2_of_scale(real ? scale : 0.f));   // (for the reference alone)
             }
-            if (c == 0) sh->good[j % kScaleStages] = (good_bits >> (4 * (j & 7))) & 15u;
+            if (lane == 0) reinterpret_cast<uint8_t*>(&sh->good[j % kScaleStages])[w] = there ? 1 : 0;
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -224,13 +234,17 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             ok = mbar_wait(&sh->v_empty[st], ph);
             if (!ok) break;
 #pragma unroll
-            for (int n = 0; n < C::kChunks; ++n) convert(from + ((C::kChunks + n) * 128 + c) * 16, at + C::kVAt + st * C::kTile, key_c + n * (128 / kPerKey));
+            for (int n = 0; n < C::kChunks; ++n) convert(from + C::kPiece / 2 + n * 512, at + C::kVAt + st * C::kTile, w * 16 + key_c + n * kPass);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh->v_full[st]);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        if (!ok && lane == 0) atomicExch(err, 26);
+        if (!ok && lane == 0) {
+            atomicExch(err, 26);
+            for (int n = 0; C::kTma && n < C::kRawStages; ++n)   // what was requested lands before the CTA leaves (bounded)
+                if ((there_bits >> n) & 1u) mbar_wait(&sh->raw_full[w][n], (phases >> n) & 1u);
+        }
     } else if (warp < row_warps) {
         // ---- a row to a thread
         const uint32_t mine_at = tmem + ((uint32_t)warp << 21);       // the warp's lanes of tensor memory
@@ -289,16 +303,16 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             const uint32_t scales = at + C::kScaleAt + (j % kScaleStages) * kScaleBytes;
             // what the row sees of the block
             const uint32_t good = sh->good[j % kScaleStages];
-            const bool masked = key0 + kKeys > s.kept || key0 + kKeys > s.klen || good != 15u;   // the same for the whole CTA
+            const bool masked = key0 + kKeys > s.kept || key0 + kKeys > s.klen || good != 0x01010101u;   // the same for the whole CTA
             unsigned long long seen = ~0ull;
             if (masked) {
                 const int d = key0 - s.kept;   // place of the first key among the drafted tokens
                 seen = d >= 64 ? 0ull : d >= 0 ? bits >> d : d > -64 ? (bits << -d) | ((1ull << -d) - 1ull) : ~0ull;
                 const int left = s.klen - key0;
                 if (left < 64) seen &= (1ull << left) - 1ull;
-                if (good != 15u)
+                if (good != 0x01010101u)
                     for (int n = 0; n < 4; ++n)
-                        if (!((good >> n) & 1u)) seen &= ~(0xffffull << (n * 16));
+                        if (!((good >> (8 * n)) & 1u)) seen &= ~(0xffffull << (n * 16));
             }
             float most = -INFINITY;
             auto two = [](const uint32_t* x) { return make_float2(__uint_as_float(x[0]), __uint_as_float(x[1])); };
@@ -466,6 +480,8 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
 
 template <int kHD>
 cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csize, int* err, cudaStream_t st) {
+    CUtensorMap codes = {};
+    if (Cfg<kHD>::kTma && p.pages > 0 && p.codes && !make_tmap_codes(&codes, p, false)) return cudaErrorInvalidValue;
     const auto kernel = attention_tree_tc_kernel<kHD>;
     static PerDeviceOnce once;
     const cudaError_t e = once.run([&] {
@@ -488,7 +504,7 @@ cudaError_t launch(const TreeParams& p, int row_tiles, long long units, int csiz
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     const bool longest_first = p.batch <= kThreads && units * csize > 2 * sm_count();
-    return cudaLaunchKernelEx(&cfg, kernel, p, row_tiles, longest_first, err);
+    return cudaLaunchKernelEx(&cfg, kernel, codes, p, row_tiles, longest_first, err);
 }
 
 }  // namespace

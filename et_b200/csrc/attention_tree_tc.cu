@@ -514,7 +514,7 @@ TreePlan attention_tree_tc_plan(const TreeParams& p) {
     const int rows = p.max_q_len * p.group;
     const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + kRows - 1) / kRows);
     const double part = (rows < kRows ? rows : kRows) / (double)kRows, places = 2.0 * sm_count();
-    const TreeCosts narrow = {1.06, 1.38, 7.2, 3.5, places, {1.0, 1.0, 0.88}, 0.21 * part}, wide = {1.13, 1.76, 8.0, 5.1, places, {1.1, 1.1, 0.60}, 0.45 * part};
+    const TreeCosts narrow = {1.03, 1.37, 7.1, 3.1, places, {1.0, 1.0, 0.78}, 0.22 * part}, wide = {1.10, 1.67, 7.7, 4.6, places, {1.1, 1.1, 0.59}, 0.445 * part};
     return tree_plan(units, (p.max_k_len + kKeys - 1) / kKeys, sm_count(), p.head_dim > 64 ? wide : narrow);
 }
 

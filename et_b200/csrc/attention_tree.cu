@@ -521,8 +521,8 @@ TreePlan attention_tree_plan(const TreeParams& p) {
     const long long units = (long long)p.batch * (p.nhead / p.group) * ((rows + 8 * tiles - 1) / (8 * tiles));
     const int turns = std::max(1, (p.max_k_len + kKeys * kWarps - 1) / (kKeys * kWarps));
     const double sm = sm_count();
-    static const TreeCosts costs[2][2] = {{{0.40, 1.04, 5.5, 2.4, 4.0, {1.0, 1.1, 1.1}, 0.0}, {0.50, 0.93, 8.3, 1.8, 3.0, {1.1, 1.1, 1.1}, 0.0}},
-                                          {{0.67, 1.77, 5.5, 3.6, 4.0, {1.1, 1.1, 0.51}, 0.0}, {0.94, 1.37, 9.2, 3.9, 3.0, {1.1, 1.1, 1.1}, 0.0}}};
+    static const TreeCosts costs[2][2] = {{{0.40, 1.04, 5.5, 2.4, 4.0, {1.0, 1.1, 1.1}, 0.0}, {0.49, 1.09, 7.6, 3.7, 3.0, {1.0, 1.1, 1.1}, 0.0}},
+                                          {{0.67, 1.77, 5.5, 3.6, 4.0, {1.1, 1.1, 0.51}, 0.0}, {0.87, 1.89, 8.0, 6.8, 3.0, {1.1, 1.1, 1.1}, 0.0}}};
     TreeCosts c = costs[p.head_dim > 64][tiles - 1];
     if (p.head_dim > 128) c = {2 * c.alone, 2 * c.shared, c.start, c.start_shared, tiles == 2 ? 1.0 : 2.0, {1.0, 1.0, 0.44}, 0.0};   // (not fitted: twice a head of 128)
     c.places *= sm;

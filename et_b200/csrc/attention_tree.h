@@ -7,8 +7,8 @@
 namespace et {
 
 // How CTAs share a sequence's keys, and what a launch takes in microseconds by a model fitted to 6200 launches (1 to 128 sequences of 200 to 16000 keys, all alike or ragged, 1 to 256 rows of
-// a K/V head, heads of 64, 96 and 128, every cluster): the kernel and the cluster taken so cost 4 % over the fastest in the mean, 26 % at the 95th percentile (with rules of thumb, tcgen05
-// from 32 rows on and clusters that fill the SMs, 26 and 100 % before).
+// a K/V head, heads of 64, 96 and 128, every cluster): the kernel and the cluster taken so cost 4 % over the fastest in the mean, 23 % at the 95th percentile (with rules of thumb, tcgen05
+// from 32 rows on and clusters that fill the SMs, 26 and 100 %).
 struct TreePlan {
     double us;
     int csize;

@@ -467,8 +467,9 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
                 }
                 few_barrier();
             }
-            ok = mbar_wait_at(smem_u32(&sh->acc_full[place]), (uint32_t)(i / kPlaces) & 1u);
-            if (!ok) break;
+            // (A warp that gives up stays in the loop without waiting again: few_barrier counts every warp.)
+            ok = ok && mbar_wait_warp_at(smem_u32(&sh->acc_full[place]), (uint32_t)(i / kPlaces) & 1u);
+            if (!ok) continue;
             tc_fence_after();
             constexpr int kStep = kCols < 16 ? kCols : 16;
 #pragma unroll

@@ -205,12 +205,12 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             const bool there = (there_bits >> place) & 1u;            // (where not, any codes are converted, which no row sees)
             asm volatile("cp.async.wait_group %0;" ::"n"(C::kRawStages - 1) : "memory");
             if (C::kTma && there) {
-                ok = mbar_wait(&sh->raw_full[w][place], (phases >> place) & 1u);
+                ok = mbar_wait_warp(&sh->raw_full[w][place], (phases >> place) & 1u);
                 if (!ok) break;
                 phases ^= 1u << place;
                 there_bits &= ~(1u << place);
             }
-            ok = mbar_wait(&sh->k_empty[st], ph);
+            ok = mbar_wait_warp(&sh->k_empty[st], ph);
             if (!ok) break;
 #pragma unroll
             for (int n = 0; n < C::kChunks; ++n) convert(from + n * 512, at + C::kKAt + st * C::kTile, w * 16 + key_c + n * kPass);
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                 mbar_arrive(&sh->scales_full[j % kScaleStages]);
                 mbar_arrive(&sh->k_full[st]);
             }
-            ok = mbar_wait(&sh->v_empty[st], ph);
+            ok = mbar_wait_warp(&sh->v_empty[st], ph);
             if (!ok) break;
 #pragma unroll
             for (int n = 0; n < C::kChunks; ++n) convert(from + C::kPiece / 2 + n * 512, at + C::kVAt + st * C::kTile, w * 16 + key_c + n * kPass);
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
         for (int j = 0; j < mine; ++j) {
             const int key0 = (crank + j * csize) * kKeys;
             // (Not for k_full: the place may be full of block j + 2 before this warp looks, and the phases of two blocks look alike. The scales of block j + 4 wait for this one's weights.)
-            ok = mbar_wait(&sh->scales_full[j % kScaleStages], (uint32_t)(j / kScaleStages) & 1u) && mbar_wait(&sh->s_full, (uint32_t)j & 1u);
+            ok = mbar_wait_warp(&sh->scales_full[j % kScaleStages], (uint32_t)(j / kScaleStages) & 1u) && mbar_wait_warp(&sh->s_full, (uint32_t)j & 1u);
             if (!ok) break;
             tc_fence_after();
             uint32_t raw[2][32];
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
             }
         }
         // O goes to shared memory where the blocks were: [row][features], 16 bytes c of a row at c ^ row, so that rows lie on different banks
-        if (ok && mine > 0) ok = mbar_wait(&sh->o_done, 0);
+        if (ok && mine > 0) ok = mbar_wait_warp(&sh->o_done, 0);
         if (!ok && lane == 0) atomicExch(err, 27);
     }
     __syncwarp();

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
                     next0 = __ldg(sw0 + kb + 1);
                     if (C::kHalves == 2) next1 = __ldg(sw1 + kb + 1);
                 }
-                if (!mbar_wait_at(acc_full + slot * 8, slot_ph)) return false;
+                if (!mbar_wait_warp_at(acc_full + slot * 8, slot_ph)) return false;
                 tc_fence_after();
 #pragma unroll
                 for (int i = 0; i < kCols; i += 32) {
@@ -350,13 +350,13 @@ __device__ __forceinline__ void st_async_cluster(uint32_t addr, uint32_t bar, ui
                  : "memory");
 }
 __device__ __forceinline__ void few_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kFewEpi) : "memory"); }
-// A bounded wait like mbar_wait, for what other CTAs of the cluster have written.
+// A bounded wait like mbar_wait_warp, for what other CTAs of the cluster have written.
 __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kMbarSpinLimit; ++i) {
         uint32_t ok;
         asm volatile("{\n.reg .pred P;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\nselp.u32 %0, 1, 0, P;\n}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
+        if (__all_sync(0xffffffffu, ok)) return true;
     }
     return false;
 }

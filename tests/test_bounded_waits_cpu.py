@@ -36,3 +36,28 @@ def test_no_warp_leaves_a_loop_whose_barriers_count_it():
     body = text[slice(*loops[0])]
     assert body.count("few_barrier();") == 2 and "acc_full" in body
     assert not re.search(r"\b(break|return|goto)\b", body)
+
+
+def by_one_lane(text, at, inside):
+    """Whether what stands here runs in one lane of a warp alone: under such a condition, or in a function of its own that only such places call."""
+    statement = text[max(text.rfind(c, 0, at) for c in ";{}") + 1:at]
+    headers = [statement] + [h for _, h, a, b in inside if a <= at < b]
+    if any(re.search(r"lane == 0|elect_one\(\)", h) for h in headers):
+        return True
+    names = [m.group(1) for h in headers for m in [re.search(r"auto (\w+) = \[&\]", h)] if m]
+    calls = [m.start() for name in names for m in re.finditer(r"(?<!auto )\b%s\(" % name, text)]
+    return bool(calls) and all(by_one_lane(text, c, inside) for c in calls)
+
+
+@pytest.mark.parametrize("name", ["fp8_gemm.cu", "attention_tree.cu", "attention_tree_tc.cu"])
+def test_a_warp_votes_on_what_it_waited_for(name):
+    """Lanes that disagree on whether their wait gave up would meet in different warp-wide operations (tensor-memory loads, barriers)."""
+    text = source(name)
+    inside = scopes(text)
+    waits = [m for m in re.finditer(r"\bmbar_wait(_at)?\(", text) if not text[:m.start()].endswith("bool ")]
+    assert waits
+    for m in waits:
+        statement = text[max(text.rfind(c, 0, m.start()) for c in ";{}") + 1:m.start()]
+        used = re.search(r"(ok|got) =|return|if \(!?$|&& $", statement)
+        behind = text[text.index(";", m.start()) + 1:].lstrip()
+        assert not used or behind.startswith("ok = __all_sync(0xffffffffu, ok);") or by_one_lane(text, m.start(), inside), statement + text[m.start():m.start() + 80]

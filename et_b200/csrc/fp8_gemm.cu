@@ -13,7 +13,7 @@
 // be read, fills the tile; K split over a cluster. Each CTA sends the others their columns' parts (asynchronous stores that count towards a barrier of the receiver) and
 // adds what it gets in the order of the ranks.
 //
-// The weight does not depend on the preceding kernel: its first copies are requested before griddepcontrol.wait. Every wait is bounded; a role that gives up records a code and all
+// The weight does not depend on the preceding kernel: its first copies are requested before griddepcontrol.wait, behind which all other roles begin. Every wait is bounded; a role that gives up records a code and all
 // threads reach the common exit.
 #include <algorithm>
 #include <cstring>
@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
                 int s = 0, kb = 0, tile = pair;
                 uint32_t ph = 1;
                 for (int c = 0; c < total; ++c) {
+                    if (!is_x && c == S) pdl_wait();   // (the weight's first copies go ahead; what follows waits for products of X)
                     ok = mbar_wait_at(smem_u32(&sh->empty[s]), ph);
                     if (!ok) break;
                     const uint32_t bar = in_cta(smem_u32(&sh->full[s]), 0);
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) fp8_pair_kernel(const __grid_
                 bool ok = true;
                 int s = C::kHalves == 2 ? 0 : m, slot = m;
                 uint32_t ph = 0, slot_ph = 1;
+                pdl_wait();   // (X's copies do: a wait for them may not begin while the preceding kernel runs, whose length has no limit)
                 for (int c = s; c < total; c += kStep) {
                     ok = mbar_wait_at(acc_empty + slot * 8, slot_ph) && mbar_wait_at(full + s * 8, ph);
                     if (!ok) break;
@@ -414,6 +416,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
             uint32_t ph = 1;
             int i = 0;
             for (; i < kn; ++i) {
+                if (!is_x && i == S) pdl_wait();   // (the weight's first copies go ahead; what follows waits for products of X)
                 ok = i < S || mbar_wait(&sh->empty[s], ph);
                 if (!ok) break;
                 mbar_expect_tx(&sh->full[s], is_x ? kXTile : kWTile);
@@ -433,6 +436,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) fp8_few_kernel(const __grid_co
             const uint64_t w0 = make_smem_desc(ring, 16, 1024, 2), x0 = make_smem_desc(ring + kWTile, 16, 1024, 2);
             int s = 0;
             uint32_t ph = 0;
+            pdl_wait();   // (X's copies do: a wait for them may not begin while the preceding kernel runs, whose length has no limit)
             for (int i = 0; i < kn; ++i) {
                 const int place = i % kPlaces;
                 ok = (i < kPlaces || mbar_wait(&sh->acc_empty[place], (uint32_t)(i / kPlaces - 1) & 1u)) && mbar_wait(&sh->full[s], ph);

@@ -46,3 +46,29 @@ def test_linear_behind_a_long_kernel(et, k, n, tokens):
     lin.handle.check()
     et.attention_check()
     assert torch.equal(out, want)
+
+
+# ------------------------------------------------------------------------------------------------ GELU
+@pytest.mark.parametrize("tokens", [3, 60, 5000])
+def test_gelu_far_to_the_left(et, tokens):
+    """Results behind -3 keep fp16's digits. Features are whole steps of 2^-6 from -7.5 to 7.5, exact in fp32. The exponent, at most 28 where fp16 has a result, is off by 2^-21.4 of itself (three
+    roundings, two constants), so the exponential by 2^-17; the reciprocal is off by 0.051^4 = 2^-17.1 and some roundings."""
+    k, n = 64, 960
+    values = (torch.arange(n, device="cuda") - 480).double() / 64
+    codes = torch.zeros(n, k, dtype=torch.float8_e4m3fn, device="cuda")
+    rest = values.clone()
+    for i in range(4):   # as sums of e4m3 numbers
+        codes[:, i] = rest.float().to(torch.float8_e4m3fn)
+        rest -= codes[:, i].double()
+    assert (rest == 0).all()
+    weight = et.Fp8Weight(k, n, codes.view(torch.uint8).cpu().numpy(), np.ones((blocks(n), 1), np.float32), is_gelu=True)
+    x = torch.zeros(tokens, k, dtype=torch.float8_e4m3fn, device="cuda")
+    x[:, :4] = 1.0
+    out = torch.zeros(tokens, n, dtype=torch.float16, device="cuda")
+    weight.run(out, x, torch.ones(1, tokens, device="cuda"))
+    want = torch.nn.functional.gelu(values, approximate="tanh").expand(tokens, n)
+    within(out, want, want.abs() * (HALF + 2.0 ** -15.9) + TINY)
+    # far out: nothing is left, or all of it
+    weight.run(out, x, torch.full((1, tokens), 2.0 ** 10, device="cuda"))
+    assert (out[:, :470] == 0).all() and torch.equal(out[:, 490:].double(), (values[490:] * 1024).half().double().expand(tokens, -1))
+    weight.check()

@@ -25,12 +25,27 @@ struct RowParams {
     float eps;
 };
 
-// What y is multiplied by to become a code, and the scale. (A code is one step off that of y / scale only where that lies within 2^-22 of the middle
-// between two codes.) An infinite maximum leaves 0 and codes that are not numbers, one that is not a number the same.
-__device__ __forceinline__ float code_factor(float top) { return top == 0.f ? 0.f : kE4m3Max / top; }
-__device__ __forceinline__ uint32_t e4m3_pair(float lo, float hi) {
+// The rounded quotient y / d, as what y * (about 1 / d) leaves of y is added to it, divided the same way.
+__device__ __forceinline__ float quotient(float y, float d, float inverse) {
+    const float q = y * inverse;
+    return fmaf(fmaf(-q, d, y), inverse, q);
+}
+__device__ __forceinline__ float2 quotient2(float a, float b, float d, float inverse) {
+    const float2 y = make_float2(a, b), i2 = make_float2(inverse, inverse), q = mul2(y, i2);
+    return fma2(fma2(q, make_float2(-d, -d), y), i2, q);
+}
+// The scale of features whose largest size is `top` (/ 448), and about 1 / scale. Codes are those of rounded quotients y / scale, since fp16 features often lie in the middle between two codes:
+// y * (448 / top) is one step beside it in some 70 of a million. A maximum that is infinite or not a number leaves a scale that is not a number.
+struct Scale {
+    float scale, inverse;
+    __device__ __forceinline__ explicit Scale(float top) : scale(quotient(top, kE4m3Max, 1.f / kE4m3Max)) {
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
+        if (top == 0.f) inverse = 0.f;
+    }
+};
+__device__ __forceinline__ uint32_t e4m3_pair(float2 v) {
     uint16_t d;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(hi), "f"(lo));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(d) : "f"(v.y), "f"(v.x));
     return d;
 }
 __device__ __forceinline__ float warp_sum(float v) {
@@ -123,13 +138,14 @@ __global__ void __launch_bounds__(kV == 4 ? 512 : 256) row_kernel(const __grid_c
             for (int i = 0; i < 8; ++i) top = max_nan(top, fabsf(h[v][i]));
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float f = code_factor(top);
+            const Scale s(top);
             if (g < granules) {
                 uint2 c;
-                c.x = e4m3_pair(h[v][0] * f, h[v][1] * f) | e4m3_pair(h[v][2] * f, h[v][3] * f) << 16;
-                c.y = e4m3_pair(h[v][4] * f, h[v][5] * f) | e4m3_pair(h[v][6] * f, h[v][7] * f) << 16;
+                auto two = [&](int i) { return e4m3_pair(quotient2(h[v][i], h[v][i + 1], s.scale, s.inverse)); };
+                c.x = two(0) | two(2) << 16;
+                c.y = two(4) | two(6) << 16;
                 *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.out) + row * p.out_pitch + g * 8) = c;
-                if ((lane & 15) == 0) p.scales[(long long)(g >> 4) * p.rows + row] = top / kE4m3Max;
+                if ((lane & 15) == 0) p.scales[(long long)(g >> 4) * p.rows + row] = s.scale;
             }
         } else if (g < granules) {
             uint4 r;
@@ -175,14 +191,14 @@ __global__ void __launch_bounds__(256) row_any_kernel(const __grid_constant__ Ro
         if constexpr (kCodes) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (lane == 0) p.scales[(long long)(b / kScaleBlock) * p.rows + row] = top / kE4m3Max;
+            if (lane == 0) p.scales[(long long)(b / kScaleBlock) * p.rows + row] = Scale(top).scale;
         }
-        const float f = code_factor(top);
+        const Scale s(top);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int c = b + i * 32 + lane;
             if (c >= p.width) continue;
-            if constexpr (kCodes) static_cast<uint8_t*>(p.out)[row * p.out_pitch + c] = (uint8_t)e4m3_pair(y[i] * f, 0.f);
+            if constexpr (kCodes) static_cast<uint8_t*>(p.out)[row * p.out_pitch + c] = (uint8_t)e4m3_pair(make_float2(quotient(y[i], s.scale, s.inverse), 0.f));
             else static_cast<half*>(p.out)[row * p.out_pitch + c] = __float2half_rn(y[i]);
         }
     }

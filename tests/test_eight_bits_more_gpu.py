@@ -72,3 +72,33 @@ def test_gelu_far_to_the_left(et, tokens):
     weight.run(out, x, torch.full((1, tokens), 2.0 ** 10, device="cuda"))
     assert (out[:, :470] == 0).all() and torch.equal(out[:, 490:].double(), (values[490:] * 1024).half().double().expand(tokens, -1))
     weight.check()
+
+
+# ------------------------------------------------------------------------------------------------ codes
+@pytest.mark.parametrize("rows,width", [(4096, 1024), (1024, 1000), (333, 250), (60000, 128)])
+def test_codes_are_those_of_the_quotient(et, rows, width):
+    """code = e4m3(x / scale), scale = largest / 448, with fp32's rounded quotients: bit for bit, ties among them."""
+    g = gen(width)
+    x = (normal(g, rows, width) * torch.exp(3 * normal(g, rows, 1))).clamp(-60000, 60000).half()
+    x[::3] = (x[::3] * 16).round().clamp(-60000, 60000)          # whole numbers: quotients meet the middles between codes often
+    x[5] = torch.arange(width, device="cuda").half() * 2.0 ** -24  # below fp16's normal numbers
+    x[6] = 0
+    out, scales = torch.zeros(rows, width, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(blocks(width), rows, device="cuda")
+    et.quantise_rows(out, scales, x)
+    top = torch.nn.functional.pad(x.float().abs(), (0, -width % 128)).view(rows, -1, 128).amax(-1).t()
+    assert torch.equal(scales, top / torch.full_like(top, 448))   # (torch divides by a number as it multiplies by its reciprocal)
+    s = spread(scales, width)
+    want = torch.where(s > 0, x.float() / s, torch.zeros_like(s)).to(torch.float8_e4m3fn)
+    assert torch.equal(out.float(), want.float())   # (of zeros either sign)
+
+
+def test_codes_of_every_number(et):
+    """Each of fp16's numbers under scales of all sizes that it is not above."""
+    numbers = torch.arange(0, 0x7c00, device="cuda", dtype=torch.int32).to(torch.int16).view(torch.float16)
+    for top in (1.0, 447.0, 449.0, 5.0, 7.0, 0.3, 65504.0, 1.375, 2047.0, 3.0):
+        some = numbers[numbers <= top]
+        some = torch.nn.functional.pad(some, (0, -len(some) % 127)).view(-1, 127)
+        x = torch.cat([torch.full((len(some), 1), top, dtype=torch.float16, device="cuda"), some], 1)
+        out, scales = torch.zeros(x.shape, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(1, len(x), device="cuda")
+        et.quantise_rows(out, scales, x)
+        assert torch.equal(out.float(), (x.float() / scales[0][:, None]).to(torch.float8_e4m3fn).float())

@@ -29,7 +29,6 @@ namespace {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kKeys = 16;                 // of a block
 constexpr int kMaxCluster = 16;
-constexpr float kRescaleStep = 8.f;       // log2 units
 
 template <int kHD, int kX>
 struct Cfg {
@@ -308,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, kHD == 256 ? 1 : kX == 2 ? 3 : 4) at
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float m = top[x][e & 1];
-                v[x][e] = ex2_fast(v[x][e] - (m == -INFINITY ? 0.f : m));
+                v[x][e] = ex2_fast(v[x][e] - (m == -INFINITY ? 0.f : m - kLift));
                 sum[x][e & 1] += v[x][e];
                 v[x][e] *= scale[x][e];
             }

@@ -99,8 +99,10 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t biased) {   // bytes
 }
 
 // Values scales enter the weights of the second product (as codes are whole numbers there), which are fp16. So the reference that is taken from a row's scores follows
-// score + log2 of the value's scale: a weight times its scale is then at most 2^8 and never small beside what it is added to. This is that logarithm; scales below 2^-40 (rows of
-// zeros: the smallest others are 2^-31) count as 2^-40.
+// score + log2 of the value's scale, in steps of kRescaleStep, and the weights are 2^kLift times as large: the largest weight times its scale lies between 2^7 and 2^15, and one that falls below half of
+// fp16's smallest step is below 2^-32 of it. (Without the lift below 2^-25: of 60000 keys with such weights nothing was left, even in features where the large one's value is 0.) This is that logarithm; scales
+// below 2^-40 (rows of zeros: the smallest others are 2^-31) count as 2^-40.
+constexpr float kRescaleStep = 8.f, kLift = 7.f;   // log2 units
 __device__ __forceinline__ float log2_of_scale(float s) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaxf(s, 9.094947017729282e-13f)));

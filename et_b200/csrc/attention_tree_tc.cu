@@ -30,7 +30,6 @@ constexpr int kRows = 128;                // of a CTA
 constexpr int kSoftmaxWarps = 4, kConvertWarps = 4, kThreads = 8 * 32;   // (two CTAs to an SM with 128 registers a thread)
 constexpr int kMaxCluster = 16;
 constexpr int kScaleStages = 4, kScaleBytes = kKeys * (4 + 4 + 2);
-constexpr float kRescaleStep = 8.f;       // log2 units
 constexpr uint32_t kTmemCols = 256;
 
 template <int kHD>
@@ -361,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) attention_tree_tc_kernel(const __
                     }
                 }
             }
-            const float shift = top == -INFINITY ? 0.f : -top;
+            const float shift = top == -INFINITY ? 0.f : kLift - top;
             auto weights = [&](auto with_masks) {
                 float2 sums = make_float2(0.f, 0.f);
                 const float2 shift2 = make_float2(shift, shift);

@@ -102,3 +102,29 @@ def test_codes_of_every_number(et):
         out, scales = torch.zeros(x.shape, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(1, len(x), device="cuda")
         et.quantise_rows(out, scales, x)
         assert torch.equal(out.float(), (x.float() / scales[0][:, None]).to(torch.float8_e4m3fn).float())
+
+
+# ------------------------------------------------------------------------------------------------ long caches
+@pytest.mark.parametrize("kernel", [0, 1])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_many_small_weights_beside_large_ones(et, kernel, hd):
+    """Keys whose weights are 2^-25.4 of those of four (one for each warp that has a reference of its own), whose values are large in one feature and 0 in the others: there the small ones are all of
+    the result, although each is below half of fp16's smallest step beside 1."""
+    n, page = 60000, 64
+    cache = Cache([n], 1, hd, page, spare=0, ratio=0.0)
+    cache.codes[:, 0], cache.codes[:, 1] = 0, 100
+    cache.scales[:, 0], cache.scales[:, 1] = 1.0, 2.0 ** -7
+    first = int(cache.table[0, 0])
+    cache.codes[first, 0, 0, ::16], cache.codes[first, 1, 0, ::16] = 1, 0
+    cache.codes[first, 1, 0, ::16, 7] = -127
+    cache.scales[first, 0, 0, ::16] = 25.4 * np.log(2.0) / hd ** 0.5       # with q = 1: the score is 25.4 log 2
+    q = torch.ones(3, 2 * hd, dtype=torch.float16, device="cuda")
+    out = torch.zeros_like(q)
+    run_kernel(et, kernel, 0, out, q, cache, None, None, 3)
+    et.attention_check()
+    for i in range(3):
+        small, v = (n - 6 + i) * 2.0 ** -25.4, torch.full((hd,), 100 / 128, dtype=torch.float64, device="cuda")
+        want, lost = v * small / (small + 4), v * (n * 2.0 ** -32) / 4
+        want[7] = (100 / 128 * small - 127 / 128 * 4) / (small + 4)
+        # rounded once, and each weight by half a step, which is 2^-11 of it or 2^-32 of the largest
+        within(out[i].view(2, hd), want, want.abs() * (2 * HALF) + lost + TINY)

@@ -103,20 +103,21 @@ __device__ __forceinline__ bool mbar_wait_at(uint32_t bar, uint32_t parity) {
     return false;
 }
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) { return mbar_wait_at(smem_u32(bar), parity); }
-// The same by a whole warp that branches on the answer: the limit may run out for some lanes just before the phase completes for others, so they vote. (At every try, which leaves the
+// Whether a phase has completed, asked without waiting by a whole warp that branches on the answer: the barrier may complete
+// between the lanes' queries, so they vote (lanes that went different ways would meet in different warp-wide operations).
+__device__ __forceinline__ bool mbar_poll_warp_at(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
+}
+__device__ __forceinline__ bool mbar_poll_warp(uint64_t* bar, uint32_t parity) { return mbar_poll_warp_at(smem_u32(bar), parity); }
+// A bounded wait by a whole warp that branches on the answer: the limit may run out for some lanes just before the phase completes for others, so they vote. (At every try, which leaves the
 // loop without lanes that part; one vote behind a loop of each lane's own took the kernels that wait most 4 % where this takes 1 %.)
 __device__ __forceinline__ bool mbar_wait_warp_at(uint32_t bar, uint32_t parity) {
 #pragma unroll 1
     for (uint32_t i = 0; i < kMbarSpinLimit; ++i)
-        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (mbar_poll_warp_at(bar, parity)) return true;
     return false;
 }
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) { return mbar_wait_warp_at(smem_u32(bar), parity); }
-// Whether a phase has completed, asked without waiting by a whole warp that branches on the answer: the barrier may complete
-// between the lanes' queries, so they vote (lanes that went different ways would meet in different warp-wide operations).
-__device__ __forceinline__ bool mbar_poll_warp(uint64_t* bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_try_wait(smem_u32(bar), parity));
-}
 // ------------------------------------------------------------------ TMA
 __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, int x, int y,
                                             uint64_t* bar) {

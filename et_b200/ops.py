@@ -5,11 +5,14 @@ function forwards to `libet_b200.so`.
 """
 import array
 import ctypes
+import importlib.util
+import os
 import struct
 
 import numpy as np
 
 from . import check, lib, ptr, raw_stream
+from .build import binding_path
 
 __all__ = [
     "skip_layernorm", "softmax_mask", "TileWeight", "tile_spmm_bias", "tile_spmm_cache_clear",
@@ -473,9 +476,15 @@ def _load_fast():
     checks below do it, which name what is wrong."""
     global _fast
     if _fast is None:
+        path = binding_path()   # (none of another Python's or torch's)
+        if path is None or not os.path.exists(path):
+            _fast = False
+            return _fast
         try:
             import torch  # noqa: F401  (its libraries are loaded first)
-            from . import _binding
+            spec = importlib.util.spec_from_file_location(__package__ + "._binding", path)
+            _binding = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(_binding)
         except ImportError:
             _fast = False
             return _fast

@@ -759,8 +759,10 @@ extern "C" int et_fp8_weight_check(const et_fp8_weight* w, int* code) {
     return ET_OK;
 }
 
-extern "C" int et_fp8_linear(const et_fp8_linear_args* a) {
-    using namespace et;
+namespace et {
+namespace {
+// forced: a plan, or null for the one that the model says.
+int fp8_linear(const et_fp8_linear_args* a, const Fp8Plan* forced) {
     ET_REQUIRE(a && a->weight, "et_fp8_linear: null weight");
     const et_fp8_weight* const w = a->weight;
     ET_REQUIRE(a->tokens >= 0 && a->tokens <= 0x7ff00000, "et_fp8_linear: negative size, or more tokens than 32 bits number");
@@ -776,6 +778,18 @@ extern "C" int et_fp8_linear(const et_fp8_linear_args* a) {
     Fp8Params p = {};
     p.Y = static_cast<half*>(a->y); p.bias = w->bias; p.x_scales = a->x_scales; p.w_scales = w->scales;
     p.y_pitch = y_pitch; p.T = a->tokens; p.N = w->N; p.k_blocks = (w->K + kBlock - 1) / kBlock; p.err = w->err;
-    const Fp8Plan plan = fp8_plan(a->tokens, w->N, p.k_blocks);
+    const Fp8Plan plan = forced ? *forced : fp8_plan(a->tokens, w->N, p.k_blocks);
     return (a->gelu ? fp8_run<true> : fp8_run<false>)(w, p, plan, a->x, x_pitch, static_cast<cudaStream_t>(a->stream));
+}
+}  // namespace
+}  // namespace et
+
+extern "C" int et_fp8_linear(const et_fp8_linear_args* a) { return et::fp8_linear(a, nullptr); }
+// Not part of the public header: one of the plans, pairs with tiles of bn features, or (bn 0) tiles of so many tokens whose K 2^log_split CTAs share, for tests that reach each of them.
+extern "C" int et_debug_fp8_linear(const et_fp8_linear_args* a, int bn, int tokens, int log_split) {
+    const et::Fp8Plan plan = {bn, tokens, log_split};
+    const bool pairs = (bn == 128 || bn == 256) && tokens == 0 && log_split == 0;
+    const bool few = bn == 0 && (tokens == 16 || tokens == 32 || tokens == 64 || tokens == 128) && log_split >= 0 && log_split < 4 && (tokens >> log_split) >= 4;
+    if (!a || !a->weight || !(pairs || (few && (1 << log_split) <= (a->weight->K + et::kBlock - 1) / et::kBlock))) return et::fail(ET_ERR_INVALID, "et_debug_fp8_linear: no such plan");
+    return et::fp8_linear(a, &plan);
 }

@@ -128,3 +128,65 @@ def test_many_small_weights_beside_large_ones(et, kernel, hd):
         want[7] = (100 / 128 * small - 127 / 128 * 4) / (small + 4)
         # rounded once, and each weight by half a step, which is 2^-11 of it or 2^-32 of the largest
         within(out[i].view(2, hd), want, want.abs() * (2 * HALF) + lost + TINY)
+
+
+# ------------------------------------------------------------------------------------------------ every plan of the linear
+def run_plan(et, plan, lin, out, x, s, gelu=False):
+    """The linear by one of its plans: (features of a pair's tile, 0, 0), or (0, tokens of a tile, log2 of the CTAs that share its K)."""
+    from et_b200 import ops
+    packed = ops._fp8_args(lin.handle._h.value, out.data_ptr(), x.data_ptr(), s.data_ptr(), torch.cuda.current_stream().cuda_stream, out.stride(0), x.stride(0), x.shape[0], 1 if gelu else 0)
+    et.check(et.lib().et_debug_fp8_linear(ctypes.create_string_buffer(packed, len(packed)), *plan))
+
+
+PLANS = [(128, 0, 0), (256, 0, 0)] + [(0, tokens, log) for tokens in (16, 32, 64, 128) for log in range(4) if tokens >> log >= 4]
+
+
+def checked(et, plan, lin, tokens, gelu):
+    """One call, X and Y as slices of wider rows: against 64 bits, nothing beside the slices, the same bits again."""
+    x, s = lin.inputs(tokens)
+    x = rows_of(x, lin.k + 48, 16)
+    wide = torch.full((tokens, lin.n + 24), 3.0, dtype=torch.float16, device="cuda")
+    out = wide[:, :lin.n]
+    run_plan(et, plan, lin, out, x, s, gelu)
+    lin.gelu = gelu
+    lin.check(out, x, s)
+    assert (wide[:, lin.n:] == 3).all()
+    again = torch.zeros_like(out)
+    run_plan(et, plan, lin, again, x, s, gelu)
+    assert torch.equal(again, out)
+    return x, s, out
+
+
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("plan", PLANS)
+@pytest.mark.parametrize("k,n,tokens", [(1040, 400, 1), (1024, 272, 130), (1168, 144, 61), (2192, 16, 257)])
+def test_every_plan(et, plan, gelu, k, n, tokens):
+    """Features, tokens and K that fill no tile. (K of 8 blocks and more: as many as the widest split.)"""
+    checked(et, plan, Linear(et, k, n), tokens, gelu)
+
+
+@pytest.mark.parametrize("gelu", [False, True])
+@pytest.mark.parametrize("plan", PLANS)
+def test_every_plan_with_more_tiles_than_places(et, plan, gelu):
+    """Several tiles to a pair (of odd numbers of blocks, so that rings and places go on where the tile before left them), and more CTAs than SMs."""
+    k, n, tokens = (1040, 2960, 2500) if plan[0] else (1040, 2960, 900)
+    checked(et, plan, Linear(et, k, n), tokens, gelu)
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_long_k_by_every_plan(et, plan):
+    """More blocks to a CTA than its scales' buffer (16) and its rings hold."""
+    checked(et, plan, Linear(et, 6416, 144), 70, False)
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_a_row_that_is_not_finite_stays_alone_by_every_plan(et, plan):
+    lin = Linear(et, 1040, 272)
+    x, s, clean = checked(et, plan, lin, 300, False)
+    x.view(torch.uint8)[3, 7] = 0x7f
+    s[1, 4] = float("inf")
+    s[8, 299] = float("nan")
+    out = torch.zeros_like(clean)
+    run_plan(et, plan, lin, out, x, s)
+    rest = [i for i in range(300) if i not in (3, 4, 299)]
+    assert out[3].isnan().all() and not out[4].isfinite().any() and out[299].isnan().all() and torch.equal(out[rest], clean[rest])

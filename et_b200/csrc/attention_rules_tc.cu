@@ -379,7 +379,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
 #define ET_BAR(name, ...) bar(offsetof(TcShared, name), ##__VA_ARGS__)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hd = r.head_dim, osteps = hd >> 4;
-    pdl_launch_dependents();
 
     if (warp == kLoadWarp) {
         if (lane == 0) {
@@ -415,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_rules_tc_kerne
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();   // (behind the allocation: columns that a dependent CTA takes first it keeps until this kernel has ended)
     const uint32_t tmem = sh->tmem_base;
 
     if (warp == kLoadWarp) {

@@ -368,7 +368,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_tc_kernel(cons
     TcShared* const sh = reinterpret_cast<TcShared*>(smem + C::kBytes);
     SeqTable* const table = reinterpret_cast<SeqTable*>(sh + 1);   // kSorted
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    pdl_launch_dependents();
     // The place of block g's mask, and how often it has been used before. The second place lies behind everything else.
     auto mask_place = [&](uint32_t g) {
         return smem + (p.mask_two && (g & 1u) ? C::template second_mask_at<kSorted>() : C::kMaskAt);
@@ -411,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_tc_kernel(cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();   // (behind the allocation: columns that a dependent CTA takes first it keeps until this kernel has ended)
     const uint32_t tmem = sh->tmem_base;
     if (warp == kSoftmaxWarps) {
         // ---- items and loads (all lanes stay together; lane 0 issues)

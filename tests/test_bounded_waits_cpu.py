@@ -61,3 +61,20 @@ def test_a_warp_votes_on_what_it_waited_for(name):
         used = re.search(r"(ok|got) =|return|if \(!?$|&& $", statement)
         behind = text[text.index(";", m.start()) + 1:].lstrip()
         assert not used or behind.startswith("ok = __all_sync(0xffffffffu, ok);") or by_one_lane(text, m.start(), inside), statement + text[m.start():m.start() + 80]
+
+
+def test_dependent_kernels_start_behind_the_allocation_of_tensor_memory():
+    """A dependent CTA takes columns as soon as it runs and waits with them for the kernel before it. A CTA of that kernel that still had to get its own could wait for the other for ever."""
+    seen = 0
+    for name in sorted(f for f in os.listdir(CSRC) if f.endswith(".cu")):
+        with open(os.path.join(CSRC, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        for kernel in re.split(r"\b__global__\b", text)[1:]:
+            allocs = [m.start() for m in re.finditer(r"\btmem_alloc\(|tcgen05\.alloc\.", kernel)]
+            starts = [m.start() for m in re.finditer(r"\bpdl_launch_dependents\(\)", kernel)]
+            if allocs and starts:
+                seen += 1
+                assert max(allocs) < min(starts), name
+                # (a barrier of the block, or a wait for what has been multiplied there)
+                assert re.search(r"__syncthreads\(\);|acc_full|acc_done", kernel[max(allocs):min(starts)]), name
+    assert seen >= 8

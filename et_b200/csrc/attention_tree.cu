@@ -4,13 +4,13 @@
 // The queries and query heads of a K/V head are rows, eight to a tile of mma.sync m16n8k16: 16 keys x 8 rows of scores, then 16 features x 8 rows of O, so that no part of a tile is empty (with the
 // rows as the tile's 16, which four query heads fill to a quarter, twice the products). Codes become halves exactly (three operations for four), the key's scale multiplies the
 // score, the value's scale the weight. A block of 16 keys of a head lies in one page: K and V of it come by one TMA copy (16 x 128 bytes each, swizzled; heads of 256 by two),
-// a block or two ahead, into a ring that each warp has for itself. (Each lane's pieces by cp.async, 60 instructions of all lanes to a block, took 69 us where this takes 58, below; heads of up to 64,
+// a block or two ahead, into a ring that each warp has for itself. (Each lane's pieces by cp.async, 60 instructions of all lanes to a block, took 69 us where this took 58, below; heads of up to 64,
 // whose copies are half as large, are 6 to 9 % faster that way and have it.)
 // Which features a step of the first product takes, and which the rows of the second are, is free: a lane has 16 neighbouring codes of a key of K, and for V of four keys the codes of 16 (8)
 // neighbouring features, by wide loads without bank conflicts. A cluster of CTAs shares a sequence's keys, its warps take blocks of 16 in turn with a reference, sum and O of their own,
 // joined in shared and then distributed shared memory in a fixed order: no workspace, one launch, the same bits every time.
 //
-// 64 sequences of up to 8192 keys, single tokens of 16 heads of 128 over 4: 58 us; codes read once 42.
+// 64 sequences of up to 8192 keys, single tokens of 16 heads of 128 over 4: 57 us; codes read once 42. (16 rows of heads of 128 and of 256 spill 12 and 52 bytes.)
 //
 // Scores, references and sums are fp32; the weights times the values' scales go to the second product as fp16 (half a step of 2^-11 of a weight).
 #include <algorithm>

@@ -7,9 +7,9 @@
 // it has to (then O is rescaled in tensor memory). Two CTAs share an SM: while one waits for its products the other takes exponentials. A cluster shares a sequence's keys; its CTAs' rows are joined
 // through distributed shared memory in a fixed order.
 //
-// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 146 us (150 with codes by cp.async, 155 with the scores' UMMAs in a loop that is not unrolled besides); codes read once 36. No unit is full
+// 16 sequences of up to 12000 keys and 48 drafted tokens, 32 heads of 128 over 8: 149 us (146 without the warps' votes on their waits; with codes by cp.async 4 more, with the scores' UMMAs in a loop that is not unrolled 5 more besides); codes read once 36. No unit is full
 // (shared-memory pipe 40 %, ALU 29 %, issue slots 38 %, tensor pipe 22 %): a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3200 clocks
-// with two CTAs to an SM. Tried: scores in halves of 32 keys, one multiplied while the other is weighed, by a warp of its own that issues UMMAs 165 (20 of them to a block instead of 12, some 45
+// with two CTAs to an SM. (Of 128 registers a thread 12 bytes are spilled.) Tried, against 146: scores in halves of 32 keys, one multiplied while the other is weighed, by a warp of its own that issues UMMAs 165 (20 of them to a block instead of 12, some 45
 // clocks of the issuing thread each); two places for scores, Q in shared memory (as tensor memory is full then), such a warp, registers handed over 174 (with Q in tensor memory and one place 163),
 // with codes fetched into registers 168 to 178 (operands from shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182.
 #include <cooperative_groups.h>

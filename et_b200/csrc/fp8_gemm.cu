@@ -5,9 +5,10 @@
 // registers while the next block is multiplied into another place. Two kernels:
 //
 // fp8_pair_kernel, many tokens: persistent pairs of CTAs (cta_group::2), 256 tokens x kBN features to a tile. A thread has a token's row of kBN / 2 columns. 16384 x 4096 -> 4096:
-// 244 us (2.2e15 operations a second), with GELU 254 (on random codes and for a quarter of a second 305: power). Of the ~900 clocks a block of 256 x 256 takes (UMMAs: 512) copies alone would take ~800 (the way from L2), sums and hand-overs
-// alone ~850. Tried: one warp that issues all UMMAs 244 / 253 us, four of them 248 / 256, sixteen warps that sum 255 / 266, eight with one
-// load from tensor memory at a time 260 / 275, waits by one lane of a warp 267, scales read behind the wait 269.
+// 255 us (2.2e15 operations a second), with GELU 273 (calls one after another for a quarter of a second 318: power). Of the ~900 clocks a block of 256 x 256 takes (UMMAs: 512) copies alone would take ~800 (the way from L2), sums and hand-overs
+// alone ~850. Tried, against 244 and with GELU 254 us (a cooler card, a GELU by tanh.approx, waits without votes): one warp that issues all UMMAs 244 / 253 us, four of them 248 / 256, sixteen warps that sum 255 / 266, eight with one
+// load from tensor memory at a time 260 / 275, waits by one lane of a warp 267, scales read behind the wait 269. A vote of the warp behind each wait, instead of at every try of it, takes 10 us more, at the end of the block 15, lanes that go on without
+// one and without a branch (which the compiler schedules worse) 20 to 40.
 //
 // fp8_few_kernel, few tokens: operands exchanged, 128 features are the tile's rows and kTokens tokens its columns, so that the weight, which is what has to
 // be read, fills the tile; K split over a cluster. Each CTA sends the others their columns' parts (asynchronous stores that count towards a barrier of the receiver) and

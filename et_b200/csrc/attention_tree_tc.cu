@@ -11,7 +11,8 @@
 // (shared-memory pipe 40 %, ALU 29 %, issue slots 38 %, tensor pipe 22 %): a CTA's block is a chain, scores -> 64 scales, maxima and exponentials -> weights -> both products, some 3200 clocks
 // with two CTAs to an SM. (Of 128 registers a thread 12 bytes are spilled.) Tried, against 146: scores in halves of 32 keys, one multiplied while the other is weighed, by a warp of its own that issues UMMAs 165 (20 of them to a block instead of 12, some 45
 // clocks of the issuing thread each); two places for scores, Q in shared memory (as tensor memory is full then), such a warp, registers handed over 174 (with Q in tensor memory and one place 163),
-// with codes fetched into registers 168 to 178 (operands from shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182.
+// with codes fetched into registers 168 to 178 (operands from shared memory take all of its bandwidth at N 64); codes fetched into registers in this form 189; clusters of two and eight 165 and 182. Weights
+// as two halves each, for results as exact as fp16 has them, take 174 us (attention_tree.cu says what one half costs them).
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "attention.h"
